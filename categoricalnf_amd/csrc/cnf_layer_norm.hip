@@ -1,0 +1,472 @@
+// Layer norm over the last axis, forward and backward, with the weight's and bias's gradients.
+//
+//   xhat = (x - mean) rstd,  y = xhat w + b,  mean and rstd per row in fp32 (variance from the centred values: two passes over
+//   registers, so a large common offset of a row does not cancel)
+//   dx = rstd (g w - mean_c(g w) - xhat mean_c(g w xhat)),   dw = sum_r g xhat,   db = sum_r g
+//
+// Bound by HBM: the forward reads x and writes y, the backward reads x and g and writes dx, each once.  A row lives in the
+// registers of the lanes that own it — a group of G lanes of a wave (up to 1024 columns; 64 / G rows per wave) or a whole
+// workgroup (up to 16 384) —, at most 16 elements per lane.  The backward's lanes own the same columns in every row they walk, so
+// the two column sums stay in registers over the whole launch; each workgroup writes one partial row of 2 C sums, and a second
+// launch adds the partial rows in their order (the same bits on every run, no atomics).  Longer rows take kernels that read a row
+// three times (forward) or twice (backward) and sum the columns in a launch of their own.
+#include <algorithm>
+#include <type_traits>
+
+#include "cnf_dtype.h"
+
+namespace cnf {
+
+constexpr int kLnElems = 16;                        // elements of a row one lane holds at most
+constexpr int kLnWaveCols = kWave * kLnElems;       // widest row of one wave
+constexpr int kLnBlockCols = 1024 * kLnElems;       // widest row of one workgroup
+constexpr int kLnMaxPartials = 1024;                // partial rows of the column sums
+
+struct LnArgs {
+    const void *x, *dy, *weight, *bias;
+    void *y, *dx;
+    float *mean, *rstd;
+    float* partials;
+    int64_t x_stride, dy_stride, y_stride;          // elements between rows (dx has y_stride)
+    int64_t rows;
+    int cols, wdtype, group;                        // group: lanes per row (wave kernels)
+    float eps;
+};
+
+// sum over the lanes that share a row: a power-of-two group of a wave, or the workgroup
+struct WaveGroup {
+    int g;
+    __device__ __forceinline__ float sum(float v) const { return group_sum(v, g); }
+    __device__ __forceinline__ Sum2 sum(Sum2 v) const { return group_sum(v, g); }
+};
+struct BlockGroup {
+    float* sh;      // 2 x 16 floats
+    __device__ __forceinline__ Sum2 sum(Sum2 v) const {
+        v = wave_sum(v);
+        const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+        __syncthreads();                            // the previous sum has been read
+        if ((threadIdx.x & 63) == 0) {
+            sh[wave] = v.a;
+            sh[16 + wave] = v.b;
+        }
+        __syncthreads();
+        Sum2 t(0);
+        for (int w = 0; w < waves; ++w) t += Sum2(sh[w], sh[16 + w]);
+        return t;
+    }
+    __device__ __forceinline__ float sum(float v) const { return sum(Sum2(v, 0.f)).a; }
+};
+
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void ln_load(const T* row, int l, int lanes, int cols, bool on, vec_t<T, VEC>* v) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = (j * lanes + l) * VEC;
+        vec_t<T, VEC> z;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) z[i] = (T)0.f;
+        v[j] = (on && c < cols) ? *reinterpret_cast<const vec_t<T, VEC>*>(row + c) : z;
+    }
+}
+
+template <int VEC, int NV>
+__device__ __forceinline__ void ln_load_weight(const void* w, int wdtype, int l, int lanes, int cols, float fill, float* out) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const int c = (j * lanes + l) * VEC + i;
+            out[j * VEC + i] = (w && c < cols) ? load_any(w, wdtype, c) : fill;
+        }
+}
+
+template <typename T, int VEC, int NV, typename Group>
+__device__ __forceinline__ void ln_fwd_row(const LnArgs& a, int64_t row, bool on, int l, int lanes, const Group& grp,
+                                           const float* w, const float* b) {
+    vec_t<T, VEC> xv[NV];
+    ln_load<T, VEC, NV>(static_cast<const T*>(a.x) + row * a.x_stride, l, lanes, a.cols, on, xv);
+    float x[NV * VEC], s = 0.f;
+#pragma unroll
+    for (int e = 0; e < NV * VEC; ++e) {
+        x[e] = (float)xv[e / VEC][e % VEC];
+        s += x[e];
+    }
+    const float inv = 1.f / (float)a.cols;
+    const float mean = grp.sum(s) * inv;
+    float q = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const bool in = (j * lanes + l) * VEC < a.cols;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            float& v = x[j * VEC + i];
+            v = in ? v - mean : 0.f;
+            q += v * v;
+        }
+    }
+    const float rstd = 1.f / sqrtf(grp.sum(q) * inv + a.eps);
+    if (!on) return;
+    T* y = static_cast<T*>(a.y) + row * a.y_stride;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = (j * lanes + l) * VEC;
+        if (c >= a.cols) continue;
+        vec_t<T, VEC> o;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o[i] = (T)(x[j * VEC + i] * rstd * w[j * VEC + i] + b[j * VEC + i]);
+        *reinterpret_cast<vec_t<T, VEC>*>(y + c) = o;
+    }
+    if (l == 0 && a.mean) {
+        a.mean[row] = mean;
+        a.rstd[row] = rstd;
+    }
+}
+
+template <typename T, int VEC, int NV>
+__global__ __launch_bounds__(kBlock) void ln_fwd_wave_kernel(const LnArgs a) {
+    const int g = a.group, rpw = kWave / g;
+    const int lane = threadIdx.x & 63, l = lane & (g - 1);
+    const int slot = (threadIdx.x >> 6) * rpw + lane / g, rpb = kWavesPerBlock * rpw;
+    float w[NV * VEC], b[NV * VEC];
+    ln_load_weight<VEC, NV>(a.weight, a.wdtype, l, g, a.cols, 1.f, w);
+    ln_load_weight<VEC, NV>(a.bias, a.wdtype, l, g, a.cols, 0.f, b);
+    const WaveGroup grp{g};
+    for (int64_t r0 = (int64_t)blockIdx.x * rpb; r0 < a.rows; r0 += (int64_t)gridDim.x * rpb)
+        ln_fwd_row<T, VEC, NV>(a, r0 + slot, r0 + slot < a.rows, l, g, grp, w, b);
+}
+
+template <typename T, int VEC, int NV>
+__global__ __launch_bounds__(1024) void ln_fwd_block_kernel(const LnArgs a) {
+    __shared__ float sh[32];
+    const BlockGroup grp{sh};
+    float w[NV * VEC], b[NV * VEC];
+    ln_load_weight<VEC, NV>(a.weight, a.wdtype, threadIdx.x, blockDim.x, a.cols, 1.f, w);
+    ln_load_weight<VEC, NV>(a.bias, a.wdtype, threadIdx.x, blockDim.x, a.cols, 0.f, b);
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x)
+        ln_fwd_row<T, VEC, NV>(a, r, true, threadIdx.x, blockDim.x, grp, w, b);
+}
+
+template <typename T, int VEC, int NV, typename Group>
+__device__ __forceinline__ void ln_bwd_row(const LnArgs& a, int64_t row, bool on, int l, int lanes, const Group& grp,
+                                           const float* w, float* dw, float* db) {
+    vec_t<T, VEC> xv[NV], gv[NV];
+    ln_load<T, VEC, NV>(static_cast<const T*>(a.x) + row * a.x_stride, l, lanes, a.cols, on, xv);
+    ln_load<T, VEC, NV>(static_cast<const T*>(a.dy) + row * a.dy_stride, l, lanes, a.cols, on, gv);
+    const float mean = on ? a.mean[row] : 0.f, rstd = on ? a.rstd[row] : 0.f;
+    float xh[NV * VEC], gw[NV * VEC];
+    Sum2 s(0);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const bool in = (j * lanes + l) * VEC < a.cols;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const int e = j * VEC + i;
+            const float g = (float)gv[j][i];
+            xh[e] = in ? ((float)xv[j][i] - mean) * rstd : 0.f;
+            gw[e] = g * w[e];
+            dw[e] += g * xh[e];
+            db[e] += g;
+            s += Sum2(gw[e], gw[e] * xh[e]);
+        }
+    }
+    s = grp.sum(s);
+    if (!on) return;
+    const float inv = 1.f / (float)a.cols, c1 = s.a * inv, c2 = s.b * inv;
+    T* dx = static_cast<T*>(a.dx) + row * a.y_stride;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = (j * lanes + l) * VEC;
+        if (c >= a.cols) continue;
+        vec_t<T, VEC> o;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o[i] = (T)(rstd * (gw[j * VEC + i] - c1 - xh[j * VEC + i] * c2));
+        *reinterpret_cast<vec_t<T, VEC>*>(dx + c) = o;
+    }
+}
+
+// partials: [gridDim.x][2][cols]
+template <typename T, int VEC, int NV>
+__global__ __launch_bounds__(kBlock) void ln_bwd_wave_kernel(const LnArgs a) {
+    __shared__ float sh[kWavesPerBlock][kLnWaveCols];
+    const int g = a.group, rpw = kWave / g;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & (g - 1);
+    const int slot = wave * rpw + lane / g, rpb = kWavesPerBlock * rpw;
+    float w[NV * VEC], acc[2][NV * VEC];
+    ln_load_weight<VEC, NV>(a.weight, a.wdtype, l, g, a.cols, 1.f, w);
+#pragma unroll
+    for (int e = 0; e < NV * VEC; ++e) acc[0][e] = acc[1][e] = 0.f;
+    const WaveGroup grp{g};
+    for (int64_t r0 = (int64_t)blockIdx.x * rpb; r0 < a.rows; r0 += (int64_t)gridDim.x * rpb)
+        ln_bwd_row<T, VEC, NV>(a, r0 + slot, r0 + slot < a.rows, l, g, grp, w, acc[0], acc[1]);
+    if (!a.partials) return;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int e = 0; e < NV * VEC; ++e) {
+            float v = acc[k][e];
+            for (int m = g; m < kWave; m <<= 1) v += __shfl_xor(v, m, kWave);       // the wave's row groups
+            const int c = ((e / VEC) * g + l) * VEC + e % VEC;
+            if (lane < g && c < a.cols) sh[wave][c] = v;
+        }
+        __syncthreads();
+        float* out = a.partials + ((size_t)blockIdx.x * 2 + k) * a.cols;
+        for (int c = threadIdx.x; c < a.cols; c += kBlock) {
+            float t = 0.f;
+#pragma unroll
+            for (int q = 0; q < kWavesPerBlock; ++q) t += sh[q][c];
+            out[c] = t;
+        }
+        __syncthreads();
+    }
+}
+
+template <typename T, int VEC, int NV>
+__global__ __launch_bounds__(1024) void ln_bwd_block_kernel(const LnArgs a) {
+    __shared__ float sh[32];
+    const BlockGroup grp{sh};
+    float w[NV * VEC], acc[2][NV * VEC];
+    ln_load_weight<VEC, NV>(a.weight, a.wdtype, threadIdx.x, blockDim.x, a.cols, 1.f, w);
+#pragma unroll
+    for (int e = 0; e < NV * VEC; ++e) acc[0][e] = acc[1][e] = 0.f;
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x)
+        ln_bwd_row<T, VEC, NV>(a, r, true, threadIdx.x, blockDim.x, grp, w, acc[0], acc[1]);
+    if (!a.partials) return;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int e = 0; e < NV * VEC; ++e) {
+            const int c = ((e / VEC) * blockDim.x + threadIdx.x) * VEC + e % VEC;
+            if (c < a.cols) a.partials[((size_t)blockIdx.x * 2 + k) * a.cols + c] = acc[k][e];
+        }
+}
+
+// ---- rows wider than a workgroup's registers: the row is read again instead of held ---------------------------------------------
+
+template <typename T>
+__global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const LnArgs a) {
+    __shared__ float sh[32];
+    const BlockGroup grp{sh};
+    const float inv = 1.f / (float)a.cols;
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
+        T* y = static_cast<T*>(a.y) + r * a.y_stride;
+        float s = 0.f, q = 0.f;
+        for (int c = threadIdx.x; c < a.cols; c += 1024) s += (float)x[c];
+        const float mean = grp.sum(s) * inv;
+        for (int c = threadIdx.x; c < a.cols; c += 1024) {
+            const float d = (float)x[c] - mean;
+            q += d * d;
+        }
+        const float rstd = 1.f / sqrtf(grp.sum(q) * inv + a.eps);
+        for (int c = threadIdx.x; c < a.cols; c += 1024) {
+            const float w = a.weight ? load_any(a.weight, a.wdtype, c) : 1.f, b = a.bias ? load_any(a.bias, a.wdtype, c) : 0.f;
+            y[c] = (T)(((float)x[c] - mean) * rstd * w + b);
+        }
+        if (threadIdx.x == 0 && a.mean) {
+            a.mean[r] = mean;
+            a.rstd[r] = rstd;
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(1024) void ln_bwd_long_kernel(const LnArgs a) {
+    __shared__ float sh[32];
+    const BlockGroup grp{sh};
+    const float inv = 1.f / (float)a.cols;
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
+        const T* g = static_cast<const T*>(a.dy) + r * a.dy_stride;
+        T* dx = static_cast<T*>(a.dx) + r * a.y_stride;
+        const float mean = a.mean[r], rstd = a.rstd[r];
+        Sum2 s(0);
+        for (int c = threadIdx.x; c < a.cols; c += 1024) {
+            const float gw = (float)g[c] * (a.weight ? load_any(a.weight, a.wdtype, c) : 1.f);
+            s += Sum2(gw, gw * (((float)x[c] - mean) * rstd));
+        }
+        s = grp.sum(s);
+        for (int c = threadIdx.x; c < a.cols; c += 1024) {
+            const float gw = (float)g[c] * (a.weight ? load_any(a.weight, a.wdtype, c) : 1.f);
+            dx[c] = (T)(rstd * (gw - s.a * inv - ((float)x[c] - mean) * rstd * (s.b * inv)));
+        }
+    }
+}
+
+// column sums of long rows: a workgroup owns 256 columns of every gridDim.y-th row
+template <typename T>
+__global__ __launch_bounds__(kBlock) void ln_columns_kernel(const LnArgs a) {
+    const int c = blockIdx.x * kBlock + threadIdx.x;
+    if (c >= a.cols) return;
+    float dw = 0.f, db = 0.f;
+    for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
+        const float g = (float)static_cast<const T*>(a.dy)[r * a.dy_stride + c];
+        dw += g * (((float)static_cast<const T*>(a.x)[r * a.x_stride + c] - a.mean[r]) * a.rstd[r]);
+        db += g;
+    }
+    a.partials[((size_t)blockIdx.y * 2) * a.cols + c] = dw;
+    a.partials[((size_t)blockIdx.y * 2 + 1) * a.cols + c] = db;
+}
+
+// partial rows -> dweight, dbias.  A workgroup owns 16 columns of the 2 C sums (one 64-byte segment per partial row); its 64 row
+// slots each add every 64th partial row, then the slots are added in order.
+__global__ __launch_bounds__(1024) void ln_reduce_kernel(const float* __restrict__ partials, int nparts, int cols, int wdtype,
+                                                         void* dweight, void* dbias) {
+    __shared__ float sh[64][17];
+    const int cl = threadIdx.x & 15, slot = threadIdx.x >> 4;
+    const int64_t k = (int64_t)blockIdx.x * 16 + cl, width = 2 * (int64_t)cols;
+    float t = 0.f;
+    if (k < width)
+        for (int p = slot; p < nparts; p += 64) t += partials[(size_t)p * width + k];
+    sh[slot][cl] = t;
+    __syncthreads();
+    if (slot == 0 && k < width) {
+        float v = 0.f;
+#pragma unroll
+        for (int q = 0; q < 64; ++q) v += sh[q][cl];
+        if (k < cols) {
+            if (dweight) store_any(dweight, wdtype, k, v);
+        } else if (dbias) {
+            store_any(dbias, wdtype, k - cols, v);
+        }
+    }
+}
+
+// How a launch deals rows to lanes.  16-byte vectors where every row allows it; otherwise single elements.
+struct LnShape {
+    int vec;        // 1: 16-byte vectors
+    int nv;         // vectors (elements) per lane: 1 or the most that keeps 16 elements
+    int group;      // lanes per row; > 64: the workgroup's size
+    int kind;       // 0 wave, 1 workgroup, 2 long rows
+};
+static LnShape ln_shape(int cols, int dtype, bool aligned) {
+    LnShape s;
+    const int per = 16 / dtype_bytes(dtype);
+    s.vec = aligned && cols % per == 0;
+    const int width = s.vec ? per : 1, units = (cols + width - 1) / width, most = kLnElems / width;
+    s.nv = units <= 16 ? 1 : most;      // short rows: one load per lane keeps the lanes of a wave busy
+    int g = 1;
+    while ((int64_t)g * s.nv < units) g <<= 1;
+    s.kind = cols > kLnBlockCols ? 2 : (g > kWave ? 1 : 0);
+    s.group = s.kind == 1 && g < kBlock ? kBlock : g;
+    return s;
+}
+
+static int ln_partials(int64_t rows, const LnShape& s) {
+    if (s.kind == 2) return (int)std::min<int64_t>(rows, 64);
+    const int rpb = s.kind == 1 ? 1 : kWavesPerBlock * (kWave / s.group);
+    const int64_t steps = (rows + rpb - 1) / rpb;
+    // at least 8 steps of rows per workgroup before there are more than 256 of them: each workgroup writes 2 C sums at its end
+    return (int)std::min<int64_t>(steps, std::max<int64_t>(256, std::min<int64_t>(kLnMaxPartials, steps / 8)));
+}
+
+template <typename T, typename Wave, typename Block>
+static void ln_pick(const LnShape& s, Wave&& wave, Block&& block) {
+    constexpr int V = 16 / (int)sizeof(T);
+    if (s.kind == 0) {
+        if (s.vec && s.nv == 1) wave(std::integral_constant<int, V>{}, std::integral_constant<int, 1>{});
+        else if (s.vec) wave(std::integral_constant<int, V>{}, std::integral_constant<int, kLnElems / V>{});
+        else if (s.nv == 1) wave(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
+        else wave(std::integral_constant<int, 1>{}, std::integral_constant<int, kLnElems>{});
+    } else if (s.vec) {
+        block(std::integral_constant<int, V>{}, std::integral_constant<int, kLnElems / V>{});
+    } else {
+        block(std::integral_constant<int, 1>{}, std::integral_constant<int, kLnElems>{});
+    }
+}
+
+}  // namespace cnf
+
+using namespace cnf;
+
+extern "C" {
+
+int cnf_layer_norm(const void* x, int64_t x_stride, const void* weight, const void* bias, void* y, float* mean, float* rstd,
+                   int64_t rows, int cols, float eps, int dtype, int wdtype, cnf_stream_t stream) {
+    CNF_REQUIRE(x && y, "cnf_layer_norm: null tensor");
+    CNF_REQUIRE(rows >= 0 && cols > 0 && x_stride >= 0, "cnf_layer_norm: bad size rows=%ld cols=%d", (long)rows, cols);
+    CNF_REQUIRE(dtype_known(dtype) && dtype_known(wdtype), "cnf_layer_norm: unknown element type");
+    CNF_REQUIRE(!mean == !rstd, "cnf_layer_norm: mean and rstd come together");
+    if (rows == 0) return CNF_OK;
+    LnArgs a{};
+    a.x = x; a.weight = weight; a.bias = bias; a.y = y; a.mean = mean; a.rstd = rstd;
+    a.x_stride = x_stride; a.y_stride = cols; a.rows = rows; a.cols = cols; a.wdtype = wdtype; a.eps = eps;
+    const LnShape s = ln_shape(cols, dtype, rows_aligned16(x, x_stride, dtype) && rows_aligned16(y, cols, dtype));
+    a.group = s.group;
+    hipStream_t st = (hipStream_t)stream;
+    return with_dtype(dtype, [&](auto t) {
+        typedef decltype(t) T;
+        if (s.kind == 2) {
+            CNF_LAUNCH((ln_fwd_long_kernel<T>), dim3((unsigned)std::min<int64_t>(rows, 2048)), dim3(1024), 0, st, a);
+        } else {
+            ln_pick<T>(s,
+                       [&](auto v, auto n) {
+                           const int rpb = kWavesPerBlock * (kWave / s.group);
+                           const unsigned grid = (unsigned)std::min<int64_t>((rows + rpb - 1) / rpb, 4096);
+                           CNF_LAUNCH((ln_fwd_wave_kernel<T, decltype(v)::value, decltype(n)::value>), dim3(grid), dim3(kBlock), 0, st, a);
+                       },
+                       [&](auto v, auto n) {
+                           CNF_LAUNCH((ln_fwd_block_kernel<T, decltype(v)::value, decltype(n)::value>),
+                                      dim3((unsigned)std::min<int64_t>(rows, 4096)), dim3(s.group), 0, st, a);
+                       });
+        }
+        return launch_status("cnf_layer_norm");
+    });
+}
+
+int64_t cnf_layer_norm_bwd_workspace_floats(int64_t rows, int cols) {
+    if (rows <= 0 || cols <= 0) return 0;
+    // the largest partials matrix over the layouts a launch of this size may take
+    int64_t most = 0;
+    for (int dtype : {CNF_DTYPE_F32, CNF_DTYPE_BF16})
+        for (int aligned = 0; aligned < 2; ++aligned)
+            most = std::max<int64_t>(most, ln_partials(rows, ln_shape(cols, dtype, aligned != 0)));
+    return most * 2 * cols;
+}
+
+int cnf_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, const void* weight,
+                       const float* mean, const float* rstd, void* dx, void* dweight, void* dbias, float* ws, int64_t ws_floats,
+                       int64_t rows, int cols, int dtype, int wdtype, cnf_stream_t stream) {
+    CNF_REQUIRE(x && dy && mean && rstd && dx, "cnf_layer_norm_bwd: null tensor");
+    CNF_REQUIRE(rows >= 0 && cols > 0 && x_stride >= 0 && dy_stride >= 0, "cnf_layer_norm_bwd: bad size rows=%ld cols=%d", (long)rows, cols);
+    CNF_REQUIRE(dtype_known(dtype) && dtype_known(wdtype), "cnf_layer_norm_bwd: unknown element type");
+    const bool sums = dweight || dbias;
+    CNF_REQUIRE(!sums || rows == 0 || (ws && ws_floats >= cnf_layer_norm_bwd_workspace_floats(rows, cols)),
+                "cnf_layer_norm_bwd: workspace smaller than cnf_layer_norm_bwd_workspace_floats");
+    LnArgs a{};
+    a.x = x; a.dy = dy; a.weight = weight; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd); a.dx = dx;
+    a.x_stride = x_stride; a.dy_stride = dy_stride; a.y_stride = cols; a.rows = rows; a.cols = cols; a.wdtype = wdtype;
+    a.partials = sums ? ws : nullptr;
+    const LnShape s = ln_shape(cols, dtype, rows_aligned16(x, x_stride, dtype) && rows_aligned16(dy, dy_stride, dtype) &&
+                                                rows_aligned16(dx, cols, dtype));
+    a.group = s.group;
+    const int parts = rows > 0 ? ln_partials(rows, s) : 0;
+    hipStream_t st = (hipStream_t)stream;
+    if (rows > 0) {
+        const int rc = with_dtype(dtype, [&](auto t) {
+            typedef decltype(t) T;
+            if (s.kind == 2) {
+                CNF_LAUNCH((ln_bwd_long_kernel<T>), dim3((unsigned)std::min<int64_t>(rows, 2048)), dim3(1024), 0, st, a);
+                if (sums)
+                    CNF_LAUNCH((ln_columns_kernel<T>), dim3((cols + kBlock - 1) / kBlock, parts), dim3(kBlock), 0, st, a);
+            } else {
+                ln_pick<T>(s,
+                           [&](auto v, auto n) {
+                               CNF_LAUNCH((ln_bwd_wave_kernel<T, decltype(v)::value, decltype(n)::value>), dim3(parts), dim3(kBlock), 0, st, a);
+                           },
+                           [&](auto v, auto n) {
+                               CNF_LAUNCH((ln_bwd_block_kernel<T, decltype(v)::value, decltype(n)::value>), dim3(parts), dim3(s.group), 0, st, a);
+                           });
+            }
+            return launch_status("cnf_layer_norm_bwd");
+        });
+        if (rc != CNF_OK) return rc;
+    }
+    if (sums) {
+        const unsigned grid = (unsigned)((2 * (int64_t)cols + 15) / 16);
+        CNF_LAUNCH(ln_reduce_kernel, dim3(grid), dim3(1024), 0, st, ws, parts, cols, wdtype, dweight, dbias);
+        return launch_status("cnf_layer_norm_bwd (column sums)");
+    }
+    return CNF_OK;
+}
+
+}  // extern "C"

@@ -34,7 +34,7 @@ from ..distributed import allreduce_nll, init_process_group, shard_bounds, wrap_
 from ..host_utils import create_channel_mask
 from ..layers.flows.distributions import LogisticDistribution
 from .language_modeling import FlowLanguageModeling
-from .run_set_modeling import checkpoint_file, load_checkpoint, save_args, save_checkpoint
+from .run_set_modeling import (add_optimizer_args, checkpoint_file, load_checkpoint, make_optimizer, optimizer_class, save_args, save_checkpoint)
 
 LOG2E = float(np.log2(np.e))
 
@@ -98,6 +98,7 @@ def parse(argv=None):
     p.add_argument("--only_eval", action="store_true")
     p.add_argument("--learning_rate", type=float, default=7.5e-4)
     p.add_argument("--lr_decay_factor", type=float, default=0.999975)
+    add_optimizer_args(p)
     p.add_argument("--max_gradient_norm", type=float, default=0.25)
     p.add_argument("--encoding_dim", type=int, default=3)
     p.add_argument("--coupling_hidden_size", type=int, default=1024)
@@ -208,7 +209,7 @@ def _main(argv=None):
     with contextlib.redirect_stdout(io.StringIO()):
         model = FlowLanguageModeling(model_params(args), None, vocab_size=args.vocab_size, vocab=Vocab()).to(device)
     prior = LogisticDistribution(mu=0.0, sigma=1.0)
-    optimizer = torch.optim.RAdam(model.parameters(), lr=args.learning_rate)
+    optimizer = make_optimizer(args, model.parameters())
     scheduler = torch.optim.lr_scheduler.LambdaLR(optimizer, lambda step: args.lr_decay_factor ** step)
     state = {"iteration": 0, "best_save_dict": {"file": None, "metric": 1e6, "detailed_metrics": None, "test": None},
              "evaluation_dict": {}}
@@ -246,7 +247,7 @@ def _main(argv=None):
         beta_t = torch.tensor(beta_at(args, state["iteration"]), dtype=torch.float32, device=device)      # the beta schedule lives in a device scalar
         graphed = GraphedTraining(model, lambda: model(s_x, reverse=False, beta=beta_t, length=s_len, noise=s_noise,
                                                        _nll=model.nll_request(length=s_len, prior=prior))[2].mean(),
-                                  device, args.max_gradient_norm, lr=lr_of(state["iteration"]), eager_optimizer=optimizer, allow_unverified=args.graph_step_unverified)
+                                  device, args.max_gradient_norm, lr=lr_of(state["iteration"]), eager_optimizer=optimizer, optimizer_cls=optimizer_class(args), allow_unverified=args.graph_step_unverified)
         optimizer = graphed.optimizer
         say("[#] --graph_step: captured training step, hipGraph nodes %s" % (graphed.nodes,))
     ddp.train()

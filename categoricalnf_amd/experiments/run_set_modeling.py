@@ -20,6 +20,7 @@ training batches of `batch_size / world` sets, DistributedDataParallel all-reduc
 the validation sets are sharded by rank with ONE all-reduce of (sum nll, count) per evaluation."""
 import argparse
 import contextlib
+import functools
 import glob
 import io
 import json
@@ -33,9 +34,28 @@ import torch
 from .. import functional as Fn
 from ..distributed import allreduce_nll, init_process_group, shard_bounds, wrap_ddp
 from ..host_utils import FlatParameters
+from ..optim import AdamW
 from .set_modeling import FlowSetModeling, SetShufflingDataset, SetSummationDataset
 
 LOG2E = float(np.log2(np.e))
+
+
+def add_optimizer_args(p):
+    p.add_argument("--optimizer", choices=["radam", "adamw", "adamw8"], default="radam",
+                   help="radam: the reference's default (torch.optim.RAdam); adamw / adamw8: categoricalnf_amd.optim.AdamW, all parameters in a few "
+                        "kernel launches, moments in fp32 / in 8 bits")
+    p.add_argument("--weight_decay", type=float, default=0.0, help="decoupled weight decay of --optimizer adamw / adamw8")
+
+
+def optimizer_class(args):
+    """The class behind --optimizer, called as cls(parameters, lr=..., [capturable=True])."""
+    if args.optimizer == "radam":
+        return torch.optim.RAdam
+    return functools.partial(AdamW, weight_decay=args.weight_decay, state_bits=8 if args.optimizer == "adamw8" else 32)
+
+
+def make_optimizer(args, parameters):
+    return optimizer_class(args)(parameters, lr=args.learning_rate)
 
 
 def parse(argv=None):
@@ -67,6 +87,7 @@ def parse(argv=None):
     p.add_argument("--compact_params", action="store_true",
                    help="the mixture couplings' sub-networks emit the transformed channels' parameter blocks only (the last Linear applies "
                         "just those rows; same parameters and checkpoints): half the parameter traffic, no zero blocks in the backward")
+    add_optimizer_args(p)
     p.add_argument("--backend", default=None, help="torch.distributed backend (default: nccl = RCCL)")
     p.add_argument("--graph_step", action="store_true",
                    help="single process only: the whole training step (forward, HIP backward kernels, clipping, RAdam) is captured "
@@ -243,7 +264,7 @@ def _main(argv=None):
         x = torch.from_numpy(train_set.sample(per_rank, rng)).long().to(device)
         return x, torch.full((x.size(0),), x.size(1), dtype=torch.long, device=device)
 
-    optimizer = torch.optim.RAdam(model.parameters(), lr=args.learning_rate)
+    optimizer = make_optimizer(args, model.parameters())
     floor = args.lr_minimum / args.learning_rate
     scheduler = torch.optim.lr_scheduler.LambdaLR(
         optimizer, lambda step: max(floor, args.lr_decay_factor ** (step // max(1, args.lr_decay_step))))
@@ -276,7 +297,7 @@ def _main(argv=None):
         say("[#] --flat_optimizer ignored: DistributedDataParallel's gradient buckets own the .grad views")
     elif args.flat_optimizer:
         flat = FlatParameters(model)                      # after the data-dependent init, which re-binds ActNorm's .data
-        optimizer = torch.optim.RAdam(flat.parameters(), lr=args.learning_rate)
+        optimizer = make_optimizer(args, flat.parameters())
         scheduler = torch.optim.lr_scheduler.LambdaLR(
             optimizer, lambda step: max(floor, args.lr_decay_factor ** (step // max(1, args.lr_decay_step))))
         advance_schedule(scheduler, state["iteration"])
@@ -292,7 +313,7 @@ def _main(argv=None):
         # the NLL assembly rides in the last coupling layer's kernel
         graphed = GraphedTraining(model, lambda: model(static_x, reverse=False, length=static_ln, beta=1, noise=static_noise,
                                                        _nll=model.nll_request(length=static_ln))[2].mean(),
-                                  device, args.max_gradient_norm, lr=lr_of(state["iteration"]), eager_optimizer=optimizer, allow_unverified=args.graph_step_unverified)
+                                  device, args.max_gradient_norm, lr=lr_of(state["iteration"]), eager_optimizer=optimizer, optimizer_cls=optimizer_class(args), allow_unverified=args.graph_step_unverified)
         optimizer = graphed.optimizer
         say("[#] --graph_step: captured training step, hipGraph nodes %s" % (graphed.nodes,))
     ddp.train()

@@ -15,6 +15,7 @@ from ..layers.flows.coupling_layer import CouplingLayer
 from ..layers.flows.flow_model import FlowModel
 from ..layers.flows.mixture_cdf_layer import MixtureCDFCoupling
 from ..layers.flows.permutation_layers import InvertibleConv
+from ..layers.networks.help_layers import LayerNorm
 
 
 class CouplingTransformerNet(nn.Module):
@@ -27,7 +28,9 @@ class CouplingTransformerNet(nn.Module):
         self.transformer_layers = nn.ModuleList([
             nn.TransformerEncoderLayer(hidden_size, nhead=4, dim_feedforward=2 * hidden_size, dropout=0.0, activation='gelu')
             for _ in range(num_layers)])
-        self.output_layer = nn.Sequential(nn.LayerNorm(hidden_size), nn.Linear(hidden_size, hidden_size), nn.GELU(),
+        for layer in self.transformer_layers:            # same parameters; torch's fused evaluation path reads them as they are
+            layer.norm1, layer.norm2 = LayerNorm(hidden_size), LayerNorm(hidden_size)
+        self.output_layer = nn.Sequential(LayerNorm(hidden_size), nn.Linear(hidden_size, hidden_size), nn.GELU(),
                                           nn.Linear(hidden_size, c_out))
 
     def forward(self, x, src_key_padding_mask, **kwargs):

@@ -6,6 +6,7 @@ sampling, benchmarks) the layer modules call `ops` directly; with it they go thr
 import ctypes
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
 from .ops import _f32, _launch, _mask_desc, _opt_f32, _pad2d, _length, _ptr, _stream
@@ -775,3 +776,28 @@ class MixtureTransformFn(torch.autograd.Function):
 
 def needs_grad(*tensors):
     return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+
+
+class LayerNormFn(torch.autograd.Function):
+    """(x, weight, bias) -> layer norm over the last axis; the backward also sums the parameters' gradients."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = ops.layer_norm(x, weight, bias, eps, want_stats=True)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.param_dtype = weight.dtype if weight is not None else (bias.dtype if bias is not None else None)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, weight, mean, rstd = ctx.saved_tensors
+        dx, dw, db = ops.layer_norm_bwd(x, g, weight, mean, rstd, ctx.param_dtype, ctx.needs_input_grad[1], ctx.needs_input_grad[2])
+        return dx, dw, db, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """Layer norm over the last axis (`ops.layer_norm`), differentiable in x, weight and bias."""
+    if needs_grad(x, weight, bias):
+        return LayerNormFn.apply(x, weight, bias, float(eps))
+    return ops.layer_norm(x, weight, bias, eps)

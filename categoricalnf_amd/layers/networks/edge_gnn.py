@@ -32,6 +32,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .graph_layers import GNNSkipConnection, SplitKLinear as _Linear
+from .help_layers import LayerNorm
 
 _NEG = -9e15        # the reference's masking constant (its softmax rows without a neighbour are zeroed afterwards)
 
@@ -95,8 +96,8 @@ class Node2EdgePlainLayer(nn.Module):
     def __init__(self, hidden_size_nodes, hidden_size_edges, skip_config=0, dp_rate=0.0, act_fn=nn.GELU):
         super().__init__()
         self.hidden_size_nodes, self.hidden_size_edges = hidden_size_nodes, hidden_size_edges
-        self.node_feat_layer = nn.Sequential(nn.LayerNorm(hidden_size_nodes), _Linear(hidden_size_nodes, hidden_size_edges))
-        self.edge_feat_layer = nn.Sequential(nn.LayerNorm(hidden_size_edges), _Linear(hidden_size_edges, hidden_size_edges))
+        self.node_feat_layer = nn.Sequential(LayerNorm(hidden_size_nodes), _Linear(hidden_size_nodes, hidden_size_edges))
+        self.edge_feat_layer = nn.Sequential(LayerNorm(hidden_size_edges), _Linear(hidden_size_edges, hidden_size_edges))
         self.skip_layer = GNNSkipConnection(hidden_size_edges, config=skip_config, dp_rate=dp_rate)
         self.dropout = nn.Dropout(dp_rate)
         self.act_fn = act_fn()
@@ -147,8 +148,8 @@ class Edge2NodeQKVAttnLayer(_Edge2NodeBase):
         self.skip_layer = GNNSkipConnection(hidden_size_nodes, config=skip_config, input_size=hidden_size_nodes, dp_rate=dp_rate)
         self.dropout = nn.Dropout(dp_rate)
         self.act_fn = act_fn()
-        self.node_normalization = nn.LayerNorm(hidden_size_nodes)
-        self.edge_normalization = nn.LayerNorm(hidden_size_edges)
+        self.node_normalization = LayerNorm(hidden_size_nodes)
+        self.edge_normalization = LayerNorm(hidden_size_edges)
 
     def forward(self, node_feat, edge_feat, x_indices, mask_valid, **kwargs):
         B, V = node_feat.size(0), node_feat.size(1)
@@ -181,8 +182,8 @@ class Edge2NodeAttnLayer(_Edge2NodeBase):
         self.skip_layer = GNNSkipConnection(hidden_size_nodes, config=skip_config, input_size=self.hidden_size_output)
         self.dropout = nn.Dropout(dp_rate)
         self.act_fn = act_fn()
-        self.node_normalization = nn.LayerNorm(hidden_size_nodes)
-        self.edge_normalization = nn.LayerNorm(hidden_size_edges)
+        self.node_normalization = LayerNorm(hidden_size_nodes)
+        self.edge_normalization = LayerNorm(hidden_size_edges)
 
     def forward(self, node_feat, edge_feat, x_indices, mask_valid, **kwargs):
         B, V = node_feat.size(0), node_feat.size(1)
@@ -232,7 +233,7 @@ class EdgeGNN(nn.Module):
             return nn.Sequential(_Linear(c_in, hidden), nn.GELU(), _Linear(hidden, hidden))
 
         def mlp_out(hidden, c_out):
-            return nn.Sequential(nn.LayerNorm(hidden), _Linear(hidden, hidden), nn.GELU(), _Linear(hidden, c_out))
+            return nn.Sequential(LayerNorm(hidden), _Linear(hidden, hidden), nn.GELU(), _Linear(hidden, c_out))
 
         self.input_layer_edges, self.input_layer_nodes = mlp_in(c_in_edges, hidden_edges), mlp_in(c_in_nodes, hidden_nodes)
         self.out_layer_edges, self.out_layer_nodes = mlp_out(hidden_edges, c_out_edges), mlp_out(hidden_nodes, c_out_nodes)

@@ -13,6 +13,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ...host_utils import one_hot
+from .help_layers import LayerNorm
 
 
 
@@ -62,7 +63,7 @@ class RelationGraphConv(nn.Module):
     def __init__(self, c_in, c_out, num_edges, **kwargs):
         super().__init__()
         self.c_in, self.c_out, self.num_edges = c_in, c_out, num_edges
-        self.norm_layer = nn.LayerNorm(self.c_in)
+        self.norm_layer = LayerNorm(self.c_in)
         self.linear_hs = nn.Linear(self.c_in, self.c_out)
         self.linear_hr = nn.Linear(self.c_in, self.c_out * self.num_edges)
 
@@ -84,7 +85,7 @@ class RelationGraphAttention(nn.Module):
         super().__init__()
         self.c_in, self.c_out, self.num_edges, self.num_heads = c_in, c_out, num_edges, num_heads
         self.c_out_per_head = self.c_out * 2 // self.num_heads
-        self.norm_layer = nn.LayerNorm(self.c_in)
+        self.norm_layer = LayerNorm(self.c_in)
         self.linear_hs = nn.Linear(self.c_in, self.c_out_per_head * self.num_heads)
         self.linear_hr = nn.Linear(self.c_in, self.c_out_per_head * self.num_heads * (self.num_edges + 1))
         self.attn_weight = nn.Parameter(torch.zeros(self.num_heads, 2, self.c_out_per_head), requires_grad=True)
@@ -162,7 +163,7 @@ class RGCNNet(nn.Module):
             for _ in range(num_layers)])
         self.input_layer = nn.Sequential(nn.Linear(c_in, hidden_size), self.act_fn,
                                          nn.Linear(hidden_size, hidden_size - neighbour_embed_size))
-        self.output_layer = nn.Sequential(nn.LayerNorm(hidden_size), nn.Linear(hidden_size, hidden_size), self.act_fn,
+        self.output_layer = nn.Sequential(LayerNorm(hidden_size), nn.Linear(hidden_size, hidden_size), self.act_fn,
                                           nn.Linear(hidden_size, c_out))
 
     def forward(self, x, adjacency, channel_padding_mask=None, embed_ext_input=None, **kwargs):

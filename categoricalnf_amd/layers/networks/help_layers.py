@@ -1,4 +1,4 @@
-"""Coupling-subnet helpers that stay plain PyTorch-ROCm (dense GEMMs -> hipBLASLt / MFMA).
+"""Coupling-subnet helpers: plain PyTorch-ROCm (dense GEMMs -> hipBLASLt / MFMA) but for the layer norm.
 
 Mirrors the names of layers/networks/help_layers.py in the reference: SimpleLinearLayer (:57-73),
 LinearNet (:76-107) and run_sequential_with_mask (:111-124).  Parameter names are kept so that the
@@ -6,6 +6,23 @@ reference's checkpoints load (`…pred_net.layer.weight`, `…nn.inp_layer.0.wei
 import numpy as np
 import torch
 import torch.nn as nn
+
+from ... import functional as Fn
+
+_KERNEL_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+class LayerNorm(nn.LayerNorm):
+    """nn.LayerNorm (same arguments, parameters and state_dict) whose last-axis norm of GPU tensors is this package's kernel,
+    forward and backward.  Host tensors, float64 and norms over several axes keep torch's: the sub-networks also run there."""
+
+    def forward(self, x):
+        if not x.is_cuda or x.dtype not in _KERNEL_DTYPES or len(self.normalized_shape) != 1 \
+                or x.shape[-1:] != self.normalized_shape:
+            return super().forward(x)
+        if torch.is_autocast_enabled():
+            x = x.float()                                # layer norm is an fp32 operation under autocast
+        return Fn.layer_norm(x, self.weight, self.bias, self.eps)
 
 
 class SimpleLinearLayer(nn.Module):

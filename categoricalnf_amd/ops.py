@@ -2,6 +2,7 @@
 stream, torch tensors out.  PyTorch is plumbing here (device memory + streams); no arithmetic of the
 hot path is done with torch ops and there is no CPU path — CPU tensors raise.
 """
+import array
 import ctypes
 import math
 import os
@@ -1028,3 +1029,165 @@ def mixture_coupling_nll_launch(z, nn_out, mask, num_mixtures, z_out, ldj_out, l
             _ptr(ws), int(ws.numel()), _ptr(flag_word(dev)), None]
     name = "cnf_mixture_coupling_compact_nll" if mixture_layout(nn_out, z, num_mixtures, act, n_act) else "cnf_mixture_coupling_nll"
     return Launch(name, getattr(lib, name), args, dev, (z, nn_out, sf, msf, m, act, pad, ln, z_out, ldj_out, neglog, nll, acc, ws))
+
+
+# ---- operators of the training step around the flow -----------------------------------------------------------------------------
+
+_DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # CNF_DTYPE_*
+
+
+def _float_code(t, name):
+    _dev(t)
+    code = _DTYPE_CODE.get(t.dtype)
+    if code is None:
+        raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
+    return code
+
+
+def _vector(t, n, name, device):
+    """An optional parameter vector of n elements on `device`: (dense tensor, dtype code) or (None, None)."""
+    if t is None:
+        return None, None
+    code = _float_code(t, name)
+    if t.device != device:
+        raise ValueError("%s is on %s, the input on %s" % (name, t.device, device))
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError("%s must have shape (%d,), got %s" % (name, n, tuple(t.shape)))
+    return (t if t.is_contiguous() else t.contiguous()), code
+
+
+def _rows(t):
+    """[..., C] as [rows, C] with unit column stride and one row stride: a view where the strides allow it, else a copy."""
+    m = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    return m if m.stride(1) == 1 or m.shape[1] == 1 else m.contiguous()
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, want_stats=False):
+    """Layer norm over the last axis of x (float32, bfloat16 or float16; any leading shape; rows may lie apart): y of x's type,
+    statistics in fp32.  weight, bias: [C], both of one type (fp32 or a 16-bit type), or None.  `want_stats`: also (mean, rstd)
+    [rows] fp32, which the backward needs."""
+    code, dev = _float_code(x, "x"), x.device
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("layer_norm needs a last axis of at least one element, got shape %s" % (tuple(x.shape),))
+    C = x.shape[-1]
+    w, wcode = _vector(weight, C, "weight", dev)
+    b, bcode = _vector(bias, C, "bias", dev)
+    if w is not None and b is not None and wcode != bcode:
+        raise TypeError("weight is %s, bias %s" % (w.dtype, b.dtype))
+    x2 = _rows(x)
+    R = x2.shape[0]
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    mean = rstd = None
+    if want_stats:
+        mean, rstd = torch.empty(2, R, dtype=torch.float32, device=dev).unbind(0)
+    _launch(dev, "cnf_layer_norm", _ptr(x2), x2.stride(0), _ptr(w), _ptr(b), _ptr(y), _ptr(mean), _ptr(rstd), R, C, float(eps), code,
+            wcode if wcode is not None else (bcode or 0), _stream(dev))
+    return (y, mean, rstd) if want_stats else y
+
+
+def layer_norm_bwd(x, dy, weight, mean, rstd, param_dtype=None, want_weight=True, want_bias=True):
+    """Gradients of layer_norm from its input, the upstream gradient and the kept statistics: (dx, dweight, dbias), the last two of
+    `param_dtype` (default: the weight's type, else x's) or None."""
+    code, dev = _float_code(x, "x"), x.device
+    C = x.shape[-1]
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError("the gradient must have the input's shape and type, got %s %s for %s %s"
+                         % (tuple(dy.shape), dy.dtype, tuple(x.shape), x.dtype))
+    w, wcode = _vector(weight, C, "weight", dev)
+    pdt = param_dtype or (w.dtype if w is not None else x.dtype)
+    if w is not None and pdt != w.dtype:
+        raise TypeError("parameter gradients have the weight's type")
+    x2, g2 = _rows(x), _rows(dy)
+    R = x2.shape[0]
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    dw = torch.empty(C, dtype=pdt, device=dev) if want_weight else None
+    db = torch.empty(C, dtype=pdt, device=dev) if want_bias else None
+    ws, n = None, 0
+    if want_weight or want_bias:
+        n = int(_lib.load().cnf_layer_norm_bwd_workspace_floats(R, C))
+        ws = torch.empty(n, dtype=torch.float32, device=dev)
+    _launch(dev, "cnf_layer_norm_bwd", _ptr(x2), x2.stride(0), _ptr(g2), g2.stride(0), _ptr(w), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dw),
+            _ptr(db), _ptr(ws), n, R, C, code, _DTYPE_CODE[pdt], _stream(dev))
+    return dx, dw, db
+
+
+ADAMW_BLOCK = 256           # consecutive elements of a tensor that share the two scales of its 8-bit moments
+
+
+def _scalar(v, name, device):
+    """A step's number: (host double, None) or (0.0, device fp32 scalar)."""
+    if not isinstance(v, torch.Tensor):
+        return float(v), None
+    if v.device != device or v.dtype != torch.float32 or v.numel() != 1:
+        raise ValueError("%s as a tensor is one float32 value on the parameters' device, got %s on %s" % (name, v.dtype, v.device))
+    return 0.0, v
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=1e-2,
+               exp_avg_scales=None, exp_avg_sq_scales=None):
+    """One AdamW step, in place, over lists of tensors in a few launches (cnf_adamw_step).
+
+    params: dense tensors of one type (fp32, bf16, fp16) on one device; grads: of that type or fp32.  Moments in fp32 — or, with
+    the two lists of scales ([ceil(n / 256)] fp32 each), in 8 bits: exp_avgs int8, exp_avg_sqs uint8 codes.  `step` (the number of
+    this step, from 1) and `lr` are numbers, or float32 device scalars that the kernel reads (for a captured step)."""
+    n = len(params)
+    bits8 = exp_avg_scales is not None
+    if (exp_avg_sq_scales is not None) != bits8:
+        raise ValueError("8-bit moments need both lists of scales")
+    lists = [params, grads, exp_avgs, exp_avg_sqs] + ([exp_avg_scales, exp_avg_sq_scales] if bits8 else [])
+    if any(len(l) != n for l in lists):
+        raise ValueError("adamw_step: lists of %s tensors" % ([len(l) for l in lists],))
+    if n == 0:
+        return
+    dev = _dev(params[0])
+    pdt, gdt = params[0].dtype, grads[0].dtype
+    pcode, gcode = _float_code(params[0], "params"), _float_code(grads[0], "grads")
+    if gdt != pdt and gdt != torch.float32:
+        raise TypeError("gradients are float32 or of the parameters' type, got %s for %s" % (gdt, pdt))
+    numel = array.array("q", [p.numel() for p in params])
+    kept = []                                             # dense copies of gradients: alive until the launches are enqueued
+    if not all(map(torch.Tensor.is_contiguous, grads)):
+        grads = kept = [g.contiguous() for g in grads]
+    want = ((params, pdt, "params"), (grads, gdt, "grads"), (exp_avgs, torch.int8 if bits8 else torch.float32, "exp_avgs"),
+            (exp_avg_sqs, torch.uint8 if bits8 else torch.float32, "exp_avg_sqs"))
+    for l, dt, name in want:
+        for t, k in zip(l, numel):
+            if t.dtype is not dt or t.numel() != k or t.device != dev or not t.is_contiguous():
+                raise ValueError("adamw_step: %s must be dense %s tensors of the parameters' sizes on %s, got %s %s on %s"
+                                 % (name, dt, dev, tuple(t.shape), t.dtype, t.device))
+    if bits8:
+        for l in (exp_avg_scales, exp_avg_sq_scales):
+            for t, k in zip(l, numel):
+                if t.dtype is not torch.float32 or t.numel() != -(-k // ADAMW_BLOCK) or t.device != dev or not t.is_contiguous():
+                    raise ValueError("adamw_step: a scale list must hold dense float32 tensors of ceil(n / %d) elements on %s" % (ADAMW_BLOCK, dev))
+    addresses = [array.array("Q", [t.data_ptr() for t in l]) for l in lists[:1] + [grads] + lists[2:]]
+    for l in (addresses[0], addresses[2], addresses[3]):
+        if len(set(l)) != n and len(set(a for a, k in zip(l, numel) if k)) != sum(k > 0 for k in numel):
+            raise ValueError("adamw_step: a parameter or a moment is listed twice")
+    if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0):
+        raise ValueError("adamw_step: betas outside [0, 1)")
+    step_host, step_dev = _scalar(step, "step", dev)
+    lr_host, lr_dev = _scalar(lr, "lr", dev)
+    if step_dev is None and step_host < 1:
+        raise ValueError("adamw_step: the first step is step 1, got %r" % (step,))
+    at = [ctypes.c_void_p(a.buffer_info()[0]) for a in addresses] + ([] if bits8 else [None, None])
+    _launch(dev, "cnf_adamw_step", n, *at, ctypes.c_void_p(numel.buffer_info()[0]), pcode, gcode, 8 if bits8 else 32, lr_host, float(beta1),
+            float(beta2), float(eps), float(weight_decay), step_host, _ptr(lr_dev), _ptr(step_dev), _stream(dev))
+    del kept
+
+
+def adamw_moments(exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale):
+    """(m, v) in fp32: the values that a tensor's 8-bit moments stand for."""
+    dev = _dev(exp_avg)
+    n = exp_avg.numel()
+    for t, dt, k, name in ((exp_avg, torch.int8, n, "exp_avg"), (exp_avg_sq, torch.uint8, n, "exp_avg_sq"),
+                           (exp_avg_scale, torch.float32, -(-n // ADAMW_BLOCK), "exp_avg_scale"),
+                           (exp_avg_sq_scale, torch.float32, -(-n // ADAMW_BLOCK), "exp_avg_sq_scale")):
+        if t.dtype != dt or t.numel() != k or t.device != dev or not t.is_contiguous():
+            raise ValueError("adamw_moments: %s must be a dense %s tensor of %d elements on %s, got %s %s on %s"
+                             % (name, dt, k, dev, tuple(t.shape), t.dtype, t.device))
+    m = torch.empty(exp_avg.shape, dtype=torch.float32, device=dev)
+    v = torch.empty(exp_avg.shape, dtype=torch.float32, device=dev)
+    _launch(dev, "cnf_adamw_moments", _ptr(exp_avg), _ptr(exp_avg_sq), _ptr(exp_avg_scale), _ptr(exp_avg_sq_scale), _ptr(m), _ptr(v), n,
+            _stream(dev))
+    return m, v

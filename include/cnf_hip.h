@@ -46,6 +46,11 @@ extern "C" {
 #define CNF_FLAG_RANGE 4       /* inverse-CDF input outside (0,1) (mixture_cdf_layer.py:238-239) */
 #define CNF_FLAG_CATEGORY 8    /* a category index outside [0, C)     (general/mutils.py:264, the one_hot assert) */
 
+/* element types of the operators that take more than fp32 (layer norm, AdamW, linear cross entropy) */
+#define CNF_DTYPE_F32 0
+#define CNF_DTYPE_BF16 1
+#define CNF_DTYPE_F16 2
+
 typedef void* cnf_stream_t;
 
 int cnf_abi_version(void);
@@ -619,6 +624,37 @@ int cnf_encoder_forward_bwd_cpl(const int64_t* categ, const float* eps, const fl
 /* d(SigmoidFlow.forward) w.r.t. its input (sigmoid_layer.py:31-37). */
 int cnf_sigmoid_flow_bwd(const float* z_in, const float* g_zout, const float* g_ldj, float* g_z,
                          int B, int L, int reverse, float alpha, cnf_stream_t stream);
+
+/* ---- operators of the training step around the flow ---------------------------------------------------------- */
+
+/* Layer norm over the last axis (nn.LayerNorm of the coupling sub-networks: set_modeling/flow_model.py:119-124,
+ * layers/networks/graph_layers.py:76,176): y = (x - mean) * rstd * weight + bias, statistics in fp32.  x [rows, cols] of `dtype`
+ * with unit column stride and `x_stride` elements between rows; y dense; weight, bias [cols] of `wdtype` (nullable: 1, 0);
+ * mean, rstd [rows] fp32 are kept for the backward (both or neither NULL).  Any number of columns. */
+int cnf_layer_norm(const void* x, int64_t x_stride, const void* weight, const void* bias, void* y, float* mean, float* rstd,
+                   int64_t rows, int cols, float eps, int dtype, int wdtype, cnf_stream_t stream);
+/* Its gradients: dx [rows, cols] dense of `dtype`; dweight, dbias [cols] of `wdtype` (nullable), summed over the rows in a fixed
+ * order (the same bits on every run).  workspace = cnf_layer_norm_bwd_workspace_floats(rows, cols) floats, needed for the column
+ * sums only. */
+int64_t cnf_layer_norm_bwd_workspace_floats(int64_t rows, int cols);
+int cnf_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, const void* weight,
+                       const float* mean, const float* rstd, void* dx, void* dweight, void* dbias, float* workspace,
+                       int64_t workspace_floats, int64_t rows, int cols, int dtype, int wdtype, cnf_stream_t stream);
+
+/* One AdamW step over `count` dense tensors: m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g^2,
+ * p = p (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps).
+ * The LISTS are HOST arrays of device pointers (and element counts), read before the call returns.  Parameters of `pdtype`,
+ * gradients of `gdtype` (= pdtype, or fp32).  state_bits 32: exp_avg, exp_avg_sq fp32, the scale lists NULL.  state_bits 8:
+ * exp_avg int8 codes q (m = s q |q|), exp_avg_sq uint8 codes q (sqrt(v) = s q^2), with one fp32 scale s for each 256 consecutive
+ * elements of a tensor.  `lr_dev` / `step_dev` (nullable): device scalars read by the kernel instead of `lr` / `step`, for a
+ * step that is captured into a graph and replayed.  No tensor may be listed twice. */
+int cnf_adamw_step(int count, void* const* params, const void* const* grads, void* const* exp_avg, void* const* exp_avg_sq,
+                   float* const* exp_avg_scale, float* const* exp_avg_sq_scale, const int64_t* numel, int pdtype, int gdtype,
+                   int state_bits, double lr, double beta1, double beta2, double eps, double weight_decay, double step,
+                   const float* lr_dev, const float* step_dev, cnf_stream_t stream);
+/* The values that a tensor's 8-bit moments stand for (n elements, ceil(n / 256) scales). */
+int cnf_adamw_moments(const int8_t* exp_avg, const uint8_t* exp_avg_sq, const float* exp_avg_scale, const float* exp_avg_sq_scale,
+                      float* m_out, float* v_out, int64_t n, cnf_stream_t stream);
 
 #ifdef __cplusplus
 }
