@@ -95,6 +95,8 @@ SIGNATURES = {
     "cnf_mixture_params_bwd": [_p, _p, _p, _p, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p],
     "cnf_layer_norm": [_p, _i64, _p, _p, _p, _p, _p, _i64, _i, _f, _i, _i, _p],
     "cnf_layer_norm_bwd": [_p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i, _i, _i, _p],
+    "cnf_linear_ce": [_p, _i64, _p, _i64, _p, _p, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i, _i, _i, _i, _p, _p],
+    "cnf_linear_ce_bwd": [_p, _i64, _p, _i64, _p, _p, _i64, _p, _p, _p, _i, _p, _p, _p, _p, _p, _i64, _i64, _i, _i, _i, _i, _p],
     "cnf_adamw_step": [_i, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _d, _d, _d, _d, _d, _d, _p, _p, _p],
     "cnf_adamw_moments": [_p, _p, _p, _p, _p, _p, _i64, _p],
     "cnf_stream_probe": [_p, _p, _p, ctypes.c_long, _i, _p],
@@ -106,7 +108,8 @@ _PLAIN = {"cnf_abi_version": ([], _i), "cnf_last_error": ([], ctypes.c_char_p),
           "cnf_set_tile_chunks": ([_i], None), "cnf_set_unroll": ([_i], None),
           "cnf_set_math_mode": ([_i], None), "cnf_set_inverse_mode": ([_i], None), "cnf_set_mixture_tile": ([_i], None),
           "cnf_set_bwd_tile": ([_i, _i], None), "cnf_set_actnorm_bwd_tiles": ([_i], None), "cnf_set_affine_bwd_tiles": ([_i], None), "cnf_set_mixture_bwd_waves": ([_i], None), "cnf_set_mixture_bwd_big_mb": ([_i], None),
-          "cnf_bwd_workspace_floats": ([_i], _i64), "cnf_layer_norm_bwd_workspace_floats": ([_i64, _i], _i64), "cnf_bwd_defer_begin": ([], None),
+          "cnf_bwd_workspace_floats": ([_i], _i64), "cnf_layer_norm_bwd_workspace_floats": ([_i64, _i], _i64),
+          "cnf_linear_ce_workspace_bytes": ([_i64, _i, _i, _i, _i], _i64), "cnf_bwd_defer_begin": ([], None),
           "cnf_mixture_workspace_bytes": ([_i], _i64), "cnf_encoder_workspace_floats": ([_i, _i, _i, _i], _i64),
           "cnf_encoder_bwd_tiled_workspace_floats": ([_i, _i, _i, _i], _i64), "cnf_set_mixture_kernel": ([_i], None), "cnf_set_encoder_kernel": ([_i], None), "cnf_set_encoder_bwd_kernel": ([_i], None), "cnf_encoder_pair_launches": ([], _i64),
           "cnf_set_mixture_lanes": ([_i], None), "cnf_set_mixture_split": ([_i], None),

@@ -1,0 +1,718 @@
+// Softmax cross entropy of a linear layer over a vocabulary, forward and backward, without keeping the logits.
+//
+//   l_rv = x_r . w_v + b_v,   m_r = max_v l_rv,   s_r = sum_v exp(l_rv - m_r),   loss_r = log s_r + (m_r - l_rt)
+//   d_rv = g_r (exp(l_rv - m_r) / s_r - [v = t_r]),   dx = d w,   dw = d^T x,   db_v = sum_r d_rv
+//
+// Forward: a product whose tiles never leave the registers.  A workgroup owns a block of rows and a part of the vocabulary; every
+// lane keeps a running maximum and sum for its rows over the vocabulary entries it sees (four of them are consecutive), the lanes and
+// waves of a row are joined once at the end, the parts of the vocabulary by a second launch, which also writes the loss.
+// Backward, in pieces of the vocabulary: the piece's logits are computed again and turned into d (rounded to the operands' type, or
+// kept as three bf16 parts for fp32), written to a workspace that fits the memory-side cache, and read by two products: dx += d w over
+// the piece, dw = d^T x complete for the piece.  db comes out of the second product: a fragment of ones in place of x.
+//
+// fp32 inputs are split once into three bf16 parts (cnf_mfma.h: pair_a): six bf16 products keep every product to 2^-26, and the
+// matrix cores do them at 16 times the fp32 rate.  16-bit inputs whose rows are not 16-byte aligned are copied once into padded rows.
+// In fp16 d is scaled by a power of two that brings the largest |g_r| to 2^14, so that small probabilities keep their bits.
+#include <algorithm>
+
+#include "cnf_mfma.h"
+
+namespace cnf {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// ---- row records -----------------------------------------------------------------------------------------------------------------
+
+struct RowState {       // backward: what an element of d needs of its row
+    float m, scale;     // maximum; g / s
+    float g;
+    int target;         // -1: ignored
+};
+
+struct CeArgs {
+    Operand w, x;                   // [V][H], [R][H]
+    int pairs, parts;
+    int64_t rows;
+    int vocab, hidden;
+    const void* bias;
+    int bias_dtype;
+    const int64_t* target;
+    int64_t ignore;
+    // forward
+    float2* partial;                // [splits][rows]
+    float* target_logit;            // [rows]
+    int splits;                     // of the vocabulary tiles
+    // backward
+    const RowState* state;          // [rows]
+    const float* unscale;           // fp16: [2] = {S, 1 / S}
+    void* d;                        // [parts][rows_pad][piece_ld]
+    int64_t d_part, d_ld;
+    int v0, v1;                     // the piece
+};
+
+// tiles in the order that lets the workgroups of one XCD (dispatched round-robin over the 8) work on neighbouring tiles
+__device__ __forceinline__ unsigned xcd_contiguous(unsigned id, unsigned n) {
+    const unsigned xcd = id & 7u, idx = id >> 3, per = n >> 3, rem = n & 7u;
+    return xcd * per + (xcd < rem ? xcd : rem) + idx;
+}
+// tile (i, j) of an ni x nj grid in column groups of 8
+__device__ __forceinline__ void grouped_tile(unsigned t, unsigned ni, unsigned nj, unsigned& i, unsigned& j) {
+    const unsigned per = 8 * ni, group = t / per, first = group * 8, width = min(8u, nj - first), in = t - group * per;
+    j = first + in % width;
+    i = in / width;
+}
+
+__device__ __forceinline__ float bias_at(const CeArgs& a, int v) { return a.bias && v < a.vocab ? load_any(a.bias, a.bias_dtype, v) : 0.f; }
+
+// ---- forward ---------------------------------------------------------------------------------------------------------------------
+
+// D[m = vocabulary][n = row]
+template <typename E, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64, 2) void ce_lse_kernel(const CeArgs a) {
+    typedef TileProduct<E, false, false, BM, BN, WM, WN> Tile;
+    __shared__ __align__(16) char lds[Tile::kLds];
+    const Tile tile(a.w, a.x, a.pairs, a.hidden, lds);
+    const unsigned t = xcd_contiguous(blockIdx.x, gridDim.x);
+    const int split = t % a.splits;
+    const int r0 = (t / a.splits) * BN;
+    const int vtiles = (a.vocab + BM - 1) / BM;
+    const int first = (int)((int64_t)vtiles * split / a.splits), last = (int)((int64_t)vtiles * (split + 1) / a.splits);
+    const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+    float mx[Tile::NT], sum[Tile::NT];
+    int want[Tile::NT];
+#pragma unroll
+    for (int n = 0; n < Tile::NT; ++n) {
+        const int64_t r = (int64_t)r0 + tile.n_wave + n * 16 + col;
+        mx[n] = -INFINITY;
+        sum[n] = 0.f;
+        const int64_t tg = r < a.rows ? a.target[r] : -1;
+        want[n] = tg >= 0 && tg < a.vocab && tg != a.ignore ? (int)tg : -1;
+    }
+    for (int vt = first; vt < last; ++vt) {
+        const int v0 = vt * BM;
+        f32x4 acc[Tile::MT][Tile::NT];
+#pragma unroll
+        for (int m = 0; m < Tile::MT; ++m)
+#pragma unroll
+            for (int n = 0; n < Tile::NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        tile.run(v0, r0, 0, a.hidden, acc, [](int) {});
+        const int vw = v0 + tile.m_wave + g * 4;        // the lane's first entry
+        if (a.bias) {
+#pragma unroll
+            for (int m = 0; m < Tile::MT; ++m) {
+                f32x4 b;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) b[i] = bias_at(a, vw + m * 16 + i);
+#pragma unroll
+                for (int n = 0; n < Tile::NT; ++n) acc[m][n] += b;
+            }
+        }
+        if (v0 + BM > a.vocab) {                        // entries past the vocabulary
+#pragma unroll
+            for (int m = 0; m < Tile::MT; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (vw + m * 16 + i >= a.vocab)
+#pragma unroll
+                        for (int n = 0; n < Tile::NT; ++n) acc[m][n][i] = -INFINITY;
+        }
+#pragma unroll
+        for (int n = 0; n < Tile::NT; ++n) {
+            const int at = want[n] - vw;                // the target's place among the lane's entries: 16 m + i
+            if (want[n] >= 0 && at >= 0 && at < Tile::MT * 16 && (at & 15) < 4) {
+#pragma unroll
+                for (int m = 0; m < Tile::MT; ++m)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (at == m * 16 + i) a.target_logit[(int64_t)r0 + tile.n_wave + n * 16 + col] = acc[m][n][i];
+            }
+            float top = mx[n];
+#pragma unroll
+            for (int m = 0; m < Tile::MT; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, acc[m][n][i]);
+            // a lane that has seen only -inf keeps the sum 0 (exp(-inf - 0)); fmaxf drops a NaN, the sum keeps it
+            const float ref = top == -INFINITY ? 0.f : top;
+            float s = sum[n] * __builtin_amdgcn_exp2f((mx[n] - ref) * kLog2e);
+#pragma unroll
+            for (int m = 0; m < Tile::MT; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s += __builtin_amdgcn_exp2f((acc[m][n][i] - ref) * kLog2e);
+            sum[n] = s;
+            mx[n] = top;
+        }
+    }
+    // join the four lane groups, then the waves that share rows
+    float2* sh = reinterpret_cast<float2*>(lds);        // [WM][BN]; every wave is past its last read of the stages
+#pragma unroll
+    for (int n = 0; n < Tile::NT; ++n) {
+        float m = mx[n], s = sum[n];
+#pragma unroll
+        for (int x = 16; x <= 32; x <<= 1) {
+            const float om = __shfl_xor(m, x, kWave), os = __shfl_xor(s, x, kWave);
+            const float nm = fmaxf(m, om), ref = nm == -INFINITY ? 0.f : nm;
+            s = s * __builtin_amdgcn_exp2f((m - ref) * kLog2e) + os * __builtin_amdgcn_exp2f((om - ref) * kLog2e);
+            m = nm;
+        }
+        if (g == 0) sh[(tile.m_wave / (BM / WM)) * BN + tile.n_wave + n * 16 + col] = make_float2(m, s);
+    }
+    __syncthreads();
+    for (int n = threadIdx.x; n < BN; n += Tile::kThreads) {
+        const int64_t r = (int64_t)r0 + n;
+        if (r >= a.rows) continue;
+        float m = -INFINITY, s = 0.f;
+#pragma unroll
+        for (int w = 0; w < WM; ++w) {
+            const float2 o = sh[w * BN + n];
+            const float nm = fmaxf(m, o.x), ref = nm == -INFINITY ? 0.f : nm;
+            s = s * __builtin_amdgcn_exp2f((m - ref) * kLog2e) + o.y * __builtin_amdgcn_exp2f((o.x - ref) * kLog2e);
+            m = nm;
+        }
+        a.partial[(int64_t)split * a.rows + r] = make_float2(m, s);
+    }
+}
+
+// the parts of the vocabulary -> row maximum, sum, loss; a category outside the vocabulary raises its flag and gives NaN
+__global__ __launch_bounds__(kBlock) void ce_join_kernel(const float2* partial, const float* target_logit, const int64_t* target,
+                                                         int64_t ignore, int vocab, int splits, int64_t rows, float* row_max,
+                                                         float* row_sum, float* loss, int* flags) {
+    const int64_t r = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (r >= rows) return;
+    float m = -INFINITY, s = 0.f;
+    for (int k = 0; k < splits; ++k) m = fmaxf(m, partial[(int64_t)k * rows + r].x);
+    const float ref = m == -INFINITY ? 0.f : m;
+    for (int k = 0; k < splits; ++k) {
+        const float2 o = partial[(int64_t)k * rows + r];
+        s += o.y * __builtin_amdgcn_exp2f((o.x - ref) * kLog2e);
+    }
+    row_max[r] = m;
+    row_sum[r] = s;
+    const int64_t t = target[r];
+    float v = 0.f;
+    if (t != ignore) {
+        if (t < 0 || t >= vocab) {
+            raise_flag(flags, CNF_FLAG_CATEGORY);
+            v = NAN;
+        } else {
+            v = logf(s) + (m - target_logit[r]);
+        }
+    }
+    loss[r] = v;
+}
+
+// reduced = {mean, sum, number} over the rows that are not ignored: one workgroup, fixed order, fp64
+__global__ __launch_bounds__(1024) void ce_reduce_kernel(const float* loss, const int64_t* target, int64_t ignore, int64_t rows,
+                                                         float* reduced) {
+    __shared__ double sh[2][16];
+    double s = 0.0, c = 0.0;
+    for (int64_t r = threadIdx.x; r < rows; r += 1024) {
+        if (target[r] != ignore) {
+            s += (double)loss[r];
+            c += 1.0;
+        }
+    }
+    s = wave_sum(s);
+    c = wave_sum(c);
+    if ((threadIdx.x & 63) == 0) {
+        sh[0][threadIdx.x >> 6] = s;
+        sh[1][threadIdx.x >> 6] = c;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s = c = 0.0;
+        for (int w = 0; w < 16; ++w) {
+            s += sh[0][w];
+            c += sh[1][w];
+        }
+        reduced[0] = (float)(s / c);    // no row left: 0 / 0 = NaN
+        reduced[1] = (float)s;
+        reduced[2] = (float)c;
+    }
+}
+
+// ---- operand layout ----------------------------------------------------------------------------------------------------------------
+
+// [rows][cols] of T -> `parts` arrays of [rows][ld] 16-bit elements, zeros behind cols; fp32: x0 + x1 + x2
+template <typename T, typename E, int PARTS>
+__global__ __launch_bounds__(kBlock) void ce_layout_kernel(const T* src, int64_t stride, int64_t rows, int cols, E* dst, int64_t ld, int64_t part) {
+    const int64_t n = rows * (ld / 8);
+    for (int64_t q = (int64_t)blockIdx.x * kBlock + threadIdx.x; q < n; q += (int64_t)gridDim.x * kBlock) {
+        const int64_t r = q / (ld / 8);
+        const int c0 = (int)(q - r * (ld / 8)) * 8;
+        vec_t<E, 8> o[PARTS];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float v = c0 + i < cols ? (float)src[r * stride + c0 + i] : 0.f;
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) {
+                E e = (E)v;
+                // the largest numbers round up to infinity: keep them finite (the next part takes the rest); infinities and NaN
+                // are whole in the first part
+                if (PARTS > 1 && __builtin_isinf((float)e) && !__builtin_isinf(v))
+                    e = __builtin_bit_cast(E, (uint16_t)(__float_as_uint(v) >> 16));
+                o[p][i] = e;
+                v = PARTS > 1 && __builtin_isfinite(v) ? v - (float)e : 0.f;
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) *reinterpret_cast<vec_t<E, 8>*>(dst + p * part + r * ld + c0) = o[p];
+    }
+}
+
+// ---- backward ----------------------------------------------------------------------------------------------------------------------
+
+// per-row upstream gradients (or one scalar over the count) -> row records; fp16: S = the power of two that brings max |g| to 2^14
+// ... 2^15 (one workgroup)
+__global__ __launch_bounds__(1024) void ce_rows_kernel(const float* g, int g_is_row, const float* count, const float* row_max, const float* row_sum,
+                                                       const int64_t* target, int64_t ignore, int vocab, int64_t rows, RowState* state,
+                                                       float* unscale) {
+    __shared__ uint32_t sh[16];
+    float scale = 1.f;
+    if (unscale) {
+        uint32_t top = 0;
+        if (g_is_row) {
+            for (int64_t r = threadIdx.x; r < rows; r += 1024)
+                if (target[r] != ignore) top = max(top, __float_as_uint(g[r]) & 0x7fffffffu);
+        } else {
+            top = __float_as_uint(*g / *count) & 0x7fffffffu;
+        }
+#pragma unroll
+        for (int m = 32; m >= 1; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, kWave));
+        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
+        __syncthreads();
+        for (int w = 0; w < 16; ++w) top = max(top, sh[w]);
+        const int e = (int)(top >> 23);                     // biased exponent; zero, subnormal, infinite and NaN gradients: no scaling
+        const int shift = e == 0 || e == 255 ? 0 : min(max(14 - (e - 127), -100), 100);
+        scale = __uint_as_float((uint32_t)(127 + shift) << 23);
+        if (threadIdx.x == 0 && blockIdx.x == 0) {
+            unscale[0] = scale;
+            unscale[1] = __uint_as_float((uint32_t)(127 - shift) << 23);
+        }
+    }
+    const float shared = g_is_row ? 0.f : *g / *count;
+    for (int64_t r = (int64_t)blockIdx.x * 1024 + threadIdx.x; r < rows; r += (int64_t)gridDim.x * 1024) {
+        const int64_t t = target[r];
+        const bool in = t != ignore && t >= 0 && t < vocab;
+        const float gr = in ? (g_is_row ? g[r] : shared) * scale : 0.f;
+        RowState s;
+        s.m = in ? row_max[r] : 0.f;
+        s.scale = in ? gr / row_sum[r] : 0.f;
+        s.g = gr;
+        s.target = in ? (int)t : -1;
+        state[r] = s;
+    }
+}
+
+// one tile of d; D[m = vocabulary][n = row]
+template <typename E, int PARTS, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
+    typedef TileProduct<E, false, false, BM, BN, WM, WN> Tile;
+    __shared__ __align__(16) char lds[Tile::kLds];
+    const Tile tile(a.w, a.x, a.pairs, a.hidden, lds);
+    const unsigned nv = (a.v1 - a.v0 + BM - 1) / BM, nr = gridDim.x / nv;
+    unsigned ti, tj;
+    grouped_tile(xcd_contiguous(blockIdx.x, gridDim.x), nv, nr, ti, tj);
+    const int v0 = a.v0 + ti * BM, r0 = tj * BN;
+    f32x4 acc[Tile::MT][Tile::NT];
+#pragma unroll
+    for (int m = 0; m < Tile::MT; ++m)
+#pragma unroll
+        for (int n = 0; n < Tile::NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    tile.run(v0, r0, 0, a.hidden, acc, [](int) {});
+    const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+    const int vw = v0 + tile.m_wave + g * 4;
+    RowState st[Tile::NT];
+#pragma unroll
+    for (int n = 0; n < Tile::NT; ++n) {
+        const int64_t r = (int64_t)r0 + tile.n_wave + n * 16 + col;
+        st[n] = r < a.rows ? a.state[r] : RowState{0.f, 0.f, 0.f, -1};
+    }
+    E* d = static_cast<E*>(a.d);
+#pragma unroll
+    for (int m = 0; m < Tile::MT; ++m) {
+        const int v = vw + m * 16;
+        f32x4 b;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[i] = bias_at(a, v + i);
+#pragma unroll
+        for (int n = 0; n < Tile::NT; ++n) {
+            const int64_t r = (int64_t)r0 + tile.n_wave + n * 16 + col;
+            vec_t<E, 4> o[PARTS];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float p = __builtin_amdgcn_exp2f((acc[m][n][i] + b[i] - st[n].m) * kLog2e) * st[n].scale;
+                if (v + i == st[n].target) p -= st[n].g;
+                if (st[n].target < 0 || v + i >= a.v1) p = 0.f;         // an ignored row, a row or an entry that is not there
+#pragma unroll
+                for (int k = 0; k < PARTS; ++k) {
+                    o[k][i] = (E)p;
+                    p = PARTS > 1 ? p - (float)o[k][i] : 0.f;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < PARTS; ++k)
+                *reinterpret_cast<vec_t<E, 4>*>(d + k * a.d_part + r * a.d_ld + (v - a.v0)) = o[k];
+        }
+    }
+}
+
+struct GradArgs {
+    Operand a, b;           // D[m = hidden][n = row or vocabulary entry]
+    int pairs, k_end, ksplit;
+    int m_end, n_end;       // extent of the output
+    void* out;              // final: [n][ld] of the output type; partial: fp32 [ksplit][n][ld]
+    int64_t ld;
+    int final_dtype;        // -1: partial sums
+    int accumulate;         // partial: add to what is there
+    const float* unscale;
+    void* db;               // nullable: row sums of B's operand (final or partial like out)
+    int db_dtype;
+};
+
+template <typename E, bool KMB, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64, 2) void ce_grad_kernel(const GradArgs a) {
+    typedef TileProduct<E, true, KMB, BM, BN, WM, WN> Tile;
+    __shared__ __align__(16) char lds[Tile::kLds];
+    const Tile tile(a.a, a.b, a.pairs, a.k_end, lds);
+    const unsigned nm = (a.m_end + BM - 1) / BM, nn = (a.n_end + BN - 1) / BN, per = nm * nn;
+    const unsigned t = xcd_contiguous(blockIdx.x, gridDim.x);
+    const unsigned ks = t / per;
+    unsigned ti, tj;
+    grouped_tile(t - ks * per, nm, nn, ti, tj);
+    const int m0 = ti * BM, n0 = tj * BN;
+    const int steps = (a.k_end + kStepK - 1) / kStepK;
+    const int k0 = (int)((int64_t)steps * ks / a.ksplit) * kStepK, k1 = min(a.k_end, (int)((int64_t)steps * (ks + 1) / a.ksplit) * kStepK);
+    const bool sums = KMB && a.db && m0 == 0 && tile.m_wave == 0;
+    f32x4 acc[Tile::MT][Tile::NT], acc1[Tile::NT];
+#pragma unroll
+    for (int n = 0; n < Tile::NT; ++n) {
+        acc1[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int m = 0; m < Tile::MT; ++m) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    s16x8 ones;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ones[i] = __builtin_bit_cast(short, (E)1.f);
+    // fp32: each part of d is once the partner of part 0 of x: pairs (0, 2), (0, 1) and (0, 0)
+    int step = 0;
+    const int per_pair = (k1 - k0 + kStepK - 1) / kStepK;
+    tile.run(m0, n0, k0, k1, acc, [&](int stage) {
+        if (!sums) return;
+        const int pair = step / per_pair;
+        ++step;
+        if (pair_a(a.pairs, pair) != 0) return;
+        const char* sb = lds + stage * Tile::kStage + Tile::kBytesA;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            s16x8 fb[4];
+            tile_frags4<KMB, BN>(sb, tile.n_wave, 0, kk, fb);
+#pragma unroll
+            for (int n = 0; n < Tile::NT; ++n) acc1[n] = mfma16<E>(ones, fb[n], acc1[n]);
+        }
+    });
+    const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+    const float scale = a.final_dtype >= 0 && a.unscale ? a.unscale[1] : 1.f;
+#pragma unroll
+    for (int n = 0; n < Tile::NT; ++n) {
+        const int64_t row = (int64_t)n0 + tile.n_wave + n * 16 + col;
+        if (row >= a.n_end) continue;
+#pragma unroll
+        for (int m = 0; m < Tile::MT; ++m) {
+            const int h = m0 + tile.m_wave + m * 16 + g * 4;
+            if (h >= a.m_end) continue;
+            if (a.final_dtype < 0) {
+                // ld is a multiple of 4: a partial row has room for the whole vector
+                f32x4* p = reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + ((int64_t)ks * a.n_end + row) * a.ld + h);
+                *p = a.accumulate ? *p + acc[m][n] : acc[m][n];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (h + i < a.m_end) store_any(a.out, a.final_dtype, row * a.ld + h + i, acc[m][n][i] * scale);
+            }
+        }
+        if (sums && g == 0) {
+            if (a.final_dtype < 0) static_cast<float*>(a.db)[(int64_t)ks * a.n_end + row] = acc1[n][0];
+            else store_any(a.db, a.db_dtype, row, acc1[n][0] * scale);
+        }
+    }
+}
+
+// sum of `parts` partial matrices in their order -> [rows][cols] of the output type (dense)
+__global__ __launch_bounds__(kBlock) void ce_sum_kernel(const float* partial, int parts, int64_t rows, int cols, int64_t ld, const float* unscale,
+                                                        void* out, int dtype) {
+    const float scale = unscale ? unscale[1] : 1.f;
+    const int64_t n = rows * cols;
+    for (int64_t q = (int64_t)blockIdx.x * kBlock + threadIdx.x; q < n; q += (int64_t)gridDim.x * kBlock) {
+        const int64_t r = q / cols;
+        const int64_t at = r * ld + (q - r * cols);
+        float s = 0.f;
+        for (int p = 0; p < parts; ++p) s += partial[(int64_t)p * rows * ld + at];
+        store_any(out, dtype, q, s * scale);
+    }
+}
+
+// ---- host: plan of a call -------------------------------------------------------------------------------------------------------
+
+constexpr int kBig = 256, kSmall = 128;         // tile edges
+constexpr int64_t kPieceBytes = 128ll << 20;    // d of one piece of the vocabulary: half the memory-side cache
+
+static int64_t round_up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+static int64_t ceil_div(int64_t n, int64_t m) { return (n + m - 1) / m; }
+
+struct CePlan {
+    int parts, pairs;
+    bool copy_x, copy_w;
+    int64_t ldh;                    // padded row of a copied operand
+    int64_t x_off, w_off, x_bytes, w_bytes;
+    // forward
+    bool big_lse;
+    int splits;
+    int64_t partial_off, logit_off;
+    // backward
+    int64_t rows_pad, piece, d_off, d_bytes, state_off, unscale_off, dx_off, dw_off, db_off;
+    int dx_split, dw_split;
+    bool big_d, big_dx, big_dw;
+    int64_t bytes;
+};
+
+static CePlan ce_plan(int64_t R, int V, int H, int dtype, bool x_ok, bool w_ok, bool backward) {
+    CePlan p{};
+    p.parts = dtype == CNF_DTYPE_F32 ? 3 : 1;
+    p.pairs = dtype == CNF_DTYPE_F32 ? 6 : 1;
+    p.copy_x = p.parts > 1 || !x_ok;
+    p.copy_w = p.parts > 1 || !w_ok;
+    p.ldh = round_up(H, 8);
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        const int64_t o = at;
+        at += round_up(bytes, 256);
+        return o;
+    };
+    if (p.copy_x) p.x_off = take(p.x_bytes = (int64_t)p.parts * R * p.ldh * 2);
+    if (p.copy_w) p.w_off = take(p.w_bytes = (int64_t)p.parts * V * p.ldh * 2);
+    if (!backward) {
+        // 256 x 256 tiles once they fill the chip; the vocabulary is split until there are two workgroups per CU (one of the big)
+        p.big_lse = ceil_div(R, kBig) * ceil_div(V, kBig) >= 512;
+        const int edge = p.big_lse ? kBig : kSmall;
+        const int64_t rt = ceil_div(R, edge), vt = ceil_div(V, edge);
+        p.splits = (int)std::min<int64_t>(vt, std::max<int64_t>(1, (p.big_lse ? 256 : 512) / rt));
+        p.partial_off = take((int64_t)p.splits * R * 8);
+        p.logit_off = take(R * 4);
+    } else {
+        p.rows_pad = round_up(R, kBig);
+        const int64_t row_bytes = p.rows_pad * 2 * p.parts;
+        p.piece = std::min<int64_t>(round_up(V, kBig), std::max<int64_t>(kBig, kPieceBytes / row_bytes / kBig * kBig));
+        p.d_off = take(p.d_bytes = row_bytes * p.piece);
+        p.state_off = take(R * (int64_t)sizeof(RowState));
+        p.unscale_off = take(8);
+        const int64_t width = std::min<int64_t>(p.piece, V);
+        p.big_d = ceil_div(R, kBig) * ceil_div(width, kBig) >= 256;
+        // dx [R][H] over k = the piece; dw [piece][H] over k = R: k is split where the tiles alone do not fill the chip
+        auto split = [&](int64_t n, int64_t k, bool& big) {
+            big = ceil_div(n, kBig) * ceil_div(H, kBig) >= 128 && H > kSmall;
+            const int edge = big ? kBig : kSmall;
+            const int64_t tiles = ceil_div(n, edge) * ceil_div(H, edge), steps = ceil_div(k, kStepK);
+            return (int)std::max<int64_t>(1, std::min<int64_t>({steps / 4, ceil_div(big ? 256 : 512, tiles), 64}));
+        };
+        p.dx_split = split(R, width, p.big_dx);
+        p.dw_split = split(width, R, p.big_dw);
+        const int64_t ld4 = round_up(H, 4);
+        if (p.dx_split > 1 || p.piece < V) p.dx_off = take((int64_t)p.dx_split * R * ld4 * 4);
+        if (p.dw_split > 1) {
+            p.dw_off = take((int64_t)p.dw_split * width * ld4 * 4);
+            p.db_off = take((int64_t)p.dw_split * width * 4);
+        }
+    }
+    p.bytes = at;
+    return p;
+}
+
+template <typename T, typename E, int PARTS>
+static void ce_layout(const void* src, int64_t stride, int64_t rows, int cols, void* dst, int64_t ld, hipStream_t st) {
+    const int64_t n = rows * (ld / 8);
+    CNF_LAUNCH((ce_layout_kernel<T, E, PARTS>), dim3((unsigned)std::min<int64_t>(ceil_div(n, kBlock), 8192)), dim3(kBlock), 0, st,
+               static_cast<const T*>(src), stride, rows, cols, static_cast<E*>(dst), ld, rows * ld);
+}
+
+// calls fn(T{}, E{}, parts): the tensors' type, the products' operand type, the parts of an operand
+template <typename Fn>
+static int ce_types(int dtype, Fn&& fn) {
+    if (dtype == CNF_DTYPE_F32) return fn(float{}, bf16_t{}, std::integral_constant<int, 3>{});
+    if (dtype == CNF_DTYPE_BF16) return fn(bf16_t{}, bf16_t{}, std::integral_constant<int, 1>{});
+    return fn(f16_t{}, f16_t{}, std::integral_constant<int, 1>{});
+}
+
+template <typename T, typename E, int PARTS>
+static void ce_operands(CeArgs& a, const CePlan& p, const void* x, int64_t x_stride, const void* w, int64_t w_stride, int64_t R, int V, int H,
+                        char* ws, hipStream_t st) {
+    if (p.copy_x) ce_layout<T, E, PARTS>(x, x_stride, R, H, ws + p.x_off, p.ldh, st);
+    if (p.copy_w) ce_layout<T, E, PARTS>(w, w_stride, V, H, ws + p.w_off, p.ldh, st);
+    a.x = p.copy_x ? Operand{ws + p.x_off, p.ldh, R * p.ldh, (int)R} : Operand{x, x_stride, 0, (int)R};
+    a.w = p.copy_w ? Operand{ws + p.w_off, p.ldh, V * p.ldh, V} : Operand{w, w_stride, 0, V};
+    a.pairs = p.pairs;
+    a.parts = p.parts;
+    a.rows = R;
+    a.vocab = V;
+    a.hidden = H;
+}
+
+static bool ce_aligned(const void* p, int64_t stride, int dtype, int H) { return rows_aligned16(p, stride, dtype) && H % 8 == 0; }
+
+}  // namespace cnf
+
+using namespace cnf;
+
+#define CE_CHECK(name)                                                                                                             \
+    CNF_REQUIRE(R >= 0 && V > 0 && H > 0 && R <= 0x7fffff00ll && V <= 0x7fffff00 && H <= 0x7fffff00, name ": bad size R=%ld V=%d H=%d", \
+                (long)R, V, H);                                                                                                    \
+    CNF_REQUIRE(dtype_known(dtype) && dtype_known(bias_dtype), name ": unknown element type");                                     \
+    CNF_REQUIRE(x_stride >= 0 && w_stride >= 0, name ": negative stride")
+
+extern "C" {
+
+int64_t cnf_linear_ce_workspace_bytes(int64_t R, int V, int H, int dtype, int backward) {
+    if (R <= 0 || V <= 0 || H <= 0 || !dtype_known(dtype)) return 0;
+    return ce_plan(R, V, H, dtype, false, false, backward != 0).bytes;
+}
+
+int cnf_linear_ce(const void* x, int64_t x_stride, const void* weight, int64_t w_stride, const void* bias, const int64_t* target,
+                  int64_t ignore_index, float* loss, float* row_max, float* row_sum, float* reduced, void* workspace, int64_t workspace_bytes,
+                  int64_t R, int V, int H, int dtype, int bias_dtype, int* flags, cnf_stream_t stream) {
+    CE_CHECK("cnf_linear_ce");
+    hipStream_t st = (hipStream_t)stream;
+    if (R > 0) {
+        CNF_REQUIRE(x && weight && target && loss && row_max && row_sum, "cnf_linear_ce: null tensor");
+        CNF_REQUIRE(workspace && workspace_bytes >= cnf_linear_ce_workspace_bytes(R, V, H, dtype, 0),
+                    "cnf_linear_ce: workspace smaller than cnf_linear_ce_workspace_bytes");
+        CNF_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "cnf_linear_ce: workspace not 16-byte aligned");
+        const CePlan p = ce_plan(R, V, H, dtype, ce_aligned(x, x_stride, dtype, H), ce_aligned(weight, w_stride, dtype, H), false);
+        char* ws = static_cast<char*>(workspace);
+        const int rc = ce_types(dtype, [&](auto t, auto e, auto parts) {
+            typedef decltype(t) T;
+            typedef decltype(e) E;
+            CeArgs a{};
+            ce_operands<T, E, decltype(parts)::value>(a, p, x, x_stride, weight, w_stride, R, V, H, ws, st);
+            a.bias = bias;
+            a.bias_dtype = bias_dtype;
+            a.target = target;
+            a.ignore = ignore_index;
+            a.partial = reinterpret_cast<float2*>(ws + p.partial_off);
+            a.target_logit = reinterpret_cast<float*>(ws + p.logit_off);
+            a.splits = p.splits;
+            if (p.big_lse)
+                CNF_LAUNCH((ce_lse_kernel<E, kBig, kBig, 2, 4>), dim3((unsigned)(ceil_div(R, kBig) * p.splits)), dim3(512), 0, st, a);
+            else
+                CNF_LAUNCH((ce_lse_kernel<E, kSmall, kSmall, 2, 2>), dim3((unsigned)(ceil_div(R, kSmall) * p.splits)), dim3(256), 0, st, a);
+            CNF_LAUNCH(ce_join_kernel, dim3((unsigned)ceil_div(R, kBlock)), dim3(kBlock), 0, st, a.partial, a.target_logit, target, ignore_index, V,
+                       p.splits, R, row_max, row_sum, loss, flags);
+            return launch_status("cnf_linear_ce");
+        });
+        if (rc != CNF_OK) return rc;
+    }
+    if (reduced) {
+        CNF_LAUNCH(ce_reduce_kernel, dim3(1), dim3(1024), 0, st, loss, target, ignore_index, R, reduced);
+        return launch_status("cnf_linear_ce (reduction)");
+    }
+    return CNF_OK;
+}
+
+int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64_t w_stride, const void* bias, const int64_t* target,
+                      int64_t ignore_index, const float* row_max, const float* row_sum, const float* g, int g_per_row, const float* count,
+                      void* dx, void* dweight, void* dbias, void* workspace, int64_t workspace_bytes, int64_t R, int V, int H, int dtype,
+                      int bias_dtype, cnf_stream_t stream) {
+    CE_CHECK("cnf_linear_ce_bwd");
+    CNF_REQUIRE(R > 0, "cnf_linear_ce_bwd: no rows");
+    CNF_REQUIRE(x && weight && target && row_max && row_sum && g && (g_per_row || count) && (dx || dweight) && (dweight || !dbias), "cnf_linear_ce_bwd: null tensor");
+    CNF_REQUIRE(workspace && workspace_bytes >= cnf_linear_ce_workspace_bytes(R, V, H, dtype, 1),
+                "cnf_linear_ce_bwd: workspace smaller than cnf_linear_ce_workspace_bytes");
+    CNF_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "cnf_linear_ce_bwd: workspace not 16-byte aligned");
+    const CePlan p = ce_plan(R, V, H, dtype, ce_aligned(x, x_stride, dtype, H), ce_aligned(weight, w_stride, dtype, H), true);
+    char* ws = static_cast<char*>(workspace);
+    hipStream_t st = (hipStream_t)stream;
+    return ce_types(dtype, [&](auto t, auto e, auto parts) {
+        typedef decltype(t) T;
+        typedef decltype(e) E;
+        constexpr int PARTS = decltype(parts)::value;
+        CeArgs a{};
+        ce_operands<T, E, PARTS>(a, p, x, x_stride, weight, w_stride, R, V, H, ws, st);
+        a.bias = bias;
+        a.bias_dtype = bias_dtype;
+        RowState* state = reinterpret_cast<RowState*>(ws + p.state_off);
+        float* unscale = dtype == CNF_DTYPE_F16 ? reinterpret_cast<float*>(ws + p.unscale_off) : nullptr;
+        a.state = state;
+        // fp16: every workgroup finds the largest |g| itself; few of them
+        CNF_LAUNCH(ce_rows_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(R, 1024), unscale && g_per_row ? 16 : 1024)), dim3(1024), 0, st, g,
+                   g_per_row, count, row_max, row_sum, target, ignore_index, V, R, state, unscale);
+        a.d = ws + p.d_off;
+        a.d_ld = p.piece;
+        a.d_part = p.rows_pad * p.piece;
+        const int64_t ld4 = round_up(H, 4);
+        const bool dx_partial = p.dx_split > 1 || p.piece < V, dw_partial = p.dw_split > 1;
+        for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
+            const int64_t v1 = std::min<int64_t>(V, v0 + p.piece), width = v1 - v0;
+            a.v0 = (int)v0;
+            a.v1 = (int)v1;
+            if (p.big_d)
+                CNF_LAUNCH((ce_d_kernel<E, PARTS, kBig, kBig, 2, 4>), dim3((unsigned)(ceil_div(width, kBig) * ceil_div(R, kBig))), dim3(512), 0, st, a);
+            else
+                CNF_LAUNCH((ce_d_kernel<E, PARTS, kSmall, kSmall, 2, 2>), dim3((unsigned)(ceil_div(width, kSmall) * ceil_div(R, kSmall))), dim3(256), 0,
+                           st, a);
+            const Operand d{a.d, a.d_ld, a.d_part, 0};
+            GradArgs q{};
+            q.pairs = p.pairs;
+            q.m_end = H;
+            // dx[r][h] += sum_v w[v][h] d[r][v]
+            q.a = Operand{static_cast<const uint16_t*>(a.w.base) + v0 * a.w.ld, a.w.ld, a.w.part, H};
+            q.b = d;
+            q.b.ext = (int)R;
+            q.k_end = (int)width;
+            q.n_end = (int)R;
+            q.ksplit = p.dx_split;
+            q.final_dtype = dx_partial ? -1 : dtype;
+            q.out = dx_partial ? static_cast<void*>(ws + p.dx_off) : dx;
+            q.ld = dx_partial ? ld4 : H;
+            q.accumulate = v0 > 0;
+            q.unscale = unscale;
+            auto grad = [&](bool kmb, bool big, int64_t n) {
+                const int64_t edge = big ? kBig : kSmall;
+                const dim3 grid((unsigned)(ceil_div(n, edge) * ceil_div(H, edge) * q.ksplit));
+                if (kmb && big) CNF_LAUNCH((ce_grad_kernel<E, true, kBig, kBig, 2, 4>), grid, dim3(512), 0, st, q);
+                else if (kmb) CNF_LAUNCH((ce_grad_kernel<E, true, kSmall, kSmall, 2, 2>), grid, dim3(256), 0, st, q);
+                else if (big) CNF_LAUNCH((ce_grad_kernel<E, false, kBig, kBig, 2, 4>), grid, dim3(512), 0, st, q);
+                else CNF_LAUNCH((ce_grad_kernel<E, false, kSmall, kSmall, 2, 2>), grid, dim3(256), 0, st, q);
+            };
+            if (dx) grad(false, p.big_dx, R);
+            if (!dweight) continue;
+            // dw[v][h] = sum_r x[r][h] d[r][v]; db[v] = sum_r d[r][v]
+            char* dw = static_cast<char*>(dweight) + v0 * H * dtype_bytes(dtype);
+            char* db = dbias ? static_cast<char*>(dbias) + v0 * dtype_bytes(bias_dtype) : nullptr;
+            q.a = a.x;
+            q.a.ext = H;
+            q.b = d;
+            q.b.ext = (int)width;
+            q.k_end = (int)R;
+            q.n_end = (int)width;
+            q.ksplit = p.dw_split;
+            q.final_dtype = dw_partial ? -1 : dtype;
+            q.out = dw_partial ? static_cast<void*>(ws + p.dw_off) : dw;
+            q.ld = dw_partial ? ld4 : H;
+            q.accumulate = 0;
+            q.db = db ? (dw_partial ? static_cast<void*>(ws + p.db_off) : db) : nullptr;
+            q.db_dtype = bias_dtype;
+            grad(true, p.big_dw, width);
+            if (dw_partial) {
+                CNF_LAUNCH(ce_sum_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(width * H, kBlock), 4096)), dim3(kBlock), 0, st,
+                           reinterpret_cast<const float*>(ws + p.dw_off), p.dw_split, width, H, ld4, unscale, dw, dtype);
+                if (db)
+                    CNF_LAUNCH(ce_sum_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(width, kBlock), 4096)), dim3(kBlock), 0, st,
+                               reinterpret_cast<const float*>(ws + p.db_off), p.dw_split, (int64_t)1, (int)width, width, unscale, db, bias_dtype);
+            }
+        }
+        if (dx && dx_partial)
+            CNF_LAUNCH(ce_sum_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(R * H, kBlock), 8192)), dim3(kBlock), 0, st,
+                       reinterpret_cast<const float*>(ws + p.dx_off), p.dx_split, R, H, ld4, unscale, dx, dtype);
+        return launch_status("cnf_linear_ce_bwd");
+    });
+}
+
+}  // extern "C"

@@ -801,3 +801,38 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     if needs_grad(x, weight, bias):
         return LayerNormFn.apply(x, weight, bias, float(eps))
     return ops.layer_norm(x, weight, bias, eps)
+
+
+class LinearCrossEntropyFn(torch.autograd.Function):
+    """(x, weight, bias) -> softmax cross entropy of the linear layer: [R] losses, or their mean or sum."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, target, ignore_index, reduction):
+        loss, row_max, row_sum, reduced = ops.linear_cross_entropy(x, weight, target, bias, ignore_index, want_reduced=reduction != "none")
+        ctx.save_for_backward(x, weight, bias, target, row_max, row_sum, reduced)
+        ctx.ignore_index, ctx.reduction = ignore_index, reduction
+        if reduction == "none":
+            return loss
+        return reduced[0 if reduction == "mean" else 1].clone()
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, weight, bias, target, row_max, row_sum, reduced = ctx.saved_tensors
+        if ctx.reduction == "sum":
+            g = g.expand(row_max.shape)
+        dx, dw, db = ops.linear_cross_entropy_bwd(x, weight, target, bias, row_max, row_sum, g.contiguous(),
+                                                  reduced[2:] if ctx.reduction == "mean" else None, ctx.ignore_index, ctx.needs_input_grad[:3])
+        return dx, dw, db, None, None, None
+
+
+def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduction="mean"):
+    """Softmax cross entropy of x @ weight.T + bias against integer targets without keeping the logits (`ops.linear_cross_entropy`),
+    differentiable in x, weight and bias.  reduction: "mean" over the rows that are not ignored (NaN if there are none), "sum",
+    or "none" (fp32 losses of target's shape; ignored rows 0)."""
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError("reduction is mean, sum or none, got %r" % (reduction,))
+    if needs_grad(x, weight, bias):
+        return LinearCrossEntropyFn.apply(x, weight, bias, target, int(ignore_index), reduction)
+    loss, _, _, reduced = ops.linear_cross_entropy(x, weight, target, bias, ignore_index, want_reduced=reduction != "none")
+    return loss if reduction == "none" else reduced[0 if reduction == "mean" else 1]

@@ -3,6 +3,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ... import functional as Fn
 from ...host_utils import get_param_val
 from ..networks.help_layers import LinearNet
 
@@ -27,7 +28,7 @@ def create_decoder(num_categories, num_dims, config, **kwargs):
 
 class DecoderLinear(nn.Module):
     """MLP latent -> class log-probabilities on the features [z, elu(z), elu(-z)] (decoder.py:35-63).
-    Dense GEMMs: stays PyTorch-ROCm."""
+    The hidden layers are dense GEMMs of PyTorch-ROCm; `class_log_prob` ends in this package's linear cross entropy."""
 
     def __init__(self, num_categories, embed_dim, hidden_size, num_layers, class_prior_log=None):
         super().__init__()
@@ -40,9 +41,18 @@ class DecoderLinear(nn.Module):
                 class_prior_log = torch.from_numpy(class_prior_log)
             self.layers.set_bias(class_prior_log)
 
+    def _features(self, z_cont):
+        return torch.cat([z_cont, F.elu(z_cont), F.elu(-z_cont)], dim=-1)
+
     def forward(self, z_cont):
-        feats = torch.cat([z_cont, F.elu(z_cont), F.elu(-z_cont)], dim=-1)
-        return self.log_softmax(self.layers(feats))
+        return self.log_softmax(self.layers(self._features(z_cont)))
+
+    def class_log_prob(self, z_cont, z_categ):
+        """log p(z_categ | z_cont) for z_categ of z_cont's shape without its last axis: forward() gathered at one class, whose
+        [..., C] log-probabilities are never written (one fused kernel per direction instead of GEMM + log-softmax + gather)."""
+        last = self.layers.main_net[-1]
+        hidden = self.layers.hidden_features(self._features(z_cont))
+        return -Fn.linear_cross_entropy(hidden, last.weight, z_categ, last.bias, ignore_index=-100, reduction="none")
 
     def info(self):
         return "Linear model with hidden size %i and %i layers" % (self.hidden_size, self.num_layers)

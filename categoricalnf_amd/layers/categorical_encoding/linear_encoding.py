@@ -203,7 +203,8 @@ class LinearCategoricalEncoding(FlowLayer):
         return z_cont, ldj
 
     def _decoder_forward(self, z_cont, z_categ, **kwargs):
-        return self.decoder(z_cont).gather(dim=-1, index=z_categ.view(-1, 1))
+        """[T] log p(class | z) from the decoder; z_cont [T, 1, D], z_categ [T, 1]."""
+        return self.decoder.class_log_prob(z_cont, z_categ).reshape(-1)
 
     def _all_class_scores(self, z_cont):
         """reverse-flow log-prob + ldj + prior for every class: [T, C] (:155-164 / :186-195)."""

@@ -1111,6 +1111,70 @@ def layer_norm_bwd(x, dy, weight, mean, rstd, param_dtype=None, want_weight=True
     return dx, dw, db
 
 
+def _ce_operands(x, weight, target, bias):
+    """Checked operands of the linear cross entropy: (x [R, H], weight, bias, target [R], R, V, H, dtype code, bias dtype code, device)."""
+    code, dev = _float_code(x, "x"), x.device
+    if weight.dtype != x.dtype or _float_code(weight, "weight") != code:
+        raise TypeError("x is %s, weight %s" % (x.dtype, weight.dtype))
+    if weight.dim() != 2 or x.dim() < 1 or weight.shape[1] != x.shape[-1] or 0 in weight.shape:
+        raise ValueError("weight must be [V, H] with the H of x, both at least 1: got %s for x %s" % (tuple(weight.shape), tuple(x.shape)))
+    if not isinstance(target, torch.Tensor) or target.dtype not in (torch.int64, torch.int32):
+        raise TypeError("target must be an integer tensor (int64 or int32)")
+    if target.shape != x.shape[:-1]:
+        raise ValueError("target must have the shape of x without its last axis: got %s for %s" % (tuple(target.shape), tuple(x.shape)))
+    for t, name in ((weight, "weight"), (target, "target")):
+        if t.device != dev:
+            raise (HipOnlyError if not t.is_cuda else ValueError)("%s is on %s, x on %s" % (name, t.device, dev))
+    V, H = weight.shape
+    b, bcode = _vector(bias, V, "bias", dev)
+    if bcode not in (None, code, 0):
+        raise TypeError("bias is float32 or of the weight's type, got %s" % (bias.dtype,))
+    return (_rows(x), _rows(weight), b, target.reshape(-1).to(torch.int64).contiguous(), target.numel(), V, H, code,
+            bcode if bcode is not None else 0, dev)
+
+
+def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, want_reduced=False):
+    """Softmax cross entropy of the linear layer x @ weight.T + bias over a vocabulary, without its logits (cnf_linear_ce).
+
+    x [..., H] and weight [V, H] float32, bfloat16 or float16; bias [V] of that type or float32; target [...] integers.  Returns
+    (loss [...] fp32, row_max [R], row_sum [R], reduced or None): rows with target == ignore_index have loss 0, a category outside
+    [0, V) raises the flag that `check_flags` reports.  reduced: [mean, sum, count] over the rows that are not ignored."""
+    x2, w2, b, t, R, V, H, code, bcode, dev = _ce_operands(x, weight, target, bias)
+    loss = torch.empty(target.shape, dtype=torch.float32, device=dev)
+    row_max, row_sum = torch.empty(2, R, dtype=torch.float32, device=dev).unbind(0)
+    reduced = torch.empty(3, dtype=torch.float32, device=dev) if want_reduced else None
+    n = int(_lib.load().cnf_linear_ce_workspace_bytes(R, V, H, code, 0))
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    _launch(dev, "cnf_linear_ce", _ptr(x2), x2.stride(0), _ptr(w2), w2.stride(0), _ptr(b), _ptr(t), int(ignore_index), _ptr(loss),
+            _ptr(row_max), _ptr(row_sum), _ptr(reduced), _ptr(ws), n, R, V, H, code, bcode, _ptr(flag_word(dev)), _stream(dev))
+    _after(dev, "linear_cross_entropy")
+    return loss, row_max, row_sum, reduced
+
+
+def linear_cross_entropy_bwd(x, weight, target, bias, row_max, row_sum, g, count=None, ignore_index=-100, want=(True, True, True)):
+    """Gradients (dx, dweight, dbias) of linear_cross_entropy for the upstream gradient g: [R] fp32, or — with `count`, the third
+    value of `reduced` — the gradient of the mean.  `want`: which of the three."""
+    x2, w2, b, t, R, V, H, code, bcode, dev = _ce_operands(x, weight, target, bias)
+    want_w = want[1] or (want[2] and b is not None)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want[0] else None
+    dw = torch.empty(V, H, dtype=x.dtype, device=dev) if want_w else None
+    db = torch.empty(V, dtype=b.dtype, device=dev) if want[2] and b is not None else None
+    if R == 0 or (dx is None and dw is None):
+        for t_ in (dw, db):
+            if t_ is not None:
+                t_.zero_()
+        return dx, dw, db
+    g = _f32(g, "g").reshape(-1)
+    if g.numel() != (1 if count is not None else R):
+        raise ValueError("the upstream gradient has %d values for %d rows" % (g.numel(), R))
+    n = int(_lib.load().cnf_linear_ce_workspace_bytes(R, V, H, code, 1))
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    _launch(dev, "cnf_linear_ce_bwd", _ptr(x2), x2.stride(0), _ptr(w2), w2.stride(0), _ptr(b), _ptr(t), int(ignore_index), _ptr(row_max),
+            _ptr(row_sum), _ptr(g), int(count is None), _ptr(count), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), n, R, V, H, code, bcode,
+            _stream(dev))
+    return dx, (dw if want[1] else None), db
+
+
 ADAMW_BLOCK = 256           # consecutive elements of a tensor that share the two scales of its 8-bit moments
 
 

@@ -641,6 +641,27 @@ int cnf_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64_t 
                        const float* mean, const float* rstd, void* dx, void* dweight, void* dbias, float* workspace,
                        int64_t workspace_floats, int64_t rows, int cols, int dtype, int wdtype, cnf_stream_t stream);
 
+/* Softmax cross entropy of a linear layer over a vocabulary, without keeping its logits: loss[r] = logsumexp_v(x_r . w_v + b_v)
+ * - (x_r . w_t + b_t), t = target[r] — minus the log-probability that the decoder's Linear + LogSoftmax + gather gives one class
+ * (layers/categorical_encoding/decoder.py:35-63, linear_encoding.py:176-180).  x [R, H] and weight [V, H] of `dtype`, unit column
+ * stride, `x_stride` / `w_stride` elements between rows; bias [V] of `bias_dtype` (nullable); target int64 [R].  Rows with target ==
+ * ignore_index have loss 0; any other target outside [0, V) raises CNF_FLAG_CATEGORY and its loss is NaN.  row_max, row_sum [R]: the
+ * maximum logit and sum_v exp(logit - maximum), which the backward takes; reduced [3] (nullable): mean (NaN over no rows), sum and
+ * number of the rows that are not ignored.  fp32 products are exact to 2^-26 each (six bf16 products of split operands), 16-bit
+ * products are exact; sums, maxima and exponentials are fp32.  workspace_bytes >= cnf_linear_ce_workspace_bytes(R, V, H, dtype, 0). */
+int64_t cnf_linear_ce_workspace_bytes(int64_t R, int V, int H, int dtype, int backward);
+int cnf_linear_ce(const void* x, int64_t x_stride, const void* weight, int64_t w_stride, const void* bias, const int64_t* target,
+                  int64_t ignore_index, float* loss, float* row_max, float* row_sum, float* reduced, void* workspace,
+                  int64_t workspace_bytes, int64_t R, int V, int H, int dtype, int bias_dtype, int* flags, cnf_stream_t stream);
+/* Its gradients: dx [R, H], dweight [V, H] dense of `dtype`, dbias [V] of `bias_dtype` (each nullable; dbias needs dweight) for the
+ * upstream gradient g: fp32 [R] (g_per_row != 0), or one value that is divided by *count (the mean's).  Ignored rows and rows with a
+ * target outside the vocabulary have gradient 0.  The gradient of the logits is computed in pieces of the vocabulary and rounded to
+ * `dtype` (fp32: kept to 24 bits); sums are fp32, in a fixed order.  workspace_bytes >= cnf_linear_ce_workspace_bytes(..., 1). */
+int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64_t w_stride, const void* bias, const int64_t* target,
+                      int64_t ignore_index, const float* row_max, const float* row_sum, const float* g, int g_per_row, const float* count,
+                      void* dx, void* dweight, void* dbias, void* workspace, int64_t workspace_bytes, int64_t R, int V, int H, int dtype,
+                      int bias_dtype, cnf_stream_t stream);
+
 /* One AdamW step over `count` dense tensors: m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g^2,
  * p = p (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps).
  * The LISTS are HOST arrays of device pointers (and element counts), read before the call returns.  Parameters of `pdtype`,
