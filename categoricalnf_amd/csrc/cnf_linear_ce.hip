@@ -10,24 +10,19 @@
 // kept as three bf16 parts for fp32), written to a workspace that fits the memory-side cache, and read by two products: dx += d w over
 // the piece, dw = d^T x complete for the piece.  db comes out of the second product: a fragment of ones in place of x.
 //
+// Few features (fp32: H <= 64, 16-bit: H <= 128) take the kernels of cnf_linear_ce_narrow.hip instead, which write nothing of size R x V.
+//
 // fp32 inputs are split once into three bf16 parts (cnf_mfma.h: pair_a): six bf16 products keep every product to 2^-26, and the
 // matrix cores do them at 16 times the fp32 rate.  16-bit inputs whose rows are not 16-byte aligned are copied once into padded rows.
-// In fp16 d is scaled by a power of two that brings the largest |g_r| to 2^14, so that small probabilities keep their bits.
+// 16-bit d is computed for g_r / max |g| (in fp16 times 2^14, so that small probabilities keep their bits) and the results are scaled
+// back: under a mean every row's -1 is then exact, where a rounded -g_r would put the same relative error on every row's largest entry.
 #include <algorithm>
 
-#include "cnf_mfma.h"
+#include "cnf_linear_ce_narrow.h"
 
 namespace cnf {
 
 constexpr float kLog2e = 1.4426950408889634f;
-
-// ---- row records -----------------------------------------------------------------------------------------------------------------
-
-struct RowState {       // backward: what an element of d needs of its row
-    float m, scale;     // maximum; g / s
-    float g;
-    int target;         // -1: ignored
-};
 
 struct CeArgs {
     Operand w, x;                   // [V][H], [R][H]
@@ -44,7 +39,6 @@ struct CeArgs {
     int splits;                     // of the vocabulary tiles
     // backward
     const RowState* state;          // [rows]
-    const float* unscale;           // fp16: [2] = {S, 1 / S}
     void* d;                        // [parts][rows_pad][piece_ld]
     int64_t d_part, d_ld;
     int v0, v1;                     // the piece
@@ -172,44 +166,69 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_lse_kernel(const CeArgs a)
     }
 }
 
-// the parts of the vocabulary -> row maximum, sum, loss; a category outside the vocabulary raises its flag and gives NaN
+// the parts of the vocabulary -> row maximum, sum, loss; a category outside the vocabulary raises its flag and gives NaN.
+// sums (with `reduced`): [workgroups][2] sum and number of the rows that are not ignored, in a fixed order; a single workgroup
+// writes `reduced` itself
 __global__ __launch_bounds__(kBlock) void ce_join_kernel(const float2* partial, const float* target_logit, const int64_t* target,
                                                          int64_t ignore, int vocab, int splits, int64_t rows, float* row_max,
-                                                         float* row_sum, float* loss, int* flags) {
+                                                         float* row_sum, float* loss, double* sums, float* reduced, int* flags) {
     const int64_t r = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-    if (r >= rows) return;
-    float m = -INFINITY, s = 0.f;
-    for (int k = 0; k < splits; ++k) m = fmaxf(m, partial[(int64_t)k * rows + r].x);
-    const float ref = m == -INFINITY ? 0.f : m;
-    for (int k = 0; k < splits; ++k) {
-        const float2 o = partial[(int64_t)k * rows + r];
-        s += o.y * __builtin_amdgcn_exp2f((o.x - ref) * kLog2e);
-    }
-    row_max[r] = m;
-    row_sum[r] = s;
-    const int64_t t = target[r];
     float v = 0.f;
-    if (t != ignore) {
-        if (t < 0 || t >= vocab) {
-            raise_flag(flags, CNF_FLAG_CATEGORY);
-            v = NAN;
+    bool counts = false;
+    if (r < rows) {
+        float m = -INFINITY, s = 0.f;
+        for (int k = 0; k < splits; ++k) m = fmaxf(m, partial[(int64_t)k * rows + r].x);
+        const float ref = m == -INFINITY ? 0.f : m;
+        for (int k = 0; k < splits; ++k) {
+            const float2 o = partial[(int64_t)k * rows + r];
+            s += o.y * __builtin_amdgcn_exp2f((o.x - ref) * kLog2e);
+        }
+        row_max[r] = m;
+        row_sum[r] = s;
+        const int64_t t = target[r];
+        counts = t != ignore;
+        if (counts) {
+            if (t < 0 || t >= vocab) {
+                raise_flag(flags, CNF_FLAG_CATEGORY);
+                v = NAN;
+            } else {
+                v = logf(s) + (m - target_logit[r]);
+            }
+        }
+        loss[r] = v;
+    }
+    if (!reduced) return;
+    __shared__ double sh[2][kWavesPerBlock];
+    const double ws = wave_sum((double)v), wc = wave_sum(counts ? 1.0 : 0.0);
+    if ((threadIdx.x & 63) == 0) {
+        sh[0][threadIdx.x >> 6] = ws;
+        sh[1][threadIdx.x >> 6] = wc;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double s = 0.0, c = 0.0;
+        for (int w = 0; w < kWavesPerBlock; ++w) {
+            s += sh[0][w];
+            c += sh[1][w];
+        }
+        if (gridDim.x == 1) {
+            reduced[0] = (float)(s / c);
+            reduced[1] = (float)s;
+            reduced[2] = (float)c;
         } else {
-            v = logf(s) + (m - target_logit[r]);
+            sums[2 * (int64_t)blockIdx.x] = s;
+            sums[2 * (int64_t)blockIdx.x + 1] = c;
         }
     }
-    loss[r] = v;
 }
 
-// reduced = {mean, sum, number} over the rows that are not ignored: one workgroup, fixed order, fp64
-__global__ __launch_bounds__(1024) void ce_reduce_kernel(const float* loss, const int64_t* target, int64_t ignore, int64_t rows,
-                                                         float* reduced) {
+// reduced = {mean, sum, number}: one workgroup, fixed order; no row left: 0 / 0 = NaN
+__global__ __launch_bounds__(1024) void ce_reduce_kernel(const double* sums, int64_t n, float* reduced) {
     __shared__ double sh[2][16];
     double s = 0.0, c = 0.0;
-    for (int64_t r = threadIdx.x; r < rows; r += 1024) {
-        if (target[r] != ignore) {
-            s += (double)loss[r];
-            c += 1.0;
-        }
+    for (int64_t i = threadIdx.x; i < n; i += 1024) {
+        s += sums[2 * i];
+        c += sums[2 * i + 1];
     }
     s = wave_sum(s);
     c = wave_sum(c);
@@ -224,7 +243,7 @@ __global__ __launch_bounds__(1024) void ce_reduce_kernel(const float* loss, cons
             s += sh[0][w];
             c += sh[1][w];
         }
-        reduced[0] = (float)(s / c);    // no row left: 0 / 0 = NaN
+        reduced[0] = (float)(s / c);
         reduced[1] = (float)s;
         reduced[2] = (float)c;
     }
@@ -232,17 +251,43 @@ __global__ __launch_bounds__(1024) void ce_reduce_kernel(const float* loss, cons
 
 // ---- operand layout ----------------------------------------------------------------------------------------------------------------
 
-// [rows][cols] of T -> `parts` arrays of [rows][ld] 16-bit elements, zeros behind cols; fp32: x0 + x1 + x2
+struct LayoutJob {
+    const void* src;                // nullable: nothing to do
+    int64_t stride, rows;
+    void* dst;
+};
+struct LayoutArgs {
+    LayoutJob job[2];               // x and w: [rows][cols] -> `parts` arrays of [rows][ld] 16-bit elements, zeros behind cols
+    int cols;
+    int64_t ld;
+    const void* bias;               // -> fp32, -inf behind the vocabulary (nullable: zeros)
+    int bias_dtype, vocab, bias_pad;
+    float* bias_out;                // nullable
+};
+
+// one launch for whatever a call has to lay out: blockIdx.y 0: x, 1: w, 2: the bias.  fp32: x0 + x1 + x2, each the bf16 nearest to what
+// is left
 template <typename T, typename E, int PARTS>
-__global__ __launch_bounds__(kBlock) void ce_layout_kernel(const T* src, int64_t stride, int64_t rows, int cols, E* dst, int64_t ld, int64_t part) {
-    const int64_t n = rows * (ld / 8);
+__global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
+    if (blockIdx.y == 2) {
+        if (a.bias_out)
+            for (int v = blockIdx.x * kBlock + threadIdx.x; v < a.bias_pad; v += gridDim.x * kBlock)
+                a.bias_out[v] = v >= a.vocab ? -INFINITY : (a.bias ? load_any(a.bias, a.bias_dtype, v) : 0.f);
+        return;
+    }
+    const LayoutJob job = a.job[blockIdx.y];
+    if (!job.src) return;
+    const T* src = static_cast<const T*>(job.src);
+    E* dst = static_cast<E*>(job.dst);
+    const int per = (int)(a.ld / 8);
+    const int64_t n = job.rows * per, part = job.rows * a.ld;
     for (int64_t q = (int64_t)blockIdx.x * kBlock + threadIdx.x; q < n; q += (int64_t)gridDim.x * kBlock) {
-        const int64_t r = q / (ld / 8);
-        const int c0 = (int)(q - r * (ld / 8)) * 8;
+        const int64_t r = q / per;
+        const int c0 = (int)(q - r * per) * 8;
         vec_t<E, 8> o[PARTS];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            float v = c0 + i < cols ? (float)src[r * stride + c0 + i] : 0.f;
+            float v = c0 + i < a.cols ? (float)src[r * job.stride + c0 + i] : 0.f;
 #pragma unroll
             for (int p = 0; p < PARTS; ++p) {
                 E e = (E)v;
@@ -255,47 +300,43 @@ __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const T* src, int64_t
             }
         }
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) *reinterpret_cast<vec_t<E, 8>*>(dst + p * part + r * ld + c0) = o[p];
+        for (int p = 0; p < PARTS; ++p) *reinterpret_cast<vec_t<E, 8>*>(dst + p * part + r * a.ld + c0) = o[p];
     }
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------------------
 
-// per-row upstream gradients (or one scalar over the count) -> row records; fp16: S = the power of two that brings max |g| to 2^14
-// ... 2^15 (one workgroup)
+// upstream gradients (per row, or one over the count) -> row records, ignored ones behind the last row up to rows_pad.
+// 16-bit operands (unscale != NULL): every g is divided by the largest |g| and multiplied by `lift`; unscale[1] undoes both
 __global__ __launch_bounds__(1024) void ce_rows_kernel(const float* g, int g_is_row, const float* count, const float* row_max, const float* row_sum,
-                                                       const int64_t* target, int64_t ignore, int vocab, int64_t rows, RowState* state,
-                                                       float* unscale) {
+                                                       const int64_t* target, int64_t ignore, int vocab, int64_t rows, int64_t rows_pad,
+                                                       float lift, RowState* state, float* unscale) {
     __shared__ uint32_t sh[16];
-    float scale = 1.f;
+    const float shared = g_is_row ? 0.f : *g / *count;
+    float top = 1.f;
     if (unscale) {
-        uint32_t top = 0;
+        uint32_t bits = 0;
         if (g_is_row) {
             for (int64_t r = threadIdx.x; r < rows; r += 1024)
-                if (target[r] != ignore) top = max(top, __float_as_uint(g[r]) & 0x7fffffffu);
+                if (target[r] != ignore) bits = max(bits, __float_as_uint(g[r]) & 0x7fffffffu);
         } else {
-            top = __float_as_uint(*g / *count) & 0x7fffffffu;
+            bits = __float_as_uint(shared) & 0x7fffffffu;
         }
 #pragma unroll
-        for (int m = 32; m >= 1; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, kWave));
-        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
+        for (int m = 32; m >= 1; m >>= 1) bits = max(bits, (uint32_t)__shfl_xor((int)bits, m, kWave));
+        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = bits;
         __syncthreads();
-        for (int w = 0; w < 16; ++w) top = max(top, sh[w]);
-        const int e = (int)(top >> 23);                     // biased exponent; zero, subnormal, infinite and NaN gradients: no scaling
-        const int shift = e == 0 || e == 255 ? 0 : min(max(14 - (e - 127), -100), 100);
-        scale = __uint_as_float((uint32_t)(127 + shift) << 23);
-        if (threadIdx.x == 0 && blockIdx.x == 0) {
-            unscale[0] = scale;
-            unscale[1] = __uint_as_float((uint32_t)(127 - shift) << 23);
-        }
+        for (int w = 0; w < 16; ++w) bits = max(bits, sh[w]);
+        // all gradients zero, or an infinite or NaN one among them: as they are
+        if (bits != 0 && bits < 0x7f800000u) top = __uint_as_float(bits);
+        if (threadIdx.x == 0 && blockIdx.x == 0) unscale[1] = top / lift;
     }
-    const float shared = g_is_row ? 0.f : *g / *count;
-    for (int64_t r = (int64_t)blockIdx.x * 1024 + threadIdx.x; r < rows; r += (int64_t)gridDim.x * 1024) {
-        const int64_t t = target[r];
-        const bool in = t != ignore && t >= 0 && t < vocab;
-        const float gr = in ? (g_is_row ? g[r] : shared) * scale : 0.f;
+    for (int64_t r = (int64_t)blockIdx.x * 1024 + threadIdx.x; r < rows_pad; r += (int64_t)gridDim.x * 1024) {
+        const int64_t t = r < rows ? target[r] : -1;
+        const bool in = r < rows && t != ignore && t >= 0 && t < vocab;
+        const float gr = in ? (g_is_row ? g[r] : shared) / top * lift : 0.f;
         RowState s;
-        s.m = in ? row_max[r] : 0.f;
+        s.m = in ? row_max[r] : INFINITY;
         s.scale = in ? gr / row_sum[r] : 0.f;
         s.g = gr;
         s.target = in ? (int)t : -1;
@@ -461,15 +502,15 @@ static int64_t ceil_div(int64_t n, int64_t m) { return (n + m - 1) / m; }
 
 struct CePlan {
     int parts, pairs;
-    bool copy_x, copy_w;
+    bool copy_x, copy_w, narrow;
     int64_t ldh;                    // padded row of a copied operand
-    int64_t x_off, w_off, x_bytes, w_bytes;
+    int64_t x_off, w_off, bias_off;
     // forward
     bool big_lse;
     int splits;
-    int64_t partial_off, logit_off;
+    int64_t partial_off, logit_off, sums_off;
     // backward
-    int64_t rows_pad, piece, d_off, d_bytes, state_off, unscale_off, dx_off, dw_off, db_off;
+    int64_t rows_pad, piece, d_off, state_off, unscale_off, dx_off, dw_off, db_off;
     int dx_split, dw_split;
     bool big_d, big_dx, big_dw;
     int64_t bytes;
@@ -481,6 +522,7 @@ static CePlan ce_plan(int64_t R, int V, int H, int dtype, bool x_ok, bool w_ok, 
     p.pairs = dtype == CNF_DTYPE_F32 ? 6 : 1;
     p.copy_x = p.parts > 1 || !x_ok;
     p.copy_w = p.parts > 1 || !w_ok;
+    p.narrow = narrow_supported(dtype, H);
     p.ldh = round_up(H, 8);
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -488,50 +530,61 @@ static CePlan ce_plan(int64_t R, int V, int H, int dtype, bool x_ok, bool w_ok, 
         at += round_up(bytes, 256);
         return o;
     };
-    if (p.copy_x) p.x_off = take(p.x_bytes = (int64_t)p.parts * R * p.ldh * 2);
-    if (p.copy_w) p.w_off = take(p.w_bytes = (int64_t)p.parts * V * p.ldh * 2);
+    if (p.copy_x) p.x_off = take((int64_t)p.parts * R * p.ldh * 2);
+    if (p.copy_w) p.w_off = take((int64_t)p.parts * V * p.ldh * 2);
+    if (p.narrow) p.bias_off = take(round_up(V, kNarrowWalk) * 4);
+    // about four workgroups for every CU, at least two steps of the walk each
+    auto narrow_split = [](int64_t own, int64_t walk) {
+        return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(1024, ceil_div(own, kNarrowOwn)), ceil_div(walk, 2 * kNarrowWalk)));
+    };
+    const int64_t ld4 = round_up(H, 4);
     if (!backward) {
         // 256 x 256 tiles once they fill the chip; the vocabulary is split until there are two workgroups per CU (one of the big)
         p.big_lse = ceil_div(R, kBig) * ceil_div(V, kBig) >= 512;
         const int edge = p.big_lse ? kBig : kSmall;
         const int64_t rt = ceil_div(R, edge), vt = ceil_div(V, edge);
-        p.splits = (int)std::min<int64_t>(vt, std::max<int64_t>(1, (p.big_lse ? 256 : 512) / rt));
+        p.splits = p.narrow ? narrow_split(R, V) : (int)std::min<int64_t>(vt, std::max<int64_t>(1, (p.big_lse ? 256 : 512) / rt));
         p.partial_off = take((int64_t)p.splits * R * 8);
         p.logit_off = take(R * 4);
-    } else {
-        p.rows_pad = round_up(R, kBig);
-        const int64_t row_bytes = p.rows_pad * 2 * p.parts;
-        p.piece = std::min<int64_t>(round_up(V, kBig), std::max<int64_t>(kBig, kPieceBytes / row_bytes / kBig * kBig));
-        p.d_off = take(p.d_bytes = row_bytes * p.piece);
-        p.state_off = take(R * (int64_t)sizeof(RowState));
-        p.unscale_off = take(8);
-        const int64_t width = std::min<int64_t>(p.piece, V);
-        p.big_d = ceil_div(R, kBig) * ceil_div(width, kBig) >= 256;
-        // dx [R][H] over k = the piece; dw [piece][H] over k = R: k is split where the tiles alone do not fill the chip
-        auto split = [&](int64_t n, int64_t k, bool& big) {
-            big = ceil_div(n, kBig) * ceil_div(H, kBig) >= 128 && H > kSmall;
-            const int edge = big ? kBig : kSmall;
-            const int64_t tiles = ceil_div(n, edge) * ceil_div(H, edge), steps = ceil_div(k, kStepK);
-            return (int)std::max<int64_t>(1, std::min<int64_t>({steps / 4, ceil_div(big ? 256 : 512, tiles), 64}));
-        };
-        p.dx_split = split(R, width, p.big_dx);
-        p.dw_split = split(width, R, p.big_dw);
-        const int64_t ld4 = round_up(H, 4);
-        if (p.dx_split > 1 || p.piece < V) p.dx_off = take((int64_t)p.dx_split * R * ld4 * 4);
+        p.sums_off = take(ceil_div(R, kBlock) * 16);
+        p.bytes = at;
+        return p;
+    }
+    p.rows_pad = round_up(R, kBig);
+    p.state_off = take(p.rows_pad * (int64_t)sizeof(RowState));
+    p.unscale_off = take(8);
+    if (p.narrow) {
+        p.dx_split = narrow_split(R, V);
+        p.dw_split = narrow_split(V, R);
+        if (p.dx_split > 1) p.dx_off = take((int64_t)p.dx_split * R * ld4 * 4);
         if (p.dw_split > 1) {
-            p.dw_off = take((int64_t)p.dw_split * width * ld4 * 4);
-            p.db_off = take((int64_t)p.dw_split * width * 4);
+            p.dw_off = take((int64_t)p.dw_split * V * ld4 * 4);
+            p.db_off = take((int64_t)p.dw_split * V * 4);
         }
+        p.bytes = at;
+        return p;
+    }
+    const int64_t row_bytes = p.rows_pad * 2 * p.parts;
+    p.piece = std::min<int64_t>(round_up(V, kBig), std::max<int64_t>(kBig, kPieceBytes / row_bytes / kBig * kBig));
+    p.d_off = take(row_bytes * p.piece);
+    const int64_t width = std::min<int64_t>(p.piece, V);
+    p.big_d = ceil_div(R, kBig) * ceil_div(width, kBig) >= 256;
+    // dx [R][H] over k = the piece; dw [piece][H] over k = R: k is split where the tiles alone do not fill the chip
+    auto split = [&](int64_t n, int64_t k, bool& big) {
+        big = ceil_div(n, kBig) * ceil_div(H, kBig) >= 128 && H > kSmall;
+        const int edge = big ? kBig : kSmall;
+        const int64_t tiles = ceil_div(n, edge) * ceil_div(H, edge), steps = ceil_div(k, kStepK);
+        return (int)std::max<int64_t>(1, std::min<int64_t>({steps / 4, ceil_div(big ? 256 : 512, tiles), 64}));
+    };
+    p.dx_split = split(R, width, p.big_dx);
+    p.dw_split = split(width, R, p.big_dw);
+    if (p.dx_split > 1 || p.piece < V) p.dx_off = take((int64_t)p.dx_split * R * ld4 * 4);
+    if (p.dw_split > 1) {
+        p.dw_off = take((int64_t)p.dw_split * width * ld4 * 4);
+        p.db_off = take((int64_t)p.dw_split * width * 4);
     }
     p.bytes = at;
     return p;
-}
-
-template <typename T, typename E, int PARTS>
-static void ce_layout(const void* src, int64_t stride, int64_t rows, int cols, void* dst, int64_t ld, hipStream_t st) {
-    const int64_t n = rows * (ld / 8);
-    CNF_LAUNCH((ce_layout_kernel<T, E, PARTS>), dim3((unsigned)std::min<int64_t>(ceil_div(n, kBlock), 8192)), dim3(kBlock), 0, st,
-               static_cast<const T*>(src), stride, rows, cols, static_cast<E*>(dst), ld, rows * ld);
 }
 
 // calls fn(T{}, E{}, parts): the tensors' type, the products' operand type, the parts of an operand
@@ -543,10 +596,25 @@ static int ce_types(int dtype, Fn&& fn) {
 }
 
 template <typename T, typename E, int PARTS>
-static void ce_operands(CeArgs& a, const CePlan& p, const void* x, int64_t x_stride, const void* w, int64_t w_stride, int64_t R, int V, int H,
-                        char* ws, hipStream_t st) {
-    if (p.copy_x) ce_layout<T, E, PARTS>(x, x_stride, R, H, ws + p.x_off, p.ldh, st);
-    if (p.copy_w) ce_layout<T, E, PARTS>(w, w_stride, V, H, ws + p.w_off, p.ldh, st);
+static void ce_operands(CeArgs& a, const CePlan& p, const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias,
+                        int bias_dtype, int64_t R, int V, int H, char* ws, hipStream_t st) {
+    LayoutArgs l{};
+    if (p.copy_x) l.job[0] = LayoutJob{x, x_stride, R, ws + p.x_off};
+    if (p.copy_w) l.job[1] = LayoutJob{w, w_stride, V, ws + p.w_off};
+    l.cols = H;
+    l.ld = p.ldh;
+    if (p.narrow) {
+        l.bias = bias;
+        l.bias_dtype = bias_dtype;
+        l.vocab = V;
+        l.bias_pad = (int)round_up(V, kNarrowWalk);
+        l.bias_out = reinterpret_cast<float*>(ws + p.bias_off);
+    }
+    if (p.copy_x || p.copy_w || p.narrow) {
+        const int64_t chunks = std::max(p.copy_x ? R * (p.ldh / 8) : 0, p.copy_w ? V * (p.ldh / 8) : 0);
+        const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(std::max<int64_t>(chunks, l.bias_pad), kBlock), 4096));
+        CNF_LAUNCH((ce_layout_kernel<T, E, PARTS>), dim3(grid, 3), dim3(kBlock), 0, st, l);
+    }
     a.x = p.copy_x ? Operand{ws + p.x_off, p.ldh, R * p.ldh, (int)R} : Operand{x, x_stride, 0, (int)R};
     a.w = p.copy_w ? Operand{ws + p.w_off, p.ldh, V * p.ldh, V} : Operand{w, w_stride, 0, V};
     a.pairs = p.pairs;
@@ -554,6 +622,30 @@ static void ce_operands(CeArgs& a, const CePlan& p, const void* x, int64_t x_str
     a.rows = R;
     a.vocab = V;
     a.hidden = H;
+    a.bias = bias;
+    a.bias_dtype = bias_dtype;
+}
+
+static NarrowArgs narrow_args(const CeArgs& a, const CePlan& p, bool rows_own, char* ws) {
+    NarrowArgs n{};
+    n.own = rows_own ? a.x : a.w;
+    n.walk = rows_own ? a.w : a.x;
+    n.hidden = a.hidden;
+    n.vocab = a.vocab;
+    n.rows = a.rows;
+    n.bias = reinterpret_cast<const float*>(ws + p.bias_off);
+    n.target = a.target;
+    n.ignore = a.ignore;
+    n.partial = a.partial;
+    n.target_logit = a.target_logit;
+    n.splits = a.splits;
+    n.state = a.state;
+    return n;
+}
+
+static void ce_sum(const void* partial, int parts, int64_t rows, int cols, int64_t ld, const float* unscale, void* out, int dtype, hipStream_t st) {
+    CNF_LAUNCH(ce_sum_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(rows * cols, kBlock), 8192)), dim3(kBlock), 0, st,
+               static_cast<const float*>(partial), parts, rows, cols, ld, unscale, out, dtype);
 }
 
 static bool ce_aligned(const void* p, int64_t stride, int dtype, int H) { return rows_aligned16(p, stride, dtype) && H % 8 == 0; }
@@ -591,27 +683,30 @@ int cnf_linear_ce(const void* x, int64_t x_stride, const void* weight, int64_t w
             typedef decltype(t) T;
             typedef decltype(e) E;
             CeArgs a{};
-            ce_operands<T, E, decltype(parts)::value>(a, p, x, x_stride, weight, w_stride, R, V, H, ws, st);
-            a.bias = bias;
-            a.bias_dtype = bias_dtype;
+            ce_operands<T, E, decltype(parts)::value>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, R, V, H, ws, st);
             a.target = target;
             a.ignore = ignore_index;
             a.partial = reinterpret_cast<float2*>(ws + p.partial_off);
             a.target_logit = reinterpret_cast<float*>(ws + p.logit_off);
             a.splits = p.splits;
-            if (p.big_lse)
+            if (p.narrow) {
+                const int rc = narrow_launch(kNarrowLse, dtype, narrow_args(a, p, true, ws), st);
+                if (rc != CNF_OK) return rc;
+            } else if (p.big_lse)
                 CNF_LAUNCH((ce_lse_kernel<E, kBig, kBig, 2, 4>), dim3((unsigned)(ceil_div(R, kBig) * p.splits)), dim3(512), 0, st, a);
             else
                 CNF_LAUNCH((ce_lse_kernel<E, kSmall, kSmall, 2, 2>), dim3((unsigned)(ceil_div(R, kSmall) * p.splits)), dim3(256), 0, st, a);
-            CNF_LAUNCH(ce_join_kernel, dim3((unsigned)ceil_div(R, kBlock)), dim3(kBlock), 0, st, a.partial, a.target_logit, target, ignore_index, V,
-                       p.splits, R, row_max, row_sum, loss, flags);
+            double* sums = reinterpret_cast<double*>(ws + p.sums_off);
+            const int64_t blocks = ceil_div(R, kBlock);
+            CNF_LAUNCH(ce_join_kernel, dim3((unsigned)blocks), dim3(kBlock), 0, st, a.partial, a.target_logit, target, ignore_index, V,
+                       p.splits, R, row_max, row_sum, loss, sums, reduced, flags);
+            if (reduced && blocks > 1) CNF_LAUNCH(ce_reduce_kernel, dim3(1), dim3(1024), 0, st, sums, blocks, reduced);
             return launch_status("cnf_linear_ce");
         });
         if (rc != CNF_OK) return rc;
-    }
-    if (reduced) {
-        CNF_LAUNCH(ce_reduce_kernel, dim3(1), dim3(1024), 0, st, loss, target, ignore_index, R, reduced);
-        return launch_status("cnf_linear_ce (reduction)");
+    } else if (reduced) {
+        CNF_LAUNCH(ce_reduce_kernel, dim3(1), dim3(1024), 0, st, nullptr, (int64_t)0, reduced);
+        return launch_status("cnf_linear_ce (no rows)");
     }
     return CNF_OK;
 }
@@ -634,19 +729,48 @@ int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64
         typedef decltype(e) E;
         constexpr int PARTS = decltype(parts)::value;
         CeArgs a{};
-        ce_operands<T, E, PARTS>(a, p, x, x_stride, weight, w_stride, R, V, H, ws, st);
-        a.bias = bias;
-        a.bias_dtype = bias_dtype;
+        ce_operands<T, E, PARTS>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, R, V, H, ws, st);
         RowState* state = reinterpret_cast<RowState*>(ws + p.state_off);
-        float* unscale = dtype == CNF_DTYPE_F16 ? reinterpret_cast<float*>(ws + p.unscale_off) : nullptr;
+        float* unscale = dtype == CNF_DTYPE_F32 ? nullptr : reinterpret_cast<float*>(ws + p.unscale_off);
         a.state = state;
-        // fp16: every workgroup finds the largest |g| itself; few of them
-        CNF_LAUNCH(ce_rows_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(R, 1024), unscale && g_per_row ? 16 : 1024)), dim3(1024), 0, st, g,
-                   g_per_row, count, row_max, row_sum, target, ignore_index, V, R, state, unscale);
+        // 16-bit, per-row gradients: every workgroup finds the largest |g| itself; few of them
+        CNF_LAUNCH(ce_rows_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(p.rows_pad, 1024), unscale && g_per_row ? 16 : 1024)), dim3(1024), 0,
+                   st, g, g_per_row, count, row_max, row_sum, target, ignore_index, V, R, p.rows_pad, dtype == CNF_DTYPE_F16 ? 16384.f : 1.f,
+                   state, unscale);
+        const int64_t ld4 = round_up(H, 4);
+        if (p.narrow) {
+            if (dx) {
+                NarrowArgs n = narrow_args(a, p, true, ws);
+                n.splits = p.dx_split;
+                n.final_dtype = n.splits > 1 ? -1 : dtype;
+                n.out = n.splits > 1 ? static_cast<void*>(ws + p.dx_off) : dx;
+                n.ld = n.splits > 1 ? ld4 : H;
+                n.unscale = unscale;
+                const int rc = narrow_launch(kNarrowDx, dtype, n, st);
+                if (rc != CNF_OK) return rc;
+                if (n.splits > 1) ce_sum(n.out, n.splits, R, H, ld4, unscale, dx, dtype, st);
+            }
+            if (dweight) {
+                NarrowArgs n = narrow_args(a, p, false, ws);
+                n.splits = p.dw_split;
+                n.final_dtype = n.splits > 1 ? -1 : dtype;
+                n.out = n.splits > 1 ? static_cast<void*>(ws + p.dw_off) : dweight;
+                n.ld = n.splits > 1 ? ld4 : H;
+                n.unscale = unscale;
+                n.db = dbias ? (n.splits > 1 ? static_cast<void*>(ws + p.db_off) : dbias) : nullptr;
+                n.db_dtype = bias_dtype;
+                const int rc = narrow_launch(kNarrowDw, dtype, n, st);
+                if (rc != CNF_OK) return rc;
+                if (n.splits > 1) {
+                    ce_sum(n.out, n.splits, V, H, ld4, unscale, dweight, dtype, st);
+                    if (dbias) ce_sum(n.db, n.splits, 1, V, V, unscale, dbias, bias_dtype, st);
+                }
+            }
+            return launch_status("cnf_linear_ce_bwd");
+        }
         a.d = ws + p.d_off;
         a.d_ld = p.piece;
         a.d_part = p.rows_pad * p.piece;
-        const int64_t ld4 = round_up(H, 4);
         const bool dx_partial = p.dx_split > 1 || p.piece < V, dw_partial = p.dw_split > 1;
         for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
             const int64_t v1 = std::min<int64_t>(V, v0 + p.piece), width = v1 - v0;
@@ -701,16 +825,11 @@ int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64
             q.db_dtype = bias_dtype;
             grad(true, p.big_dw, width);
             if (dw_partial) {
-                CNF_LAUNCH(ce_sum_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(width * H, kBlock), 4096)), dim3(kBlock), 0, st,
-                           reinterpret_cast<const float*>(ws + p.dw_off), p.dw_split, width, H, ld4, unscale, dw, dtype);
-                if (db)
-                    CNF_LAUNCH(ce_sum_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(width, kBlock), 4096)), dim3(kBlock), 0, st,
-                               reinterpret_cast<const float*>(ws + p.db_off), p.dw_split, (int64_t)1, (int)width, width, unscale, db, bias_dtype);
+                ce_sum(ws + p.dw_off, p.dw_split, width, H, ld4, unscale, dw, dtype, st);
+                if (db) ce_sum(ws + p.db_off, p.dw_split, 1, (int)width, width, unscale, db, bias_dtype, st);
             }
         }
-        if (dx && dx_partial)
-            CNF_LAUNCH(ce_sum_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(R * H, kBlock), 8192)), dim3(kBlock), 0, st,
-                       reinterpret_cast<const float*>(ws + p.dx_off), p.dx_split, R, H, ld4, unscale, dx, dtype);
+        if (dx && dx_partial) ce_sum(ws + p.dx_off, p.dx_split, R, H, ld4, unscale, dx, dtype, st);
         return launch_status("cnf_linear_ce_bwd");
     });
 }

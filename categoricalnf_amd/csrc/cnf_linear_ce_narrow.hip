@@ -1,0 +1,351 @@
+// Linear cross entropy of few features: forward, gradient of the rows, gradient of the weights (formulas: cnf_linear_ce.hip).
+//
+// A workgroup of four waves keeps 128 rows (for dw: 128 vocabulary entries) as matrix-core operands in registers, 32 a wave, and walks
+// through its part of the other side in steps of 64, copied into LDS one step ahead.  Per step and wave:
+//   S = walk . own^T, starting from the bias            (six bf16 products for fp32 operands, one for 16-bit ones)
+//   forward:  running maximum and sum per lane;  backward:  d from S in place, and  out^T += walk^T . d
+// S has four consecutive walk entries of one own entry per lane (fragment layout in cnf_mfma.h); two 16-row tiles of it are exactly
+// the eight k of a lane in the second product, whose other operand is the transposed LDS read of the same tile: d never moves
+// between lanes.  For fp32 d is split into three bf16 parts there.
+//
+// Bound by the matrix cores and the vector work beside them (exponentials, splitting): 5 products of 2 R V H operations against the
+// 3 of the definition — the logits are computed three times — but nothing of size R x V is written or read.
+#include <algorithm>
+
+#include "cnf_linear_ce_narrow.h"
+
+namespace cnf {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// LDS tile: [PARTS][64][HP] 16-bit elements; 16-byte chunk c of row r at c ^ f(r): row reads (16 rows, one chunk each) and transposing
+// reads (16 rows, 32 bytes each) both touch every bank equally often
+template <int HP>
+__device__ __forceinline__ int narrow_swizzle(int row) {
+    return HP == 32 ? (row >> 2) & 3 : (HP == 64 ? row & 7 : row & 15);
+}
+
+template <int HP, int PARTS>
+struct NarrowTile {
+    static constexpr int kChunks = HP / 8;
+    static constexpr int kPart = kNarrowWalk * HP * 2;              // bytes
+    static constexpr int kBytes = PARTS * kPart;
+    static constexpr int kCopies = PARTS * kNarrowWalk * kChunks / kBlock;
+
+    __device__ static void copy(const Operand& o, int64_t m0, int hidden, char* lds) {
+        const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const uint16_t* base = static_cast<const uint16_t*>(o.base);
+#pragma unroll
+        for (int j = 0; j < kCopies; ++j) {
+            const int q = j * kBlock + tid;
+            const int part = j * kBlock / (kNarrowWalk * kChunks);
+            const int row = (q / kChunks) % kNarrowWalk, c = (q % kChunks) ^ narrow_swizzle<HP>(row);
+            const int64_t e = m0 + row;
+            const void* src = (e < o.ext && c * 8 < hidden) ? static_cast<const void*>(base + (int64_t)part * o.part + e * o.ld + c * 8)
+                                                            : static_cast<const void*>(kZeroChunk);
+            __builtin_amdgcn_global_load_lds((glb_cvoid_t*)src, (lds_void16_t*)(lds + (j * kBlock + wave * 64) * 16), 16, 0, 0);
+        }
+    }
+    // rows row0 ... row0 + 15, k = 32 kk ...
+    __device__ static s16x8 frag(const char* lds, int part, int row0, int kk) {
+        const int l = threadIdx.x & 63, row = row0 + (l & 15), c = kk * 4 + (l >> 4);
+        return *reinterpret_cast<const s16x8*>(lds + part * kPart + row * (HP * 2) + ((c ^ narrow_swizzle<HP>(row)) << 4));
+    }
+    // transposed: columns 16 h ... for h = h0, h0 + 1, k = the 32 rows from row0: lane group g holds rows 4 g ... + 3 and 16 + 4 g ... + 3
+    __device__ static void frag_t2(const char* lds, int part, int row0, int h0, s16x8 (&out)[2]) {
+        const int l = threadIdx.x & 63, g = l >> 4, i = l & 15, row = row0 + g * 4 + (i >> 2);
+        uint32_t at[2][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int r = row + k * 16, c = (h0 + h) * 2 + ((i & 3) >> 1);
+                at[h][k] = (uint32_t)(uintptr_t)(lds_void16_t*)lds + part * kPart + r * (HP * 2) + ((c ^ narrow_swizzle<HP>(r)) << 4) + (i & 1) * 8;
+            }
+        // in assembly, waited for in the same block, like the transposing reads of cnf_mfma.h
+        s16x4 v[2][2];
+        asm volatile(
+            "ds_read_b64_tr_b16 %0, %4\n\t"
+            "ds_read_b64_tr_b16 %1, %5\n\t"
+            "ds_read_b64_tr_b16 %2, %6\n\t"
+            "ds_read_b64_tr_b16 %3, %7\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1])
+            : "v"(at[0][0]), "v"(at[0][1]), "v"(at[1][0]), "v"(at[1][1])
+            : "memory");
+#pragma unroll
+        for (int h = 0; h < 2; ++h) out[h] = __builtin_shufflevector(v[h][0], v[h][1], 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
+
+template <typename E, int PARTS, int HP, NarrowJob JOB>
+__global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a) {
+    typedef NarrowTile<HP, PARTS> Tile;
+    constexpr int NT = 2, KK = HP / 32, HT = HP / 16;
+    constexpr int kAux = JOB == kNarrowDw ? kNarrowWalk * 16 : kNarrowWalk * 4;       // row records, or biases
+    constexpr int kStage = Tile::kBytes + kAux;
+    __shared__ __align__(16) char lds[2 * kStage];
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int split = blockIdx.x % a.splits;
+    const int64_t own_n = JOB == kNarrowDw ? a.vocab : a.rows, walk_n = JOB == kNarrowDw ? a.rows : a.vocab;
+    const int64_t n_wave = (int64_t)(blockIdx.x / a.splits) * kNarrowOwn + wave * (NT * 16);
+    const int64_t tiles = (walk_n + kNarrowWalk - 1) / kNarrowWalk;
+    const int64_t first = tiles * split / a.splits, last = tiles * (split + 1) / a.splits;
+
+    auto copy = [&](int64_t tile, int stage) {
+        char* s = lds + stage * kStage;
+        Tile::copy(a.walk, tile * kNarrowWalk, a.hidden, s);
+        // every wave copies the step's records (the same bytes to the same place): all waves have the same number of copies in flight
+        if (JOB == kNarrowDw)
+            __builtin_amdgcn_global_load_lds((glb_cvoid_t*)(a.state + tile * kNarrowWalk + lane), (lds_void16_t*)(s + Tile::kBytes), 16, 0, 0);
+        else
+            __builtin_amdgcn_global_load_lds((glb_cvoid_t*)(a.bias + tile * kNarrowWalk + lane), (lds_void16_t*)(s + Tile::kBytes), 4, 0, 0);
+    };
+    if (first < last) copy(first, 0);
+
+    // this lane's own entries
+    RowState st[NT];
+    float bias_n[NT];
+    int want[NT];
+    s16x8 own[PARTS][KK][NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int64_t e = n_wave + n * 16 + col;
+        bool in = e < own_n;
+        st[n] = RowState{INFINITY, 0.f, 0.f, -1};
+        bias_n[n] = 0.f;
+        want[n] = -1;
+        if (JOB == kNarrowLse) {
+            const int64_t t = in ? a.target[e] : -1;
+            want[n] = t >= 0 && t < a.vocab && t != a.ignore ? (int)t : -1;
+        } else if (JOB == kNarrowDx) {
+            if (in) st[n] = a.state[e];
+            in = in && st[n].target >= 0;               // an ignored row: operand 0, maximum +inf, so that d = 0 whatever the row holds
+        } else {
+            bias_n[n] = in ? a.bias[e] : -INFINITY;     // d = 0
+        }
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) {
+                const int k = kk * 32 + g * 8;
+                s16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+                own[p][kk][n] = in && k < a.hidden ? *reinterpret_cast<const s16x8*>(static_cast<const uint16_t*>(a.own.base) +
+                                                                                       (int64_t)p * a.own.part + e * a.own.ld + k)
+                                                   : z;
+            }
+    }
+    float mx[NT], sum[NT];
+    f32x4 acc[HT][NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        mx[n] = -INFINITY;
+        sum[n] = 0.f;
+#pragma unroll
+        for (int h = 0; h < HT; ++h) acc[h][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    int stage = 0;
+    for (int64_t tile = first; tile < last; ++tile, stage ^= 1) {
+        if (tile + 1 < last) {
+            copy(tile + 1, stage ^ 1);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Tile::kCopies + 1) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const char* s = lds + stage * kStage;
+        const int64_t m_tile = tile * kNarrowWalk;
+#pragma unroll
+        for (int mp = 0; mp < 2; ++mp) {
+            f32x4 sc[2][NT];
+            RowState row[2][4];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if (JOB == kNarrowDw) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        row[t][i] = reinterpret_cast<const RowState*>(s + Tile::kBytes)[mp * 32 + t * 16 + g * 4 + i];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) sc[t][n] = f32x4{bias_n[n], bias_n[n], bias_n[n], bias_n[n]};
+                } else {
+                    const f32x4 b = *reinterpret_cast<const f32x4*>(s + Tile::kBytes + (mp * 32 + t * 16 + g * 4) * 4);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) sc[t][n] = b;
+                }
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) {
+                    s16x8 f[PARTS];
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) f[p] = Tile::frag(s, p, mp * 32 + t * 16, kk);
+#pragma unroll
+                    for (int order = PARTS - 1; order >= 0; --order)          // smallest products first
+#pragma unroll
+                        for (int p = 0; p <= order; ++p)
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) sc[t][n] = mfma16<E>(f[p], own[order - p][kk][n], sc[t][n]);
+                }
+            }
+            const int64_t m0 = m_tile + mp * 32 + g * 4;            // the lane's first walk entry: 16 t + i further
+            if (JOB == kNarrowLse) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const int64_t at = want[n] - m0;
+                    if (want[n] >= 0 && at >= 0 && at < 32 && (at & 15) < 4) {
+#pragma unroll
+                        for (int t = 0; t < 2; ++t)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (at == t * 16 + i) a.target_logit[n_wave + n * 16 + col] = sc[t][n][i];
+                    }
+                    float top = mx[n];
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[t][n][i]);
+                    const float ref = top == -INFINITY ? 0.f : top;
+                    float q = sum[n] * __builtin_amdgcn_exp2f((mx[n] - ref) * kLog2e);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) q += __builtin_amdgcn_exp2f((sc[t][n][i] - ref) * kLog2e);
+                    sum[n] = q;
+                    mx[n] = top;
+                }
+                continue;
+            }
+            // d, split into its parts: the second product's operand
+            s16x8 d[PARTS][NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float m = JOB == kNarrowDw ? row[e / 4][e % 4].m : st[n].m;
+                    const float f = JOB == kNarrowDw ? row[e / 4][e % 4].scale : st[n].scale;
+                    v[e] = __builtin_amdgcn_exp2f((sc[e / 4][n][e % 4] - m) * kLog2e) * f;
+                }
+                if (JOB == kNarrowDx) {
+                    const int64_t at = st[n].target - m0;
+                    if (__ballot(st[n].target >= 0 && at >= 0 && at < 32)) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (at == (e / 4) * 16 + e % 4) v[e] -= st[n].g;
+                    }
+                } else {
+                    const int e0 = (int)(n_wave + n * 16 + col);
+                    bool hit = false;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) hit |= row[e / 4][e % 4].target == e0;
+                    if (__ballot(hit)) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (row[e / 4][e % 4].target == e0) v[e] -= row[e / 4][e % 4].g;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sum[n] += v[e];
+                }
+                vec_t<E, 8> o[PARTS];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) {
+                        o[p][e] = (E)v[e];
+                        v[e] = PARTS > 1 ? v[e] - (float)o[p][e] : 0.f;
+                    }
+                }
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) d[p][n] = __builtin_bit_cast(s16x8, o[p]);
+            }
+#pragma unroll
+            for (int h = 0; h < HT; h += 2)
+#pragma unroll
+                for (int p = PARTS - 1; p >= 0; --p) {
+                    s16x8 f[2];
+                    Tile::frag_t2(s, p, mp * 32, h, f);
+#pragma unroll
+                    for (int b = PARTS - 1 - p; b >= 0; --b)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) acc[h + i][n] = mfma16<E>(f[i], d[b][n], acc[h + i][n]);
+                }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // this wave has read the stage ...
+        __builtin_amdgcn_s_barrier();                               // ... and the others: the next copy may overwrite it
+        asm volatile("" ::: "memory");
+    }
+
+    if (JOB == kNarrowLse) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float m = mx[n], q = sum[n];
+#pragma unroll
+            for (int x = 16; x <= 32; x <<= 1) {
+                const float om = __shfl_xor(m, x, kWave), oq = __shfl_xor(q, x, kWave);
+                const float nm = fmaxf(m, om), ref = nm == -INFINITY ? 0.f : nm;
+                q = q * __builtin_amdgcn_exp2f((m - ref) * kLog2e) + oq * __builtin_amdgcn_exp2f((om - ref) * kLog2e);
+                m = nm;
+            }
+            const int64_t r = n_wave + n * 16 + col;
+            if (g == 0 && r < a.rows) a.partial[(int64_t)split * a.rows + r] = make_float2(m, q);
+        }
+        return;
+    }
+    const float unscale = a.final_dtype >= 0 && a.unscale ? a.unscale[1] : 1.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int64_t e = n_wave + n * 16 + col;
+        float b = sum[n];
+        if (JOB == kNarrowDw) {
+#pragma unroll
+            for (int x = 16; x <= 32; x <<= 1) b += __shfl_xor(b, x, kWave);
+        }
+        if (e >= own_n) continue;
+        if (JOB == kNarrowDw && a.db && g == 0) {
+            if (a.final_dtype >= 0) store_any(a.db, a.db_dtype, e, b * unscale);
+            else static_cast<float*>(a.db)[(int64_t)split * own_n + e] = b;
+        }
+#pragma unroll
+        for (int h = 0; h < HT; ++h) {
+            const int k = h * 16 + g * 4;
+            if (k >= a.hidden) continue;
+            if (a.final_dtype < 0) {
+                *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + ((int64_t)split * own_n + e) * a.ld + k) = acc[h][n];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (k + i < a.hidden) store_any(a.out, a.final_dtype, e * a.ld + k + i, acc[h][n][i] * unscale);
+            }
+        }
+    }
+}
+
+template <typename E, int PARTS, int HP>
+static void narrow_job(NarrowJob job, const NarrowArgs& a, hipStream_t st) {
+    const int64_t own_n = job == kNarrowDw ? a.vocab : a.rows;
+    const dim3 grid((unsigned)((own_n + kNarrowOwn - 1) / kNarrowOwn * a.splits));
+    if (job == kNarrowLse) CNF_LAUNCH((ce_narrow_kernel<E, PARTS, HP, kNarrowLse>), grid, dim3(kBlock), 0, st, a);
+    else if (job == kNarrowDx) CNF_LAUNCH((ce_narrow_kernel<E, PARTS, HP, kNarrowDx>), grid, dim3(kBlock), 0, st, a);
+    else CNF_LAUNCH((ce_narrow_kernel<E, PARTS, HP, kNarrowDw>), grid, dim3(kBlock), 0, st, a);
+}
+
+template <typename E, int PARTS>
+static void narrow_width(NarrowJob job, const NarrowArgs& a, hipStream_t st) {
+    if (a.hidden <= 32) narrow_job<E, PARTS, 32>(job, a, st);
+    else if (PARTS > 1 || a.hidden <= 64) narrow_job<E, PARTS, 64>(job, a, st);
+    else if constexpr (PARTS == 1) narrow_job<E, PARTS, 128>(job, a, st);
+}
+
+// three parts of 128 features would take more registers than a lane has
+bool narrow_supported(int dtype, int hidden) { return hidden <= (dtype == CNF_DTYPE_F32 ? 64 : 128); }
+
+int narrow_launch(NarrowJob job, int dtype, const NarrowArgs& a, hipStream_t st) {
+    if (dtype == CNF_DTYPE_F32) narrow_width<bf16_t, 3>(job, a, st);
+    else if (dtype == CNF_DTYPE_BF16) narrow_width<bf16_t, 1>(job, a, st);
+    else narrow_width<f16_t, 1>(job, a, st);
+    return launch_status("cnf_linear_ce (few features)");
+}
+
+}  // namespace cnf
