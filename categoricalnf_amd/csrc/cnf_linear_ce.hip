@@ -22,8 +22,6 @@
 
 namespace cnf {
 
-constexpr float kLog2e = 1.4426950408889634f;
-
 struct CeArgs {
     Operand w, x;                   // [V][H], [R][H]
     int pairs, parts;
@@ -258,7 +256,7 @@ struct LayoutJob {
 };
 struct LayoutArgs {
     LayoutJob job[2];               // x and w: [rows][cols] -> `parts` arrays of [rows][ld] 16-bit elements, zeros behind cols
-    int cols;
+    int cols, vec;                  // vec: bit j: 8 elements of job j's rows may be read as vectors of 16 bytes
     int64_t ld;
     const void* bias;               // -> fp32, -inf behind the vocabulary (nullable: zeros)
     int bias_dtype, vocab, bias_pad;
@@ -284,10 +282,17 @@ __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
     for (int64_t q = (int64_t)blockIdx.x * kBlock + threadIdx.x; q < n; q += (int64_t)gridDim.x * kBlock) {
         const int64_t r = q / per;
         const int c0 = (int)(q - r * per) * 8;
+        vec_t<T, 8> in;
+        if ((a.vec >> blockIdx.y) & 1) {
+            in = *reinterpret_cast<const vec_t<T, 8>*>(src + r * job.stride + c0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) in[i] = c0 + i < a.cols ? src[r * job.stride + c0 + i] : (T)0.f;
+        }
         vec_t<E, 8> o[PARTS];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            float v = c0 + i < a.cols ? (float)src[r * job.stride + c0 + i] : 0.f;
+            float v = (float)in[i];
 #pragma unroll
             for (int p = 0; p < PARTS; ++p) {
                 E e = (E)v;
@@ -336,8 +341,10 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(const float* g, int g_is_
         const bool in = r < rows && t != ignore && t >= 0 && t < vocab;
         const float gr = in ? (g_is_row ? g[r] : shared) / top * lift : 0.f;
         RowState s;
-        s.m = in ? row_max[r] : INFINITY;
-        s.scale = in ? gr / row_sum[r] : 0.f;
+        // exp(l - m) = exp2(l L - m2) exp2(m2 - m L), L = log2 e, m2 = m L rounded: one fma per element, the row's rest in its scale
+        const float m2 = in ? row_max[r] * kLog2e : INFINITY;
+        s.m2 = m2;
+        s.scale = in ? gr / row_sum[r] * __builtin_amdgcn_exp2f(-__builtin_fmaf(row_max[r], kLog2e, -m2)) : 0.f;
         s.g = gr;
         s.target = in ? (int)t : -1;
         state[r] = s;
@@ -366,30 +373,52 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
 #pragma unroll
     for (int n = 0; n < Tile::NT; ++n) {
         const int64_t r = (int64_t)r0 + tile.n_wave + n * 16 + col;
-        st[n] = r < a.rows ? a.state[r] : RowState{0.f, 0.f, 0.f, -1};
+        st[n] = r < a.rows ? a.state[r] : RowState{INFINITY, 0.f, 0.f, -1};
     }
     E* d = static_cast<E*>(a.d);
+    // targets among the wave's entries are rare: their -g is applied behind a branch that most waves do not take
+    int at[Tile::NT];
+    bool hit = false;
+#pragma unroll
+    for (int n = 0; n < Tile::NT; ++n) {
+        at[n] = st[n].target - vw;
+        hit |= st[n].target >= 0 && at[n] >= 0 && at[n] < Tile::MT * 16;
+    }
+    const bool any_hit = __ballot(hit) != 0, edge = v0 + BM > a.v1;
 #pragma unroll
     for (int m = 0; m < Tile::MT; ++m) {
         const int v = vw + m * 16;
-        f32x4 b;
+        f32x4 b = {0.f, 0.f, 0.f, 0.f};
+        if (a.bias) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) b[i] = bias_at(a, v + i);
+            for (int i = 0; i < 4; ++i) b[i] = bias_at(a, v + i);
+        }
 #pragma unroll
         for (int n = 0; n < Tile::NT; ++n) {
             const int64_t r = (int64_t)r0 + tile.n_wave + n * 16 + col;
+            f32x4 p;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[m][n][i] + b[i], kLog2e, -st[n].m2)) * st[n].scale;
+            if (any_hit) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (at[n] == m * 16 + i && st[n].target >= 0) p[i] -= st[n].g;
+            }
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (v + i >= a.v1) p[i] = 0.f;
+            }
+            // an ignored row, or one that is not there (x may hold anything)
+            if (st[n].target < 0) p = f32x4{0.f, 0.f, 0.f, 0.f};
             vec_t<E, 4> o[PARTS];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float p = __builtin_amdgcn_exp2f((acc[m][n][i] + b[i] - st[n].m) * kLog2e) * st[n].scale;
-                if (v + i == st[n].target) p -= st[n].g;
-                if (st[n].target < 0 || v + i >= a.v1) p = 0.f;         // an ignored row, a row or an entry that is not there
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int k = 0; k < PARTS; ++k) {
-                    o[k][i] = (E)p;
-                    p = PARTS > 1 ? p - (float)o[k][i] : 0.f;
+                    o[k][i] = (E)p[i];
+                    p[i] = PARTS > 1 ? p[i] - (float)o[k][i] : 0.f;
                 }
-            }
 #pragma unroll
             for (int k = 0; k < PARTS; ++k)
                 *reinterpret_cast<vec_t<E, 4>*>(d + k * a.d_part + r * a.d_ld + (v - a.v0)) = o[k];
@@ -406,7 +435,7 @@ struct GradArgs {
     int final_dtype;        // -1: partial sums
     int accumulate;         // partial: add to what is there
     const float* unscale;
-    void* db;               // nullable: row sums of B's operand (final or partial like out)
+    void* db;               // nullable: row sums of B's operand; partial: in column ld - 4 of out
     int db_dtype;
 };
 
@@ -472,30 +501,75 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_grad_kernel(const GradArgs
             }
         }
         if (sums && g == 0) {
-            if (a.final_dtype < 0) static_cast<float*>(a.db)[(int64_t)ks * a.n_end + row] = acc1[n][0];
+            if (a.final_dtype < 0) static_cast<float*>(a.out)[((int64_t)ks * a.n_end + row) * a.ld + a.ld - 4] = acc1[n][0];
             else store_any(a.db, a.db_dtype, row, acc1[n][0] * scale);
         }
     }
 }
 
-// sum of `parts` partial matrices in their order -> [rows][cols] of the output type (dense)
-__global__ __launch_bounds__(kBlock) void ce_sum_kernel(const float* partial, int parts, int64_t rows, int cols, int64_t ld, const float* unscale,
-                                                        void* out, int dtype) {
-    const float scale = unscale ? unscale[1] : 1.f;
-    const int64_t n = rows * cols;
+struct SumArgs {
+    const float* partial;           // [parts][rows][ld]
+    int parts;
+    int64_t rows, ld;
+    int cols;
+    const float* unscale;
+    void* out;                      // [rows][cols] dense
+    int dtype;
+    void* db;                       // nullable: [rows], from column ld - 4
+    int db_dtype;
+};
+// where output q lies in a partial matrix
+__device__ __forceinline__ int64_t sum_source(const SumArgs& a, int64_t q) {
+    const int per = a.cols + (a.db ? 1 : 0);
+    const int64_t r = q / per;
+    const int c = (int)(q - r * per);
+    return r * a.ld + (c < a.cols ? c : a.ld - 4);
+}
+__device__ __forceinline__ void sum_store(const SumArgs& a, int64_t q, float v) {
+    const int per = a.cols + (a.db ? 1 : 0);
+    const int64_t r = q / per;
+    const int c = (int)(q - r * per);
+    if (a.unscale) v *= a.unscale[1];
+    if (c < a.cols) store_any(a.out, a.dtype, r * a.cols + c, v);
+    else store_any(a.db, a.db_dtype, r, v);
+}
+
+// the partial matrices added in their order: a lane per output
+__global__ __launch_bounds__(kBlock) void ce_sum_kernel(const SumArgs a) {
+    const int64_t n = a.rows * (a.cols + (a.db ? 1 : 0)), part = a.rows * a.ld;
     for (int64_t q = (int64_t)blockIdx.x * kBlock + threadIdx.x; q < n; q += (int64_t)gridDim.x * kBlock) {
-        const int64_t r = q / cols;
-        const int64_t at = r * ld + (q - r * cols);
+        const float* p = a.partial + sum_source(a, q);
         float s = 0.f;
-        for (int p = 0; p < parts; ++p) s += partial[(int64_t)p * rows * ld + at];
-        store_any(out, dtype, q, s * scale);
+        for (int k = 0; k < a.parts; ++k) s += p[k * part];
+        sum_store(a, q, s);
+    }
+}
+
+// many partial matrices of few outputs (51 classes x 64 features x 288 parts: 67 us with a lane per output): 16 outputs a workgroup,
+// 64 lanes each add every 64th part, then the 64 sums are added in order
+__global__ __launch_bounds__(1024) void ce_sum_many_kernel(const SumArgs a) {
+    __shared__ float sh[64][17];
+    const int cl = threadIdx.x & 15, slot = threadIdx.x >> 4;
+    const int64_t n = a.rows * (a.cols + (a.db ? 1 : 0)), part = a.rows * a.ld, q = (int64_t)blockIdx.x * 16 + cl;
+    float t = 0.f;
+    if (q < n) {
+        const float* p = a.partial + sum_source(a, q);
+        for (int k = slot; k < a.parts; k += 64) t += p[k * part];
+    }
+    sh[slot][cl] = t;
+    __syncthreads();
+    if (slot == 0 && q < n) {
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < 64; ++k) v += sh[k][cl];
+        sum_store(a, q, v);
     }
 }
 
 // ---- host: plan of a call -------------------------------------------------------------------------------------------------------
 
 constexpr int kBig = 256, kSmall = 128;         // tile edges
-constexpr int64_t kPieceBytes = 128ll << 20;    // d of one piece of the vocabulary: half the memory-side cache
+constexpr int64_t kPieceBytes = 256ll << 20;    // d of one piece of the vocabulary
 
 static int64_t round_up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 static int64_t ceil_div(int64_t n, int64_t m) { return (n + m - 1) / m; }
@@ -510,7 +584,7 @@ struct CePlan {
     int splits;
     int64_t partial_off, logit_off, sums_off;
     // backward
-    int64_t rows_pad, piece, d_off, state_off, unscale_off, dx_off, dw_off, db_off;
+    int64_t rows_pad, piece, d_off, state_off, unscale_off, dx_off, dw_off;
     int dx_split, dw_split;
     bool big_d, big_dx, big_dw;
     int64_t bytes;
@@ -557,10 +631,7 @@ static CePlan ce_plan(int64_t R, int V, int H, int dtype, bool x_ok, bool w_ok, 
         p.dx_split = narrow_split(R, V);
         p.dw_split = narrow_split(V, R);
         if (p.dx_split > 1) p.dx_off = take((int64_t)p.dx_split * R * ld4 * 4);
-        if (p.dw_split > 1) {
-            p.dw_off = take((int64_t)p.dw_split * V * ld4 * 4);
-            p.db_off = take((int64_t)p.dw_split * V * 4);
-        }
+        if (p.dw_split > 1) p.dw_off = take((int64_t)p.dw_split * V * (ld4 + 4) * 4);
         p.bytes = at;
         return p;
     }
@@ -579,10 +650,7 @@ static CePlan ce_plan(int64_t R, int V, int H, int dtype, bool x_ok, bool w_ok, 
     p.dx_split = split(R, width, p.big_dx);
     p.dw_split = split(width, R, p.big_dw);
     if (p.dx_split > 1 || p.piece < V) p.dx_off = take((int64_t)p.dx_split * R * ld4 * 4);
-    if (p.dw_split > 1) {
-        p.dw_off = take((int64_t)p.dw_split * width * ld4 * 4);
-        p.db_off = take((int64_t)p.dw_split * width * 4);
-    }
+    if (p.dw_split > 1) p.dw_off = take((int64_t)p.dw_split * width * (ld4 + 4) * 4);
     p.bytes = at;
     return p;
 }
@@ -595,6 +663,9 @@ static int ce_types(int dtype, Fn&& fn) {
     return fn(f16_t{}, f16_t{}, std::integral_constant<int, 1>{});
 }
 
+// fp32 rows that vectors of 8 elements may be read from
+static bool rows_aligned32(const void* p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0 && stride % 8 == 0; }
+
 template <typename T, typename E, int PARTS>
 static void ce_operands(CeArgs& a, const CePlan& p, const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias,
                         int bias_dtype, int64_t R, int V, int H, char* ws, hipStream_t st) {
@@ -602,6 +673,8 @@ static void ce_operands(CeArgs& a, const CePlan& p, const void* x, int64_t x_str
     if (p.copy_x) l.job[0] = LayoutJob{x, x_stride, R, ws + p.x_off};
     if (p.copy_w) l.job[1] = LayoutJob{w, w_stride, V, ws + p.w_off};
     l.cols = H;
+    // fp32 rows of whole 32-byte groups; 16-bit rows are only copied where they cannot be read that way
+    if (sizeof(T) == 4 && H % 8 == 0) l.vec = (rows_aligned32(x, x_stride) ? 1 : 0) | (rows_aligned32(w, w_stride) ? 2 : 0);
     l.ld = p.ldh;
     if (p.narrow) {
         l.bias = bias;
@@ -643,9 +716,12 @@ static NarrowArgs narrow_args(const CeArgs& a, const CePlan& p, bool rows_own, c
     return n;
 }
 
-static void ce_sum(const void* partial, int parts, int64_t rows, int cols, int64_t ld, const float* unscale, void* out, int dtype, hipStream_t st) {
-    CNF_LAUNCH(ce_sum_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(rows * cols, kBlock), 8192)), dim3(kBlock), 0, st,
-               static_cast<const float*>(partial), parts, rows, cols, ld, unscale, out, dtype);
+static void ce_sum(const void* partial, int parts, int64_t rows, int cols, int64_t ld, const float* unscale, void* out, int dtype, void* db,
+                   int db_dtype, hipStream_t st) {
+    const SumArgs a{static_cast<const float*>(partial), parts, rows, ld, cols, unscale, out, dtype, db, db_dtype};
+    const int64_t n = rows * (cols + (db ? 1 : 0));
+    if (parts > 16) CNF_LAUNCH(ce_sum_many_kernel, dim3((unsigned)ceil_div(n, 16)), dim3(1024), 0, st, a);
+    else CNF_LAUNCH(ce_sum_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(n, kBlock), 8192)), dim3(kBlock), 0, st, a);
 }
 
 static bool ce_aligned(const void* p, int64_t stride, int dtype, int H) { return rows_aligned16(p, stride, dtype) && H % 8 == 0; }
@@ -748,23 +824,20 @@ int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64
                 n.unscale = unscale;
                 const int rc = narrow_launch(kNarrowDx, dtype, n, st);
                 if (rc != CNF_OK) return rc;
-                if (n.splits > 1) ce_sum(n.out, n.splits, R, H, ld4, unscale, dx, dtype, st);
+                if (n.splits > 1) ce_sum(n.out, n.splits, R, H, ld4, unscale, dx, dtype, nullptr, 0, st);
             }
             if (dweight) {
                 NarrowArgs n = narrow_args(a, p, false, ws);
                 n.splits = p.dw_split;
                 n.final_dtype = n.splits > 1 ? -1 : dtype;
                 n.out = n.splits > 1 ? static_cast<void*>(ws + p.dw_off) : dweight;
-                n.ld = n.splits > 1 ? ld4 : H;
+                n.ld = n.splits > 1 ? ld4 + 4 : H;
                 n.unscale = unscale;
-                n.db = dbias ? (n.splits > 1 ? static_cast<void*>(ws + p.db_off) : dbias) : nullptr;
+                n.db = dbias;
                 n.db_dtype = bias_dtype;
                 const int rc = narrow_launch(kNarrowDw, dtype, n, st);
                 if (rc != CNF_OK) return rc;
-                if (n.splits > 1) {
-                    ce_sum(n.out, n.splits, V, H, ld4, unscale, dweight, dtype, st);
-                    if (dbias) ce_sum(n.db, n.splits, 1, V, V, unscale, dbias, bias_dtype, st);
-                }
+                if (n.splits > 1) ce_sum(n.out, n.splits, V, H, n.ld, unscale, dweight, dtype, dbias, bias_dtype, st);
             }
             return launch_status("cnf_linear_ce_bwd");
         }
@@ -819,17 +892,14 @@ int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64
             q.ksplit = p.dw_split;
             q.final_dtype = dw_partial ? -1 : dtype;
             q.out = dw_partial ? static_cast<void*>(ws + p.dw_off) : dw;
-            q.ld = dw_partial ? ld4 : H;
+            q.ld = dw_partial ? ld4 + 4 : H;
             q.accumulate = 0;
-            q.db = db ? (dw_partial ? static_cast<void*>(ws + p.db_off) : db) : nullptr;
+            q.db = db;
             q.db_dtype = bias_dtype;
             grad(true, p.big_dw, width);
-            if (dw_partial) {
-                ce_sum(ws + p.dw_off, p.dw_split, width, H, ld4, unscale, dw, dtype, st);
-                if (db) ce_sum(ws + p.db_off, p.dw_split, 1, (int)width, width, unscale, db, bias_dtype, st);
-            }
+            if (dw_partial) ce_sum(ws + p.dw_off, p.dw_split, width, H, q.ld, unscale, dw, dtype, db, bias_dtype, st);
         }
-        if (dx && dx_partial) ce_sum(ws + p.dx_off, p.dx_split, R, H, ld4, unscale, dx, dtype, st);
+        if (dx && dx_partial) ce_sum(ws + p.dx_off, p.dx_split, R, H, ld4, unscale, dx, dtype, nullptr, 0, st);
         return launch_status("cnf_linear_ce_bwd");
     });
 }

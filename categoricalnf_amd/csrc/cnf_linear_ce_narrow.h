@@ -5,8 +5,10 @@
 
 namespace cnf {
 
-struct RowState {       // backward: what an element of d needs of its row
-    float m, scale;     // maximum (+inf: the row is ignored); g / s
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct RowState {       // backward: what an element d = exp2(l log2 e - m2) scale - [target] g needs of its row
+    float m2, scale;    // maximum times log2 e (+inf: the row is ignored); g / s
     float g;
     int target;         // -1: ignored
 };
@@ -31,7 +33,7 @@ struct NarrowArgs {
     int64_t ld;
     int final_dtype;
     const float* unscale;
-    void* db;
+    void* db;                           // nullable; partial sums: in column ld - 4 of out
     int db_dtype;
 };
 

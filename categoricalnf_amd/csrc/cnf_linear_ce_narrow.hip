@@ -11,12 +11,12 @@
 // Bound by the matrix cores and the vector work beside them (exponentials, splitting): 5 products of 2 R V H operations against the
 // 3 of the definition — the logits are computed three times — but nothing of size R x V is written or read.
 #include <algorithm>
+#include <type_traits>
+#include <utility>
 
 #include "cnf_linear_ce_narrow.h"
 
 namespace cnf {
-
-constexpr float kLog2e = 1.4426950408889634f;
 
 // LDS tile: [PARTS][64][HP] 16-bit elements; 16-byte chunk c of row r at c ^ f(r): row reads (16 rows, one chunk each) and transposing
 // reads (16 rows, 32 bytes each) both touch every bank equally often
@@ -51,32 +51,41 @@ struct NarrowTile {
         const int l = threadIdx.x & 63, row = row0 + (l & 15), c = kk * 4 + (l >> 4);
         return *reinterpret_cast<const s16x8*>(lds + part * kPart + row * (HP * 2) + ((c ^ narrow_swizzle<HP>(row)) << 4));
     }
-    // transposed: columns 16 h ... for h = h0, h0 + 1, k = the 32 rows from row0: lane group g holds rows 4 g ... + 3 and 16 + 4 g ... + 3
-    __device__ static void frag_t2(const char* lds, int part, int row0, int h0, s16x8 (&out)[2]) {
-        const int l = threadIdx.x & 63, g = l >> 4, i = l & 15, row = row0 + g * 4 + (i >> 2);
-        uint32_t at[2][2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int r = row + k * 16, c = (h0 + h) * 2 + ((i & 3) >> 1);
-                at[h][k] = (uint32_t)(uintptr_t)(lds_void16_t*)lds + part * kPart + r * (HP * 2) + ((c ^ narrow_swizzle<HP>(r)) << 4) + (i & 1) * 8;
-            }
-        // in assembly, waited for in the same block, like the transposing reads of cnf_mfma.h
+    // Transposed: columns 16 h ..., k = 32 rows, lane group g holding rows 4 g ... + 3 and 16 + 4 g ... + 3.  The
+    // swizzle of a row depends on its place within 16 rows only, so one address per h serves every part and row block through the
+    // instruction's offset (held per block, they took 80 registers more).
+    __device__ static uint32_t frag_t_base(int h) {
+        const int l = threadIdx.x & 63, i = l & 15, row = (l >> 4) * 4 + (i >> 2), c = h * 2 + ((i & 3) >> 1);
+        return row * (HP * 2) + ((c ^ narrow_swizzle<HP>(row)) << 4) + (i & 1) * 8;
+    }
+    // two of them, h and h + 1; in assembly, waited for in the same block, like the transposing reads of cnf_mfma.h
+    template <int PART>
+    __device__ static void frag_t2(uint32_t at0, uint32_t at1, s16x8 (&out)[2]) {
+        constexpr int kOff = PART * kPart;
         s16x4 v[2][2];
         asm volatile(
-            "ds_read_b64_tr_b16 %0, %4\n\t"
-            "ds_read_b64_tr_b16 %1, %5\n\t"
-            "ds_read_b64_tr_b16 %2, %6\n\t"
-            "ds_read_b64_tr_b16 %3, %7\n\t"
+            "ds_read_b64_tr_b16 %0, %4 offset:%6\n\t"
+            "ds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+            "ds_read_b64_tr_b16 %2, %5 offset:%6\n\t"
+            "ds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
             "s_waitcnt lgkmcnt(0)"
             : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1])
-            : "v"(at[0][0]), "v"(at[0][1]), "v"(at[1][0]), "v"(at[1][1])
+            : "v"(at0), "v"(at1), "n"(kOff), "n"(kOff + 16 * HP * 2)
             : "memory");
 #pragma unroll
         for (int h = 0; h < 2; ++h) out[h] = __builtin_shufflevector(v[h][0], v[h][1], 0, 1, 2, 3, 4, 5, 6, 7);
     }
 };
+
+// fn(integral_constant 0) ... fn(integral_constant N - 1)
+template <typename Fn, int... I>
+__device__ __forceinline__ void static_for_impl(Fn&& fn, std::integer_sequence<int, I...>) {
+    (fn(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename Fn>
+__device__ __forceinline__ void static_for(Fn&& fn) {
+    static_for_impl(static_cast<Fn&&>(fn), std::make_integer_sequence<int, N>{});
+}
 
 template <typename E, int PARTS, int HP, NarrowJob JOB>
 __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a) {
@@ -135,6 +144,9 @@ __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a
                                                    : z;
             }
     }
+    uint32_t t_base[HT];
+#pragma unroll
+    for (int h = 0; h < HT; ++h) t_base[h] = (uint32_t)(uintptr_t)(lds_void16_t*)lds + Tile::frag_t_base(h);
     float mx[NT], sum[NT];
     f32x4 acc[HT][NT];
 #pragma unroll
@@ -157,16 +169,12 @@ __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a
         asm volatile("" ::: "memory");
         const char* s = lds + stage * kStage;
         const int64_t m_tile = tile * kNarrowWalk;
-#pragma unroll
+#pragma unroll 1
         for (int mp = 0; mp < 2; ++mp) {
             f32x4 sc[2][NT];
-            RowState row[2][4];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 if (JOB == kNarrowDw) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        row[t][i] = reinterpret_cast<const RowState*>(s + Tile::kBytes)[mp * 32 + t * 16 + g * 4 + i];
 #pragma unroll
                     for (int n = 0; n < NT; ++n) sc[t][n] = f32x4{bias_n[n], bias_n[n], bias_n[n], bias_n[n]};
                 } else {
@@ -217,14 +225,27 @@ __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a
             }
             // d, split into its parts: the second product's operand
             s16x8 d[PARTS][NT];
+            // dw: the records of the lane's rows; their g is read only where a target is met
+            const RowState* row = reinterpret_cast<const RowState*>(s + Tile::kBytes) + mp * 32 + g * 4;
+            float row_m2[8], row_scale[8];
+            int row_target[8];
+            if (JOB == kNarrowDw) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const RowState& q = row[(e / 4) * 16 + e % 4];
+                    row_m2[e] = q.m2;
+                    row_scale[e] = q.scale;
+                    row_target[e] = q.target;
+                }
+            }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float v[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float m = JOB == kNarrowDw ? row[e / 4][e % 4].m : st[n].m;
-                    const float f = JOB == kNarrowDw ? row[e / 4][e % 4].scale : st[n].scale;
-                    v[e] = __builtin_amdgcn_exp2f((sc[e / 4][n][e % 4] - m) * kLog2e) * f;
+                    const float m = JOB == kNarrowDw ? row_m2[e] : st[n].m2;
+                    const float f = JOB == kNarrowDw ? row_scale[e] : st[n].scale;
+                    v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e / 4][n][e % 4], kLog2e, -m)) * f;
                 }
                 if (JOB == kNarrowDx) {
                     const int64_t at = st[n].target - m0;
@@ -237,11 +258,11 @@ __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a
                     const int e0 = (int)(n_wave + n * 16 + col);
                     bool hit = false;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) hit |= row[e / 4][e % 4].target == e0;
+                    for (int e = 0; e < 8; ++e) hit |= row_target[e] == e0;
                     if (__ballot(hit)) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            if (row[e / 4][e % 4].target == e0) v[e] -= row[e / 4][e % 4].g;
+                            if (row_target[e] == e0) v[e] -= row[(e / 4) * 16 + e % 4].g;
                     }
 #pragma unroll
                     for (int e = 0; e < 8; ++e) sum[n] += v[e];
@@ -258,19 +279,21 @@ __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a
 #pragma unroll
                 for (int p = 0; p < PARTS; ++p) d[p][n] = __builtin_bit_cast(s16x8, o[p]);
             }
-#pragma unroll
-            for (int h = 0; h < HT; h += 2)
-#pragma unroll
-                for (int p = PARTS - 1; p >= 0; --p) {
+            const uint32_t tile_at = stage * kStage + mp * (32 * HP * 2);
+            static_for<HT / 2>([&](auto h_c) {
+                constexpr int h = decltype(h_c)::value * 2;
+                static_for<PARTS>([&](auto q_c) {
+                    constexpr int p = PARTS - 1 - decltype(q_c)::value;          // smallest products first
                     s16x8 f[2];
-                    Tile::frag_t2(s, p, mp * 32, h, f);
+                    Tile::template frag_t2<p>(t_base[h] + tile_at, t_base[h + 1] + tile_at, f);
 #pragma unroll
                     for (int b = PARTS - 1 - p; b >= 0; --b)
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
 #pragma unroll
                             for (int n = 0; n < NT; ++n) acc[h + i][n] = mfma16<E>(f[i], d[b][n], acc[h + i][n]);
-                }
+                });
+            });
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // this wave has read the stage ...
         __builtin_amdgcn_s_barrier();                               // ... and the others: the next copy may overwrite it
@@ -305,7 +328,7 @@ __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a
         if (e >= own_n) continue;
         if (JOB == kNarrowDw && a.db && g == 0) {
             if (a.final_dtype >= 0) store_any(a.db, a.db_dtype, e, b * unscale);
-            else static_cast<float*>(a.db)[(int64_t)split * own_n + e] = b;
+            else static_cast<float*>(a.out)[((int64_t)split * own_n + e) * a.ld + a.ld - 4] = b;
         }
 #pragma unroll
         for (int h = 0; h < HT; ++h) {
