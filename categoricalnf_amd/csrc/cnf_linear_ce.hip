@@ -7,16 +7,18 @@
 // lane keeps a running maximum and sum for its rows over the vocabulary entries it sees (four of them are consecutive), the lanes and
 // waves of a row are joined once at the end, the parts of the vocabulary by a second launch, which also writes the loss.
 // Backward, in pieces of the vocabulary: the piece's logits are computed again and turned into d (rounded to the operands' type, or
-// kept as three bf16 parts for fp32), written to a workspace that fits the memory-side cache, and read by two products: dx += d w over
+// kept as two fp16 parts for fp32), written to a workspace that fits the memory-side cache, and read by two products: dx += d w over
 // the piece, dw = d^T x complete for the piece.  db comes out of the second product: a fragment of ones in place of x.
 //
-// Few features (fp32: H <= 64, 16-bit: H <= 128) take the kernels of cnf_linear_ce_narrow.hip instead, which write nothing of size R x V.
+// Few features (H <= 128) take the kernels of cnf_linear_ce_narrow.hip instead, which write nothing of size R x V.
 //
-// fp32 inputs are split once into three bf16 parts (cnf_mfma.h: pair_a): six bf16 products keep every product to 2^-26, and the
-// matrix cores do them at 16 times the fp32 rate.  16-bit inputs whose rows are not 16-byte aligned are copied once into padded rows.
-// 16-bit d is computed for g_r / max |g| (in fp16 times 2^14, so that small probabilities keep their bits) and the results are scaled
+// fp32 inputs are scaled by a power of two per tensor and split once into two fp16 parts (cnf_mfma.h: pair_a): three fp16 products keep
+// every product to 2^-22, and the matrix cores do them at 16 times the fp32 rate.  16-bit inputs whose rows are not 16-byte aligned
+// are copied once into padded rows.
+// d is computed for g_r / max |g| (for fp16 operands times 2^14, so that small probabilities keep their bits) and the results are scaled
 // back: under a mean every row's -1 is then exact, where a rounded -g_r would put the same relative error on every row's largest entry.
 #include <algorithm>
+#include <type_traits>
 
 #include "cnf_linear_ce_narrow.h"
 
@@ -37,6 +39,9 @@ struct CeArgs {
     int splits;                     // of the vocabulary tiles
     // backward
     const RowState* state;          // [rows]
+    const CeScales* scales;
+    int scaled;                     // fp32 operands: scales->ex holds
+    float lift;                     // of d
     void* d;                        // [parts][rows_pad][piece_ld]
     int64_t d_part, d_ld;
     int v0, v1;                     // the piece
@@ -55,6 +60,11 @@ __device__ __forceinline__ void grouped_tile(unsigned t, unsigned ni, unsigned n
 }
 
 __device__ __forceinline__ float bias_at(const CeArgs& a, int v) { return a.bias && v < a.vocab ? load_any(a.bias, a.bias_dtype, v) : 0.f; }
+
+// what takes a product of scaled operands to unit * logit
+__device__ __forceinline__ float logit_scale(const CeArgs& a, float unit) {
+    return a.scaled ? ldexpf(unit, max(min(-(a.scales->ex[0] + a.scales->ex[1]), 126), -300)) : unit;
+}
 
 // ---- forward ---------------------------------------------------------------------------------------------------------------------
 
@@ -89,15 +99,16 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_lse_kernel(const CeArgs a)
             for (int n = 0; n < Tile::NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
         tile.run(v0, r0, 0, a.hidden, acc, [](int) {});
         const int vw = v0 + tile.m_wave + g * 4;        // the lane's first entry
-        if (a.bias) {
+        if (a.bias || a.scaled) {
+            const float back = logit_scale(a, 1.f);
 #pragma unroll
-            for (int m = 0; m < Tile::MT; ++m) {
-                f32x4 b;
+            for (int m = 0; m < Tile::MT; ++m)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) b[i] = bias_at(a, vw + m * 16 + i);
+                for (int i = 0; i < 4; ++i) {
+                    const float b = bias_at(a, vw + m * 16 + i);
 #pragma unroll
-                for (int n = 0; n < Tile::NT; ++n) acc[m][n] += b;
-            }
+                    for (int n = 0; n < Tile::NT; ++n) acc[m][n][i] = __builtin_fmaf(acc[m][n][i], back, b);
+                }
         }
         if (v0 + BM > a.vocab) {                        // entries past the vocabulary
 #pragma unroll
@@ -249,6 +260,37 @@ __global__ __launch_bounds__(1024) void ce_reduce_kernel(const double* sums, int
 
 // ---- operand layout ----------------------------------------------------------------------------------------------------------------
 
+constexpr int kMaxBlocks = 256;
+// fp32: the largest finite |element| of x (blockIdx.y 0) and w (1), one value per workgroup
+__global__ __launch_bounds__(kBlock) void ce_largest_kernel(const float* x, int64_t x_stride, int64_t R, const float* w, int64_t w_stride, int V,
+                                                            int H, uint32_t* largest) {
+    __shared__ uint32_t sh[kWavesPerBlock];
+    const float* src = blockIdx.y ? w : x;
+    const int64_t stride = blockIdx.y ? w_stride : x_stride, rows = blockIdx.y ? V : R;
+    uint32_t top = 0;
+    if (stride == H) {
+        const int64_t n = rows * H;
+        for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (int64_t)kMaxBlocks * kBlock) {
+            const uint32_t b = __float_as_uint(src[i]) & 0x7fffffffu;
+            if (b < 0x7f800000u) top = max(top, b);
+        }
+    } else {
+        for (int64_t r = blockIdx.x; r < rows; r += kMaxBlocks)
+            for (int c = threadIdx.x; c < H; c += kBlock) {
+                const uint32_t b = __float_as_uint(src[r * stride + c]) & 0x7fffffffu;
+                if (b < 0x7f800000u) top = max(top, b);
+            }
+    }
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, kWave));
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int k = 1; k < kWavesPerBlock; ++k) top = max(top, sh[k]);
+        largest[blockIdx.y * kMaxBlocks + blockIdx.x] = top;
+    }
+}
+
 struct LayoutJob {
     const void* src;                // nullable: nothing to do
     int64_t stride, rows;
@@ -261,20 +303,37 @@ struct LayoutArgs {
     const void* bias;               // -> fp32, -inf behind the vocabulary (nullable: zeros)
     int bias_dtype, vocab, bias_pad;
     float* bias_out;                // nullable
+    float bias_unit;
+    const uint32_t* largest;        // fp32: what ce_largest_kernel found ...
+    CeScales* scales;               // ... and where the exponents go
 };
 
-// one launch for whatever a call has to lay out: blockIdx.y 0: x, 1: w, 2: the bias.  fp32: x0 + x1 + x2, each the bf16 nearest to what
-// is left
+// one launch for whatever a call has to lay out: blockIdx.y 0: x, 1: w, 2: the bias.  fp32: scaled, then x0 + x1, each the fp16 nearest
+// to what is left
 template <typename T, typename E, int PARTS>
 __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
     if (blockIdx.y == 2) {
         if (a.bias_out)
             for (int v = blockIdx.x * kBlock + threadIdx.x; v < a.bias_pad; v += gridDim.x * kBlock)
-                a.bias_out[v] = v >= a.vocab ? -INFINITY : (a.bias ? load_any(a.bias, a.bias_dtype, v) : 0.f);
+                a.bias_out[v] = v >= a.vocab ? -INFINITY : (a.bias ? load_any(a.bias, a.bias_dtype, v) * a.bias_unit : 0.f);
         return;
     }
     const LayoutJob job = a.job[blockIdx.y];
     if (!job.src) return;
+    int ex = 0;
+    if (PARTS > 1) {
+        __shared__ uint32_t sh[kWavesPerBlock];
+        uint32_t top = a.largest[blockIdx.y * kMaxBlocks + threadIdx.x];
+        static_assert(kMaxBlocks == kBlock, "a lane reads one workgroup's value");
+#pragma unroll
+        for (int m = 32; m >= 1; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, kWave));
+        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
+        __syncthreads();
+        for (int k = 0; k < kWavesPerBlock; ++k) top = max(top, sh[k]);
+        // the largest into 2^14 ... 2^15 (subnormal numbers: as if of exponent -126); zeros alone stay as they are
+        if (top) ex = 14 - (max((int)(top >> 23), 1) - 127);
+        if (blockIdx.x == 0 && threadIdx.x == 0) a.scales->ex[blockIdx.y] = ex;
+    }
     const T* src = static_cast<const T*>(job.src);
     E* dst = static_cast<E*>(job.dst);
     const int per = (int)(a.ld / 8);
@@ -292,16 +351,12 @@ __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
         vec_t<E, 8> o[PARTS];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            float v = (float)in[i];
+            float v = PARTS > 1 ? ldexpf((float)in[i], ex) : (float)in[i];
 #pragma unroll
             for (int p = 0; p < PARTS; ++p) {
-                E e = (E)v;
-                // the largest numbers round up to infinity: keep them finite (the next part takes the rest); infinities and NaN
-                // are whole in the first part
-                if (PARTS > 1 && __builtin_isinf((float)e) && !__builtin_isinf(v))
-                    e = __builtin_bit_cast(E, (uint16_t)(__float_as_uint(v) >> 16));
-                o[p][i] = e;
-                v = PARTS > 1 && __builtin_isfinite(v) ? v - (float)e : 0.f;
+                o[p][i] = (E)v;
+                // infinities and NaN are whole in the first part
+                v = PARTS > 1 && __builtin_isfinite(v) ? v - (float)o[p][i] : 0.f;
             }
         }
 #pragma unroll
@@ -311,41 +366,34 @@ __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
 
 // ---- backward ----------------------------------------------------------------------------------------------------------------------
 
-// upstream gradients (per row, or one over the count) -> row records, ignored ones behind the last row up to rows_pad.
-// 16-bit operands (unscale != NULL): every g is divided by the largest |g| and multiplied by `lift`; unscale[1] undoes both
+// upstream gradients (per row, or one over the count) -> row records, ignored ones behind the last row up to rows_pad.  Every g is
+// divided by the largest |g|, which goes to scales
 __global__ __launch_bounds__(1024) void ce_rows_kernel(const float* g, int g_is_row, const float* count, const float* row_max, const float* row_sum,
                                                        const int64_t* target, int64_t ignore, int vocab, int64_t rows, int64_t rows_pad,
-                                                       float lift, RowState* state, float* unscale) {
+                                                       RowState* state, CeScales* scales) {
     __shared__ uint32_t sh[16];
     const float shared = g_is_row ? 0.f : *g / *count;
-    float top = 1.f;
-    if (unscale) {
-        uint32_t bits = 0;
-        if (g_is_row) {
-            for (int64_t r = threadIdx.x; r < rows; r += 1024)
-                if (target[r] != ignore) bits = max(bits, __float_as_uint(g[r]) & 0x7fffffffu);
-        } else {
-            bits = __float_as_uint(shared) & 0x7fffffffu;
-        }
+    uint32_t bits = __float_as_uint(shared) & 0x7fffffffu;
+    if (g_is_row) {
+        for (int64_t r = threadIdx.x; r < rows; r += 1024)
+            if (target[r] != ignore) bits = max(bits, __float_as_uint(g[r]) & 0x7fffffffu);
 #pragma unroll
         for (int m = 32; m >= 1; m >>= 1) bits = max(bits, (uint32_t)__shfl_xor((int)bits, m, kWave));
         if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = bits;
         __syncthreads();
         for (int w = 0; w < 16; ++w) bits = max(bits, sh[w]);
-        // all gradients zero, or an infinite or NaN one among them: as they are
-        if (bits != 0 && bits < 0x7f800000u) top = __uint_as_float(bits);
-        if (threadIdx.x == 0 && blockIdx.x == 0) unscale[1] = top / lift;
     }
+    // all gradients zero, or an infinite or NaN one among them: as they are
+    const float top = bits != 0 && bits < 0x7f800000u ? __uint_as_float(bits) : 1.f;
+    if (threadIdx.x == 0 && blockIdx.x == 0) scales->top = top;
     for (int64_t r = (int64_t)blockIdx.x * 1024 + threadIdx.x; r < rows_pad; r += (int64_t)gridDim.x * 1024) {
         const int64_t t = r < rows ? target[r] : -1;
         const bool in = r < rows && t != ignore && t >= 0 && t < vocab;
-        const float gr = in ? (g_is_row ? g[r] : shared) / top * lift : 0.f;
         RowState s;
         // exp(l - m) = exp2(l L - m2) exp2(m2 - m L), L = log2 e, m2 = m L rounded: one fma per element, the row's rest in its scale
-        const float m2 = in ? row_max[r] * kLog2e : INFINITY;
-        s.m2 = m2;
-        s.scale = in ? gr / row_sum[r] * __builtin_amdgcn_exp2f(-__builtin_fmaf(row_max[r], kLog2e, -m2)) : 0.f;
-        s.g = gr;
+        s.m2 = in ? row_max[r] * kLog2e : INFINITY;
+        s.inv_s = in ? __builtin_amdgcn_exp2f(-__builtin_fmaf(row_max[r], kLog2e, -s.m2)) / row_sum[r] : 0.f;
+        s.g = in ? (g_is_row ? g[r] : shared) / top : 0.f;
         s.target = in ? (int)t : -1;
         state[r] = s;
     }
@@ -376,6 +424,13 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
         st[n] = r < a.rows ? a.state[r] : RowState{INFINITY, 0.f, 0.f, -1};
     }
     E* d = static_cast<E*>(a.d);
+    const float back = logit_scale(a, kLog2e);
+    float scale[Tile::NT], own_g[Tile::NT];
+#pragma unroll
+    for (int n = 0; n < Tile::NT; ++n) {
+        own_g[n] = st[n].g * a.lift;
+        scale[n] = st[n].inv_s * own_g[n];
+    }
     // targets among the wave's entries are rare: their -g is applied behind a branch that most waves do not take
     int at[Tile::NT];
     bool hit = false;
@@ -391,18 +446,18 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
         f32x4 b = {0.f, 0.f, 0.f, 0.f};
         if (a.bias) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) b[i] = bias_at(a, v + i);
+            for (int i = 0; i < 4; ++i) b[i] = bias_at(a, v + i) * kLog2e;
         }
 #pragma unroll
         for (int n = 0; n < Tile::NT; ++n) {
             const int64_t r = (int64_t)r0 + tile.n_wave + n * 16 + col;
             f32x4 p;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[m][n][i] + b[i], kLog2e, -st[n].m2)) * st[n].scale;
+            for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[m][n][i], back, b[i] - st[n].m2)) * scale[n];
             if (any_hit) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (at[n] == m * 16 + i && st[n].target >= 0) p[i] -= st[n].g;
+                    if (at[n] == m * 16 + i && st[n].target >= 0) p[i] -= own_g[n];
             }
             if (edge) {
 #pragma unroll
@@ -434,7 +489,9 @@ struct GradArgs {
     int64_t ld;
     int final_dtype;        // -1: partial sums
     int accumulate;         // partial: add to what is there
-    const float* unscale;
+    const CeScales* scales;
+    int scaled;             // fp32: which of scales->ex to take back (1 + index), 0: none
+    float lift;
     void* db;               // nullable: row sums of B's operand; partial: in column ld - 4 of out
     int db_dtype;
 };
@@ -463,7 +520,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_grad_kernel(const GradArgs
     s16x8 ones;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ones[i] = __builtin_bit_cast(short, (E)1.f);
-    // fp32: each part of d is once the partner of part 0 of x: pairs (0, 2), (0, 1) and (0, 0)
+    // fp32: each part of d is once the partner of part 0 of x: pairs (0, 1) and (0, 0)
     int step = 0;
     const int per_pair = (k1 - k0 + kStepK - 1) / kStepK;
     tile.run(m0, n0, k0, k1, acc, [&](int stage) {
@@ -481,7 +538,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_grad_kernel(const GradArgs
         }
     });
     const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
-    const float scale = a.final_dtype >= 0 && a.unscale ? a.unscale[1] : 1.f;
+    const float down = a.scales->top / a.lift;
+    const int ex = a.scaled ? -a.scales->ex[a.scaled - 1] : 0;
 #pragma unroll
     for (int n = 0; n < Tile::NT; ++n) {
         const int64_t row = (int64_t)n0 + tile.n_wave + n * 16 + col;
@@ -490,6 +548,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_grad_kernel(const GradArgs
         for (int m = 0; m < Tile::MT; ++m) {
             const int h = m0 + tile.m_wave + m * 16 + g * 4;
             if (h >= a.m_end) continue;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[m][n][i] = a.scaled ? ldexpf(acc[m][n][i] * down, ex) : acc[m][n][i] * down;
             if (a.final_dtype < 0) {
                 // ld is a multiple of 4: a partial row has room for the whole vector
                 f32x4* p = reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + ((int64_t)ks * a.n_end + row) * a.ld + h);
@@ -497,12 +557,12 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_grad_kernel(const GradArgs
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (h + i < a.m_end) store_any(a.out, a.final_dtype, row * a.ld + h + i, acc[m][n][i] * scale);
+                    if (h + i < a.m_end) store_any(a.out, a.final_dtype, row * a.ld + h + i, acc[m][n][i]);
             }
         }
         if (sums && g == 0) {
-            if (a.final_dtype < 0) static_cast<float*>(a.out)[((int64_t)ks * a.n_end + row) * a.ld + a.ld - 4] = acc1[n][0];
-            else store_any(a.db, a.db_dtype, row, acc1[n][0] * scale);
+            if (a.final_dtype < 0) static_cast<float*>(a.out)[((int64_t)ks * a.n_end + row) * a.ld + a.ld - 4] = acc1[n][0] * down;
+            else store_any(a.db, a.db_dtype, row, acc1[n][0] * down);
         }
     }
 }
@@ -512,7 +572,6 @@ struct SumArgs {
     int parts;
     int64_t rows, ld;
     int cols;
-    const float* unscale;
     void* out;                      // [rows][cols] dense
     int dtype;
     void* db;                       // nullable: [rows], from column ld - 4
@@ -529,7 +588,6 @@ __device__ __forceinline__ void sum_store(const SumArgs& a, int64_t q, float v) 
     const int per = a.cols + (a.db ? 1 : 0);
     const int64_t r = q / per;
     const int c = (int)(q - r * per);
-    if (a.unscale) v *= a.unscale[1];
     if (c < a.cols) store_any(a.out, a.dtype, r * a.cols + c, v);
     else store_any(a.db, a.db_dtype, r, v);
 }
@@ -578,13 +636,13 @@ struct CePlan {
     int parts, pairs;
     bool copy_x, copy_w, narrow;
     int64_t ldh;                    // padded row of a copied operand
-    int64_t x_off, w_off, bias_off;
+    int64_t x_off, w_off, bias_off, scales_off, largest_off;
     // forward
     bool big_lse;
     int splits;
     int64_t partial_off, logit_off, sums_off;
     // backward
-    int64_t rows_pad, piece, d_off, state_off, unscale_off, dx_off, dw_off;
+    int64_t rows_pad, piece, d_off, state_off, dx_off, dw_off;
     int dx_split, dw_split;
     bool big_d, big_dx, big_dw;
     int64_t bytes;
@@ -592,11 +650,11 @@ struct CePlan {
 
 static CePlan ce_plan(int64_t R, int V, int H, int dtype, bool x_ok, bool w_ok, bool backward) {
     CePlan p{};
-    p.parts = dtype == CNF_DTYPE_F32 ? 3 : 1;
-    p.pairs = dtype == CNF_DTYPE_F32 ? 6 : 1;
+    p.parts = dtype == CNF_DTYPE_F32 ? 2 : 1;
+    p.pairs = dtype == CNF_DTYPE_F32 ? 3 : 1;
     p.copy_x = p.parts > 1 || !x_ok;
     p.copy_w = p.parts > 1 || !w_ok;
-    p.narrow = narrow_supported(dtype, H);
+    p.narrow = narrow_supported(H);
     p.ldh = round_up(H, 8);
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -606,6 +664,8 @@ static CePlan ce_plan(int64_t R, int V, int H, int dtype, bool x_ok, bool w_ok, 
     };
     if (p.copy_x) p.x_off = take((int64_t)p.parts * R * p.ldh * 2);
     if (p.copy_w) p.w_off = take((int64_t)p.parts * V * p.ldh * 2);
+    p.scales_off = take(sizeof(CeScales));
+    if (p.parts > 1) p.largest_off = take(2 * kMaxBlocks * 4);
     if (p.narrow) p.bias_off = take(round_up(V, kNarrowWalk) * 4);
     // about four workgroups for every CU, at least two steps of the walk each
     auto narrow_split = [](int64_t own, int64_t walk) {
@@ -626,7 +686,6 @@ static CePlan ce_plan(int64_t R, int V, int H, int dtype, bool x_ok, bool w_ok, 
     }
     p.rows_pad = round_up(R, kBig);
     p.state_off = take(p.rows_pad * (int64_t)sizeof(RowState));
-    p.unscale_off = take(8);
     if (p.narrow) {
         p.dx_split = narrow_split(R, V);
         p.dw_split = narrow_split(V, R);
@@ -658,7 +717,7 @@ static CePlan ce_plan(int64_t R, int V, int H, int dtype, bool x_ok, bool w_ok, 
 // calls fn(T{}, E{}, parts): the tensors' type, the products' operand type, the parts of an operand
 template <typename Fn>
 static int ce_types(int dtype, Fn&& fn) {
-    if (dtype == CNF_DTYPE_F32) return fn(float{}, bf16_t{}, std::integral_constant<int, 3>{});
+    if (dtype == CNF_DTYPE_F32) return fn(float{}, f16_t{}, std::integral_constant<int, 2>{});
     if (dtype == CNF_DTYPE_BF16) return fn(bf16_t{}, bf16_t{}, std::integral_constant<int, 1>{});
     return fn(f16_t{}, f16_t{}, std::integral_constant<int, 1>{});
 }
@@ -668,8 +727,16 @@ static bool rows_aligned32(const void* p, int64_t stride) { return (reinterpret_
 
 template <typename T, typename E, int PARTS>
 static void ce_operands(CeArgs& a, const CePlan& p, const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias,
-                        int bias_dtype, int64_t R, int V, int H, char* ws, hipStream_t st) {
+                        int bias_dtype, float bias_unit, int64_t R, int V, int H, char* ws, hipStream_t st) {
     LayoutArgs l{};
+    CeScales* scales = reinterpret_cast<CeScales*>(ws + p.scales_off);
+    if constexpr (PARTS > 1) {
+        uint32_t* largest = reinterpret_cast<uint32_t*>(ws + p.largest_off);
+        CNF_LAUNCH(ce_largest_kernel, dim3(kMaxBlocks, 2), dim3(kBlock), 0, st, static_cast<const float*>(x), x_stride, R,
+                   static_cast<const float*>(w), w_stride, V, H, largest);
+        l.largest = largest;
+        l.scales = scales;
+    }
     if (p.copy_x) l.job[0] = LayoutJob{x, x_stride, R, ws + p.x_off};
     if (p.copy_w) l.job[1] = LayoutJob{w, w_stride, V, ws + p.w_off};
     l.cols = H;
@@ -679,6 +746,7 @@ static void ce_operands(CeArgs& a, const CePlan& p, const void* x, int64_t x_str
     if (p.narrow) {
         l.bias = bias;
         l.bias_dtype = bias_dtype;
+        l.bias_unit = bias_unit;
         l.vocab = V;
         l.bias_pad = (int)round_up(V, kNarrowWalk);
         l.bias_out = reinterpret_cast<float*>(ws + p.bias_off);
@@ -697,6 +765,9 @@ static void ce_operands(CeArgs& a, const CePlan& p, const void* x, int64_t x_str
     a.hidden = H;
     a.bias = bias;
     a.bias_dtype = bias_dtype;
+    a.scales = scales;
+    a.scaled = PARTS > 1;
+    a.lift = sizeof(E) == 2 && std::is_same<E, f16_t>::value ? 16384.f : 1.f;
 }
 
 static NarrowArgs narrow_args(const CeArgs& a, const CePlan& p, bool rows_own, char* ws) {
@@ -713,12 +784,15 @@ static NarrowArgs narrow_args(const CeArgs& a, const CePlan& p, bool rows_own, c
     n.target_logit = a.target_logit;
     n.splits = a.splits;
     n.state = a.state;
+    n.scales = a.scales;
+    n.scaled = a.scaled;
+    n.lift = a.lift;
     return n;
 }
 
-static void ce_sum(const void* partial, int parts, int64_t rows, int cols, int64_t ld, const float* unscale, void* out, int dtype, void* db,
-                   int db_dtype, hipStream_t st) {
-    const SumArgs a{static_cast<const float*>(partial), parts, rows, ld, cols, unscale, out, dtype, db, db_dtype};
+static void ce_sum(const void* partial, int parts, int64_t rows, int cols, int64_t ld, void* out, int dtype, void* db, int db_dtype,
+                   hipStream_t st) {
+    const SumArgs a{static_cast<const float*>(partial), parts, rows, ld, cols, out, dtype, db, db_dtype};
     const int64_t n = rows * (cols + (db ? 1 : 0));
     if (parts > 16) CNF_LAUNCH(ce_sum_many_kernel, dim3((unsigned)ceil_div(n, 16)), dim3(1024), 0, st, a);
     else CNF_LAUNCH(ce_sum_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(n, kBlock), 8192)), dim3(kBlock), 0, st, a);
@@ -759,7 +833,7 @@ int cnf_linear_ce(const void* x, int64_t x_stride, const void* weight, int64_t w
             typedef decltype(t) T;
             typedef decltype(e) E;
             CeArgs a{};
-            ce_operands<T, E, decltype(parts)::value>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, R, V, H, ws, st);
+            ce_operands<T, E, decltype(parts)::value>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, 1.f, R, V, H, ws, st);
             a.target = target;
             a.ignore = ignore_index;
             a.partial = reinterpret_cast<float2*>(ws + p.partial_off);
@@ -805,14 +879,12 @@ int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64
         typedef decltype(e) E;
         constexpr int PARTS = decltype(parts)::value;
         CeArgs a{};
-        ce_operands<T, E, PARTS>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, R, V, H, ws, st);
+        ce_operands<T, E, PARTS>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, kLog2e, R, V, H, ws, st);
         RowState* state = reinterpret_cast<RowState*>(ws + p.state_off);
-        float* unscale = dtype == CNF_DTYPE_F32 ? nullptr : reinterpret_cast<float*>(ws + p.unscale_off);
         a.state = state;
-        // 16-bit, per-row gradients: every workgroup finds the largest |g| itself; few of them
-        CNF_LAUNCH(ce_rows_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(p.rows_pad, 1024), unscale && g_per_row ? 16 : 1024)), dim3(1024), 0,
-                   st, g, g_per_row, count, row_max, row_sum, target, ignore_index, V, R, p.rows_pad, dtype == CNF_DTYPE_F16 ? 16384.f : 1.f,
-                   state, unscale);
+        // per-row gradients: every workgroup finds the largest |g| itself; few of them
+        CNF_LAUNCH(ce_rows_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(p.rows_pad, 1024), g_per_row ? 16 : 1024)), dim3(1024), 0, st, g,
+                   g_per_row, count, row_max, row_sum, target, ignore_index, V, R, p.rows_pad, state, reinterpret_cast<CeScales*>(ws + p.scales_off));
         const int64_t ld4 = round_up(H, 4);
         if (p.narrow) {
             if (dx) {
@@ -821,10 +893,9 @@ int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64
                 n.final_dtype = n.splits > 1 ? -1 : dtype;
                 n.out = n.splits > 1 ? static_cast<void*>(ws + p.dx_off) : dx;
                 n.ld = n.splits > 1 ? ld4 : H;
-                n.unscale = unscale;
                 const int rc = narrow_launch(kNarrowDx, dtype, n, st);
                 if (rc != CNF_OK) return rc;
-                if (n.splits > 1) ce_sum(n.out, n.splits, R, H, ld4, unscale, dx, dtype, nullptr, 0, st);
+                if (n.splits > 1) ce_sum(n.out, n.splits, R, H, ld4, dx, dtype, nullptr, 0, st);
             }
             if (dweight) {
                 NarrowArgs n = narrow_args(a, p, false, ws);
@@ -832,12 +903,11 @@ int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64
                 n.final_dtype = n.splits > 1 ? -1 : dtype;
                 n.out = n.splits > 1 ? static_cast<void*>(ws + p.dw_off) : dweight;
                 n.ld = n.splits > 1 ? ld4 + 4 : H;
-                n.unscale = unscale;
                 n.db = dbias;
                 n.db_dtype = bias_dtype;
                 const int rc = narrow_launch(kNarrowDw, dtype, n, st);
                 if (rc != CNF_OK) return rc;
-                if (n.splits > 1) ce_sum(n.out, n.splits, V, H, n.ld, unscale, dweight, dtype, dbias, bias_dtype, st);
+                if (n.splits > 1) ce_sum(n.out, n.splits, V, H, n.ld, dweight, dtype, dbias, bias_dtype, st);
             }
             return launch_status("cnf_linear_ce_bwd");
         }
@@ -869,7 +939,9 @@ int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64
             q.out = dx_partial ? static_cast<void*>(ws + p.dx_off) : dx;
             q.ld = dx_partial ? ld4 : H;
             q.accumulate = v0 > 0;
-            q.unscale = unscale;
+            q.scales = a.scales;
+            q.scaled = a.scaled ? 2 : 0;
+            q.lift = a.lift;
             auto grad = [&](bool kmb, bool big, int64_t n) {
                 const int64_t edge = big ? kBig : kSmall;
                 const dim3 grid((unsigned)(ceil_div(n, edge) * ceil_div(H, edge) * q.ksplit));
@@ -894,12 +966,13 @@ int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64
             q.out = dw_partial ? static_cast<void*>(ws + p.dw_off) : dw;
             q.ld = dw_partial ? ld4 + 4 : H;
             q.accumulate = 0;
+            q.scaled = a.scaled ? 1 : 0;
             q.db = db;
             q.db_dtype = bias_dtype;
             grad(true, p.big_dw, width);
-            if (dw_partial) ce_sum(ws + p.dw_off, p.dw_split, width, H, q.ld, unscale, dw, dtype, db, bias_dtype, st);
+            if (dw_partial) ce_sum(ws + p.dw_off, p.dw_split, width, H, q.ld, dw, dtype, db, bias_dtype, st);
         }
-        if (dx && dx_partial) ce_sum(ws + p.dx_off, p.dx_split, R, H, ld4, unscale, dx, dtype, nullptr, 0, st);
+        if (dx && dx_partial) ce_sum(ws + p.dx_off, p.dx_split, R, H, ld4, dx, dtype, nullptr, 0, st);
         return launch_status("cnf_linear_ce_bwd");
     });
 }

@@ -7,10 +7,16 @@ namespace cnf {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-struct RowState {       // backward: what an element d = exp2(l log2 e - m2) scale - [target] g needs of its row
-    float m2, scale;    // maximum times log2 e (+inf: the row is ignored); g / s
-    float g;
+struct RowState {       // backward: what an element d = (exp2(l log2 e - m2) inv_s - [target]) g needs of its row
+    float m2, inv_s;    // maximum times log2 e (+inf: the row is ignored); 1 / s
+    float g;            // over the largest |g|
     int target;         // -1: ignored
+};
+
+// what the operands of a call were scaled by; in device memory
+struct CeScales {
+    int ex[2];          // fp32: x was multiplied by 2^ex[0], w by 2^ex[1]
+    float top;          // largest |g|
 };
 
 constexpr int kNarrowOwn = 128;         // rows (or vocabulary entries) of a workgroup
@@ -21,7 +27,7 @@ struct NarrowArgs {
     int hidden, vocab;
     int64_t rows;
     int splits;                         // of the walk
-    const float* bias;                  // [vocabulary rounded up to kNarrowWalk] fp32, -inf behind the last entry
+    const float* bias;                  // [vocabulary rounded up to kNarrowWalk] fp32, -inf behind the last entry; backward: times log2 e
     // forward
     const int64_t* target;
     int64_t ignore;
@@ -32,14 +38,16 @@ struct NarrowArgs {
     void* out;                          // final_dtype >= 0: [n][hidden] of that type; otherwise fp32 [splits][n][ld]
     int64_t ld;
     int final_dtype;
-    const float* unscale;
+    const CeScales* scales;
+    int scaled;                         // fp32 operands: scales->ex holds
+    float lift;                         // d is computed times lift (a power of two): small probabilities stay normal numbers in fp16
     void* db;                           // nullable; partial sums: in column ld - 4 of out
     int db_dtype;
 };
 
 enum NarrowJob { kNarrowLse, kNarrowDx, kNarrowDw };
 
-bool narrow_supported(int dtype, int hidden);
+bool narrow_supported(int hidden);
 int narrow_launch(NarrowJob job, int dtype, const NarrowArgs& a, hipStream_t st);
 
 }  // namespace cnf

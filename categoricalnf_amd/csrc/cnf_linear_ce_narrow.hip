@@ -2,11 +2,11 @@
 //
 // A workgroup of four waves keeps 128 rows (for dw: 128 vocabulary entries) as matrix-core operands in registers, 32 a wave, and walks
 // through its part of the other side in steps of 64, copied into LDS one step ahead.  Per step and wave:
-//   S = walk . own^T, starting from the bias            (six bf16 products for fp32 operands, one for 16-bit ones)
+//   S = walk . own^T            (three fp16 products for fp32 operands, one for 16-bit ones)
 //   forward:  running maximum and sum per lane;  backward:  d from S in place, and  out^T += walk^T . d
 // S has four consecutive walk entries of one own entry per lane (fragment layout in cnf_mfma.h); two 16-row tiles of it are exactly
 // the eight k of a lane in the second product, whose other operand is the transposed LDS read of the same tile: d never moves
-// between lanes.  For fp32 d is split into three bf16 parts there.
+// between lanes.  For fp32 d is split into two fp16 parts there.
 //
 // Bound by the matrix cores and the vector work beside them (exponentials, splitting): 5 products of 2 R V H operations against the
 // 3 of the definition — the logits are computed three times — but nothing of size R x V is written or read.
@@ -116,6 +116,9 @@ __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a
     RowState st[NT];
     float bias_n[NT];
     int want[NT];
+    // a logit is its product times `back` plus the bias
+    const int ex = a.scaled ? a.scales->ex[0] + a.scales->ex[1] : 0;
+    const float back = ldexpf(JOB == kNarrowLse ? 1.f : kLog2e, max(min(-ex, 126), -300));
     s16x8 own[PARTS][KK][NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -129,6 +132,7 @@ __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a
             want[n] = t >= 0 && t < a.vocab && t != a.ignore ? (int)t : -1;
         } else if (JOB == kNarrowDx) {
             if (in) st[n] = a.state[e];
+            st[n].inv_s *= a.lift;
             in = in && st[n].target >= 0;               // an ignored row: operand 0, maximum +inf, so that d = 0 whatever the row holds
         } else {
             bias_n[n] = in ? a.bias[e] : -INFINITY;     // d = 0
@@ -169,19 +173,13 @@ __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a
         asm volatile("" ::: "memory");
         const char* s = lds + stage * kStage;
         const int64_t m_tile = tile * kNarrowWalk;
-#pragma unroll 1
+#pragma unroll(JOB == kNarrowLse ? 2 : 1)
         for (int mp = 0; mp < 2; ++mp) {
             f32x4 sc[2][NT];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                if (JOB == kNarrowDw) {
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) sc[t][n] = f32x4{bias_n[n], bias_n[n], bias_n[n], bias_n[n]};
-                } else {
-                    const f32x4 b = *reinterpret_cast<const f32x4*>(s + Tile::kBytes + (mp * 32 + t * 16 + g * 4) * 4);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) sc[t][n] = b;
-                }
+                for (int n = 0; n < NT; ++n) sc[t][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int kk = 0; kk < KK; ++kk) {
                     s16x8 f[PARTS];
@@ -196,7 +194,18 @@ __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a
                 }
             }
             const int64_t m0 = m_tile + mp * 32 + g * 4;            // the lane's first walk entry: 16 t + i further
+            f32x4 bias[2];
+            if (JOB != kNarrowDw) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) bias[t] = *reinterpret_cast<const f32x4*>(s + Tile::kBytes + (mp * 32 + t * 16 + g * 4) * 4);
+            }
             if (JOB == kNarrowLse) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sc[t][n][i] = __builtin_fmaf(sc[t][n][i], back, bias[t][i]);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const int64_t at = want[n] - m0;
@@ -227,14 +236,14 @@ __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a
             s16x8 d[PARTS][NT];
             // dw: the records of the lane's rows; their g is read only where a target is met
             const RowState* row = reinterpret_cast<const RowState*>(s + Tile::kBytes) + mp * 32 + g * 4;
-            float row_m2[8], row_scale[8];
+            float row_m2[8], row_scale[8];          // dw: the row's g and the lift in its scale
             int row_target[8];
             if (JOB == kNarrowDw) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const RowState& q = row[(e / 4) * 16 + e % 4];
                     row_m2[e] = q.m2;
-                    row_scale[e] = q.scale;
+                    row_scale[e] = q.inv_s * q.g * a.lift;
                     row_target[e] = q.target;
                 }
             }
@@ -244,15 +253,16 @@ __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float m = JOB == kNarrowDw ? row_m2[e] : st[n].m2;
-                    const float f = JOB == kNarrowDw ? row_scale[e] : st[n].scale;
-                    v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e / 4][n][e % 4], kLog2e, -m)) * f;
+                    const float f = JOB == kNarrowDw ? row_scale[e] : st[n].inv_s;      // dx: times the lift; g comes at the end
+                    const float b = JOB == kNarrowDw ? bias_n[n] : bias[e / 4][e % 4];
+                    v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e / 4][n][e % 4], back, b - m)) * f;
                 }
                 if (JOB == kNarrowDx) {
                     const int64_t at = st[n].target - m0;
                     if (__ballot(st[n].target >= 0 && at >= 0 && at < 32)) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            if (at == (e / 4) * 16 + e % 4) v[e] -= st[n].g;
+                            if (at == (e / 4) * 16 + e % 4) v[e] -= a.lift;
                     }
                 } else {
                     const int e0 = (int)(n_wave + n * 16 + col);
@@ -262,7 +272,7 @@ __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a
                     if (__ballot(hit)) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            if (row_target[e] == e0) v[e] -= row[(e / 4) * 16 + e % 4].g;
+                            if (row_target[e] == e0) v[e] -= row[(e / 4) * 16 + e % 4].g * a.lift;
                     }
 #pragma unroll
                     for (int e = 0; e < 8; ++e) sum[n] += v[e];
@@ -316,7 +326,8 @@ __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a
         }
         return;
     }
-    const float unscale = a.final_dtype >= 0 && a.unscale ? a.unscale[1] : 1.f;
+    const float down = a.scales->top / a.lift;
+    const int ex_out = a.scaled ? -a.scales->ex[JOB == kNarrowDw ? 0 : 1] : 0;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int64_t e = n_wave + n * 16 + col;
@@ -326,20 +337,23 @@ __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a
             for (int x = 16; x <= 32; x <<= 1) b += __shfl_xor(b, x, kWave);
         }
         if (e >= own_n) continue;
+        const float scale = JOB == kNarrowDx ? down * st[n].g : down;
         if (JOB == kNarrowDw && a.db && g == 0) {
-            if (a.final_dtype >= 0) store_any(a.db, a.db_dtype, e, b * unscale);
-            else static_cast<float*>(a.out)[((int64_t)split * own_n + e) * a.ld + a.ld - 4] = b;
+            if (a.final_dtype >= 0) store_any(a.db, a.db_dtype, e, b * down);
+            else static_cast<float*>(a.out)[((int64_t)split * own_n + e) * a.ld + a.ld - 4] = b * down;
         }
 #pragma unroll
         for (int h = 0; h < HT; ++h) {
             const int k = h * 16 + g * 4;
             if (k >= a.hidden) continue;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[h][n][i] = ldexpf(acc[h][n][i] * scale, ex_out);
             if (a.final_dtype < 0) {
                 *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + ((int64_t)split * own_n + e) * a.ld + k) = acc[h][n];
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (k + i < a.hidden) store_any(a.out, a.final_dtype, e * a.ld + k + i, acc[h][n][i] * unscale);
+                    if (k + i < a.hidden) store_any(a.out, a.final_dtype, e * a.ld + k + i, acc[h][n][i]);
             }
         }
     }
@@ -357,15 +371,14 @@ static void narrow_job(NarrowJob job, const NarrowArgs& a, hipStream_t st) {
 template <typename E, int PARTS>
 static void narrow_width(NarrowJob job, const NarrowArgs& a, hipStream_t st) {
     if (a.hidden <= 32) narrow_job<E, PARTS, 32>(job, a, st);
-    else if (PARTS > 1 || a.hidden <= 64) narrow_job<E, PARTS, 64>(job, a, st);
-    else if constexpr (PARTS == 1) narrow_job<E, PARTS, 128>(job, a, st);
+    else if (a.hidden <= 64) narrow_job<E, PARTS, 64>(job, a, st);
+    else narrow_job<E, PARTS, 128>(job, a, st);
 }
 
-// three parts of 128 features would take more registers than a lane has
-bool narrow_supported(int dtype, int hidden) { return hidden <= (dtype == CNF_DTYPE_F32 ? 64 : 128); }
+bool narrow_supported(int hidden) { return hidden <= 128; }
 
 int narrow_launch(NarrowJob job, int dtype, const NarrowArgs& a, hipStream_t st) {
-    if (dtype == CNF_DTYPE_F32) narrow_width<bf16_t, 3>(job, a, st);
+    if (dtype == CNF_DTYPE_F32) narrow_width<f16_t, 2>(job, a, st);
     else if (dtype == CNF_DTYPE_BF16) narrow_width<bf16_t, 1>(job, a, st);
     else narrow_width<f16_t, 1>(job, a, st);
     return launch_status("cnf_linear_ce (few features)");

@@ -35,7 +35,7 @@ __device__ __forceinline__ f32x4 mfma16<f16_t>(s16x8 a, s16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec_t<f16_t, 8>, a), __builtin_bit_cast(vec_t<f16_t, 8>, b), c, 0, 0, 0);
 }
 
-// One operand: `parts` arrays of 16-bit elements, `part` elements apart (fp32 values split into three bf16 parts; 16-bit values: one).
+// One operand: `parts` arrays of 16-bit elements, `part` elements apart (fp32 values split into two fp16 parts; 16-bit values: one).
 // ld is a multiple of 8 and the base 16-byte aligned; a row has room for its extent rounded up to 8.
 struct Operand {
     const void* base;
@@ -109,10 +109,11 @@ __device__ __forceinline__ void tile_frags4(const char* lds, int ext0, int t0, i
     }
 }
 
-// Which parts are multiplied: 16-bit values (0, 0); fp32 values as x0 + x1 + x2 (each the bf16 nearest to what is left, 2^-9 of the
-// one before): the products of order up to 2, smallest first.  What is dropped is below 2^-26 of |a| |b| per product.
-__device__ __forceinline__ int pair_a(int pairs, int s) { return pairs == 1 ? 0 : (0x021010 >> (4 * (5 - s))) & 3; }
-__device__ __forceinline__ int pair_b(int pairs, int s) { return pairs == 1 ? 0 : (0x201100 >> (4 * (5 - s))) & 3; }
+// Which parts are multiplied: 16-bit values (0, 0); fp32 values, scaled so that the largest of their tensor lies in 2^14 ... 2^15, as
+// x0 + x1 (each the fp16 nearest to what is left: 2^-23 of the value, or 2^-25 in the scaled unit, stays out): (0, 1), (1, 0), (0, 0).
+// What is dropped, x1 y1, is below 2^-22 of |x| |y| and has either sign; fp32 products and sums round by 2^-24 each.
+__device__ __forceinline__ int pair_a(int pairs, int s) { return pairs == 3 && s == 1 ? 1 : 0; }
+__device__ __forceinline__ int pair_b(int pairs, int s) { return pairs == 3 && s == 0 ? 1 : 0; }
 
 template <typename E, bool KMA, bool KMB, int BM, int BN, int WM, int WN>
 struct TileProduct {
