@@ -5,6 +5,7 @@ compute entry point raises.  The library is built in-tree by ``categoricalnf_amd
 (``make -C categoricalnf_amd/csrc``); it is git-ignored but travels with the working tree.
 """
 import ctypes
+import importlib.util
 import os
 import re
 
@@ -95,8 +96,8 @@ SIGNATURES = {
     "cnf_mixture_params_bwd": [_p, _p, _p, _p, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p],
     "cnf_layer_norm": [_p, _i64, _p, _p, _p, _p, _p, _i64, _i, _f, _i, _i, _p],
     "cnf_layer_norm_bwd": [_p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i, _i, _i, _p],
-    "cnf_linear_ce": [_p, _i64, _p, _i64, _p, _p, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i, _i, _i, _i, _p, _p],
-    "cnf_linear_ce_bwd": [_p, _i64, _p, _i64, _p, _p, _i64, _p, _p, _p, _i, _p, _p, _p, _p, _p, _i64, _i64, _i, _i, _i, _i, _p],
+    "cnf_linear_ce": [_p, _i64, _p, _i64, _p, _p, _i64, _p, _p, _p, _p, _p, _p, _i64, _i64, _i, _i, _i, _i, _p, _p],
+    "cnf_linear_ce_bwd": [_p, _i64, _p, _i64, _p, _p, _i64, _p, _p, _p, _p, _i, _p, _p, _p, _p, _p, _i64, _i64, _i, _i, _i, _i, _p],
     "cnf_adamw_step": [_i, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _d, _d, _d, _d, _d, _d, _p, _p, _p],
     "cnf_adamw_moments": [_p, _p, _p, _p, _p, _p, _i64, _p],
     "cnf_stream_probe": [_p, _p, _p, ctypes.c_long, _i, _p],
@@ -158,6 +159,27 @@ def load():
                               "PyTorch-ROCm" % ", ".join(sorted(runtimes)))
     _lib = lib
     return lib
+
+
+TORCH_LIB_PATH = os.path.join(_HERE, "lib", "_cnf_torch.so")
+_native = None
+
+
+def native(hip_only_error):
+    """The host-side extension of the training step's operators (csrc/cnf_torch.cpp), bound to the loaded libcnf_hip.so."""
+    global _native
+    if _native is None:
+        lib = load()
+        if not os.path.exists(TORCH_LIB_PATH):
+            raise CnfLibraryError("host extension %s not found - build it with `make -C categoricalnf_amd/csrc`" % TORCH_LIB_PATH)
+        spec = importlib.util.spec_from_file_location("_cnf_torch", TORCH_LIB_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        names = ("cnf_last_error", "cnf_layer_norm", "cnf_layer_norm_bwd", "cnf_layer_norm_bwd_workspace_floats", "cnf_linear_ce",
+                 "cnf_linear_ce_bwd", "cnf_linear_ce_workspace_bytes", "cnf_adamw_step")
+        module.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names}, hip_only_error)
+        _native = module
+    return _native
 
 
 def exported_symbols():

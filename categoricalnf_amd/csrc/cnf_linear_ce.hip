@@ -268,18 +268,30 @@ __global__ __launch_bounds__(kBlock) void ce_largest_kernel(const float* x, int6
     const float* src = blockIdx.y ? w : x;
     const int64_t stride = blockIdx.y ? w_stride : x_stride, rows = blockIdx.y ? V : R;
     uint32_t top = 0;
-    if (stride == H) {
-        const int64_t n = rows * H;
-        for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (int64_t)kMaxBlocks * kBlock) {
-            const uint32_t b = __float_as_uint(src[i]) & 0x7fffffffu;
-            if (b < 0x7f800000u) top = max(top, b);
+    auto see = [&](float v) {
+        const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+        if (b < 0x7f800000u) top = max(top, b);
+    };
+    const int64_t step = (int64_t)kMaxBlocks * kBlock, at = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (stride == H && rows * H % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+        const f32x4* v = reinterpret_cast<const f32x4*>(src);
+        const int64_t n = rows * H / 4;
+        int64_t i = at;
+        for (; i + 3 * step < n; i += 4 * step) {           // four loads in flight
+            const f32x4 q[4] = {v[i], v[i + step], v[i + 2 * step], v[i + 3 * step]};
+#pragma unroll
+            for (int k = 0; k < 16; ++k) see(q[k / 4][k % 4]);
         }
+        for (; i < n; i += step) {
+            const f32x4 q = v[i];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) see(q[k]);
+        }
+    } else if (stride == H) {
+        for (int64_t i = at; i < rows * H; i += step) see(src[i]);
     } else {
         for (int64_t r = blockIdx.x; r < rows; r += kMaxBlocks)
-            for (int c = threadIdx.x; c < H; c += kBlock) {
-                const uint32_t b = __float_as_uint(src[r * stride + c]) & 0x7fffffffu;
-                if (b < 0x7f800000u) top = max(top, b);
-            }
+            for (int c = threadIdx.x; c < H; c += kBlock) see(src[r * stride + c]);
     }
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, kWave));
@@ -304,8 +316,10 @@ struct LayoutArgs {
     int bias_dtype, vocab, bias_pad;
     float* bias_out;                // nullable
     float bias_unit;
-    const uint32_t* largest;        // fp32: what ce_largest_kernel found ...
-    CeScales* scales;               // ... and where the exponents go
+    const uint32_t* largest;        // fp32: what ce_largest_kernel found,
+    const int* known;               // or the exponents themselves;
+    CeScales* scales;               // where they go ...
+    int* exponents;                 // ... and here (nullable)
 };
 
 // one launch for whatever a call has to lay out: blockIdx.y 0: x, 1: w, 2: the bias.  fp32: scaled, then x0 + x1, each the fp16 nearest
@@ -322,17 +336,24 @@ __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
     if (!job.src) return;
     int ex = 0;
     if (PARTS > 1) {
-        __shared__ uint32_t sh[kWavesPerBlock];
-        uint32_t top = a.largest[blockIdx.y * kMaxBlocks + threadIdx.x];
-        static_assert(kMaxBlocks == kBlock, "a lane reads one workgroup's value");
+        if (a.known) {
+            ex = a.known[blockIdx.y];
+        } else {
+            __shared__ uint32_t sh[kWavesPerBlock];
+            uint32_t top = a.largest[blockIdx.y * kMaxBlocks + threadIdx.x];
+            static_assert(kMaxBlocks == kBlock, "a lane reads one workgroup's value");
 #pragma unroll
-        for (int m = 32; m >= 1; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, kWave));
-        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
-        __syncthreads();
-        for (int k = 0; k < kWavesPerBlock; ++k) top = max(top, sh[k]);
-        // the largest into 2^14 ... 2^15 (subnormal numbers: as if of exponent -126); zeros alone stay as they are
-        if (top) ex = 14 - (max((int)(top >> 23), 1) - 127);
-        if (blockIdx.x == 0 && threadIdx.x == 0) a.scales->ex[blockIdx.y] = ex;
+            for (int m = 32; m >= 1; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, kWave));
+            if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
+            __syncthreads();
+            for (int k = 0; k < kWavesPerBlock; ++k) top = max(top, sh[k]);
+            // the largest into 2^14 ... 2^15 (subnormal numbers: as if of exponent -126); zeros alone stay as they are
+            if (top) ex = 14 - (max((int)(top >> 23), 1) - 127);
+        }
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            a.scales->ex[blockIdx.y] = ex;
+            if (a.exponents) a.exponents[blockIdx.y] = ex;
+        }
     }
     const T* src = static_cast<const T*>(job.src);
     E* dst = static_cast<E*>(job.dst);
@@ -727,15 +748,19 @@ static bool rows_aligned32(const void* p, int64_t stride) { return (reinterpret_
 
 template <typename T, typename E, int PARTS>
 static void ce_operands(CeArgs& a, const CePlan& p, const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias,
-                        int bias_dtype, float bias_unit, int64_t R, int V, int H, char* ws, hipStream_t st) {
+                        int bias_dtype, float bias_unit, const int* known, int* exponents, int64_t R, int V, int H, char* ws, hipStream_t st) {
     LayoutArgs l{};
     CeScales* scales = reinterpret_cast<CeScales*>(ws + p.scales_off);
     if constexpr (PARTS > 1) {
-        uint32_t* largest = reinterpret_cast<uint32_t*>(ws + p.largest_off);
-        CNF_LAUNCH(ce_largest_kernel, dim3(kMaxBlocks, 2), dim3(kBlock), 0, st, static_cast<const float*>(x), x_stride, R,
-                   static_cast<const float*>(w), w_stride, V, H, largest);
-        l.largest = largest;
+        if (!known) {
+            uint32_t* largest = reinterpret_cast<uint32_t*>(ws + p.largest_off);
+            CNF_LAUNCH(ce_largest_kernel, dim3(kMaxBlocks, 2), dim3(kBlock), 0, st, static_cast<const float*>(x), x_stride, R,
+                       static_cast<const float*>(w), w_stride, V, H, largest);
+            l.largest = largest;
+        }
+        l.known = known;
         l.scales = scales;
+        l.exponents = exponents;
     }
     if (p.copy_x) l.job[0] = LayoutJob{x, x_stride, R, ws + p.x_off};
     if (p.copy_w) l.job[1] = LayoutJob{w, w_stride, V, ws + p.w_off};
@@ -818,7 +843,7 @@ int64_t cnf_linear_ce_workspace_bytes(int64_t R, int V, int H, int dtype, int ba
 }
 
 int cnf_linear_ce(const void* x, int64_t x_stride, const void* weight, int64_t w_stride, const void* bias, const int64_t* target,
-                  int64_t ignore_index, float* loss, float* row_max, float* row_sum, float* reduced, void* workspace, int64_t workspace_bytes,
+                  int64_t ignore_index, float* loss, float* row_max, float* row_sum, float* reduced, int* exponents, void* workspace, int64_t workspace_bytes,
                   int64_t R, int V, int H, int dtype, int bias_dtype, int* flags, cnf_stream_t stream) {
     CE_CHECK("cnf_linear_ce");
     hipStream_t st = (hipStream_t)stream;
@@ -833,7 +858,7 @@ int cnf_linear_ce(const void* x, int64_t x_stride, const void* weight, int64_t w
             typedef decltype(t) T;
             typedef decltype(e) E;
             CeArgs a{};
-            ce_operands<T, E, decltype(parts)::value>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, 1.f, R, V, H, ws, st);
+            ce_operands<T, E, decltype(parts)::value>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, 1.f, nullptr, exponents, R, V, H, ws, st);
             a.target = target;
             a.ignore = ignore_index;
             a.partial = reinterpret_cast<float2*>(ws + p.partial_off);
@@ -862,8 +887,8 @@ int cnf_linear_ce(const void* x, int64_t x_stride, const void* weight, int64_t w
 }
 
 int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64_t w_stride, const void* bias, const int64_t* target,
-                      int64_t ignore_index, const float* row_max, const float* row_sum, const float* g, int g_per_row, const float* count,
-                      void* dx, void* dweight, void* dbias, void* workspace, int64_t workspace_bytes, int64_t R, int V, int H, int dtype,
+                      int64_t ignore_index, const float* row_max, const float* row_sum, const int* exponents, const float* g, int g_per_row,
+                      const float* count, void* dx, void* dweight, void* dbias, void* workspace, int64_t workspace_bytes, int64_t R, int V, int H, int dtype,
                       int bias_dtype, cnf_stream_t stream) {
     CE_CHECK("cnf_linear_ce_bwd");
     CNF_REQUIRE(R > 0, "cnf_linear_ce_bwd: no rows");
@@ -879,7 +904,7 @@ int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64
         typedef decltype(e) E;
         constexpr int PARTS = decltype(parts)::value;
         CeArgs a{};
-        ce_operands<T, E, PARTS>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, kLog2e, R, V, H, ws, st);
+        ce_operands<T, E, PARTS>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, kLog2e, exponents, nullptr, R, V, H, ws, st);
         RowState* state = reinterpret_cast<RowState*>(ws + p.state_off);
         a.state = state;
         // per-row gradients: every workgroup finds the largest |g| itself; few of them

@@ -6,7 +6,6 @@ sampling, benchmarks) the layer modules call `ops` directly; with it they go thr
 import ctypes
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
 from .ops import _f32, _launch, _mask_desc, _opt_f32, _pad2d, _length, _ptr, _stream
@@ -778,61 +777,20 @@ def needs_grad(*tensors):
     return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
 
 
-class LayerNormFn(torch.autograd.Function):
-    """(x, weight, bias) -> layer norm over the last axis; the backward also sums the parameters' gradients."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = ops.layer_norm(x, weight, bias, eps, want_stats=True)
-        ctx.save_for_backward(x, weight, mean, rstd)
-        ctx.param_dtype = weight.dtype if weight is not None else (bias.dtype if bias is not None else None)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        x, weight, mean, rstd = ctx.saved_tensors
-        dx, dw, db = ops.layer_norm_bwd(x, g, weight, mean, rstd, ctx.param_dtype, ctx.needs_input_grad[1], ctx.needs_input_grad[2])
-        return dx, dw, db, None
-
-
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
-    """Layer norm over the last axis (`ops.layer_norm`), differentiable in x, weight and bias."""
-    if needs_grad(x, weight, bias):
-        return LayerNormFn.apply(x, weight, bias, float(eps))
-    return ops.layer_norm(x, weight, bias, eps)
+    """Layer norm over the last axis (`ops.layer_norm`), differentiable (once) in x, weight and bias."""
+    return ops.native().layer_norm(x, weight, bias, eps)
 
 
-class LinearCrossEntropyFn(torch.autograd.Function):
-    """(x, weight, bias) -> softmax cross entropy of the linear layer: [R] losses, or their mean or sum."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, target, ignore_index, reduction):
-        loss, row_max, row_sum, reduced = ops.linear_cross_entropy(x, weight, target, bias, ignore_index, want_reduced=reduction != "none")
-        ctx.save_for_backward(x, weight, bias, target, row_max, row_sum, reduced)
-        ctx.ignore_index, ctx.reduction = ignore_index, reduction
-        if reduction == "none":
-            return loss
-        return reduced[0 if reduction == "mean" else 1].clone()
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        x, weight, bias, target, row_max, row_sum, reduced = ctx.saved_tensors
-        if ctx.reduction == "sum":
-            g = g.expand(row_max.shape)
-        dx, dw, db = ops.linear_cross_entropy_bwd(x, weight, target, bias, row_max, row_sum, g.contiguous(),
-                                                  reduced[2:] if ctx.reduction == "mean" else None, ctx.ignore_index, ctx.needs_input_grad[:3])
-        return dx, dw, db, None, None, None
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
 def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduction="mean"):
     """Softmax cross entropy of x @ weight.T + bias against integer targets without keeping the logits (`ops.linear_cross_entropy`),
-    differentiable in x, weight and bias.  reduction: "mean" over the rows that are not ignored (NaN if there are none), "sum",
+    differentiable (once) in x, weight and bias.  reduction: "mean" over the rows that are not ignored (NaN if there are none), "sum",
     or "none" (fp32 losses of target's shape; ignored rows 0)."""
-    if reduction not in ("mean", "sum", "none"):
+    if reduction not in _REDUCTIONS:
         raise ValueError("reduction is mean, sum or none, got %r" % (reduction,))
-    if needs_grad(x, weight, bias):
-        return LinearCrossEntropyFn.apply(x, weight, bias, target, int(ignore_index), reduction)
-    loss, _, _, reduced = ops.linear_cross_entropy(x, weight, target, bias, ignore_index, want_reduced=reduction != "none")
-    return loss if reduction == "none" else reduced[0 if reduction == "mean" else 1]
+    loss = ops.native().linear_ce(x, weight, target, bias, ignore_index, _REDUCTIONS[reduction], ops.flag_word(ops._dev(x)))
+    ops._after(x.device, "linear_cross_entropy")
+    return loss

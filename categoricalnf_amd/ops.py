@@ -2,7 +2,6 @@
 stream, torch tensors out.  PyTorch is plumbing here (device memory + streams); no arithmetic of the
 hot path is done with torch ops and there is no CPU path — CPU tensors raise.
 """
-import array
 import ctypes
 import math
 import os
@@ -1033,158 +1032,45 @@ def mixture_coupling_nll_launch(z, nn_out, mask, num_mixtures, z_out, ldj_out, l
 
 # ---- operators of the training step around the flow -----------------------------------------------------------------------------
 
-_DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # CNF_DTYPE_*
-
-
-def _float_code(t, name):
-    _dev(t)
-    code = _DTYPE_CODE.get(t.dtype)
-    if code is None:
-        raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
-    return code
-
-
-def _vector(t, n, name, device):
-    """An optional parameter vector of n elements on `device`: (dense tensor, dtype code) or (None, None)."""
-    if t is None:
-        return None, None
-    code = _float_code(t, name)
-    if t.device != device:
-        raise ValueError("%s is on %s, the input on %s" % (name, t.device, device))
-    if t.dim() != 1 or t.shape[0] != n:
-        raise ValueError("%s must have shape (%d,), got %s" % (name, n, tuple(t.shape)))
-    return (t if t.is_contiguous() else t.contiguous()), code
-
-
-def _rows(t):
-    """[..., C] as [rows, C] with unit column stride and one row stride: a view where the strides allow it, else a copy."""
-    m = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    return m if m.stride(1) == 1 or m.shape[1] == 1 else m.contiguous()
+def native():
+    """The host-side extension of these operators (argument checks, outputs, autograd nodes, tensor lists: csrc/cnf_torch.cpp)."""
+    return _lib.native(HipOnlyError)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, want_stats=False):
     """Layer norm over the last axis of x (float32, bfloat16 or float16; any leading shape; rows may lie apart): y of x's type,
     statistics in fp32.  weight, bias: [C], both of one type (fp32 or a 16-bit type), or None.  `want_stats`: also (mean, rstd)
     [rows] fp32, which the backward needs."""
-    code, dev = _float_code(x, "x"), x.device
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError("layer_norm needs a last axis of at least one element, got shape %s" % (tuple(x.shape),))
-    C = x.shape[-1]
-    w, wcode = _vector(weight, C, "weight", dev)
-    b, bcode = _vector(bias, C, "bias", dev)
-    if w is not None and b is not None and wcode != bcode:
-        raise TypeError("weight is %s, bias %s" % (w.dtype, b.dtype))
-    x2 = _rows(x)
-    R = x2.shape[0]
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    mean = rstd = None
-    if want_stats:
-        mean, rstd = torch.empty(2, R, dtype=torch.float32, device=dev).unbind(0)
-    _launch(dev, "cnf_layer_norm", _ptr(x2), x2.stride(0), _ptr(w), _ptr(b), _ptr(y), _ptr(mean), _ptr(rstd), R, C, float(eps), code,
-            wcode if wcode is not None else (bcode or 0), _stream(dev))
-    return (y, mean, rstd) if want_stats else y
+    out = native().layer_norm_raw(x, weight, bias, eps, want_stats)
+    return out if want_stats else out[0]
 
 
 def layer_norm_bwd(x, dy, weight, mean, rstd, param_dtype=None, want_weight=True, want_bias=True):
     """Gradients of layer_norm from its input, the upstream gradient and the kept statistics: (dx, dweight, dbias), the last two of
     `param_dtype` (default: the weight's type, else x's) or None."""
-    code, dev = _float_code(x, "x"), x.device
-    C = x.shape[-1]
-    if dy.shape != x.shape or dy.dtype != x.dtype:
-        raise ValueError("the gradient must have the input's shape and type, got %s %s for %s %s"
-                         % (tuple(dy.shape), dy.dtype, tuple(x.shape), x.dtype))
-    w, wcode = _vector(weight, C, "weight", dev)
-    pdt = param_dtype or (w.dtype if w is not None else x.dtype)
-    if w is not None and pdt != w.dtype:
-        raise TypeError("parameter gradients have the weight's type")
-    x2, g2 = _rows(x), _rows(dy)
-    R = x2.shape[0]
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    dw = torch.empty(C, dtype=pdt, device=dev) if want_weight else None
-    db = torch.empty(C, dtype=pdt, device=dev) if want_bias else None
-    ws, n = None, 0
-    if want_weight or want_bias:
-        n = int(_lib.load().cnf_layer_norm_bwd_workspace_floats(R, C))
-        ws = torch.empty(n, dtype=torch.float32, device=dev)
-    _launch(dev, "cnf_layer_norm_bwd", _ptr(x2), x2.stride(0), _ptr(g2), g2.stride(0), _ptr(w), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dw),
-            _ptr(db), _ptr(ws), n, R, C, code, _DTYPE_CODE[pdt], _stream(dev))
-    return dx, dw, db
-
-
-def _ce_operands(x, weight, target, bias):
-    """Checked operands of the linear cross entropy: (x [R, H], weight, bias, target [R], R, V, H, dtype code, bias dtype code, device)."""
-    code, dev = _float_code(x, "x"), x.device
-    if weight.dtype != x.dtype or _float_code(weight, "weight") != code:
-        raise TypeError("x is %s, weight %s" % (x.dtype, weight.dtype))
-    if weight.dim() != 2 or x.dim() < 1 or weight.shape[1] != x.shape[-1] or 0 in weight.shape:
-        raise ValueError("weight must be [V, H] with the H of x, both at least 1: got %s for x %s" % (tuple(weight.shape), tuple(x.shape)))
-    if not isinstance(target, torch.Tensor) or target.dtype not in (torch.int64, torch.int32):
-        raise TypeError("target must be an integer tensor (int64 or int32)")
-    if target.shape != x.shape[:-1]:
-        raise ValueError("target must have the shape of x without its last axis: got %s for %s" % (tuple(target.shape), tuple(x.shape)))
-    for t, name in ((weight, "weight"), (target, "target")):
-        if t.device != dev:
-            raise (HipOnlyError if not t.is_cuda else ValueError)("%s is on %s, x on %s" % (name, t.device, dev))
-    V, H = weight.shape
-    b, bcode = _vector(bias, V, "bias", dev)
-    if bcode not in (None, code, 0):
-        raise TypeError("bias is float32 or of the weight's type, got %s" % (bias.dtype,))
-    return (_rows(x), _rows(weight), b, target.reshape(-1).to(torch.int64).contiguous(), target.numel(), V, H, code,
-            bcode if bcode is not None else 0, dev)
+    return native().layer_norm_bwd_raw(x, dy, weight, mean, rstd, param_dtype or (weight.dtype if weight is not None else x.dtype), want_weight,
+                                       want_bias)
 
 
 def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, want_reduced=False):
     """Softmax cross entropy of the linear layer x @ weight.T + bias over a vocabulary, without its logits (cnf_linear_ce).
 
     x [..., H] and weight [V, H] float32, bfloat16 or float16; bias [V] of that type or float32; target [...] integers.  Returns
-    (loss [...] fp32, row_max [R], row_sum [R], reduced or None): rows with target == ignore_index have loss 0, a category outside
-    [0, V) raises the flag that `check_flags` reports.  reduced: [mean, sum, count] over the rows that are not ignored."""
-    x2, w2, b, t, R, V, H, code, bcode, dev = _ce_operands(x, weight, target, bias)
-    loss = torch.empty(target.shape, dtype=torch.float32, device=dev)
-    row_max, row_sum = torch.empty(2, R, dtype=torch.float32, device=dev).unbind(0)
-    reduced = torch.empty(3, dtype=torch.float32, device=dev) if want_reduced else None
-    n = int(_lib.load().cnf_linear_ce_workspace_bytes(R, V, H, code, 0))
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    _launch(dev, "cnf_linear_ce", _ptr(x2), x2.stride(0), _ptr(w2), w2.stride(0), _ptr(b), _ptr(t), int(ignore_index), _ptr(loss),
-            _ptr(row_max), _ptr(row_sum), _ptr(reduced), _ptr(ws), n, R, V, H, code, bcode, _ptr(flag_word(dev)), _stream(dev))
-    _after(dev, "linear_cross_entropy")
-    return loss, row_max, row_sum, reduced
+    (loss [...] fp32, stats [2, R]: the rows' maximum logit and sum of exponentials, reduced [mean, sum, count] over the rows that
+    are not ignored or None, exponents); rows with target == ignore_index have loss 0, a category outside [0, V) raises the flag that
+    `check_flags` reports."""
+    out = native().linear_ce_raw(x, weight, target, bias, ignore_index, want_reduced, flag_word(_dev(x)))
+    _after(x.device, "linear_cross_entropy")
+    return out
 
 
-def linear_cross_entropy_bwd(x, weight, target, bias, row_max, row_sum, g, count=None, ignore_index=-100, want=(True, True, True)):
+def linear_cross_entropy_bwd(x, weight, target, bias, stats, g, count=None, ignore_index=-100, exponents=None, want=(True, True, True)):
     """Gradients (dx, dweight, dbias) of linear_cross_entropy for the upstream gradient g: [R] fp32, or — with `count`, the third
-    value of `reduced` — the gradient of the mean.  `want`: which of the three."""
-    x2, w2, b, t, R, V, H, code, bcode, dev = _ce_operands(x, weight, target, bias)
-    want_w = want[1] or (want[2] and b is not None)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want[0] else None
-    dw = torch.empty(V, H, dtype=x.dtype, device=dev) if want_w else None
-    db = torch.empty(V, dtype=b.dtype, device=dev) if want[2] and b is not None else None
-    if R == 0 or (dx is None and dw is None):
-        for t_ in (dw, db):
-            if t_ is not None:
-                t_.zero_()
-        return dx, dw, db
-    g = _f32(g, "g").reshape(-1)
-    if g.numel() != (1 if count is not None else R):
-        raise ValueError("the upstream gradient has %d values for %d rows" % (g.numel(), R))
-    n = int(_lib.load().cnf_linear_ce_workspace_bytes(R, V, H, code, 1))
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    _launch(dev, "cnf_linear_ce_bwd", _ptr(x2), x2.stride(0), _ptr(w2), w2.stride(0), _ptr(b), _ptr(t), int(ignore_index), _ptr(row_max),
-            _ptr(row_sum), _ptr(g), int(count is None), _ptr(count), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), n, R, V, H, code, bcode,
-            _stream(dev))
-    return dx, (dw if want[1] else None), db
+    value of `reduced` — the gradient of the mean.  `exponents`: the forward's, or None.  `want`: which of the three."""
+    return native().linear_ce_bwd_raw(x, weight, target, bias, stats, exponents, g, count, ignore_index, *want)
 
 
 ADAMW_BLOCK = 256           # consecutive elements of a tensor that share the two scales of its 8-bit moments
-
-
-def _scalar(v, name, device):
-    """A step's number: (host double, None) or (0.0, device fp32 scalar)."""
-    if not isinstance(v, torch.Tensor):
-        return float(v), None
-    if v.device != device or v.dtype != torch.float32 or v.numel() != 1:
-        raise ValueError("%s as a tensor is one float32 value on the parameters' device, got %s on %s" % (name, v.dtype, v.device))
-    return 0.0, v
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=1e-2,
@@ -1194,50 +1080,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, beta1=0.9, bet
     params: dense tensors of one type (fp32, bf16, fp16) on one device; grads: of that type or fp32.  Moments in fp32 — or, with
     the two lists of scales ([ceil(n / 256)] fp32 each), in 8 bits: exp_avgs int8, exp_avg_sqs uint8 codes.  `step` (the number of
     this step, from 1) and `lr` are numbers, or float32 device scalars that the kernel reads (for a captured step)."""
-    n = len(params)
-    bits8 = exp_avg_scales is not None
-    if (exp_avg_sq_scales is not None) != bits8:
-        raise ValueError("8-bit moments need both lists of scales")
-    lists = [params, grads, exp_avgs, exp_avg_sqs] + ([exp_avg_scales, exp_avg_sq_scales] if bits8 else [])
-    if any(len(l) != n for l in lists):
-        raise ValueError("adamw_step: lists of %s tensors" % ([len(l) for l in lists],))
-    if n == 0:
-        return
-    dev = _dev(params[0])
-    pdt, gdt = params[0].dtype, grads[0].dtype
-    pcode, gcode = _float_code(params[0], "params"), _float_code(grads[0], "grads")
-    if gdt != pdt and gdt != torch.float32:
-        raise TypeError("gradients are float32 or of the parameters' type, got %s for %s" % (gdt, pdt))
-    numel = array.array("q", [p.numel() for p in params])
-    kept = []                                             # dense copies of gradients: alive until the launches are enqueued
-    if not all(map(torch.Tensor.is_contiguous, grads)):
-        grads = kept = [g.contiguous() for g in grads]
-    want = ((params, pdt, "params"), (grads, gdt, "grads"), (exp_avgs, torch.int8 if bits8 else torch.float32, "exp_avgs"),
-            (exp_avg_sqs, torch.uint8 if bits8 else torch.float32, "exp_avg_sqs"))
-    for l, dt, name in want:
-        for t, k in zip(l, numel):
-            if t.dtype is not dt or t.numel() != k or t.device != dev or not t.is_contiguous():
-                raise ValueError("adamw_step: %s must be dense %s tensors of the parameters' sizes on %s, got %s %s on %s"
-                                 % (name, dt, dev, tuple(t.shape), t.dtype, t.device))
-    if bits8:
-        for l in (exp_avg_scales, exp_avg_sq_scales):
-            for t, k in zip(l, numel):
-                if t.dtype is not torch.float32 or t.numel() != -(-k // ADAMW_BLOCK) or t.device != dev or not t.is_contiguous():
-                    raise ValueError("adamw_step: a scale list must hold dense float32 tensors of ceil(n / %d) elements on %s" % (ADAMW_BLOCK, dev))
-    addresses = [array.array("Q", [t.data_ptr() for t in l]) for l in lists[:1] + [grads] + lists[2:]]
-    for l in (addresses[0], addresses[2], addresses[3]):
-        if len(set(l)) != n and len(set(a for a, k in zip(l, numel) if k)) != sum(k > 0 for k in numel):
-            raise ValueError("adamw_step: a parameter or a moment is listed twice")
-    if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0):
-        raise ValueError("adamw_step: betas outside [0, 1)")
-    step_host, step_dev = _scalar(step, "step", dev)
-    lr_host, lr_dev = _scalar(lr, "lr", dev)
-    if step_dev is None and step_host < 1:
-        raise ValueError("adamw_step: the first step is step 1, got %r" % (step,))
-    at = [ctypes.c_void_p(a.buffer_info()[0]) for a in addresses] + ([] if bits8 else [None, None])
-    _launch(dev, "cnf_adamw_step", n, *at, ctypes.c_void_p(numel.buffer_info()[0]), pcode, gcode, 8 if bits8 else 32, lr_host, float(beta1),
-            float(beta2), float(eps), float(weight_decay), step_host, _ptr(lr_dev), _ptr(step_dev), _stream(dev))
-    del kept
+    native().adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps, weight_decay, exp_avg_scales, exp_avg_sq_scales,
+                        ADAMW_BLOCK)
 
 
 def adamw_moments(exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale):

@@ -647,20 +647,21 @@ int cnf_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64_t 
  * stride, `x_stride` / `w_stride` elements between rows; bias [V] of `bias_dtype` (nullable); target int64 [R].  Rows with target ==
  * ignore_index have loss 0; any other target outside [0, V) raises CNF_FLAG_CATEGORY and its loss is NaN.  row_max, row_sum [R]: the
  * maximum logit and sum_v exp(logit - maximum), which the backward takes; reduced [3] (nullable): mean (NaN over no rows), sum and
- * number of the rows that are not ignored.  fp32 products are exact to 2^-22 of the operands' sizes (three fp16
+ * number of the rows that are not ignored; exponents [2] (nullable): the powers of two that fp32 operands were scaled by, which the
+ * backward takes back instead of looking for the largest elements again.  fp32 products are exact to 2^-22 of the operands' sizes (three fp16
  * products of operands scaled by a power of two per tensor and split in two), 16-bit products are exact; sums, maxima and exponentials
  * are fp32.  workspace_bytes >= cnf_linear_ce_workspace_bytes(R, V, H, dtype, 0). */
 int64_t cnf_linear_ce_workspace_bytes(int64_t R, int V, int H, int dtype, int backward);
 int cnf_linear_ce(const void* x, int64_t x_stride, const void* weight, int64_t w_stride, const void* bias, const int64_t* target,
-                  int64_t ignore_index, float* loss, float* row_max, float* row_sum, float* reduced, void* workspace,
-                  int64_t workspace_bytes, int64_t R, int V, int H, int dtype, int bias_dtype, int* flags, cnf_stream_t stream);
-/* Its gradients: dx [R, H], dweight [V, H] dense of `dtype`, dbias [V] of `bias_dtype` (each nullable; dbias needs dweight) for the
+                  int64_t ignore_index, float* loss, float* row_max, float* row_sum, float* reduced, int* exponents,
+                  void* workspace, int64_t workspace_bytes, int64_t R, int V, int H, int dtype, int bias_dtype, int* flags, cnf_stream_t stream);
+/* Its gradients (exponents: the forward's, or NULL): dx [R, H], dweight [V, H] dense of `dtype`, dbias [V] of `bias_dtype` (each nullable; dbias needs dweight) for the
  * upstream gradient g: fp32 [R] (g_per_row != 0), or one value that is divided by *count (the mean's).  Ignored rows and rows with a
  * target outside the vocabulary have gradient 0.  The gradient of the logits is computed in pieces of the vocabulary and rounded to
  * `dtype` (fp32: to 2^-22), relative to the largest |g|; sums are fp32, in a fixed order.  workspace_bytes >= cnf_linear_ce_workspace_bytes(..., 1). */
 int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64_t w_stride, const void* bias, const int64_t* target,
-                      int64_t ignore_index, const float* row_max, const float* row_sum, const float* g, int g_per_row, const float* count,
-                      void* dx, void* dweight, void* dbias, void* workspace, int64_t workspace_bytes, int64_t R, int V, int H, int dtype,
+                      int64_t ignore_index, const float* row_max, const float* row_sum, const int* exponents, const float* g,
+                      int g_per_row, const float* count, void* dx, void* dweight, void* dbias, void* workspace, int64_t workspace_bytes, int64_t R, int V, int H, int dtype,
                       int bias_dtype, cnf_stream_t stream);
 
 /* One AdamW step over `count` dense tensors: m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g^2,

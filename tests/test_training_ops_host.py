@@ -58,8 +58,50 @@ def test_adamw_refuses_before_launching(lib):
     assert lib.cnf_adamw_moments(None, P, P, P, P, P, 4, None) == 1 and lib.cnf_adamw_moments(P, P, P, P, P, P, 0, None) == 0
 
 
+def test_linear_ce_refuses_before_launching(lib):
+    need = lib.cnf_linear_ce_workspace_bytes(100, 50, 16, 0, 0)
+    assert need > 0 and lib.cnf_linear_ce_workspace_bytes(0, 50, 16, 0, 0) == 0 and lib.cnf_linear_ce_workspace_bytes(10, 50, 16, 9, 0) == 0
+    #     x  xs  w  ws  b     t  ign   loss max sum red   exp   ws bytes R    V   H   dt bdt flags stream
+    ok = [P, 16, P, 16, None, P, -100, P, P, P, None, None, P, need, 100, 50, 16, 0, 0, None, None]
+    for i, bad in ((0, None), (2, None), (5, None), (7, None), (8, None), (9, None), (12, None), (13, need - 1), (14, -1), (15, 0), (16, 0), (17, 3),
+                   (18, -1), (1, -16), (12, ctypes.c_void_p(24))):
+        args = list(ok)
+        args[i] = bad
+        assert lib.cnf_linear_ce(*args) == 1 and b"cnf_linear_ce" in lib.cnf_last_error(), i
+    assert lib.cnf_linear_ce(*(ok[:14] + [0] + ok[15:])) == 0                     # no rows and nothing to reduce
+    need = lib.cnf_linear_ce_workspace_bytes(100, 50, 16, 0, 1)
+    #     x  xs  w  ws  b     t  ign   max sum exp   g  per count dx dw db   ws bytes R    V   H   dt bdt stream
+    ok = [P, 16, P, 16, None, P, -100, P, P, None, P, 1, None, P, P, None, P, need, 100, 50, 16, 0, 0, None]
+    for i, bad in ((0, None), (2, None), (5, None), (7, None), (8, None), (10, None), (11, 0), (16, None), (17, need - 1), (18, 0), (19, 0), (21, 4),
+                   (16, ctypes.c_void_p(20))):
+        args = list(ok)
+        args[i] = bad
+        assert lib.cnf_linear_ce_bwd(*args) == 1 and b"cnf_linear_ce_bwd" in lib.cnf_last_error(), i
+    for none in ((13, 14), (14,)):                                               # nothing asked for; dbias without dweight
+        args = list(ok)
+        args[15] = P if none == (14,) else None
+        for i in none:
+            args[i] = None
+        assert lib.cnf_linear_ce_bwd(*args) == 1
+
+
+def test_linear_ce_workspace_is_bounded(lib):
+    """The gradient of the logits never takes more than 256 MiB beyond what one strip of 256 classes needs, however large the
+    vocabulary: nothing of size rows x vocabulary is kept."""
+    for rows, vocab, hidden in ((8192, 200_000, 1024), (100_000, 50_000, 512), (1, 10 ** 6, 4096)):
+        for dtype, parts in ((0, 2), (1, 1), (2, 1)):
+            n = lib.cnf_linear_ce_workspace_bytes(rows, vocab, hidden, dtype, 1)
+            copies = parts * 2 * (rows + vocab) * (hidden + 8)
+            partial = 64 * rows * (hidden + 8) * 4 + 64 * vocab * (hidden + 8) * 4 if rows < 1000 else 3 * (rows + vocab) * (hidden + 8) * 4
+            assert n <= copies + partial + max(256 << 20, (rows + 256) * 256 * 2 * parts) + (rows + 256) * 16 + (1 << 20), (rows, vocab, n)
+
+
 def test_cpu_tensors_are_refused():
     x = torch.randn(3, 4)
+    with pytest.raises(ops.HipOnlyError):
+        Fn.linear_cross_entropy(x, torch.randn(5, 4), torch.tensor([0, 1, 2]))
+    with pytest.raises(ops.HipOnlyError):
+        ops.linear_cross_entropy(x, torch.randn(5, 4), torch.tensor([0, 1, 2]))
     with pytest.raises(ops.HipOnlyError):
         ops.layer_norm(x)
     with pytest.raises(ops.HipOnlyError):
