@@ -73,7 +73,7 @@ template <typename E, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 2) void ce_lse_kernel(const CeArgs a) {
     typedef TileProduct<E, false, false, BM, BN, WM, WN> Tile;
     __shared__ __align__(16) char lds[Tile::kLds];
-    const Tile tile(a.w, a.x, a.pairs, a.hidden, lds);
+    Tile tile(a.w, a.x, a.pairs, a.hidden, lds);
     const unsigned t = xcd_contiguous(blockIdx.x, gridDim.x);
     const int split = t % a.splits;
     const int r0 = (t / a.splits) * BN;
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_lse_kernel(const CeArgs a)
         for (int m = 0; m < Tile::MT; ++m)
 #pragma unroll
             for (int n = 0; n < Tile::NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-        tile.run(v0, r0, 0, a.hidden, acc, [](int) {});
+        tile.run(v0, r0, 0, a.hidden, acc, [](int, int) {});
         const int vw = v0 + tile.m_wave + g * 4;        // the lane's first entry
         if (a.bias || a.scaled) {
             const float back = logit_scale(a, 1.f);
@@ -425,7 +425,7 @@ template <typename E, int PARTS, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
     typedef TileProduct<E, false, false, BM, BN, WM, WN> Tile;
     __shared__ __align__(16) char lds[Tile::kLds];
-    const Tile tile(a.w, a.x, a.pairs, a.hidden, lds);
+    Tile tile(a.w, a.x, a.pairs, a.hidden, lds);
     const unsigned nv = (a.v1 - a.v0 + BM - 1) / BM, nr = gridDim.x / nv;
     unsigned ti, tj;
     grouped_tile(xcd_contiguous(blockIdx.x, gridDim.x), nv, nr, ti, tj);
@@ -435,7 +435,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
     for (int m = 0; m < Tile::MT; ++m)
 #pragma unroll
         for (int n = 0; n < Tile::NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    tile.run(v0, r0, 0, a.hidden, acc, [](int) {});
+    tile.run(v0, r0, 0, a.hidden, acc, [](int, int) {});
     const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
     const int vw = v0 + tile.m_wave + g * 4;
     RowState st[Tile::NT];
@@ -521,7 +521,7 @@ template <typename E, bool KMB, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 2) void ce_grad_kernel(const GradArgs a) {
     typedef TileProduct<E, true, KMB, BM, BN, WM, WN> Tile;
     __shared__ __align__(16) char lds[Tile::kLds];
-    const Tile tile(a.a, a.b, a.pairs, a.k_end, lds);
+    Tile tile(a.a, a.b, a.pairs, a.k_end, lds);
     const unsigned nm = (a.m_end + BM - 1) / BM, nn = (a.n_end + BN - 1) / BN, per = nm * nn;
     const unsigned t = xcd_contiguous(blockIdx.x, gridDim.x);
     const unsigned ks = t / per;
@@ -542,21 +542,13 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_grad_kernel(const GradArgs
 #pragma unroll
     for (int i = 0; i < 8; ++i) ones[i] = __builtin_bit_cast(short, (E)1.f);
     // fp32: each part of d is once the partner of part 0 of x: pairs (0, 1) and (0, 0)
-    int step = 0;
-    const int per_pair = (k1 - k0 + kStepK - 1) / kStepK;
-    tile.run(m0, n0, k0, k1, acc, [&](int stage) {
-        if (!sums) return;
-        const int pair = step / per_pair;
-        ++step;
-        if (pair_a(a.pairs, pair) != 0) return;
+    tile.run(m0, n0, k0, k1, acc, [&](int stage, int pair) {
+        if (!sums || pair_a(a.pairs, pair) != 0) return;
         const char* sb = lds + stage * Tile::kStage + Tile::kBytesA;
+        s16x8 fb[4];
+        tile_frags4<KMB, BN>(sb, tile.n_wave, 0, fb);
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            s16x8 fb[4];
-            tile_frags4<KMB, BN>(sb, tile.n_wave, 0, kk, fb);
-#pragma unroll
-            for (int n = 0; n < Tile::NT; ++n) acc1[n] = mfma16<E>(ones, fb[n], acc1[n]);
-        }
+        for (int n = 0; n < Tile::NT; ++n) acc1[n] = mfma16<E>(ones, fb[n], acc1[n]);
     });
     const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
     const float down = a.scales->top / a.lift;
@@ -725,7 +717,7 @@ static CePlan ce_plan(int64_t R, int V, int H, int dtype, bool x_ok, bool w_ok, 
         big = ceil_div(n, kBig) * ceil_div(H, kBig) >= 128 && H > kSmall;
         const int edge = big ? kBig : kSmall;
         const int64_t tiles = ceil_div(n, edge) * ceil_div(H, edge), steps = ceil_div(k, kStepK);
-        return (int)std::max<int64_t>(1, std::min<int64_t>({steps / 4, ceil_div(big ? 256 : 512, tiles), 64}));
+        return (int)std::max<int64_t>(1, std::min<int64_t>({steps / 8, ceil_div(big ? 256 : 512, tiles), 64}));
     };
     p.dx_split = split(R, width, p.big_dx);
     p.dw_split = split(width, R, p.big_dw);
@@ -823,7 +815,10 @@ static void ce_sum(const void* partial, int parts, int64_t rows, int cols, int64
     else CNF_LAUNCH(ce_sum_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(n, kBlock), 8192)), dim3(kBlock), 0, st, a);
 }
 
-static bool ce_aligned(const void* p, int64_t stride, int dtype, int H) { return rows_aligned16(p, stride, dtype) && H % 8 == 0; }
+// rows that the products may read as they are: whole 16-byte chunks, and 256 of them within reach of a 31-bit offset
+static bool ce_aligned(const void* p, int64_t stride, int dtype, int H) {
+    return rows_aligned16(p, stride, dtype) && H % 8 == 0 && stride < (1 << 21);
+}
 
 }  // namespace cnf
 

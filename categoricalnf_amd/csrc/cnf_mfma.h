@@ -1,12 +1,14 @@
 // 16-bit matrix products on the matrix cores (v_mfma_f32_16x16x32), shared by the kernels of the linear cross entropy.
 //
-// A workgroup computes a BM x BN tile of D[m][n] = sum_k A[m][k] B[n][k] in steps of 64 k.  Both operands of a step are copied
-// straight into LDS (16 bytes per lane, no registers) while the step before it is multiplied.  Either operand may lie in memory
-//   * k-contiguous ([ext][k]: a row of 64 k is 128 bytes = 8 chunks), or
+// A workgroup computes a BM x BN tile of D[m][n] = sum_k A[m][k] B[n][k] in steps of 32 k.  Both operands of a step are copied
+// straight into LDS (16 bytes per lane, no registers), three steps ahead into a ring of four stages; a step issues its copies between
+// its matrix instructions (issued together in front of them they held every wave for the time the address unit takes).  Either operand
+// may lie in memory
+//   * k-contiguous ([ext][k]: a row of 32 k is 64 bytes = 4 chunks), or
 //   * k-major ([k][ext]: fragments are then read with the transposing LDS read, 4 k x 16 columns for 16 lanes).
-// Chunks are stored permuted (k-contiguous: chunk c of row r at c ^ (r & 7); k-major: 32-byte unit u of row k at u ^ f(k)), so that
-// the 64 lanes of a fragment read touch all banks evenly; the copy applies the permutation to its source addresses.  Chunks outside
-// an operand are copied from a block of zeros: edges cost no branch in the inner loop, and nothing outside a tensor is read.
+// Chunks are stored permuted (k-contiguous: chunk c of row r at c ^ (r / 4 & 3); k-major: 32-byte unit u of row k at u ^ f(k)), so that
+// the 64 lanes of a fragment read touch all banks evenly; the copy applies the permutation to its source addresses.  Nothing outside a
+// tensor is read.
 //
 // Fragment layout (lane l, g = l / 16): A and B hold k = 8 g ... 8 g + 7 of row l % 16; D holds n = l % 16, m = 4 g ... 4 g + 3.
 #pragma once
@@ -20,7 +22,8 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kStepK = 64;
+constexpr int kStepK = 32;
+constexpr int kStages = 4;
 
 __device__ const uint32_t kZeroChunk[4] = {0, 0, 0, 0};
 
@@ -43,50 +46,71 @@ struct Operand {
     int ext;            // rows of D (columns) that exist
 };
 
-// copies the ext0 ... ext0 + EXT - 1, k0 ... k0 + 63 tile
+// Copies the ext0 ... ext0 + EXT - 1, k0 ... k0 + 31 tile.  A lane's chunk lies at the same offset from the tile's first element in every
+// step, so a step whose 32 k all exist costs no vector arithmetic: a scalar base moves on.  Chunks outside `ext` repeat one that exists
+// (they reach outputs that are not there); the last, partial step takes chunks behind k_end from a block of zeros.
 template <bool KMAJOR, int EXT, int THREADS>
-__device__ __forceinline__ void tile_copy(const Operand& o, int part, int ext0, int k0, int k_end, char* lds) {
-    constexpr int CH = EXT * 8 / THREADS;
-    static_assert(CH * THREADS == EXT * 8, "whole chunks per lane");
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint16_t* base = static_cast<const uint16_t*>(o.base) + (int64_t)part * o.part;
-#pragma unroll
-    for (int j = 0; j < CH; ++j) {
-        const int q = j * THREADS + tid;
-        int e, k;
-        int64_t off;
+struct TileCopy {
+    static constexpr int CH = EXT * 4 / THREADS;
+    static_assert(CH * THREADS == EXT * 4, "whole chunks per lane");
+    uint32_t off[CH];           // bytes
+
+    __device__ __forceinline__ static void place(int j, int& e, int& k) {
+        const int q = j * THREADS + threadIdx.x;
         if (!KMAJOR) {
-            const int row = q >> 3, c = (q & 7) ^ (row & 7);
-            e = ext0 + row;
-            k = k0 + c * 8;
-            off = (int64_t)e * o.ld + k;
+            const int row = q >> 2;
+            e = row;
+            k = ((q & 3) ^ ((row >> 2) & 3)) * 8;
         } else {
             constexpr int CPR = EXT / 8;
             const int kr = q / CPR, slot = q % CPR;
-            const int c = (((slot >> 1) ^ ((kr & 3) | ((kr >> 1) & 4))) << 1) | (slot & 1);
-            e = ext0 + c * 8;
-            k = k0 + kr;
-            off = (int64_t)k * o.ld + e;
+            e = (((((slot >> 1) ^ ((kr & 3) | ((kr >> 1) & 4))) << 1) | (slot & 1))) * 8;
+            k = kr;
         }
-        const void* src = (e < o.ext && k < k_end) ? static_cast<const void*>(base + off) : static_cast<const void*>(kZeroChunk);
-        __builtin_amdgcn_global_load_lds((glb_cvoid_t*)src, (lds_void16_t*)(lds + (j * THREADS + wave * 64) * 16), 16, 0, 0);
     }
-}
+    __device__ __forceinline__ void aim(const Operand& o, int ext0) {
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+            int e, k;
+            place(j, e, k);
+            if (ext0 + e >= o.ext) e = KMAJOR ? 0 : o.ext - 1 - ext0;
+            off[j] = (uint32_t)(KMAJOR ? k * (int)o.ld + e : e * (int)o.ld + k) * 2u;
+        }
+    }
+    __device__ __forceinline__ void copy(const Operand& o, int part, int ext0, int k0, int k_end, char* lds) const {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const char* base = static_cast<const char*>(o.base) +
+                           2 * ((int64_t)part * o.part + (KMAJOR ? (int64_t)k0 * o.ld + ext0 : (int64_t)ext0 * o.ld + k0));
+        if (k0 + kStepK <= k_end) {
+#pragma unroll
+            for (int j = 0; j < CH; ++j)
+                __builtin_amdgcn_global_load_lds((glb_cvoid_t*)(base + off[j]), (lds_void16_t*)(lds + (j * THREADS + wave * 64) * 16), 16, 0, 0);
+        } else {
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+                int e, k;
+                place(j, e, k);
+                const void* src = k0 + k < k_end ? static_cast<const void*>(base + off[j]) : static_cast<const void*>(kZeroChunk);
+                __builtin_amdgcn_global_load_lds((glb_cvoid_t*)src, (lds_void16_t*)(lds + (j * THREADS + wave * 64) * 16), 16, 0, 0);
+            }
+        }
+    }
+};
 
-// the fragments of rows (columns) ext0 + 16 t ... + 15, t = t0 ... t0 + 3, k = 32 kk ... 32 kk + 31 of a tile
+// the fragments of rows (columns) ext0 + 16 t ... + 15, t = t0 ... t0 + 3, of a tile
 template <bool KMAJOR, int EXT>
-__device__ __forceinline__ void tile_frags4(const char* lds, int ext0, int t0, int kk, s16x8 (&out)[4]) {
+__device__ __forceinline__ void tile_frags4(const char* lds, int ext0, int t0, s16x8 (&out)[4]) {
     const int l = threadIdx.x & 63, g = l >> 4, i = l & 15;
     if (!KMAJOR) {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
-            out[t] = *reinterpret_cast<const s16x8*>(lds + (ext0 + (t0 + t) * 16 + i) * 128 + (((kk * 4 + g) ^ (i & 7)) << 4));
+            out[t] = *reinterpret_cast<const s16x8*>(lds + (ext0 + (t0 + t) * 16 + i) * 64 + ((g ^ (i >> 2)) << 4));
     } else {
         // In assembly: in front of the builtin the compiler drains every copy to LDS that is in flight (it cannot tell which stage a
         // transposing read touches), which would undo the overlap.  The reads are waited for in the same block; the outputs are
         // early-clobbered, so no read in flight lands on an address of a later one.
         const int f = (i >> 2) | ((g & 1) << 2);
-        const uint32_t row = (uint32_t)(uintptr_t)(lds_void16_t*)lds + (kk * 32 + g * 8 + (i >> 2)) * (EXT * 2) + (i & 3) * 8;
+        const uint32_t row = (uint32_t)(uintptr_t)(lds_void16_t*)lds + (g * 8 + (i >> 2)) * (EXT * 2) + (i & 3) * 8;
         uint32_t at[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) at[t] = row + (((ext0 >> 4) + t0 + t) ^ f) * 32;
@@ -120,8 +144,8 @@ struct TileProduct {
     static constexpr int kThreads = WM * WN * 64;
     static constexpr int MT = BM / WM / 16, NT = BN / WN / 16;
     static constexpr int kBytesA = BM * kStepK * 2, kBytesB = BN * kStepK * 2, kStage = kBytesA + kBytesB;
-    static constexpr int kLds = 2 * kStage;
-    static constexpr int kCopies = (BM + BN) * 8 / kThreads;        // copies in flight per lane and step
+    static constexpr int kLds = kStages * kStage;
+    static constexpr int kCopies = (BM + BN) * 4 / kThreads;        // copies per lane and step
 
     static_assert(NT == 4 && MT % 4 == 0, "fragments are read in fours");
 
@@ -137,72 +161,74 @@ struct TileProduct {
         n_wave = (wave / WM) * (BN / WN);
     }
 
-    __device__ __forceinline__ void copy(int m0, int n0, int pair, int k0, int stage) const {
-        char* s = lds + stage * kStage;
-        tile_copy<KMA, BM, kThreads>(a, pair_a(pairs, pair), m0, k0, k_end, s);
-        tile_copy<KMB, BN, kThreads>(b, pair_b(pairs, pair), n0, k0, k_end, s + kBytesA);
-    }
+    TileCopy<KMA, BM, kThreads> ca;
+    TileCopy<KMB, BN, kThreads> cb;
 
-    // wait until all copies but the `newer` last ones of this lane have landed, then for the other waves
+    // wait until this wave's copies but the `NEWER` last steps' have landed and its fragments have been read, then for the other waves:
+    // the oldest step in flight is there for everyone, and the stage before it may be overwritten
     template <int NEWER>
-    __device__ __forceinline__ static void landed() {
-        if (NEWER == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        else if (NEWER == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-        else if (NEWER == 6) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-        static_assert(NEWER == 0 || NEWER == 4 || NEWER == 6 || NEWER == 8, "a wait for this many copies is missing");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-    }
-    // every wave has read its fragments of the stage: it may be overwritten
-    __device__ __forceinline__ static void read_done() {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __device__ __forceinline__ static void arrive() {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(NEWER * kCopies) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     }
 
-    __device__ __forceinline__ void multiply(int stage, f32x4 (&acc)[MT][NT]) const {
-        const char* sa = lds + stage * kStage;
-        const char* sb = sa + kBytesA;
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
+    // acc += the tile's product over k0 ... k1 - 1 (k0 a multiple of 32); extra(stage, pair) sees every stage before it is given up
+    template <typename Extra>
+    __device__ __forceinline__ void run(int m0, int n0, int k0, int k1, f32x4 (&acc)[MT][NT], Extra&& extra) {
+        const int ksteps = (k1 - k0 + kStepK - 1) / kStepK, total = ksteps * pairs;
+        if (total <= 0) return;
+        ca.aim(a, m0);
+        cb.aim(b, n0);
+        int cp = 0, ck = 0;         // the next step to be copied: its pair and k step
+        auto next = [&]() {
+            if (++ck == ksteps) {
+                ck = 0;
+                ++cp;
+            }
+        };
+        for (int s = 0; s < kStages - 1 && s < total; ++s, next()) {
+            ca.copy(a, pair_a(pairs, cp), m0, k0 + ck * kStepK, k_end, lds + s * kStage);
+            cb.copy(b, pair_b(pairs, cp), n0, k0 + ck * kStepK, k_end, lds + s * kStage + kBytesA);
+        }
+        int pair = 0, ks = 0;
+        for (int s = 0; s < total; ++s) {
+            const int left = total - 1 - s;
+            if (left >= 2) arrive<2>();
+            else if (left == 1) arrive<1>();
+            else arrive<0>();
+            const char* sa = lds + (s % kStages) * kStage;
+            const char* sb = sa + kBytesA;
+            char* ahead = lds + ((s + kStages - 1) % kStages) * kStage;
+            const bool more = left >= kStages - 1;
             s16x8 fb[4];
-            tile_frags4<KMB, BN>(sb, n_wave, 0, kk, fb);
+            tile_frags4<KMB, BN>(sb, n_wave, 0, fb);
 #pragma unroll
             for (int m = 0; m < MT; m += 4) {
                 s16x8 fa[4];
-                tile_frags4<KMA, BM>(sa, m_wave, m, kk, fa);
+                tile_frags4<KMA, BM>(sa, m_wave, m, fa);
+                if (more && m == 0) ca.copy(a, pair_a(pairs, cp), m0, k0 + ck * kStepK, k_end, ahead);
+                if (more && m == MT - 4) {
+                    cb.copy(b, pair_b(pairs, cp), n0, k0 + ck * kStepK, k_end, ahead + kBytesA);
+                    next();
+                }
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int n = 0; n < NT; ++n) acc[m + i][n] = mfma16<E>(fa[i], fb[n], acc[m + i][n]);
+                __builtin_amdgcn_s_setprio(0);
             }
-        }
-    }
-
-    // acc += the tile's product over k0 ... k1 - 1 (k0 a multiple of 64); extra(stage) sees every stage before it is given up
-    template <typename Extra>
-    __device__ __forceinline__ void run(int m0, int n0, int k0, int k1, f32x4 (&acc)[MT][NT], Extra&& extra) const {
-        const int ksteps = (k1 - k0 + kStepK - 1) / kStepK, total = ksteps * pairs;
-        if (total <= 0) return;
-        int pair = 0, ks = 0, stage = 0;
-        copy(m0, n0, 0, k0, 0);
-        for (int s = 0; s < total; ++s) {
+            extra(s % kStages, pair);
             if (++ks == ksteps) {
                 ks = 0;
                 ++pair;
             }
-            if (s + 1 < total) {
-                copy(m0, n0, pair, k0 + ks * kStepK, stage ^ 1);
-                landed<kCopies>();
-            } else {
-                landed<0>();
-            }
-            multiply(stage, acc);
-            extra(stage);
-            read_done();
-            stage ^= 1;
         }
+        // the ring may be used again
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
     }
 };
 
