@@ -28,7 +28,7 @@ struct CeArgs {
     Operand w, x;                   // [V][H], [R][H]
     int pairs, parts;
     int64_t rows;
-    int vocab, hidden;
+    int vocab, hidden, k_end;       // k_end: of the products (copied operands: the padded row)
     const void* bias;
     int bias_dtype;
     const int64_t* target;
@@ -73,7 +73,7 @@ template <typename E, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 2) void ce_lse_kernel(const CeArgs a) {
     typedef TileProduct<E, false, false, BM, BN, WM, WN> Tile;
     __shared__ __align__(16) char lds[Tile::kLds];
-    Tile tile(a.w, a.x, a.pairs, a.hidden, lds);
+    Tile tile(a.w, a.x, a.pairs, a.k_end, lds);
     const unsigned t = xcd_contiguous(blockIdx.x, gridDim.x);
     const int split = t % a.splits;
     const int r0 = (t / a.splits) * BN;
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_lse_kernel(const CeArgs a)
         for (int m = 0; m < Tile::MT; ++m)
 #pragma unroll
             for (int n = 0; n < Tile::NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-        tile.run(v0, r0, 0, a.hidden, acc, [](int, int) {});
+        tile.run(v0, r0, 0, a.k_end, acc, [](int, int) {});
         const int vw = v0 + tile.m_wave + g * 4;        // the lane's first entry
         if (a.bias || a.scaled) {
             const float back = logit_scale(a, 1.f);
@@ -363,7 +363,7 @@ __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
         const int64_t r = q / per;
         const int c0 = (int)(q - r * per) * 8;
         vec_t<T, 8> in;
-        if ((a.vec >> blockIdx.y) & 1) {
+        if (((a.vec >> blockIdx.y) & 1) && c0 + 8 <= a.cols) {
             in = *reinterpret_cast<const vec_t<T, 8>*>(src + r * job.stride + c0);
         } else {
 #pragma unroll
@@ -425,7 +425,7 @@ template <typename E, int PARTS, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
     typedef TileProduct<E, false, false, BM, BN, WM, WN> Tile;
     __shared__ __align__(16) char lds[Tile::kLds];
-    Tile tile(a.w, a.x, a.pairs, a.hidden, lds);
+    Tile tile(a.w, a.x, a.pairs, a.k_end, lds);
     const unsigned nv = (a.v1 - a.v0 + BM - 1) / BM, nr = gridDim.x / nv;
     unsigned ti, tj;
     grouped_tile(xcd_contiguous(blockIdx.x, gridDim.x), nv, nr, ti, tj);
@@ -435,7 +435,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
     for (int m = 0; m < Tile::MT; ++m)
 #pragma unroll
         for (int n = 0; n < Tile::NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    tile.run(v0, r0, 0, a.hidden, acc, [](int, int) {});
+    tile.run(v0, r0, 0, a.k_end, acc, [](int, int) {});
     const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
     const int vw = v0 + tile.m_wave + g * 4;
     RowState st[Tile::NT];
@@ -668,7 +668,7 @@ static CePlan ce_plan(int64_t R, int V, int H, int dtype, bool x_ok, bool w_ok, 
     p.copy_x = p.parts > 1 || !x_ok;
     p.copy_w = p.parts > 1 || !w_ok;
     p.narrow = narrow_supported(H);
-    p.ldh = round_up(H, 8);
+    p.ldh = round_up(H, p.narrow ? 8 : kStepK);     // whole steps of the products
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         const int64_t o = at;
@@ -780,6 +780,7 @@ static void ce_operands(CeArgs& a, const CePlan& p, const void* x, int64_t x_str
     a.rows = R;
     a.vocab = V;
     a.hidden = H;
+    a.k_end = p.copy_x && p.copy_w ? (int)p.ldh : H;
     a.bias = bias;
     a.bias_dtype = bias_dtype;
     a.scales = scales;

@@ -2,7 +2,8 @@
 //
 // A workgroup computes a BM x BN tile of D[m][n] = sum_k A[m][k] B[n][k] in steps of 32 k.  Both operands of a step are copied
 // straight into LDS (16 bytes per lane, no registers), three steps ahead into a ring of four stages; a step issues its copies between
-// its matrix instructions (issued together in front of them they held every wave for the time the address unit takes).  Either operand
+// its matrix instructions (issued together in front of them they held every wave for the time the address unit takes), and the steps in
+// the middle are unrolled over the ring (its bookkeeping cost 8 %).  8192 x 8192 x 1024 bf16: 1.26 PFLOP/s, the library's 8192^3 1.24.  Either operand
 // may lie in memory
 //   * k-contiguous ([ext][k]: a row of 32 k is 64 bytes = 4 chunks), or
 //   * k-major ([k][ext]: fragments are then read with the transposing LDS read, 4 k x 16 columns for 16 lanes).
@@ -77,22 +78,27 @@ struct TileCopy {
             off[j] = (uint32_t)(KMAJOR ? k * (int)o.ld + e : e * (int)o.ld + k) * 2u;
         }
     }
-    __device__ __forceinline__ void copy(const Operand& o, int part, int ext0, int k0, int k_end, char* lds) const {
+    // the tile's first element, and how far the next step's is
+    __device__ __forceinline__ static const char* base(const Operand& o, int part, int ext0, int k0) {
+        return static_cast<const char*>(o.base) + 2 * ((int64_t)part * o.part + (KMAJOR ? (int64_t)k0 * o.ld + ext0 : (int64_t)ext0 * o.ld + k0));
+    }
+    __device__ __forceinline__ static int64_t advance(const Operand& o) { return 2 * (KMAJOR ? kStepK * o.ld : (int64_t)kStepK); }
+    __device__ __forceinline__ void copy_whole(const char* from, char* lds) const {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const char* base = static_cast<const char*>(o.base) +
-                           2 * ((int64_t)part * o.part + (KMAJOR ? (int64_t)k0 * o.ld + ext0 : (int64_t)ext0 * o.ld + k0));
-        if (k0 + kStepK <= k_end) {
 #pragma unroll
-            for (int j = 0; j < CH; ++j)
-                __builtin_amdgcn_global_load_lds((glb_cvoid_t*)(base + off[j]), (lds_void16_t*)(lds + (j * THREADS + wave * 64) * 16), 16, 0, 0);
-        } else {
+        for (int j = 0; j < CH; ++j)
+            __builtin_amdgcn_global_load_lds((glb_cvoid_t*)(from + off[j]), (lds_void16_t*)(lds + (j * THREADS + wave * 64) * 16), 16, 0, 0);
+    }
+    // k0: the step's first k
+    __device__ __forceinline__ void copy(const char* from, int k0, int k_end, char* lds) const {
+        if (k0 + kStepK <= k_end) return copy_whole(from, lds);
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
-            for (int j = 0; j < CH; ++j) {
-                int e, k;
-                place(j, e, k);
-                const void* src = k0 + k < k_end ? static_cast<const void*>(base + off[j]) : static_cast<const void*>(kZeroChunk);
-                __builtin_amdgcn_global_load_lds((glb_cvoid_t*)src, (lds_void16_t*)(lds + (j * THREADS + wave * 64) * 16), 16, 0, 0);
-            }
+        for (int j = 0; j < CH; ++j) {
+            int e, k;
+            place(j, e, k);
+            const void* src = k0 + k < k_end ? static_cast<const void*>(from + off[j]) : static_cast<const void*>(kZeroChunk);
+            __builtin_amdgcn_global_load_lds((glb_cvoid_t*)src, (lds_void16_t*)(lds + (j * THREADS + wave * 64) * 16), 16, 0, 0);
         }
     }
 };
@@ -101,19 +107,24 @@ struct TileCopy {
 template <bool KMAJOR, int EXT>
 __device__ __forceinline__ void tile_frags4(const char* lds, int ext0, int t0, s16x8 (&out)[4]) {
     const int l = threadIdx.x & 63, g = l >> 4, i = l & 15;
+    // the stage's address as a scalar of its own: with the unrolled steps' stages folded in, every fragment's address of every stage is
+    // kept in a register (26 of them spilled)
+    uint32_t stage = (uint32_t)(uintptr_t)(lds_void16_t*)lds;
+    asm volatile("" : "+s"(stage));
     if (!KMAJOR) {
+        typedef __attribute__((address_space(3))) const s16x8 lds_s16x8;
+        const uint32_t at = stage + (ext0 + t0 * 16 + i) * 64 + ((g ^ (i >> 2)) << 4);
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-            out[t] = *reinterpret_cast<const s16x8*>(lds + (ext0 + (t0 + t) * 16 + i) * 64 + ((g ^ (i >> 2)) << 4));
+        for (int t = 0; t < 4; ++t) out[t] = *(lds_s16x8*)(uintptr_t)(at + t * 1024);
     } else {
         // In assembly: in front of the builtin the compiler drains every copy to LDS that is in flight (it cannot tell which stage a
         // transposing read touches), which would undo the overlap.  The reads are waited for in the same block; the outputs are
         // early-clobbered, so no read in flight lands on an address of a later one.
         const int f = (i >> 2) | ((g & 1) << 2);
-        const uint32_t row = (uint32_t)(uintptr_t)(lds_void16_t*)lds + (g * 8 + (i >> 2)) * (EXT * 2) + (i & 3) * 8;
+        const uint32_t row = (g * 8 + (i >> 2)) * (EXT * 2) + (i & 3) * 8;
         uint32_t at[4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) at[t] = row + (((ext0 >> 4) + t0 + t) ^ f) * 32;
+        for (int t = 0; t < 4; ++t) at[t] = stage + (row + (((ext0 >> 4) + t0 + t) ^ f) * 32);
         s16x4 lo[4], hi[4];
         asm volatile(
             "ds_read_b64_tr_b16 %0, %8\n\t"
@@ -173,6 +184,32 @@ struct TileProduct {
         asm volatile("" ::: "memory");
     }
 
+    __device__ __forceinline__ void multiply4(int m, const s16x8 (&fa)[4], const s16x8 (&fb)[4], f32x4 (&acc)[MT][NT]) const {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[m + i][n] = mfma16<E>(fa[i], fb[n], acc[m + i][n]);
+        __builtin_amdgcn_s_setprio(0);
+    }
+
+    // a step in the middle: its stage is known, three more steps follow, and the one it copies is whole
+    template <int STAGE, typename Extra>
+    __device__ __forceinline__ void middle_step(const char* pa, const char* pb, int pair, f32x4 (&acc)[MT][NT], Extra&& extra) const {
+        constexpr int kAhead = (STAGE + kStages - 1) % kStages;
+        arrive<2>();
+        const char* sa = lds + STAGE * kStage;
+        s16x8 fb[4], fa[MT / 4][4];
+        tile_frags4<KMB, BN>(sa + kBytesA, n_wave, 0, fb);
+        tile_frags4<KMA, BM>(sa, m_wave, 0, fa[0]);
+        ca.copy_whole(pa, lds + kAhead * kStage);
+        multiply4(0, fa[0], fb, acc);
+        if (MT > 4) tile_frags4<KMA, BM>(sa, m_wave, 4, fa[MT / 4 - 1]);
+        cb.copy_whole(pb, lds + kAhead * kStage + kBytesA);
+        if (MT > 4) multiply4(MT - 4, fa[MT / 4 - 1], fb, acc);
+        extra(STAGE, pair);
+    }
+
     // acc += the tile's product over k0 ... k1 - 1 (k0 a multiple of 32); extra(stage, pair) sees every stage before it is given up
     template <typename Extra>
     __device__ __forceinline__ void run(int m0, int n0, int k0, int k1, f32x4 (&acc)[MT][NT], Extra&& extra) {
@@ -180,50 +217,61 @@ struct TileProduct {
         if (total <= 0) return;
         ca.aim(a, m0);
         cb.aim(b, n0);
-        int cp = 0, ck = 0;         // the next step to be copied: its pair and k step
+        int cp = 0, ck = 0;         // the next step to be copied: its pair and k step ...
+        const char *pa = ca.base(a, pair_a(pairs, 0), m0, k0), *pb = cb.base(b, pair_b(pairs, 0), n0, k0);      // ... and where it begins
+        const int64_t da = ca.advance(a), db = cb.advance(b);
         auto next = [&]() {
             if (++ck == ksteps) {
                 ck = 0;
                 ++cp;
+                pa = ca.base(a, pair_a(pairs, cp), m0, k0);
+                pb = cb.base(b, pair_b(pairs, cp), n0, k0);
+            } else {
+                pa += da;
+                pb += db;
+            }
+        };
+        int pair = 0, ks = 0;
+        auto done = [&]() {
+            if (++ks == ksteps) {
+                ks = 0;
+                ++pair;
             }
         };
         for (int s = 0; s < kStages - 1 && s < total; ++s, next()) {
-            ca.copy(a, pair_a(pairs, cp), m0, k0 + ck * kStepK, k_end, lds + s * kStage);
-            cb.copy(b, pair_b(pairs, cp), n0, k0 + ck * kStepK, k_end, lds + s * kStage + kBytesA);
+            ca.copy(pa, k0 + ck * kStepK, k_end, lds + s * kStage);
+            cb.copy(pb, k0 + ck * kStepK, k_end, lds + s * kStage + kBytesA);
         }
-        int pair = 0, ks = 0;
-        for (int s = 0; s < total; ++s) {
+        // whole steps, four at a time; a partial one can only be the last of a pair
+        const int whole = k0 + ksteps * kStepK <= k_end ? total : (pairs == 1 ? total - 1 : 0);
+        int s = 0;
+        for (; s + 2 * kStages - 1 <= whole; s += kStages) {
+            middle_step<0>(pa, pb, pair, acc, extra); next(); done();
+            middle_step<1>(pa, pb, pair, acc, extra); next(); done();
+            middle_step<2>(pa, pb, pair, acc, extra); next(); done();
+            middle_step<3>(pa, pb, pair, acc, extra); next(); done();
+        }
+        for (; s < total; ++s, done()) {
             const int left = total - 1 - s;
             if (left >= 2) arrive<2>();
             else if (left == 1) arrive<1>();
             else arrive<0>();
             const char* sa = lds + (s % kStages) * kStage;
-            const char* sb = sa + kBytesA;
-            char* ahead = lds + ((s + kStages - 1) % kStages) * kStage;
-            const bool more = left >= kStages - 1;
+            if (left >= kStages - 1) {
+                char* ahead = lds + ((s + kStages - 1) % kStages) * kStage;
+                ca.copy(pa, k0 + ck * kStepK, k_end, ahead);
+                cb.copy(pb, k0 + ck * kStepK, k_end, ahead + kBytesA);
+                next();
+            }
             s16x8 fb[4];
-            tile_frags4<KMB, BN>(sb, n_wave, 0, fb);
+            tile_frags4<KMB, BN>(sa + kBytesA, n_wave, 0, fb);
 #pragma unroll
             for (int m = 0; m < MT; m += 4) {
                 s16x8 fa[4];
                 tile_frags4<KMA, BM>(sa, m_wave, m, fa);
-                if (more && m == 0) ca.copy(a, pair_a(pairs, cp), m0, k0 + ck * kStepK, k_end, ahead);
-                if (more && m == MT - 4) {
-                    cb.copy(b, pair_b(pairs, cp), n0, k0 + ck * kStepK, k_end, ahead + kBytesA);
-                    next();
-                }
-                __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) acc[m + i][n] = mfma16<E>(fa[i], fb[n], acc[m + i][n]);
-                __builtin_amdgcn_s_setprio(0);
+                multiply4(m, fa, fb, acc);
             }
             extra(s % kStages, pair);
-            if (++ks == ksteps) {
-                ks = 0;
-                ++pair;
-            }
         }
         // the ring may be used again
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
