@@ -1,6 +1,7 @@
 // Softmax cross entropy of a linear layer over a vocabulary, forward and backward, without keeping the logits.
 //
 //   l_rv = x_r . w_v + b_v,   m_r = max_v l_rv,   s_r = sum_v exp(l_rv - m_r),   loss_r = log s_r + (m_r - l_rt)
+//   (the kernels keep l and m in units of log 2: one instruction less per exponential)
 //   d_rv = g_r (exp(l_rv - m_r) / s_r - [v = t_r]),   dx = d w,   dw = d^T x,   db_v = sum_r d_rv
 //
 // Forward: a product whose tiles never leave the registers.  A workgroup owns a block of rows and a part of the vocabulary; every
@@ -99,13 +100,13 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_lse_kernel(const CeArgs a)
             for (int n = 0; n < Tile::NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
         tile.run(v0, r0, 0, a.k_end, acc, [](int, int) {});
         const int vw = v0 + tile.m_wave + g * 4;        // the lane's first entry
-        if (a.bias || a.scaled) {
-            const float back = logit_scale(a, 1.f);
+        {
+            const float back = logit_scale(a, kLog2e);
 #pragma unroll
             for (int m = 0; m < Tile::MT; ++m)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float b = bias_at(a, vw + m * 16 + i);
+                    const float b = a.bias ? bias_at(a, vw + m * 16 + i) * kLog2e : 0.f;
 #pragma unroll
                     for (int n = 0; n < Tile::NT; ++n) acc[m][n][i] = __builtin_fmaf(acc[m][n][i], back, b);
                 }
@@ -136,11 +137,11 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_lse_kernel(const CeArgs a)
                 for (int i = 0; i < 4; ++i) top = fmaxf(top, acc[m][n][i]);
             // a lane that has seen only -inf keeps the sum 0 (exp(-inf - 0)); fmaxf drops a NaN, the sum keeps it
             const float ref = top == -INFINITY ? 0.f : top;
-            float s = sum[n] * __builtin_amdgcn_exp2f((mx[n] - ref) * kLog2e);
+            float s = sum[n] * __builtin_amdgcn_exp2f(mx[n] - ref);
 #pragma unroll
             for (int m = 0; m < Tile::MT; ++m)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s += __builtin_amdgcn_exp2f((acc[m][n][i] - ref) * kLog2e);
+                for (int i = 0; i < 4; ++i) s += __builtin_amdgcn_exp2f(acc[m][n][i] - ref);
             sum[n] = s;
             mx[n] = top;
         }
@@ -154,7 +155,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_lse_kernel(const CeArgs a)
         for (int x = 16; x <= 32; x <<= 1) {
             const float om = __shfl_xor(m, x, kWave), os = __shfl_xor(s, x, kWave);
             const float nm = fmaxf(m, om), ref = nm == -INFINITY ? 0.f : nm;
-            s = s * __builtin_amdgcn_exp2f((m - ref) * kLog2e) + os * __builtin_amdgcn_exp2f((om - ref) * kLog2e);
+            s = s * __builtin_amdgcn_exp2f(m - ref) + os * __builtin_amdgcn_exp2f(om - ref);
             m = nm;
         }
         if (g == 0) sh[(tile.m_wave / (BM / WM)) * BN + tile.n_wave + n * 16 + col] = make_float2(m, s);
@@ -168,7 +169,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_lse_kernel(const CeArgs a)
         for (int w = 0; w < WM; ++w) {
             const float2 o = sh[w * BN + n];
             const float nm = fmaxf(m, o.x), ref = nm == -INFINITY ? 0.f : nm;
-            s = s * __builtin_amdgcn_exp2f((m - ref) * kLog2e) + o.y * __builtin_amdgcn_exp2f((o.x - ref) * kLog2e);
+            s = s * __builtin_amdgcn_exp2f(m - ref) + o.y * __builtin_amdgcn_exp2f(o.x - ref);
             m = nm;
         }
         a.partial[(int64_t)split * a.rows + r] = make_float2(m, s);
@@ -190,7 +191,7 @@ __global__ __launch_bounds__(kBlock) void ce_join_kernel(const float2* partial, 
         const float ref = m == -INFINITY ? 0.f : m;
         for (int k = 0; k < splits; ++k) {
             const float2 o = partial[(int64_t)k * rows + r];
-            s += o.y * __builtin_amdgcn_exp2f((o.x - ref) * kLog2e);
+            s += o.y * __builtin_amdgcn_exp2f(o.x - ref);
         }
         row_max[r] = m;
         row_sum[r] = s;
@@ -201,7 +202,7 @@ __global__ __launch_bounds__(kBlock) void ce_join_kernel(const float2* partial, 
                 raise_flag(flags, CNF_FLAG_CATEGORY);
                 v = NAN;
             } else {
-                v = logf(s) + (m - target_logit[r]);
+                v = logf(s) + (m - target_logit[r]) * kLn2;
             }
         }
         loss[r] = v;
@@ -312,10 +313,9 @@ struct LayoutArgs {
     LayoutJob job[2];               // x and w: [rows][cols] -> `parts` arrays of [rows][ld] 16-bit elements, zeros behind cols
     int cols, vec;                  // vec: bit j: 8 elements of job j's rows may be read as vectors of 16 bytes
     int64_t ld;
-    const void* bias;               // -> fp32, -inf behind the vocabulary (nullable: zeros)
+    const void* bias;               // -> fp32, times log2 e, -inf behind the vocabulary (nullable: zeros)
     int bias_dtype, vocab, bias_pad;
     float* bias_out;                // nullable
-    float bias_unit;
     const uint32_t* largest;        // fp32: what ce_largest_kernel found,
     const int* known;               // or the exponents themselves;
     CeScales* scales;               // where they go ...
@@ -329,7 +329,7 @@ __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
     if (blockIdx.y == 2) {
         if (a.bias_out)
             for (int v = blockIdx.x * kBlock + threadIdx.x; v < a.bias_pad; v += gridDim.x * kBlock)
-                a.bias_out[v] = v >= a.vocab ? -INFINITY : (a.bias ? load_any(a.bias, a.bias_dtype, v) * a.bias_unit : 0.f);
+                a.bias_out[v] = v >= a.vocab ? -INFINITY : (a.bias ? load_any(a.bias, a.bias_dtype, v) * kLog2e : 0.f);
         return;
     }
     const LayoutJob job = a.job[blockIdx.y];
@@ -411,9 +411,8 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(const float* g, int g_is_
         const int64_t t = r < rows ? target[r] : -1;
         const bool in = r < rows && t != ignore && t >= 0 && t < vocab;
         RowState s;
-        // exp(l - m) = exp2(l L - m2) exp2(m2 - m L), L = log2 e, m2 = m L rounded: one fma per element, the row's rest in its scale
-        s.m2 = in ? row_max[r] * kLog2e : INFINITY;
-        s.inv_s = in ? __builtin_amdgcn_exp2f(-__builtin_fmaf(row_max[r], kLog2e, -s.m2)) / row_sum[r] : 0.f;
+        s.m2 = in ? row_max[r] : INFINITY;
+        s.inv_s = in ? 1.f / row_sum[r] : 0.f;
         s.g = in ? (g_is_row ? g[r] : shared) / top : 0.f;
         s.target = in ? (int)t : -1;
         state[r] = s;
@@ -474,11 +473,12 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
             const int64_t r = (int64_t)r0 + tile.n_wave + n * 16 + col;
             f32x4 p;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[m][n][i], back, b[i] - st[n].m2)) * scale[n];
+            for (int i = 0; i < 4; ++i)             // the logit rounded as in the forward, then the difference: the row's maximum gives 1
+                p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[m][n][i], back, b[i]) - st[n].m2) * scale[n];
             if (any_hit) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (at[n] == m * 16 + i && st[n].target >= 0) p[i] -= own_g[n];
+                    if (at[n] == m * 16 + i) p[i] -= own_g[n];          // an ignored row's is negative
             }
             if (edge) {
 #pragma unroll
@@ -489,11 +489,17 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
             if (st[n].target < 0) p = f32x4{0.f, 0.f, 0.f, 0.f};
             vec_t<E, 4> o[PARTS];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; i += 2)
 #pragma unroll
                 for (int k = 0; k < PARTS; ++k) {
-                    o[k][i] = (E)p[i];
-                    p[i] = PARTS > 1 ? p[i] - (float)o[k][i] : 0.f;
+                    const uint32_t h = pack2<E>(p[i], p[i + 1]);
+                    reinterpret_cast<uint32_t*>(&o[k])[i / 2] = h;
+                    if (k + 1 < PARTS) {
+                        float lo = p[i], hi = p[i + 1];
+                        minus_halves(h, lo, hi);
+                        p[i] = lo;
+                        p[i + 1] = hi;
+                    }
                 }
 #pragma unroll
             for (int k = 0; k < PARTS; ++k)
@@ -740,7 +746,7 @@ static bool rows_aligned32(const void* p, int64_t stride) { return (reinterpret_
 
 template <typename T, typename E, int PARTS>
 static void ce_operands(CeArgs& a, const CePlan& p, const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias,
-                        int bias_dtype, float bias_unit, const int* known, int* exponents, int64_t R, int V, int H, char* ws, hipStream_t st) {
+                        int bias_dtype, const int* known, int* exponents, int64_t R, int V, int H, char* ws, hipStream_t st) {
     LayoutArgs l{};
     CeScales* scales = reinterpret_cast<CeScales*>(ws + p.scales_off);
     if constexpr (PARTS > 1) {
@@ -763,7 +769,6 @@ static void ce_operands(CeArgs& a, const CePlan& p, const void* x, int64_t x_str
     if (p.narrow) {
         l.bias = bias;
         l.bias_dtype = bias_dtype;
-        l.bias_unit = bias_unit;
         l.vocab = V;
         l.bias_pad = (int)round_up(V, kNarrowWalk);
         l.bias_out = reinterpret_cast<float*>(ws + p.bias_off);
@@ -854,7 +859,7 @@ int cnf_linear_ce(const void* x, int64_t x_stride, const void* weight, int64_t w
             typedef decltype(t) T;
             typedef decltype(e) E;
             CeArgs a{};
-            ce_operands<T, E, decltype(parts)::value>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, 1.f, nullptr, exponents, R, V, H, ws, st);
+            ce_operands<T, E, decltype(parts)::value>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, nullptr, exponents, R, V, H, ws, st);
             a.target = target;
             a.ignore = ignore_index;
             a.partial = reinterpret_cast<float2*>(ws + p.partial_off);
@@ -900,7 +905,7 @@ int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64
         typedef decltype(e) E;
         constexpr int PARTS = decltype(parts)::value;
         CeArgs a{};
-        ce_operands<T, E, PARTS>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, kLog2e, exponents, nullptr, R, V, H, ws, st);
+        ce_operands<T, E, PARTS>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, exponents, nullptr, R, V, H, ws, st);
         RowState* state = reinterpret_cast<RowState*>(ws + p.state_off);
         a.state = state;
         // per-row gradients: every workgroup finds the largest |g| itself; few of them

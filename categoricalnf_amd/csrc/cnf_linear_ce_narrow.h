@@ -5,9 +5,9 @@
 
 namespace cnf {
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
-struct RowState {       // backward: what an element d = (exp2(l log2 e - m2) inv_s - [target]) g needs of its row
+struct RowState {       // backward: what an element d = (exp2(l2 - m2) inv_s - [target]) g, l2 = l log2 e, needs of its row
     float m2, inv_s;    // maximum times log2 e (+inf: the row is ignored); 1 / s
     float g;            // over the largest |g|
     int target;         // -1: ignored
@@ -27,7 +27,7 @@ struct NarrowArgs {
     int hidden, vocab;
     int64_t rows;
     int splits;                         // of the walk
-    const float* bias;                  // [vocabulary rounded up to kNarrowWalk] fp32, -inf behind the last entry; backward: times log2 e
+    const float* bias;                  // [vocabulary rounded up to kNarrowWalk] fp32, times log2 e, -inf behind the last entry
     // forward
     const int64_t* target;
     int64_t ignore;

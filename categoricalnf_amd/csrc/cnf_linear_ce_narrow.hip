@@ -58,22 +58,41 @@ struct NarrowTile {
         const int l = threadIdx.x & 63, i = l & 15, row = (l >> 4) * 4 + (i >> 2), c = h * 2 + ((i & 3) >> 1);
         return row * (HP * 2) + ((c ^ narrow_swizzle<HP>(row)) << 4) + (i & 1) * 8;
     }
-    // two of them, h and h + 1; in assembly, waited for in the same block, like the transposing reads of cnf_mfma.h
-    template <int PART>
-    __device__ static void frag_t2(uint32_t at0, uint32_t at1, s16x8 (&out)[2]) {
+    // N of them (2 or 4); in assembly, waited for in the same block, like the transposing reads of cnf_mfma.h
+    template <int PART, int N>
+    __device__ static void frag_t(const uint32_t* base, uint32_t tile_at, s16x8 (&out)[N]) {
         constexpr int kOff = PART * kPart;
-        s16x4 v[2][2];
-        asm volatile(
-            "ds_read_b64_tr_b16 %0, %4 offset:%6\n\t"
-            "ds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
-            "ds_read_b64_tr_b16 %2, %5 offset:%6\n\t"
-            "ds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
-            "s_waitcnt lgkmcnt(0)"
-            : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1])
-            : "v"(at0), "v"(at1), "n"(kOff), "n"(kOff + 16 * HP * 2)
-            : "memory");
+        static_assert(N == 2 || N == 4, "two or four");
+        uint32_t at[N];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) out[h] = __builtin_shufflevector(v[h][0], v[h][1], 0, 1, 2, 3, 4, 5, 6, 7);
+        for (int h = 0; h < N; ++h) at[h] = base[h] + tile_at;
+        s16x4 v[N][2];
+        if constexpr (N == 2)
+            asm volatile(
+                "ds_read_b64_tr_b16 %0, %4 offset:%6\n\t"
+                "ds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+                "ds_read_b64_tr_b16 %2, %5 offset:%6\n\t"
+                "ds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+                "s_waitcnt lgkmcnt(0)"
+                : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1])
+                : "v"(at[0]), "v"(at[1]), "n"(kOff), "n"(kOff + 16 * HP * 2)
+                : "memory");
+        else
+            asm volatile(
+                "ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
+                "ds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+                "ds_read_b64_tr_b16 %2, %9 offset:%12\n\t"
+                "ds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+                "ds_read_b64_tr_b16 %4, %10 offset:%12\n\t"
+                "ds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+                "ds_read_b64_tr_b16 %6, %11 offset:%12\n\t"
+                "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+                "s_waitcnt lgkmcnt(0)"
+                : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1]), "=&v"(v[2][0]), "=&v"(v[2][1]), "=&v"(v[3][0]), "=&v"(v[3][1])
+                : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(kOff), "n"(kOff + 16 * HP * 2)
+                : "memory");
+#pragma unroll
+        for (int h = 0; h < N; ++h) out[h] = __builtin_shufflevector(v[h][0], v[h][1], 0, 1, 2, 3, 4, 5, 6, 7);
     }
 };
 
@@ -88,9 +107,10 @@ __device__ __forceinline__ void static_for(Fn&& fn) {
 }
 
 template <typename E, int PARTS, int HP, NarrowJob JOB>
-__global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a) {
+__global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(const NarrowArgs a) {
     typedef NarrowTile<HP, PARTS> Tile;
     constexpr int NT = 2, KK = HP / 32, HT = HP / 16;
+    constexpr int HB = HT < 4 || JOB == kNarrowDw ? 2 : 4;           // fragments read together; dw has registers for two
     constexpr int kAux = JOB == kNarrowDw ? kNarrowWalk * 16 : kNarrowWalk * 4;       // row records, or biases
     constexpr int kStage = Tile::kBytes + kAux;
     __shared__ __align__(16) char lds[2 * kStage];
@@ -116,9 +136,9 @@ __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a
     RowState st[NT];
     float bias_n[NT];
     int want[NT];
-    // a logit is its product times `back` plus the bias
+    // a logit (times log2 e) is its product times `back` plus the bias
     const int ex = a.scaled ? a.scales->ex[0] + a.scales->ex[1] : 0;
-    const float back = ldexpf(JOB == kNarrowLse ? 1.f : kLog2e, max(min(-ex, 126), -300));
+    const float back = ldexpf(kLog2e, max(min(-ex, 126), -300));
     s16x8 own[PARTS][KK][NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -222,17 +242,22 @@ __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a
 #pragma unroll
                         for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[t][n][i]);
                     const float ref = top == -INFINITY ? 0.f : top;
-                    float q = sum[n] * __builtin_amdgcn_exp2f((mx[n] - ref) * kLog2e);
+                    float q = sum[n] * __builtin_amdgcn_exp2f(mx[n] - ref);
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) q += __builtin_amdgcn_exp2f((sc[t][n][i] - ref) * kLog2e);
+                        for (int i = 0; i < 4; ++i) q += __builtin_amdgcn_exp2f(sc[t][n][i] - ref);
                     sum[n] = q;
                     mx[n] = top;
                 }
                 continue;
             }
             // d, split into its parts: the second product's operand
+            // the second product's first fragments, read while the matrix cores work on the first product
+            const uint32_t tile_at = stage * kStage + mp * (32 * HP * 2);
+            // (dx only: dw has no registers left for them, 393 us against 364 at 36864 x 10000 x 64 fp32)
+            s16x8 early[HB];
+            if constexpr (JOB == kNarrowDx) Tile::template frag_t<PARTS - 1, HB>(t_base, tile_at, early);
             s16x8 d[PARTS][NT];
             // dw: the records of the lane's rows; their g is read only where a target is met
             const RowState* row = reinterpret_cast<const RowState*>(s + Tile::kBytes) + mp * 32 + g * 4;
@@ -255,7 +280,8 @@ __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a
                     const float m = JOB == kNarrowDw ? row_m2[e] : st[n].m2;
                     const float f = JOB == kNarrowDw ? row_scale[e] : st[n].inv_s;      // dx: times the lift; g comes at the end
                     const float b = JOB == kNarrowDw ? bias_n[n] : bias[e / 4][e % 4];
-                    v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e / 4][n][e % 4], back, b - m)) * f;
+                    // the logit rounded as in the forward, then the difference: the row's maximum gives 1
+                    v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e / 4][n][e % 4], back, b) - m) * f;
                 }
                 if (JOB == kNarrowDx) {
                     const int64_t at = st[n].target - m0;
@@ -279,27 +305,32 @@ __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a
                 }
                 vec_t<E, 8> o[PARTS];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
+                for (int e = 0; e < 8; e += 2) {
 #pragma unroll
                     for (int p = 0; p < PARTS; ++p) {
-                        o[p][e] = (E)v[e];
-                        v[e] = PARTS > 1 ? v[e] - (float)o[p][e] : 0.f;
+                        const uint32_t h = pack2<E>(v[e], v[e + 1]);
+                        reinterpret_cast<uint32_t*>(&o[p])[e / 2] = h;
+                        if (p + 1 < PARTS) minus_halves(h, v[e], v[e + 1]);
                     }
                 }
 #pragma unroll
                 for (int p = 0; p < PARTS; ++p) d[p][n] = __builtin_bit_cast(s16x8, o[p]);
             }
-            const uint32_t tile_at = stage * kStage + mp * (32 * HP * 2);
-            static_for<HT / 2>([&](auto h_c) {
-                constexpr int h = decltype(h_c)::value * 2;
+            static_for<HT / HB>([&](auto h_c) {
+                constexpr int h = decltype(h_c)::value * HB;
                 static_for<PARTS>([&](auto q_c) {
                     constexpr int p = PARTS - 1 - decltype(q_c)::value;          // smallest products first
-                    s16x8 f[2];
-                    Tile::template frag_t2<p>(t_base[h] + tile_at, t_base[h + 1] + tile_at, f);
+                    s16x8 f[HB];
+                    if constexpr (JOB == kNarrowDx && h == 0 && p == PARTS - 1) {
+#pragma unroll
+                        for (int i = 0; i < HB; ++i) f[i] = early[i];
+                    } else {
+                        Tile::template frag_t<p, HB>(t_base + h, tile_at, f);
+                    }
 #pragma unroll
                     for (int b = PARTS - 1 - p; b >= 0; --b)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i)
+                        for (int i = 0; i < HB; ++i)
 #pragma unroll
                             for (int n = 0; n < NT; ++n) acc[h + i][n] = mfma16<E>(f[i], d[b][n], acc[h + i][n]);
                 });
@@ -318,7 +349,7 @@ __global__ __launch_bounds__(kBlock, 2) void ce_narrow_kernel(const NarrowArgs a
             for (int x = 16; x <= 32; x <<= 1) {
                 const float om = __shfl_xor(m, x, kWave), oq = __shfl_xor(q, x, kWave);
                 const float nm = fmaxf(m, om), ref = nm == -INFINITY ? 0.f : nm;
-                q = q * __builtin_amdgcn_exp2f((m - ref) * kLog2e) + oq * __builtin_amdgcn_exp2f((om - ref) * kLog2e);
+                q = q * __builtin_amdgcn_exp2f(m - ref) + oq * __builtin_amdgcn_exp2f(om - ref);
                 m = nm;
             }
             const int64_t r = n_wave + n * 16 + col;

@@ -144,6 +144,27 @@ __device__ __forceinline__ void tile_frags4(const char* lds, int ext0, int t0, s
     }
 }
 
+// two numbers rounded to nearest into one register
+template <typename E>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<bf16_t>(float lo, float hi) {
+    const vec_t<bf16_t, 2> v = {(bf16_t)lo, (bf16_t)hi};
+    return __builtin_bit_cast(uint32_t, v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<f16_t>(float lo, float hi) {
+    uint32_t v;         // the compiler converts one by one and permutes where both halves are needed again
+    asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(v) : "v"(lo), "v"(hi));
+    return v;
+}
+// v - h for both halves of a register of two fp16 numbers, exactly: the mixed fma reads the halves as they lie, where conversions take
+// two instructions more per element
+__device__ __forceinline__ void minus_halves(uint32_t h, float& lo, float& hi) {
+    asm("v_fma_mix_f32 %0, %1, -1.0, %0 op_sel_hi:[1,0,0]" : "+v"(lo) : "v"(h));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %0 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(hi) : "v"(h));
+}
+
 // Which parts are multiplied: 16-bit values (0, 0); fp32 values, scaled so that the largest of their tensor lies in 2^14 ... 2^15, as
 // x0 + x1 (each the fp16 nearest to what is left: 2^-23 of the value, or 2^-25 in the scaled unit, stays out): (0, 1), (1, 0), (0, 0).
 // What is dropped, x1 y1, is below 2^-22 of |x| |y| and has either sign; fp32 products and sums round by 2^-24 each.

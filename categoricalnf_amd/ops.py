@@ -1056,7 +1056,7 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, want_r
     """Softmax cross entropy of the linear layer x @ weight.T + bias over a vocabulary, without its logits (cnf_linear_ce).
 
     x [..., H] and weight [V, H] float32, bfloat16 or float16; bias [V] of that type or float32; target [...] integers.  Returns
-    (loss [...] fp32, stats [2, R]: the rows' maximum logit and sum of exponentials, reduced [mean, sum, count] over the rows that
+    (loss [...] fp32, stats [2, R]: the rows' maximum logit times log2(e) and sum of exponentials, reduced [mean, sum, count] over the rows that
     are not ignored or None, exponents); rows with target == ignore_index have loss 0, a category outside [0, V) raises the flag that
     `check_flags` reports."""
     out = native().linear_ce_raw(x, weight, target, bias, ignore_index, want_reduced, flag_word(_dev(x)))

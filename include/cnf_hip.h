@@ -646,7 +646,7 @@ int cnf_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64_t 
  * (layers/categorical_encoding/decoder.py:35-63, linear_encoding.py:176-180).  x [R, H] and weight [V, H] of `dtype`, unit column
  * stride, `x_stride` / `w_stride` elements between rows; bias [V] of `bias_dtype` (nullable); target int64 [R].  Rows with target ==
  * ignore_index have loss 0; any other target outside [0, V) raises CNF_FLAG_CATEGORY and its loss is NaN.  row_max, row_sum [R]: the
- * maximum logit and sum_v exp(logit - maximum), which the backward takes; reduced [3] (nullable): mean (NaN over no rows), sum and
+ * maximum logit times log2(e) and sum_v exp(logit - maximum), which the backward takes; reduced [3] (nullable): mean (NaN over no rows), sum and
  * number of the rows that are not ignored; exponents [2] (nullable): the powers of two that fp32 operands were scaled by, which the
  * backward takes back instead of looking for the largest elements again.  fp32 products are exact to 2^-22 of the operands' sizes (three fp16
  * products of operands scaled by a power of two per tensor and split in two), 16-bit products are exact; sums, maxima and exponentials
