@@ -31,8 +31,12 @@ struct NarrowArgs {
     // forward
     const int64_t* target;
     int64_t ignore;
-    float2* partial;                    // [splits][rows]
+    float2* partial;                    // [splits][rows]; with one split the kernel finishes its rows itself:
     float* target_logit;                // [rows]
+    float *row_max, *row_sum, *loss;    // [rows]
+    double* sums;                       // [workgroups][2] sum and number of the rows that count
+    float* reduced;                     // nullable: nobody asks for the sums; written by a single workgroup
+    int* flags;
     // backward
     const RowState* state;              // [rows rounded up to kNarrowWalk]
     void* out;                          // final_dtype >= 0: [n][hidden] of that type; otherwise fp32 [splits][n][ld]

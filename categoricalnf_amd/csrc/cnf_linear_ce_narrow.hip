@@ -111,6 +111,7 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
     typedef NarrowTile<HP, PARTS> Tile;
     constexpr int NT = 2, KK = HP / 32, HT = HP / 16;
     constexpr int HB = HT < 4 || JOB == kNarrowDw ? 2 : 4;           // fragments read together; dw has registers for two
+    constexpr int kHalves = JOB == kNarrowLse ? 2 : 1;               // halves of a step in flight: the gradients have registers for one
     constexpr int kAux = JOB == kNarrowDw ? kNarrowWalk * 16 : kNarrowWalk * 4;       // row records, or biases
     constexpr int kStage = Tile::kBytes + kAux;
     __shared__ __align__(16) char lds[2 * kStage];
@@ -171,12 +172,12 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
     uint32_t t_base[HT];
 #pragma unroll
     for (int h = 0; h < HT; ++h) t_base[h] = (uint32_t)(uintptr_t)(lds_void16_t*)lds + Tile::frag_t_base(h);
-    float mx[NT], sum[NT];
+    float mx[NT], sum[NT], own_logit[NT];
     f32x4 acc[HT][NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         mx[n] = -INFINITY;
-        sum[n] = 0.f;
+        sum[n] = own_logit[n] = 0.f;
 #pragma unroll
         for (int h = 0; h < HT; ++h) acc[h][n] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -193,7 +194,7 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
         asm volatile("" ::: "memory");
         const char* s = lds + stage * kStage;
         const int64_t m_tile = tile * kNarrowWalk;
-#pragma unroll(JOB == kNarrowLse ? 2 : 1)
+#pragma unroll kHalves
         for (int mp = 0; mp < 2; ++mp) {
             f32x4 sc[2][NT];
 #pragma unroll
@@ -234,7 +235,8 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
                         for (int t = 0; t < 2; ++t)
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                if (at == t * 16 + i) a.target_logit[n_wave + n * 16 + col] = sc[t][n][i];
+                                if (at == t * 16 + i) own_logit[n] = sc[t][n][i];
+                        if (a.splits > 1) a.target_logit[n_wave + n * 16 + col] = own_logit[n];
                     }
                     float top = mx[n];
 #pragma unroll
@@ -342,6 +344,7 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
     }
 
     if (JOB == kNarrowLse) {
+        double total = 0.0, count = 0.0;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             float m = mx[n], q = sum[n];
@@ -353,7 +356,47 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
                 m = nm;
             }
             const int64_t r = n_wave + n * 16 + col;
-            if (g == 0 && r < a.rows) a.partial[(int64_t)split * a.rows + r] = make_float2(m, q);
+            if (a.splits > 1) {
+                if (g == 0 && r < a.rows) a.partial[(int64_t)split * a.rows + r] = make_float2(m, q);
+                continue;
+            }
+            // the whole vocabulary has gone by: one lane of the row's four has met the target
+            float t = own_logit[n];
+#pragma unroll
+            for (int x = 16; x <= 32; x <<= 1) t += __shfl_xor(t, x, kWave);
+            if (g == 0 && r < a.rows) {
+                const int64_t cat = a.target[r];
+                float v = 0.f;
+                if (cat != a.ignore) {
+                    if (want[n] < 0) raise_flag(a.flags, CNF_FLAG_CATEGORY);
+                    v = want[n] < 0 ? NAN : logf(q) + (m - t) * kLn2;
+                    total += (double)v;
+                    count += 1.0;
+                }
+                a.row_max[r] = m;
+                a.row_sum[r] = q;
+                a.loss[r] = v;
+            }
+        }
+        if (a.splits > 1 || !a.reduced) return;
+        double* sh = reinterpret_cast<double*>(lds);            // every wave is past its last read of the stages
+        total = wave_sum(total);
+        count = wave_sum(count);
+        if (lane == 0) {
+            sh[wave] = total;
+            sh[4 + wave] = count;
+        }
+        __syncthreads();
+        if (tid == 0) {
+            const double s = ((sh[0] + sh[1]) + sh[2]) + sh[3], c = ((sh[4] + sh[5]) + sh[6]) + sh[7];
+            if (gridDim.x == 1) {
+                a.reduced[0] = (float)(s / c);
+                a.reduced[1] = (float)s;
+                a.reduced[2] = (float)c;
+            } else {
+                a.sums[2 * (int64_t)blockIdx.x] = s;
+                a.sums[2 * (int64_t)blockIdx.x + 1] = c;
+            }
         }
         return;
     }
