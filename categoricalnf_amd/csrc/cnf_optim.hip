@@ -14,8 +14,8 @@
 //
 // Bound by HBM: 28 bytes per fp32 element (16 with 8-bit moments, plus 8 / 256).  The tensors' addresses travel in the kernel
 // arguments (up to 4 KB: 80 tensors a launch, 56 with scales): nothing is uploaded, so a launch may be captured and replayed, and
-// nothing on the device has to outlive it.  A workgroup owns 4096 consecutive elements of one tensor, found by counting the
-// tensors that begin at or before it; each lane has four 4-element units of every array in flight.
+// nothing on the device has to outlive it.  A workgroup owns 1024 (2048 with 8-bit moments) consecutive elements of one tensor, found by counting
+// the tensors that begin at or before it; each lane has one or two 4-element units of every array in flight.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -25,8 +25,10 @@
 
 namespace cnf {
 
-constexpr int kAdamChunk = 4096;
-constexpr int kAdamUnits = kAdamChunk / (4 * kBlock);       // 4-element units per lane
+// elements of a workgroup, 4 or 8 a lane: fp32 moments want many short workgroups (420 M bf16 elements with 4096, 2048, 1024 each: 1730,
+// 1721, 1597 us), 8-bit ones a little arithmetic to hide loads behind (84 M: 340, 285, 308 us)
+template <int BITS>
+constexpr int kAdamChunk = BITS == 8 ? 2048 : 1024;
 
 struct AdamConst {
     float beta1, one_beta1, beta2, one_beta2, eps, keep, size, root;
@@ -51,10 +53,18 @@ struct AdamArgs {
 };
 static_assert(sizeof(AdamArgs<32>) <= 4096 && sizeof(AdamArgs<8>) <= 4096, "kernel arguments");
 
+// largest value of the wave, in every lane: within rows of 16 lanes, then row by row into lane 63
 __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, m, kWave));
-    return v;
+    auto step = [&](auto ctrl) {
+        v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xf, 0xf, false));
+    };
+    step(std::integral_constant<int, 0xb1>{});      // lanes 1 0 3 2
+    step(std::integral_constant<int, 0x4e>{});      // lanes 2 3 0 1
+    step(std::integral_constant<int, 0x141>{});     // mirrored within 8
+    step(std::integral_constant<int, 0x140>{});     // mirrored within 16
+    step(std::integral_constant<int, 0x142>{});     // lane 15 of a row to the next row
+    step(std::integral_constant<int, 0x143>{});     // lane 31 to the upper half
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, kWave - 1);
 }
 __device__ __forceinline__ bool is_finite(float v) { return (__float_as_uint(v) & 0x7fffffffu) < 0x7f800000u; }
 
@@ -63,18 +73,34 @@ __device__ __forceinline__ float code_scale(uint32_t bits, float inv_steps2) {
     const float s = __uint_as_float(bits) * inv_steps2;
     return is_finite(s) ? s : __uint_as_float(0x7fc00000u);
 }
-__device__ __forceinline__ int code_m(float m, float s) {
-    if (!(s > 0.f)) return 0;
-    const int q = (int)fminf(rintf(sqrtf(fabsf(m) / s)), 127.f);
-    return m < 0.f ? -q : q;
-}
-__device__ __forceinline__ int code_v(float r, float s) {
-    if (!(s > 0.f) || !(r > 0.f)) return 0;
-    return (int)fminf(fmaxf(rintf(sqrtf(r / s)), 1.f), 255.f);
-}
-__device__ __forceinline__ float decode_m(int q, float s) { return (float)(q * (q < 0 ? -q : q)) * s; }
-__device__ __forceinline__ float decode_v(int q, float s) {
-    const float r = (float)(q * q) * s;
+// q = rint(sqrt(|x| / s)), quotient and root correctly rounded.  The short form differs from it by less than 2^-21 of the
+// root (reciprocal 2^-23, product 2^-24 and quotient 2^-24, halved by the root; the root instruction 2^-23 and the rounded root 2^-24:
+// 2^-21.6): it settles every root that is further than that from half an integer, and the wave computes the long form where one of its
+// roots is not
+struct CodeScale {
+    float s, inv;
+    bool ok;            // the short form applies
+    __device__ __forceinline__ explicit CodeScale(float scale) : s(scale), inv(__builtin_amdgcn_rcpf(scale)), ok(s > 0.f && s < 0x1p100f && inv < 0x1p100f) {}
+    __device__ __forceinline__ float exact(float x) const { return s > 0.f ? rintf(sqrtf(fabsf(x) / s)) : 0.f; }
+    __device__ __forceinline__ float quick(float x, bool& unsure) const {
+        const float y = __builtin_amdgcn_sqrtf(fabsf(x) * inv), q = rintf(y);
+        unsure |= !(__builtin_fmaf(y, 0x1p-21f, fabsf(y - q)) < 0.5f);
+        return q;
+    }
+    __device__ __forceinline__ void four(const float* x, float* q) const {
+        bool unsure = !ok;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = quick(x[i], unsure);
+        if (__ballot(unsure)) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[i] = exact(x[i]);
+        }
+    }
+};
+// q as whole numbers in fp32: every product of two is exact
+__device__ __forceinline__ float decode_m(float q, float s) { return q * fabsf(q) * s; }
+__device__ __forceinline__ float decode_v(float q, float s) {
+    const float r = q * q * s;
     return r * r;
 }
 
@@ -104,6 +130,22 @@ __device__ __forceinline__ void store4(T* p, int64_t e, int64_t n, bool whole, c
     }
 }
 
+// four codes as bytes: q + bias in 0 .. 255, with the bits of `flip` turned over (127 + 1 and the top bit: two's complement)
+template <typename T>
+__device__ __forceinline__ void store_codes(T* p, int64_t e, int64_t n, bool whole, const float* q, float bias, uint32_t flip) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w = __builtin_amdgcn_cvt_pk_u8_f32(q[i] + bias, i, w);
+    w ^= flip;
+    if (whole) {
+        *reinterpret_cast<uint32_t*>(p + e) = w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (e + i < n) p[e + i] = (T)(w >> (8 * i));
+    }
+}
+
 template <int BITS, typename PT, typename GT>
 __global__ __launch_bounds__(kBlock) void adamw_kernel(const AdamArgs<BITS> a) {
     typedef typename std::conditional<BITS == 8, int8_t, float>::type MT;
@@ -120,7 +162,7 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(const AdamArgs<BITS> a) {
     const GT* g = static_cast<const GT*>(a.g[t]);
     MT* m = static_cast<MT*>(a.m[t]);
     VT* v = static_cast<VT*>(a.v[t]);
-    const int64_t n = a.n[t], base = (int64_t)(chunk - a.first[t]) * kAdamChunk;
+    const int64_t n = a.n[t], base = (int64_t)(chunk - a.first[t]) * kAdamChunk<BITS>;
     const bool aligned = ((reinterpret_cast<uintptr_t>(p) & (4 * sizeof(PT) - 1)) | (reinterpret_cast<uintptr_t>(g) & (4 * sizeof(GT) - 1)) |
                           (reinterpret_cast<uintptr_t>(m) & (4 * sizeof(MT) - 1)) | (reinterpret_cast<uintptr_t>(v) & (4 * sizeof(VT) - 1))) == 0;
     AdamConst c = a.c;
@@ -131,6 +173,7 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(const AdamArgs<BITS> a) {
         c.size = (float)(lr / (1.0 - exp2(step * a.log2_beta1)));
         c.root = (float)(1.0 / sqrt(1.0 - exp2(step * a.log2_beta2)));
     }
+    constexpr int kAdamUnits = kAdamChunk<BITS> / (4 * kBlock);         // 4-element units per lane
     float pv[kAdamUnits][4], gv[kAdamUnits][4], mv[kAdamUnits][4], vv[kAdamUnits][4];
 #pragma unroll
     for (int j = 0; j < kAdamUnits; ++j) {
@@ -151,8 +194,8 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(const AdamArgs<BITS> a) {
             const float sm = in ? a.ms[t][block] : 0.f, sv = in ? a.vs[t][block] : 0.f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                mv[j][i] = decode_m((int)mv[j][i], sm);
-                vv[j][i] = decode_v((int)vv[j][i], sv);
+                mv[j][i] = decode_m(mv[j][i], sm);
+                vv[j][i] = decode_v(vv[j][i], sv);
             }
         }
 #pragma unroll
@@ -181,13 +224,15 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(const AdamArgs<BITS> a) {
             }
             const float sm = code_scale(wave_umax(am), 1.f / 16129.f), sv = code_scale(wave_umax(ar), 1.f / 65025.f);
             float qm[4], qv[4];
+            CodeScale(sm).four(mv[j], qm);
+            CodeScale(sv).four(r, qv);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                qm[i] = (float)code_m(mv[j][i], sm);
-                qv[i] = (float)code_v(r[i], sv);
+                qm[i] = copysignf(fminf(qm[i], 127.f), mv[j][i]);
+                qv[i] = r[i] > 0.f && sv > 0.f ? fminf(fmaxf(qv[i], 1.f), 255.f) : 0.f;
             }
-            store4(m, e, n, whole, qm);
-            store4(v, e, n, whole, qv);
+            store_codes(m, e, n, whole, qm, 128.f, 0x80808080u);
+            store_codes(v, e, n, whole, qv, 0.f, 0u);
             if ((threadIdx.x & 63) == 0 && block * 256 < n) {
                 a.ms[t][block] = sm;
                 a.vs[t][block] = sv;
@@ -210,8 +255,8 @@ __global__ __launch_bounds__(kBlock) void adamw_moments_kernel(const int8_t* m, 
         const float sm = ms[b], sv = vs[b];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            qm[i] = decode_m((int)qm[i], sm);
-            qv[i] = decode_v((int)qv[i], sv);
+            qm[i] = decode_m(qm[i], sm);
+            qv[i] = decode_v(qv[i], sv);
         }
         store4(m_out, e, n, whole, qm);
         store4(v_out, e, n, whole, qv);
@@ -227,7 +272,7 @@ static int adamw_launch(int count, void* const* p, const void* const* g, void* c
         uint64_t chunks = 0;
         for (; i < count && k < AdamArgs<BITS>::kTensors; ++i) {
             if (n[i] == 0) continue;
-            const uint64_t c = ((uint64_t)n[i] + kAdamChunk - 1) / kAdamChunk;
+            const uint64_t c = ((uint64_t)n[i] + kAdamChunk<BITS> - 1) / kAdamChunk<BITS>;
             if (k > 0 && chunks + c > 0x7fffffffull) break;
             a.p[k] = p[i];
             a.g[k] = g[i];
