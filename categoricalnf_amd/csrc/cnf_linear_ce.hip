@@ -98,7 +98,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_lse_kernel(const CeArgs a)
         for (int m = 0; m < Tile::MT; ++m)
 #pragma unroll
             for (int n = 0; n < Tile::NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-        tile.run(v0, r0, 0, a.k_end, acc, [](int, int) {});
+        tile.begin(v0, r0, 0, a.k_end);         // (ahead of the last epilogue, as in ce_d_kernel, it spills more and gains nothing: 578 -> 588 us)
+        tile.multiply(acc, [](int, int) {});
         const int vw = v0 + tile.m_wave + g * 4;        // the lane's first entry
         {
             const float back = logit_scale(a, kLog2e);
@@ -428,91 +429,113 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(const float* g, int g_is_
     }
 }
 
-// one tile of d; D[m = vocabulary][n = row]
+// d, a few tiles per workgroup (as many workgroups as run at once), so that a tile's first copies land during the epilogue of the one
+// before; D[m = vocabulary][n = row].  An XCD's workgroups share one run of tiles.  8192 x 16128 x 1024 bf16: 363 -> 341 us (790 TF) with
+// the copies ahead and 16-byte stores
 template <typename E, int PARTS, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
     typedef TileProduct<E, false, false, BM, BN, WM, WN> Tile;
     __shared__ __align__(16) char lds[Tile::kLds];
     Tile tile(a.w, a.x, a.pairs, a.k_end, lds);
-    const unsigned nv = (a.v1 - a.v0 + BM - 1) / BM, nr = gridDim.x / nv;
-    unsigned ti, tj;
-    grouped_tile(xcd_contiguous(blockIdx.x, gridDim.x), nv, nr, ti, tj);
-    const int v0 = a.v0 + ti * BM, r0 = tj * BN;
-    f32x4 acc[Tile::MT][Tile::NT];
-#pragma unroll
-    for (int m = 0; m < Tile::MT; ++m)
-#pragma unroll
-        for (int n = 0; n < Tile::NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    tile.run(v0, r0, 0, a.k_end, acc, [](int, int) {});
+    const unsigned nv = (a.v1 - a.v0 + BM - 1) / BM, nr = (unsigned)((a.rows + BN - 1) / BN), tiles = nv * nr;
+    const unsigned xcds = min(8u, gridDim.x), xcd = blockIdx.x % xcds, step = gridDim.x / xcds + (xcd < gridDim.x % xcds ? 1 : 0);
+    const unsigned end = (unsigned)((uint64_t)tiles * (xcd + 1) / xcds);
+    unsigned t = (unsigned)((uint64_t)tiles * xcd / xcds) + blockIdx.x / xcds;
     const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
-    const int vw = v0 + tile.m_wave + g * 4;
-    RowState st[Tile::NT];
-#pragma unroll
-    for (int n = 0; n < Tile::NT; ++n) {
-        const int64_t r = (int64_t)r0 + tile.n_wave + n * 16 + col;
-        st[n] = r < a.rows ? a.state[r] : RowState{INFINITY, 0.f, 0.f, -1};
-    }
     E* d = static_cast<E*>(a.d);
     const float back = logit_scale(a, kLog2e);
-    float scale[Tile::NT], own_g[Tile::NT];
+    int v0 = 0, r0 = 0;
+    auto begin = [&]() {
+        unsigned ti, tj;
+        grouped_tile(t, nv, nr, ti, tj);
+        v0 = a.v0 + ti * BM;
+        r0 = tj * BN;
+        tile.begin(v0, r0, 0, a.k_end);
+    };
+    if (t < end) begin();
+    while (t < end) {
+        f32x4 acc[Tile::MT][Tile::NT];
 #pragma unroll
-    for (int n = 0; n < Tile::NT; ++n) {
-        own_g[n] = st[n].g * a.lift;
-        scale[n] = st[n].inv_s * own_g[n];
-    }
-    // targets among the wave's entries are rare: their -g is applied behind a branch that most waves do not take
-    int at[Tile::NT];
-    bool hit = false;
+        for (int m = 0; m < Tile::MT; ++m)
 #pragma unroll
-    for (int n = 0; n < Tile::NT; ++n) {
-        at[n] = st[n].target - vw;
-        hit |= st[n].target >= 0 && at[n] >= 0 && at[n] < Tile::MT * 16;
-    }
-    const bool any_hit = __ballot(hit) != 0, edge = v0 + BM > a.v1;
-#pragma unroll
-    for (int m = 0; m < Tile::MT; ++m) {
-        const int v = vw + m * 16;
-        f32x4 b = {0.f, 0.f, 0.f, 0.f};
-        if (a.bias) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) b[i] = bias_at(a, v + i) * kLog2e;
-        }
+            for (int n = 0; n < Tile::NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        tile.multiply(acc, [](int, int) {});
+        const int vw = v0 + tile.m_wave + g * 4;
+        const int64_t rw = (int64_t)r0 + tile.n_wave + col;
+        const bool edge = v0 + BM > a.v1;
+        RowState st[Tile::NT];
+        float scale[Tile::NT], own_g[Tile::NT];
+        // targets among the wave's entries are rare: their -g is applied behind a branch that most waves do not take
+        int at[Tile::NT];
+        bool hit = false;
 #pragma unroll
         for (int n = 0; n < Tile::NT; ++n) {
-            const int64_t r = (int64_t)r0 + tile.n_wave + n * 16 + col;
-            f32x4 p;
+            st[n] = rw + n * 16 < a.rows ? a.state[rw + n * 16] : RowState{INFINITY, 0.f, 0.f, -1};
+            own_g[n] = st[n].g * a.lift;
+            scale[n] = st[n].inv_s * own_g[n];
+            at[n] = st[n].target - vw;
+            hit |= st[n].target >= 0 && at[n] >= 0 && at[n] < Tile::MT * 16;
+        }
+        const bool any_hit = __ballot(hit) != 0;        // the rows' records have arrived: no wait for them behind the copies
+        const int v_tile = v0;
+        t += step;
+        if (t < end) begin();
 #pragma unroll
-            for (int i = 0; i < 4; ++i)             // the logit rounded as in the forward, then the difference: the row's maximum gives 1
-                p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[m][n][i], back, b[i]) - st[n].m2) * scale[n];
-            if (any_hit) {
+        for (int m = 0; m < Tile::MT; m += 2) {
+            f32x4 b[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            if (a.bias) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (at[n] == m * 16 + i) p[i] -= own_g[n];          // an ignored row's is negative
+                for (int i = 0; i < 8; ++i) b[i / 4][i % 4] = bias_at(a, vw + (m + i / 4) * 16 + i % 4) * kLog2e;
             }
-            if (edge) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (v + i >= a.v1) p[i] = 0.f;
-            }
-            // an ignored row, or one that is not there (x may hold anything)
-            if (st[n].target < 0) p = f32x4{0.f, 0.f, 0.f, 0.f};
-            vec_t<E, 4> o[PARTS];
+            for (int n = 0; n < Tile::NT; ++n) {
+                uint32_t o[PARTS][2][2];
 #pragma unroll
-            for (int i = 0; i < 4; i += 2)
+                for (int q = 0; q < 2; ++q) {
+                    f32x4 p;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)         // the logit rounded as in the forward, then the difference: the row's maximum gives 1
+                        p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[m + q][n][i], back, b[q][i]) - st[n].m2) * scale[n];
+                    if (any_hit) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (at[n] == (m + q) * 16 + i) p[i] -= own_g[n];        // an ignored row's is negative
+                    }
+                    if (edge) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (vw + (m + q) * 16 + i >= a.v1) p[i] = 0.f;
+                    }
+                    // an ignored row, or one that is not there (x may hold anything)
+                    if (st[n].target < 0) p = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < 4; i += 2)
+#pragma unroll
+                        for (int k = 0; k < PARTS; ++k) {
+                            o[k][q][i / 2] = pack2<E>(p[i], p[i + 1]);
+                            if (k + 1 < PARTS) {
+                                float lo = p[i], hi = p[i + 1];
+                                minus_halves(o[k][q][i / 2], lo, hi);
+                                p[i] = lo;
+                                p[i + 1] = hi;
+                            }
+                        }
+                }
+                // lanes 16 ... 31 hand their entries 4 ... 7 of block m to lanes 0 ... 15 and get 0 ... 3 of block m + 1 (lanes 48 and 32
+                // likewise): a lane then holds 8 consecutive entries, a row's 32 are one 64-byte run
+                const int v = v_tile - a.v0 + tile.m_wave + (m + (g & 1)) * 16 + (g >> 1) * 8;
 #pragma unroll
                 for (int k = 0; k < PARTS; ++k) {
-                    const uint32_t h = pack2<E>(p[i], p[i + 1]);
-                    reinterpret_cast<uint32_t*>(&o[k])[i / 2] = h;
-                    if (k + 1 < PARTS) {
-                        float lo = p[i], hi = p[i + 1];
-                        minus_halves(h, lo, hi);
-                        p[i] = lo;
-                        p[i + 1] = hi;
-                    }
-                }
+                    vec_t<uint32_t, 4> w;
 #pragma unroll
-            for (int k = 0; k < PARTS; ++k)
-                *reinterpret_cast<vec_t<E, 4>*>(d + k * a.d_part + r * a.d_ld + (v - a.v0)) = o[k];
+                    for (int i = 0; i < 2; ++i) {
+                        const auto r = __builtin_amdgcn_permlane16_swap(o[k][0][i], o[k][1][i], false, false);
+                        w[i] = r[0];
+                        w[2 + i] = r[1];
+                    }
+                    *reinterpret_cast<vec_t<uint32_t, 4>*>(d + k * a.d_part + (rw + n * 16) * a.d_ld + v) = w;
+                }
+            }
         }
     }
 }
@@ -557,7 +580,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_grad_kernel(const GradArgs
 #pragma unroll
     for (int i = 0; i < 8; ++i) ones[i] = __builtin_bit_cast(short, (E)1.f);
     // fp32: each part of d is once the partner of part 0 of x: pairs (0, 1) and (0, 0)
-    tile.run(m0, n0, k0, k1, acc, [&](int stage, int pair) {
+    tile.begin(m0, n0, k0, k1);
+    tile.multiply(acc, [&](int stage, int pair) {
         if (!sums || pair_a(a.pairs, pair) != 0) return;
         const char* sb = lds + stage * Tile::kStage + Tile::kBytesA;
         s16x8 fb[4];
@@ -966,11 +990,10 @@ int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64
             const int64_t v1 = std::min<int64_t>(V, v0 + p.piece), width = v1 - v0;
             a.v0 = (int)v0;
             a.v1 = (int)v1;
-            if (p.big_d)
-                CNF_LAUNCH((ce_d_kernel<E, PARTS, kBig, kBig, 2, 4>), dim3((unsigned)(ceil_div(width, kBig) * ceil_div(R, kBig))), dim3(512), 0, st, a);
-            else
-                CNF_LAUNCH((ce_d_kernel<E, PARTS, kSmall, kSmall, 2, 2>), dim3((unsigned)(ceil_div(width, kSmall) * ceil_div(R, kSmall))), dim3(256), 0,
-                           st, a);
+            const int edge = p.big_d ? kBig : kSmall;
+            const unsigned d_grid = (unsigned)std::min<int64_t>(ceil_div(width, edge) * ceil_div(R, edge), p.big_d ? 256 : 512);
+            if (p.big_d) CNF_LAUNCH((ce_d_kernel<E, PARTS, kBig, kBig, 2, 4>), dim3(d_grid), dim3(512), 0, st, a);
+            else CNF_LAUNCH((ce_d_kernel<E, PARTS, kSmall, kSmall, 2, 2>), dim3(d_grid), dim3(256), 0, st, a);
             const Operand d{a.d, a.d_ld, a.d_part, 0};
             GradArgs q{};
             q.pairs = p.pairs;

@@ -231,27 +231,47 @@ struct TileProduct {
         extra(STAGE, pair);
     }
 
-    // acc += the tile's product over k0 ... k1 - 1 (k0 a multiple of 32); extra(stage, pair) sees every stage before it is given up
-    template <typename Extra>
-    __device__ __forceinline__ void run(int m0, int n0, int k0, int k1, f32x4 (&acc)[MT][NT], Extra&& extra) {
-        const int ksteps = (k1 - k0 + kStepK - 1) / kStepK, total = ksteps * pairs;
-        if (total <= 0) return;
+    // the tile being multiplied: its corner and k steps; the next step to be copied: its pair, its k step and where it begins
+    int m_at, n_at, k_first, ksteps, cp, ck;
+    const char *pa, *pb;
+
+    __device__ __forceinline__ void next() {
+        if (++ck == ksteps) {
+            ck = 0;
+            ++cp;
+            pa = ca.base(a, pair_a(pairs, cp), m_at, k_first);
+            pb = cb.base(b, pair_b(pairs, cp), n_at, k_first);
+        } else {
+            pa += ca.advance(a);
+            pb += cb.advance(b);
+        }
+    }
+
+    // starts the product of the tile at m0, n0 over k0 ... k1 - 1 (k0 a multiple of 32): its first copies.  The ring must be free: at the
+    // start, or after multiply().  What a wave stores or loads between the two is newer than these copies, so that waiting for all but
+    // the newest operations still waits for them.
+    __device__ __forceinline__ void begin(int m0, int n0, int k0, int k1) {
+        m_at = m0;
+        n_at = n0;
+        k_first = k0;
+        ksteps = (k1 - k0 + kStepK - 1) / kStepK;
+        if (ksteps <= 0) return;
         ca.aim(a, m0);
         cb.aim(b, n0);
-        int cp = 0, ck = 0;         // the next step to be copied: its pair and k step ...
-        const char *pa = ca.base(a, pair_a(pairs, 0), m0, k0), *pb = cb.base(b, pair_b(pairs, 0), n0, k0);      // ... and where it begins
-        const int64_t da = ca.advance(a), db = cb.advance(b);
-        auto next = [&]() {
-            if (++ck == ksteps) {
-                ck = 0;
-                ++cp;
-                pa = ca.base(a, pair_a(pairs, cp), m0, k0);
-                pb = cb.base(b, pair_b(pairs, cp), n0, k0);
-            } else {
-                pa += da;
-                pb += db;
-            }
-        };
+        cp = ck = 0;
+        pa = ca.base(a, pair_a(pairs, 0), m0, k0);
+        pb = cb.base(b, pair_b(pairs, 0), n0, k0);
+        for (int s = 0; s < kStages - 1 && s < ksteps * pairs; ++s, next()) {
+            ca.copy(pa, k0 + ck * kStepK, k_end, lds + s * kStage);
+            cb.copy(pb, k0 + ck * kStepK, k_end, lds + s * kStage + kBytesA);
+        }
+    }
+
+    // acc += the product begun; extra(stage, pair) sees every stage before it is given up
+    template <typename Extra>
+    __device__ __forceinline__ void multiply(f32x4 (&acc)[MT][NT], Extra&& extra) {
+        const int total = ksteps * pairs, k0 = k_first;
+        if (total <= 0) return;
         int pair = 0, ks = 0;
         auto done = [&]() {
             if (++ks == ksteps) {
@@ -259,10 +279,6 @@ struct TileProduct {
                 ++pair;
             }
         };
-        for (int s = 0; s < kStages - 1 && s < total; ++s, next()) {
-            ca.copy(pa, k0 + ck * kStepK, k_end, lds + s * kStage);
-            cb.copy(pb, k0 + ck * kStepK, k_end, lds + s * kStage + kBytesA);
-        }
         // whole steps, four at a time; a partial one can only be the last of a pair
         const int whole = k0 + ksteps * kStepK <= k_end ? total : (pairs == 1 ? total - 1 : 0);
         int s = 0;
