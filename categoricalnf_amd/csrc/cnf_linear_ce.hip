@@ -8,8 +8,8 @@
 // lane keeps a running maximum and sum for its rows over the vocabulary entries it sees (four of them are consecutive), the lanes and
 // waves of a row are joined once at the end, the parts of the vocabulary by a second launch, which also writes the loss.
 // Backward, in pieces of the vocabulary: the piece's logits are computed again and turned into d (rounded to the operands' type, or
-// kept as two fp16 parts for fp32), written to a workspace that fits the memory-side cache, and read by two products: dx += d w over
-// the piece, dw = d^T x complete for the piece.  db comes out of the second product: a fragment of ones in place of x.
+// kept as two fp16 parts for fp32), written to a workspace and read by two products: dx += d w over the piece, dw = d^T x complete for
+// the piece.  db comes out of the second product: a fragment of ones in place of x.
 //
 // Few features (H <= 128) take the kernels of cnf_linear_ce_narrow.hip instead, which write nothing of size R x V.
 //
@@ -430,7 +430,7 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(const float* g, int g_is_
 }
 
 // d, a few tiles per workgroup (as many workgroups as run at once), so that a tile's first copies land during the epilogue of the one
-// before; D[m = vocabulary][n = row].  An XCD's workgroups share one run of tiles.  8192 x 16128 x 1024 bf16: 363 -> 341 us (790 TF) with
+// before; D[m = vocabulary][n = row].  An XCD's workgroups share one run of tiles.  8192 x 32000 x 1024 bf16: 726 -> 682 us (790 TF) with
 // the copies ahead and 16-byte stores
 template <typename E, int PARTS, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
@@ -679,7 +679,9 @@ __global__ __launch_bounds__(1024) void ce_sum_many_kernel(const SumArgs a) {
 // ---- host: plan of a call -------------------------------------------------------------------------------------------------------
 
 constexpr int kBig = 256, kSmall = 128;         // tile edges
-constexpr int64_t kPieceBytes = 256ll << 20;    // d of one piece of the vocabulary
+// d of one piece of the vocabulary.  A second piece costs dx another pass through memory: 8192 x 32000 x 1024 bf16 takes 2197 us as one
+// piece, 2285 as two of 256 MiB, which would fit the memory-side cache
+constexpr int64_t kPieceBytes = 512ll << 20;
 
 static int64_t round_up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 static int64_t ceil_div(int64_t n, int64_t m) { return (n + m - 1) / m; }

@@ -234,6 +234,7 @@ struct TileProduct {
     // the tile being multiplied: its corner and k steps; the next step to be copied: its pair, its k step and where it begins
     int m_at, n_at, k_first, ksteps, cp, ck;
     const char *pa, *pb;
+    int64_t da, db;             // from one k step to the next
 
     __device__ __forceinline__ void next() {
         if (++ck == ksteps) {
@@ -242,8 +243,8 @@ struct TileProduct {
             pa = ca.base(a, pair_a(pairs, cp), m_at, k_first);
             pb = cb.base(b, pair_b(pairs, cp), n_at, k_first);
         } else {
-            pa += ca.advance(a);
-            pb += cb.advance(b);
+            pa += da;
+            pb += db;
         }
     }
 
@@ -259,6 +260,8 @@ struct TileProduct {
         ca.aim(a, m0);
         cb.aim(b, n0);
         cp = ck = 0;
+        da = ca.advance(a);
+        db = cb.advance(b);
         pa = ca.base(a, pair_a(pairs, 0), m0, k0);
         pb = cb.base(b, pair_b(pairs, 0), n0, k0);
         for (int s = 0; s < kStages - 1 && s < ksteps * pairs; ++s, next()) {
