@@ -1,7 +1,8 @@
 """Linear cross entropy (ops.linear_cross_entropy, functional.linear_cross_entropy) against the definition in 64 bits.
 
-Tolerances, u = 2^-24, h = half a step of the operands' type, P = 6 products per term for fp32 operands and 1 otherwise:
-  * a logit is a sum of P H exact (fp32: to 2^-26) products, at most 2 u lost per addition (the matrix unit may cut where it aligns):
+Tolerances, u = 2^-24, h = half a step of the operands' type, P = 6 roundings per term for fp32 operands (three products of fp16
+parts; the part left out, below 2^-22 = 4 u of |x w|, counts less than the other three) and 1 otherwise:
+  * a logit is a sum of P H exact products, at most 2 u lost per addition (the matrix unit may cut where it aligns):
     e_l = 2 (P H + 16) u sum_k |x w| + 2 u |b|;
   * exp2 of a rounded argument: relative (2 |l - m| + 4) u per term; the sum of V terms: at most V / 8 + 64 additions in a lane and
     the tree; the logarithm and the two differences add 4 u of their magnitudes.  The loss is off by at most e_l of its target
@@ -112,6 +113,13 @@ def test_values_and_gradients(shape, dtype):
                                          (BF16, (600, 9000, 1024)), (F32, (3000, 9000, 100)), (F32, (520, 9000, 520))], ids=str)
 def test_large_tiles_and_pieces_of_the_vocabulary(shape, dtype):
     run_and_check(*make(*shape, dtype, bias=dtype != BF16))
+
+
+@pytest.mark.parametrize("dtype,rows", [(BF16, 16500), (F16, 16500), (F32, 8300)])
+def test_two_pieces_of_the_vocabulary(dtype, rows):
+    """More than 512 MiB of d: the second piece adds to dx and writes its own rows of dw and db."""
+    x, w, b, t, g = make(rows, 17000, 136, dtype)
+    run_and_check(x, w, b, t, g)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
