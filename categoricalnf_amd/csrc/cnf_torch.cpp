@@ -3,7 +3,7 @@
 // every function ends in the C entry points of libcnf_hip.so (include/cnf_hip.h), whose addresses Python hands over once (`bind`), so
 // that there is one loaded library whichever build it is.
 //
-// Measured on the host of an MI355X box: layer norm step (forward + torch.autograd.grad) 123 us as a Python autograd Function, whose
+// Measured beside an MI355X: layer norm step (forward + torch.autograd.grad) 123 us as a Python autograd Function, whose
 // backward waits for the interpreter lock on the engine's thread; torch's own 35 us.
 #include <algorithm>
 #include <string>
