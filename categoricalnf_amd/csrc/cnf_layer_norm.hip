@@ -25,6 +25,7 @@ constexpr int kLnElems = 16;                        // elements of a row one lan
 constexpr int kLnWaveCols = kWave * kLnElems;       // widest row of one wave
 constexpr int kLnBlockCols = 1024 * kLnElems;       // widest row of one workgroup
 constexpr int kLnMaxPartials = 1024;                // partial rows of the column sums
+constexpr int kLnMaxCols = 1 << 30;                 // what 32-bit column counters reach
 
 struct LnArgs {
     const void *x, *dy, *weight, *bias;
@@ -438,7 +439,7 @@ extern "C" {
 int cnf_layer_norm(const void* x, int64_t x_stride, const void* weight, const void* bias, void* y, float* mean, float* rstd,
                    int64_t rows, int cols, float eps, int dtype, int wdtype, cnf_stream_t stream) {
     CNF_REQUIRE(x && y, "cnf_layer_norm: null tensor");
-    CNF_REQUIRE(rows >= 0 && cols > 0 && x_stride >= 0, "cnf_layer_norm: bad size rows=%ld cols=%d", (long)rows, cols);
+    CNF_REQUIRE(rows >= 0 && cols > 0 && cols <= kLnMaxCols && x_stride >= 0, "cnf_layer_norm: bad size rows=%ld cols=%d", (long)rows, cols);
     CNF_REQUIRE(dtype_known(dtype) && dtype_known(wdtype), "cnf_layer_norm: unknown element type");
     CNF_REQUIRE(!mean == !rstd, "cnf_layer_norm: mean and rstd come together");
     if (rows == 0) return CNF_OK;
@@ -469,7 +470,7 @@ int cnf_layer_norm(const void* x, int64_t x_stride, const void* weight, const vo
 }
 
 int64_t cnf_layer_norm_bwd_workspace_floats(int64_t rows, int cols) {
-    if (rows <= 0 || cols <= 0) return 0;
+    if (rows <= 0 || cols <= 0 || cols > kLnMaxCols) return 0;
     // the largest partials matrix over the layouts a launch of this size may take
     int64_t most = 0;
     for (int dtype : {CNF_DTYPE_F32, CNF_DTYPE_BF16})
@@ -482,7 +483,7 @@ int cnf_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64_t 
                        const float* mean, const float* rstd, void* dx, void* dweight, void* dbias, float* ws, int64_t ws_floats,
                        int64_t rows, int cols, int dtype, int wdtype, cnf_stream_t stream) {
     CNF_REQUIRE(x && dy && mean && rstd && dx, "cnf_layer_norm_bwd: null tensor");
-    CNF_REQUIRE(rows >= 0 && cols > 0 && x_stride >= 0 && dy_stride >= 0, "cnf_layer_norm_bwd: bad size rows=%ld cols=%d", (long)rows, cols);
+    CNF_REQUIRE(rows >= 0 && cols > 0 && cols <= kLnMaxCols && x_stride >= 0 && dy_stride >= 0, "cnf_layer_norm_bwd: bad size rows=%ld cols=%d", (long)rows, cols);
     CNF_REQUIRE(dtype_known(dtype) && dtype_known(wdtype), "cnf_layer_norm_bwd: unknown element type");
     const bool sums = dweight || dbias;
     CNF_REQUIRE(!sums || rows == 0 || (ws && ws_floats >= cnf_layer_norm_bwd_workspace_floats(rows, cols)),

@@ -18,8 +18,9 @@
 //
 // Few features (H <= 128) take the kernels of cnf_linear_ce_narrow.hip instead, which write nothing of size R x V.
 //
-// fp32 inputs are scaled by a power of two per tensor and split once into two fp16 parts (cnf_mfma.h: pair_a): three fp16 products keep
-// every product to 2^-22, and the matrix cores do them at 16 times the fp32 rate.  16-bit inputs whose rows are not 16-byte aligned
+// fp32 inputs are scaled by a power of two per tensor (small rows of x: of their own) and split once into two fp16 parts (cnf_mfma.h:
+// pair_a): three fp16 products keep every product to 2^-22, and the matrix cores do them at 16 times the fp32 rate.  What is below
+// 2^-16 of the largest |w| keeps 2^-39 of that largest, not 2^-23 of itself; so does a small row's part in dw beside large rows.  16-bit inputs whose rows are not 16-byte aligned
 // are copied once into padded rows.
 // d is computed for g_r / max |g| (for fp16 operands times 2^14, so that small probabilities keep their bits) and the results are scaled
 // back: under a mean every row's -1 is then exact, where a rounded -g_r would put the same relative error on every row's largest entry.
@@ -46,7 +47,9 @@ struct CeArgs {
     // backward
     const RowState* state;          // [rows]
     const CeScales* scales;
-    int scaled;                     // fp32 operands: scales->ex holds
+    int scaled;                     // fp32 operands: scales->ex holds, and
+    const uint8_t* shift;           // [rows] what the rows of x were scaled by beyond it
+    Operand x_even;                 // x for the product over the rows: fp32: without the rows' shifts, else x
     float lift;                     // of d
     void* d;                        // [parts][rows_pad][piece_ld]
     int64_t d_part, d_ld;
@@ -67,9 +70,10 @@ __device__ __forceinline__ void grouped_tile(unsigned t, unsigned ni, unsigned n
 
 __device__ __forceinline__ float bias_at(const CeArgs& a, int v) { return a.bias && v < a.vocab ? load_any(a.bias, a.bias_dtype, v) : 0.f; }
 
-// what takes a product of scaled operands to unit * logit
-__device__ __forceinline__ float logit_scale(const CeArgs& a, float unit) {
-    return a.scaled ? ldexpf(unit, max(min(-(a.scales->ex[0] + a.scales->ex[1]), 126), -300)) : unit;
+// what takes a product of row r to its logit, times log2 e
+__device__ __forceinline__ float logit_scale(const CeArgs& a, int64_t r) {
+    const int shift = a.scaled && r < a.rows ? a.shift[r] : 0;
+    return a.scaled ? ldexpf(kLog2e, max(min(-(a.scales->ex[0] + a.scales->ex[1] + shift), 126), -300)) : kLog2e;
 }
 
 // ---- forward ---------------------------------------------------------------------------------------------------------------------
@@ -107,14 +111,16 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_lse_kernel(const CeArgs a)
         tile.multiply(acc, [](int, int) {});
         const int vw = v0 + tile.m_wave + g * 4;        // the lane's first entry
         {
-            const float back = logit_scale(a, kLog2e);
+            float back[Tile::NT];
+#pragma unroll
+            for (int n = 0; n < Tile::NT; ++n) back[n] = logit_scale(a, (int64_t)r0 + tile.n_wave + n * 16 + col);
 #pragma unroll
             for (int m = 0; m < Tile::MT; ++m)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float b = a.bias ? bias_at(a, vw + m * 16 + i) * kLog2e : 0.f;
 #pragma unroll
-                    for (int n = 0; n < Tile::NT; ++n) acc[m][n][i] = __builtin_fmaf(acc[m][n][i], back, b);
+                    for (int n = 0; n < Tile::NT; ++n) acc[m][n][i] = __builtin_fmaf(acc[m][n][i], back[n], b);
                 }
         }
         if (v0 + BM > a.vocab) {                        // entries past the vocabulary
@@ -268,16 +274,17 @@ __global__ __launch_bounds__(1024) void ce_reduce_kernel(const double* sums, int
 // ---- operand layout ----------------------------------------------------------------------------------------------------------------
 
 constexpr int kMaxBlocks = 256;
-// fp32: the largest finite |element| of x (blockIdx.y 0) and w (1), one value per workgroup
-__global__ __launch_bounds__(kBlock) void ce_largest_kernel(const float* x, int64_t x_stride, int64_t R, const float* w, int64_t w_stride, int V,
-                                                            int H, uint32_t* largest) {
+// fp32: the largest finite |element| of x's rows that count (blockIdx.y 0) and of w (1), one value per workgroup
+__global__ __launch_bounds__(kBlock) void ce_largest_kernel(const float* x, int64_t x_stride, int64_t R, const int64_t* target, int64_t ignore,
+                                                            const float* w, int64_t w_stride, int V, int H, uint32_t* largest) {
     __shared__ uint32_t sh[kWavesPerBlock];
     const float* src = blockIdx.y ? w : x;
     const int64_t stride = blockIdx.y ? w_stride : x_stride, rows = blockIdx.y ? V : R;
     uint32_t top = 0;
-    auto see = [&](float v) {
+    // row: asked for only where an element exceeds all that the lane has seen
+    auto see = [&](float v, auto row) {
         const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
-        if (b < 0x7f800000u) top = max(top, b);
+        if (b > top && b < 0x7f800000u && (blockIdx.y || target[row()] != ignore)) top = b;
     };
     const int64_t step = (int64_t)kMaxBlocks * kBlock, at = (int64_t)blockIdx.x * kBlock + threadIdx.x;
     if (stride == H && rows * H % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
@@ -287,18 +294,18 @@ __global__ __launch_bounds__(kBlock) void ce_largest_kernel(const float* x, int6
         for (; i + 3 * step < n; i += 4 * step) {           // four loads in flight
             const f32x4 q[4] = {v[i], v[i + step], v[i + 2 * step], v[i + 3 * step]};
 #pragma unroll
-            for (int k = 0; k < 16; ++k) see(q[k / 4][k % 4]);
+            for (int k = 0; k < 16; ++k) see(q[k / 4][k % 4], [&] { return (4 * (i + k / 4 * step) + k % 4) / H; });
         }
         for (; i < n; i += step) {
             const f32x4 q = v[i];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) see(q[k]);
+            for (int k = 0; k < 4; ++k) see(q[k], [&] { return (4 * i + k) / H; });
         }
     } else if (stride == H) {
-        for (int64_t i = at; i < rows * H; i += step) see(src[i]);
+        for (int64_t i = at; i < rows * H; i += step) see(src[i], [&] { return i / H; });
     } else {
         for (int64_t r = blockIdx.x; r < rows; r += kMaxBlocks)
-            for (int c = threadIdx.x; c < H; c += kBlock) see(src[r * stride + c]);
+            for (int c = threadIdx.x; c < H; c += kBlock) see(src[r * stride + c], [&] { return r; });
     }
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, kWave));
@@ -316,8 +323,12 @@ struct LayoutJob {
     void* dst;
 };
 struct LayoutArgs {
-    LayoutJob job[2];               // x and w: [rows][cols] -> `parts` arrays of [rows][ld] 16-bit elements, zeros behind cols
+    LayoutJob job[4];               // 0: x, 1: w, 3: x without its rows' shifts; [rows][cols] -> `parts` arrays of [rows][ld] 16-bit elements, zeros behind cols
     int cols, vec;                  // vec: bit j: 8 elements of job j's rows may be read as vectors of 16 bytes
+    int group;                      // lanes that share a row of x (a power of two)
+    const int64_t* target;          // fp32: ignored rows of x are laid out as zeros, whatever they hold
+    int64_t ignore;
+    uint8_t* shift;
     int64_t ld;
     const void* bias;               // -> fp32, times log2 e, -inf behind the vocabulary (nullable: zeros)
     int bias_dtype, vocab, bias_pad;
@@ -328,8 +339,9 @@ struct LayoutArgs {
     int* exponents;                 // ... and here (nullable)
 };
 
-// one launch for whatever a call has to lay out: blockIdx.y 0: x, 1: w, 2: the bias.  fp32: scaled, then x0 + x1, each the fp16 nearest
-// to what is left
+// one launch for whatever a call has to lay out: blockIdx.y 0: x, 1: w, 2: the bias, 3: x for the product over the rows.  fp32: scaled,
+// then x0 + x1, each the fp16 nearest to what is left.  A row of x whose largest element is below 2^-11 of the tensor's is scaled by
+// itself (its shift): a row's results do not depend on the size of the others
 template <typename T, typename E, int PARTS>
 __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
     if (blockIdx.y == 2) {
@@ -341,21 +353,28 @@ __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
     const LayoutJob job = a.job[blockIdx.y];
     if (!job.src) return;
     const T* src = static_cast<const T*>(job.src);
+    E* dst = static_cast<E*>(job.dst);
+    const int which = blockIdx.y == 1 ? 1 : 0;
+    auto counts = [&](int64_t r) { return which == 1 || a.target[r] != a.ignore; };
+    auto exponent = [](uint32_t top) {
+        // the largest into 2^14 ... 2^15 (subnormal numbers: as if of exponent -126); zeros alone stay as they are
+        return top ? 14 - (max((int)(top >> 23), 1) - 127) : 0;
+    };
     int ex = 0;
     if (PARTS > 1) {
         if (a.known) {
-            ex = a.known[blockIdx.y];
+            ex = a.known[which];
         } else {
             __shared__ uint32_t sh[kWavesPerBlock];
             static_assert(kMaxBlocks == kBlock, "a lane reads one workgroup's value");
             uint32_t top = 0;
             if (a.largest) {
-                top = a.largest[blockIdx.y * kMaxBlocks + threadIdx.x];
+                top = a.largest[which * kMaxBlocks + threadIdx.x];
             } else {
                 for (int i = threadIdx.x; i < (int)job.rows * a.cols; i += kBlock) {
                     const int r = i / a.cols;
                     const uint32_t b = __float_as_uint((float)src[r * job.stride + i - r * a.cols]) & 0x7fffffffu;
-                    if (b < 0x7f800000u) top = max(top, b);
+                    if (b < 0x7f800000u && counts(r)) top = max(top, b);
                 }
             }
 #pragma unroll
@@ -363,31 +382,30 @@ __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
             if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
             __syncthreads();
             for (int k = 0; k < kWavesPerBlock; ++k) top = max(top, sh[k]);
-            // the largest into 2^14 ... 2^15 (subnormal numbers: as if of exponent -126); zeros alone stay as they are
-            if (top) ex = 14 - (max((int)(top >> 23), 1) - 127);
+            ex = exponent(top);
         }
-        if (blockIdx.x == 0 && threadIdx.x == 0) {
-            a.scales->ex[blockIdx.y] = ex;
-            if (a.exponents) a.exponents[blockIdx.y] = ex;
+        if (blockIdx.x == 0 && blockIdx.y < 2 && threadIdx.x == 0) {
+            a.scales->ex[which] = ex;
+            if (a.exponents) a.exponents[which] = ex;
         }
     }
-    E* dst = static_cast<E*>(job.dst);
     const int per = (int)(a.ld / 8);
-    const int64_t n = job.rows * per, part = job.rows * a.ld;
-    for (int64_t q = (int64_t)blockIdx.x * kBlock + threadIdx.x; q < n; q += (int64_t)gridDim.x * kBlock) {
-        const int64_t r = q / per;
-        const int c0 = (int)(q - r * per) * 8;
+    const int64_t part = job.rows * a.ld;
+    auto read = [&](int64_t r, int c0) {
         vec_t<T, 8> in;
-        if (((a.vec >> blockIdx.y) & 1) && c0 + 8 <= a.cols) {
+        if (((a.vec >> which) & 1) && c0 + 8 <= a.cols) {
             in = *reinterpret_cast<const vec_t<T, 8>*>(src + r * job.stride + c0);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) in[i] = c0 + i < a.cols ? src[r * job.stride + c0 + i] : (T)0.f;
         }
+        return in;
+    };
+    auto write = [&](int64_t r, int c0, const vec_t<T, 8>& in, int by, bool live) {
         vec_t<E, 8> o[PARTS];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            float v = PARTS > 1 ? ldexpf((float)in[i], ex) : (float)in[i];
+            float v = PARTS > 1 ? (live ? ldexpf((float)in[i], by) : 0.f) : (float)in[i];
 #pragma unroll
             for (int p = 0; p < PARTS; ++p) {
                 o[p][i] = (E)v;
@@ -397,6 +415,36 @@ __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
         }
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) *reinterpret_cast<vec_t<E, 8>*>(dst + p * part + r * a.ld + c0) = o[p];
+    };
+    if (PARTS > 1 && blockIdx.y == 0) {
+        const int l = threadIdx.x & (a.group - 1), rpb = kBlock / a.group;
+        for (int64_t r = (int64_t)blockIdx.x * rpb + threadIdx.x / a.group; r < job.rows; r += (int64_t)gridDim.x * rpb) {
+            const bool live = counts(r);
+            uint32_t top = 0;
+            vec_t<T, 8> in;
+            for (int c = l; c < per; c += a.group) {
+                in = read(r, c * 8);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t b = __float_as_uint((float)in[i]) & 0x7fffffffu;
+                    if (b < 0x7f800000u) top = max(top, b);
+                }
+            }
+            for (int m = 1; m < a.group; m <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, kWave));
+            const int more = live && top ? exponent(top) - ex : 0, shift = more >= 12 ? min(more, 255) : 0;
+            if (l == 0) a.shift[r] = (uint8_t)shift;
+            for (int c = l; c < per; c += a.group) {
+                if (per > a.group) in = read(r, c * 8);
+                write(r, c * 8, in, ex + shift, live);
+            }
+        }
+        return;
+    }
+    const int64_t n = job.rows * per;
+    for (int64_t q = (int64_t)blockIdx.x * kBlock + threadIdx.x; q < n; q += (int64_t)gridDim.x * kBlock) {
+        const int64_t r = q / per;
+        const int c0 = (int)(q - r * per) * 8;
+        write(r, c0, read(r, c0), ex, PARTS == 1 || counts(r));
     }
 }
 
@@ -406,7 +454,7 @@ __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
 // divided by the largest |g|, which goes to scales
 __global__ __launch_bounds__(1024) void ce_rows_kernel(const float* g, int g_is_row, const float* count, const float* row_max, const float* row_sum,
                                                        const int64_t* target, int64_t ignore, int vocab, int64_t rows, int64_t rows_pad,
-                                                       RowState* state, CeScales* scales) {
+                                                       const uint8_t* shift, int narrow, RowState* state, CeScales* scales) {
     __shared__ uint32_t sh[16];
     const float shared = g_is_row ? 0.f : *g / *count;
     uint32_t bits = __float_as_uint(shared) & 0x7fffffffu;
@@ -430,6 +478,7 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(const float* g, int g_is_
         s.inv_s = in ? 1.f / row_sum[r] : 0.f;
         s.g = in ? (g_is_row ? g[r] : shared) / top : 0.f;
         s.target = in ? (int)t : -1;
+        if (narrow) s.target = in ? (int)((uint32_t)t | (shift ? (uint32_t)shift[r] << 24 : 0)) : kNarrowVocab;
         state[r] = s;
     }
 }
@@ -448,7 +497,6 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
     unsigned t = (unsigned)((uint64_t)tiles * xcd / xcds) + blockIdx.x / xcds;
     const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
     E* d = static_cast<E*>(a.d);
-    const float back = logit_scale(a, kLog2e);
     int v0 = 0, r0 = 0;
     auto begin = [&]() {
         unsigned ti, tj;
@@ -469,7 +517,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
         const int64_t rw = (int64_t)r0 + tile.n_wave + col;
         const bool edge = v0 + BM > a.v1;
         RowState st[Tile::NT];
-        float scale[Tile::NT], own_g[Tile::NT];
+        float scale[Tile::NT], own_g[Tile::NT], back[Tile::NT];
         // targets among the wave's entries are rare: their -g is applied behind a branch that most waves do not take
         int at[Tile::NT];
         bool hit = false;
@@ -478,6 +526,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
             st[n] = rw + n * 16 < a.rows ? a.state[rw + n * 16] : RowState{INFINITY, 0.f, 0.f, -1};
             own_g[n] = st[n].g * a.lift;
             scale[n] = st[n].inv_s * own_g[n];
+            back[n] = logit_scale(a, rw + n * 16);
             at[n] = st[n].target - vw;
             hit |= st[n].target >= 0 && at[n] >= 0 && at[n] < Tile::MT * 16;
         }
@@ -500,7 +549,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
                     f32x4 p;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)         // the logit rounded as in the forward, then the difference: the row's maximum gives 1
-                        p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[m + q][n][i], back, b[q][i]) - st[n].m2) * scale[n];
+                        p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[m + q][n][i], back[n], b[q][i]) - st[n].m2) * scale[n];
                     if (any_hit) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
@@ -684,6 +733,8 @@ __global__ __launch_bounds__(1024) void ce_sum_many_kernel(const SumArgs a) {
 // ---- host: plan of a call -------------------------------------------------------------------------------------------------------
 
 constexpr int kBig = 256, kSmall = 128;         // tile edges
+// what 32-bit loop counters and a tile's 31-bit offsets (256 rows) reach
+constexpr int kMaxVocab = 1 << 30, kMaxHidden = 1 << 21;
 // d of one piece of the vocabulary.  A second piece costs dx another pass through memory: 8192 x 32000 x 1024 bf16 takes 2197 us as one
 // piece, 2285 as two of 256 MiB, which would fit the memory-side cache
 constexpr int64_t kPieceBytes = 512ll << 20;
@@ -695,7 +746,7 @@ struct CePlan {
     int parts, pairs;
     bool copy_x, copy_w, narrow;
     int64_t ldh;                    // padded row of a copied operand
-    int64_t x_off, w_off, bias_off, scales_off, largest_off;
+    int64_t x_off, w_off, even_off, shift_off, bias_off, scales_off, largest_off;
     // forward
     bool big_lse;
     int splits;
@@ -713,7 +764,7 @@ static CePlan ce_plan(int64_t R, int V, int H, int dtype, bool x_ok, bool w_ok, 
     p.pairs = dtype == CNF_DTYPE_F32 ? 3 : 1;
     p.copy_x = p.parts > 1 || !x_ok;
     p.copy_w = p.parts > 1 || !w_ok;
-    p.narrow = narrow_supported(H);
+    p.narrow = narrow_supported(H, V);
     p.ldh = round_up(H, p.narrow ? 8 : kStepK);     // whole steps of the products
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -724,7 +775,11 @@ static CePlan ce_plan(int64_t R, int V, int H, int dtype, bool x_ok, bool w_ok, 
     if (p.copy_x) p.x_off = take((int64_t)p.parts * R * p.ldh * 2);
     if (p.copy_w) p.w_off = take((int64_t)p.parts * V * p.ldh * 2);
     p.scales_off = take(sizeof(CeScales));
-    if (p.parts > 1) p.largest_off = take(2 * kMaxBlocks * 4);
+    if (p.parts > 1) {
+        p.largest_off = take(2 * kMaxBlocks * 4);
+        p.shift_off = take(R);
+        if (backward && !p.narrow) p.even_off = take((int64_t)p.parts * R * p.ldh * 2);
+    }
     if (p.narrow) p.bias_off = take(round_up(V, kNarrowWalk) * 4);
     // about four workgroups for every CU, at least two steps of the walk each
     auto narrow_split = [](int64_t own, int64_t walk) {
@@ -786,7 +841,8 @@ static bool rows_aligned32(const void* p, int64_t stride) { return (reinterpret_
 
 template <typename T, typename E, int PARTS>
 static void ce_operands(CeArgs& a, const CePlan& p, const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias,
-                        int bias_dtype, const int* known, int* exponents, int64_t R, int V, int H, char* ws, hipStream_t st) {
+                        int bias_dtype, const int64_t* target, int64_t ignore, const int* known, int* exponents, bool even, int64_t R, int V, int H,
+                        char* ws, hipStream_t st) {
     LayoutArgs l{};
     CeScales* scales = reinterpret_cast<CeScales*>(ws + p.scales_off);
     if constexpr (PARTS > 1) {
@@ -794,13 +850,20 @@ static void ce_operands(CeArgs& a, const CePlan& p, const void* x, int64_t x_str
         // the join, 64 tokens of 51 classes and 64 features take 11.6 us instead of 17.1
         if (!known && std::max<int64_t>(R, V) * H > 8192) {
             uint32_t* largest = reinterpret_cast<uint32_t*>(ws + p.largest_off);
-            CNF_LAUNCH(ce_largest_kernel, dim3(kMaxBlocks, 2), dim3(kBlock), 0, st, static_cast<const float*>(x), x_stride, R,
+            CNF_LAUNCH(ce_largest_kernel, dim3(kMaxBlocks, 2), dim3(kBlock), 0, st, static_cast<const float*>(x), x_stride, R, target, ignore,
                        static_cast<const float*>(w), w_stride, V, H, largest);
             l.largest = largest;
         }
         l.known = known;
         l.scales = scales;
         l.exponents = exponents;
+        l.shift = reinterpret_cast<uint8_t*>(ws + p.shift_off);
+        l.target = target;
+        l.ignore = ignore;
+        l.group = 8;
+        while (l.group < kWave && l.group < p.ldh / 8) l.group *= 2;
+        if (even) l.job[3] = LayoutJob{x, x_stride, R, ws + p.even_off};
+        a.shift = l.shift;
     }
     if (p.copy_x) l.job[0] = LayoutJob{x, x_stride, R, ws + p.x_off};
     if (p.copy_w) l.job[1] = LayoutJob{w, w_stride, V, ws + p.w_off};
@@ -818,10 +881,11 @@ static void ce_operands(CeArgs& a, const CePlan& p, const void* x, int64_t x_str
     if (p.copy_x || p.copy_w || p.narrow) {
         const int64_t chunks = std::max(p.copy_x ? R * (p.ldh / 8) : 0, p.copy_w ? V * (p.ldh / 8) : 0);
         const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(std::max<int64_t>(chunks, l.bias_pad), kBlock), 4096));
-        CNF_LAUNCH((ce_layout_kernel<T, E, PARTS>), dim3(grid, 3), dim3(kBlock), 0, st, l);
+        CNF_LAUNCH((ce_layout_kernel<T, E, PARTS>), dim3(grid, even ? 4 : 3), dim3(kBlock), 0, st, l);
     }
     a.x = p.copy_x ? Operand{ws + p.x_off, p.ldh, R * p.ldh, (int)R} : Operand{x, x_stride, 0, (int)R};
     a.w = p.copy_w ? Operand{ws + p.w_off, p.ldh, V * p.ldh, V} : Operand{w, w_stride, 0, V};
+    a.x_even = even ? Operand{ws + p.even_off, p.ldh, R * p.ldh, (int)R} : a.x;
     a.pairs = p.pairs;
     a.parts = p.parts;
     a.rows = R;
@@ -851,6 +915,7 @@ static NarrowArgs narrow_args(const CeArgs& a, const CePlan& p, bool rows_own, c
     n.state = a.state;
     n.scales = a.scales;
     n.scaled = a.scaled;
+    n.shift = a.shift;
     n.lift = a.lift;
     return n;
 }
@@ -873,7 +938,7 @@ static bool ce_aligned(const void* p, int64_t stride, int dtype, int H) {
 using namespace cnf;
 
 #define CE_CHECK(name)                                                                                                             \
-    CNF_REQUIRE(R >= 0 && V > 0 && H > 0 && R <= 0x7fffff00ll && V <= 0x7fffff00 && H <= 0x7fffff00, name ": bad size R=%ld V=%d H=%d", \
+    CNF_REQUIRE(R >= 0 && V > 0 && H > 0 && R <= 0x7fffff00ll && V <= kMaxVocab && H <= kMaxHidden, name ": bad size R=%ld V=%d H=%d", \
                 (long)R, V, H);                                                                                                    \
     CNF_REQUIRE(dtype_known(dtype) && dtype_known(bias_dtype), name ": unknown element type");                                     \
     CNF_REQUIRE(x_stride >= 0 && w_stride >= 0, name ": negative stride")
@@ -881,7 +946,7 @@ using namespace cnf;
 extern "C" {
 
 int64_t cnf_linear_ce_workspace_bytes(int64_t R, int V, int H, int dtype, int backward) {
-    if (R <= 0 || V <= 0 || H <= 0 || !dtype_known(dtype)) return 0;
+    if (R <= 0 || R > 0x7fffff00ll || V <= 0 || V > kMaxVocab || H <= 0 || H > kMaxHidden || !dtype_known(dtype)) return 0;
     return ce_plan(R, V, H, dtype, false, false, backward != 0).bytes;
 }
 
@@ -901,7 +966,8 @@ int cnf_linear_ce(const void* x, int64_t x_stride, const void* weight, int64_t w
             typedef decltype(t) T;
             typedef decltype(e) E;
             CeArgs a{};
-            ce_operands<T, E, decltype(parts)::value>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, nullptr, exponents, R, V, H, ws, st);
+            ce_operands<T, E, decltype(parts)::value>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, target, ignore_index, nullptr, exponents, false, R, V, H,
+                                                     ws, st);
             a.target = target;
             a.ignore = ignore_index;
             a.partial = reinterpret_cast<float2*>(ws + p.partial_off);
@@ -957,12 +1023,14 @@ int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64
         typedef decltype(e) E;
         constexpr int PARTS = decltype(parts)::value;
         CeArgs a{};
-        ce_operands<T, E, PARTS>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, exponents, nullptr, R, V, H, ws, st);
+        ce_operands<T, E, PARTS>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, target, ignore_index, exponents, nullptr,
+                                 PARTS > 1 && !p.narrow && dweight, R, V, H, ws, st);
         RowState* state = reinterpret_cast<RowState*>(ws + p.state_off);
         a.state = state;
         // per-row gradients: every workgroup finds the largest |g| itself; few of them
         CNF_LAUNCH(ce_rows_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(p.rows_pad, 1024), g_per_row ? 16 : 1024)), dim3(1024), 0, st, g,
-                   g_per_row, count, row_max, row_sum, target, ignore_index, V, R, p.rows_pad, state, reinterpret_cast<CeScales*>(ws + p.scales_off));
+                   g_per_row, count, row_max, row_sum, target, ignore_index, V, R, p.rows_pad, a.shift, p.narrow, state,
+                   reinterpret_cast<CeScales*>(ws + p.scales_off));
         const int64_t ld4 = round_up(H, 4);
         if (p.narrow) {
             if (dx) {
@@ -1032,7 +1100,7 @@ int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64
             // dw[v][h] = sum_r x[r][h] d[r][v]; db[v] = sum_r d[r][v]
             char* dw = static_cast<char*>(dweight) + v0 * H * dtype_bytes(dtype);
             char* db = dbias ? static_cast<char*>(dbias) + v0 * dtype_bytes(bias_dtype) : nullptr;
-            q.a = a.x;
+            q.a = a.x_even;
             q.a.ext = H;
             q.b = d;
             q.b.ext = (int)width;

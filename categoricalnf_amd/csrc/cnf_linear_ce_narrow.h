@@ -10,12 +10,15 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 struct RowState {       // backward: what an element d = (exp2(l2 - m2) inv_s - [target]) g, l2 = l log2 e, needs of its row
     float m2, inv_s;    // maximum times log2 e (+inf: the row is ignored); 1 / s
     float g;            // over the largest |g|
-    int target;         // -1: ignored
+    int target;         // -1: ignored.  Few features: target_of(), and in the upper 8 bits the row's shift
 };
+constexpr int kNarrowVocab = (1 << 24) - 1;             // so many classes at most; its value as a target: ignored
+__device__ __forceinline__ int target_of(int word) { return word & kNarrowVocab; }
+__device__ __forceinline__ int shift_of(int word) { return (int)((uint32_t)word >> 24); }
 
 // what the operands of a call were scaled by; in device memory
 struct CeScales {
-    int ex[2];          // fp32: x was multiplied by 2^ex[0], w by 2^ex[1]
+    int ex[2];          // fp32: x was multiplied by 2^ex[0] (its row r by 2^(ex[0] + shift[r])), w by 2^ex[1]
     float top;          // largest |g|
 };
 
@@ -43,7 +46,8 @@ struct NarrowArgs {
     int64_t ld;
     int final_dtype;
     const CeScales* scales;
-    int scaled;                         // fp32 operands: scales->ex holds
+    int scaled;                         // fp32 operands: scales->ex holds, and
+    const uint8_t* shift;               // [rows] what the rows of x were scaled by beyond it (forward)
     float lift;                         // d is computed times lift (a power of two): small probabilities stay normal numbers in fp16
     void* db;                           // nullable; partial sums: in column ld - 4 of out
     int db_dtype;
@@ -51,7 +55,7 @@ struct NarrowArgs {
 
 enum NarrowJob { kNarrowLse, kNarrowDx, kNarrowDw };
 
-bool narrow_supported(int hidden);
+bool narrow_supported(int hidden, int vocab);
 int narrow_launch(NarrowJob job, int dtype, const NarrowArgs& a, hipStream_t st);
 
 }  // namespace cnf

@@ -141,26 +141,30 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
     float bias_n[NT];
     int want[NT];
     // a logit (times log2 e) is its product times `back` plus the bias
-    const int ex = a.scaled ? a.scales->ex[0] + a.scales->ex[1] : 0;
-    const float back = ldexpf(kLog2e, max(min(-ex, 126), -300));
+    float back[NT];
     s16x8 own[PARTS][KK][NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int64_t e = n_wave + n * 16 + col;
         bool in = e < own_n;
-        st[n] = RowState{INFINITY, 0.f, 0.f, -1};
+        st[n] = RowState{INFINITY, 0.f, 0.f, kNarrowVocab};
         bias_n[n] = 0.f;
         want[n] = -1;
+        int shift = 0;
         if (JOB == kNarrowLse) {
             const int64_t t = in ? a.target[e] : -1;
+            shift = in && a.scaled ? a.shift[e] : 0;
             want[n] = t >= 0 && t < a.vocab && t != a.ignore ? (int)t : -1;
         } else if (JOB == kNarrowDx) {
             if (in) st[n] = a.state[e];
             st[n].inv_s *= a.lift;
-            in = in && st[n].target >= 0;               // an ignored row: operand 0, maximum +inf, so that d = 0 whatever the row holds
+            shift = shift_of(st[n].target);
+            st[n].target = target_of(st[n].target);
+            in = in && st[n].target != kNarrowVocab;               // an ignored row: operand 0, maximum +inf, so that d = 0 whatever the row holds
         } else {
             bias_n[n] = in ? a.bias[e] : -INFINITY;     // d = 0
         }
+        back[n] = a.scaled ? ldexpf(kLog2e, max(min(-(a.scales->ex[0] + a.scales->ex[1] + shift), 126), -300)) : kLog2e;
 #pragma unroll
         for (int p = 0; p < PARTS; ++p)
 #pragma unroll
@@ -210,11 +214,13 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
 #pragma unroll
                     for (int p = 0; p < PARTS; ++p) f[p] = Tile::frag(s, p, mp * 32 + t * 16, kk);
 #pragma unroll
-                    for (int order = PARTS - 1; order >= 0; --order)          // smallest products first
-#pragma unroll
-                        for (int p = 0; p <= order; ++p)
+                    for (int order = PARTS - 1; order >= 0; --order)          // smallest products first, w's first part before its second:
+#pragma unroll                                                                // the forward's logit to the bit, whichever side is walked
+                        for (int i = 0; i <= order; ++i) {
+                            const int p = JOB == kNarrowDw ? order - i : i;
 #pragma unroll
                             for (int n = 0; n < NT; ++n) sc[t][n] = mfma16<E>(f[p], own[order - p][kk][n], sc[t][n]);
+                        }
                 }
             }
             const int64_t m0 = m_tile + mp * 32 + g * 4;            // the lane's first walk entry: 16 t + i further
@@ -229,7 +235,7 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) sc[t][n][i] = __builtin_fmaf(sc[t][n][i], back, bias[t][i]);
+                        for (int i = 0; i < 4; ++i) sc[t][n][i] = __builtin_fmaf(sc[t][n][i], back[n], bias[t][i]);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const int64_t at = want[n] - m0;
@@ -268,13 +274,25 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
             const RowState* row = reinterpret_cast<const RowState*>(s + Tile::kBytes) + mp * 32 + g * 4;
             float row_m2[8], row_scale[8];          // dw: the row's g and the lift in its scale
             int row_target[8];
+            bool shifted = false;                   // rows that were scaled by more than the others: rare
             if (JOB == kNarrowDw) {
+                int words = 0;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const RowState& q = row[(e / 4) * 16 + e % 4];
                     row_m2[e] = q.m2;
                     row_scale[e] = q.inv_s * q.g * a.lift;
-                    row_target[e] = q.target;
+                    row_target[e] = target_of(q.target);
+                    words |= q.target;
+                }
+                shifted = PARTS > 1 && __ballot(shift_of(words) != 0) != 0;
+                if (shifted) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int s = shift_of(row[(e / 4) * 16 + e % 4].target);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) sc[e / 4][n][e % 4] = ldexpf(sc[e / 4][n][e % 4], -s);
+                    }
                 }
             }
 #pragma unroll
@@ -286,11 +304,13 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
                     const float f = JOB == kNarrowDw ? row_scale[e] : st[n].inv_s;      // dx: times the lift; g comes at the end
                     const float b = JOB == kNarrowDw ? bias_n[n] : bias[e / 4][e % 4];
                     // the logit rounded as in the forward, then the difference: the row's maximum gives 1
-                    v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e / 4][n][e % 4], back, b) - m) * f;
+                    v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e / 4][n][e % 4], back[n], b) - m) * f;
+                    // an ignored row of x read as it is: its logits may have overflowed (fp32 ones are laid out as zeros)
+                    if (JOB == kNarrowDw && PARTS == 1) v[e] = row_target[e] == kNarrowVocab ? 0.f : v[e];
                 }
                 if (JOB == kNarrowDx) {
                     const int64_t at = st[n].target - m0;
-                    if (__ballot(st[n].target >= 0 && at >= 0 && at < 32)) {
+                    if (__ballot(st[n].target != kNarrowVocab && at >= 0 && at < 32)) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
                             if (at == (e / 4) * 16 + e % 4) v[e] -= a.lift;
@@ -307,6 +327,10 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
                     }
 #pragma unroll
                     for (int e = 0; e < 8; ++e) sum[n] += v[e];
+                    if (shifted) {                  // x's row is that much larger in the second product
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], -shift_of(row[(e / 4) * 16 + e % 4].target));
+                    }
                 }
                 vec_t<E, 8> o[PARTS];
 #pragma unroll
@@ -452,7 +476,7 @@ static void narrow_width(NarrowJob job, const NarrowArgs& a, hipStream_t st) {
     else narrow_job<E, PARTS, 128>(job, a, st);
 }
 
-bool narrow_supported(int hidden) { return hidden <= 128; }
+bool narrow_supported(int hidden, int vocab) { return hidden <= 128 && vocab <= kNarrowVocab; }
 
 int narrow_launch(NarrowJob job, int dtype, const NarrowArgs& a, hipStream_t st) {
     if (dtype == CNF_DTYPE_F32) narrow_width<f16_t, 2>(job, a, st);

@@ -112,7 +112,7 @@ Tensor opt(const std::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(
 std::tuple<Tensor, Tensor, Tensor> layer_norm_raw(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, bool want_stats) {
     const int code = dtype_code(x, "x");
     TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0, "layer_norm needs a last axis of at least one element, got shape ", x.sizes());
-    TORCH_CHECK_VALUE(x.size(-1) <= 0x7fffffff, "layer_norm: ", x.size(-1), " columns");
+    TORCH_CHECK_VALUE(x.size(-1) <= 1 << 30, "layer_norm: ", x.size(-1), " columns");
     const int64_t C = x.size(-1);
     const Tensor w = vector_of(weight, C, "weight", x.device()), b = vector_of(bias, C, "bias", x.device());
     TORCH_CHECK_TYPE(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(), "weight is ", w.defined() ? w.scalar_type() : at::kFloat,
@@ -215,7 +215,7 @@ CeOperands ce_operands(const Tensor& x, const Tensor& weight, const Tensor& targ
     o.V = weight.size(0);
     o.H = weight.size(1);
     o.R = target.numel();
-    TORCH_CHECK_VALUE(o.V <= 0x7fffff00 && o.H <= 0x7fffff00 && o.R <= 0x7fffff00, "linear_cross_entropy: sizes ", o.R, " x ", o.V, " x ", o.H);
+    TORCH_CHECK_VALUE(o.V <= 1 << 30 && o.H <= 1 << 21 && o.R <= 0x7fffff00, "linear_cross_entropy: sizes ", o.R, " x ", o.V, " x ", o.H);
     o.b = vector_of(bias, o.V, "bias", x.device());
     o.bcode = o.b.defined() ? dtype_code(o.b, "bias") : CNF_DTYPE_F32;
     TORCH_CHECK_TYPE(o.bcode == o.code || o.bcode == CNF_DTYPE_F32, "bias is float32 or of the weight's type, got ", o.b.scalar_type());
@@ -280,17 +280,20 @@ std::tuple<Tensor, Tensor, Tensor> linear_ce_bwd_raw(const Tensor& x, const Tens
 
 enum Reduction { kNone = 0, kMean = 1, kSum = 2 };
 
+// one of the reduced values as a tensor of its own, no view: a caller may change a loss in place while the count is kept for the backward
+Tensor value_of(const Tensor& reduced, int64_t k) { return at::empty({0}, reduced.options()).set_(reduced.storage(), k, {}, {}); }
+
 struct LinearCeNode : torch::autograd::Function<LinearCeNode> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const std::optional<Tensor>& b, const Tensor& target,
                           int64_t ignore_index, int64_t reduction, const Tensor& flags) {
         const Tensor bias = opt(b);
         auto [loss, stats, reduced, exps] = linear_ce_raw(x, weight, target, bias, ignore_index, reduction != kNone, flags);
         Tensor count;
-        if (reduction == kMean) count = reduced.select(0, 2);
+        if (reduction == kMean) count = value_of(reduced, 2);
         ctx->save_for_backward({x, weight, bias, target, stats, exps, count});
         ctx->saved_data["ignore"] = ignore_index;
         ctx->saved_data["reduction"] = reduction;
-        return reduction == kNone ? loss : reduced.select(0, reduction - 1);
+        return reduction == kNone ? loss : value_of(reduced, reduction - 1);
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         const auto s = ctx->get_saved_variables();
@@ -307,7 +310,7 @@ Tensor linear_ce(const Tensor& x, const Tensor& weight, const Tensor& target, co
     const Tensor b = opt(bias);
     if (wants_grad({&x, &weight, &b})) return LinearCeNode::apply(x, weight, bias, target, ignore_index, reduction, flags);
     auto [loss, stats, reduced, exps] = linear_ce_raw(x, weight, target, b, ignore_index, reduction != kNone, flags);
-    return reduction == kNone ? loss : reduced.select(0, reduction - 1);
+    return reduction == kNone ? loss : value_of(reduced, reduction - 1);
 }
 
 // ---- AdamW -------------------------------------------------------------------------------------------------------------------------
@@ -330,15 +333,18 @@ struct TensorList {
     }
 };
 
-// no two tensors of a list share memory
-void check_apart(const std::vector<void*>& at, const std::vector<int64_t>& n, int64_t size, const char* name) {
+// no two of the tensors that are written share memory: [list][tensor] addresses, elements and bytes of an element
+void check_apart(const std::vector<std::vector<void*>>& at, const std::vector<int64_t>& numel, const std::vector<int64_t>& size, int64_t block) {
     std::vector<std::pair<uintptr_t, uintptr_t>> spans;
-    spans.reserve(at.size());
-    for (size_t i = 0; i < at.size(); ++i)
-        if (n[i]) spans.emplace_back((uintptr_t)at[i], (uintptr_t)at[i] + n[i] * size);
+    spans.reserve(at.size() * numel.size());
+    for (size_t k = 0; k < at.size(); ++k) {
+        if (k == 1) continue;                   // gradients are read only
+        for (size_t i = 0; i < numel.size(); ++i)
+            if (numel[i]) spans.emplace_back((uintptr_t)at[k][i], (uintptr_t)at[k][i] + (k < 4 ? numel[i] : (numel[i] + block - 1) / block) * size[k]);
+    }
     std::sort(spans.begin(), spans.end());
     for (size_t i = 1; i < spans.size(); ++i)
-        TORCH_CHECK_VALUE(spans[i].first >= spans[i - 1].second, "adamw_step: two tensors of ", name, " share memory");
+        TORCH_CHECK_VALUE(spans[i].first >= spans[i - 1].second, "adamw_step: two of the parameters and moments share memory");
 }
 
 // a step's number: a host value, or one float32 on the device
@@ -395,9 +401,7 @@ void adamw_step(const py::object& params, const py::object& grads, const py::obj
             at_[k][i] = t->data_ptr();
         }
     }
-    check_apart(at_[0], numel, p0.element_size(), names[0]);
-    check_apart(at_[2], numel, bits8 ? 1 : 4, names[2]);
-    check_apart(at_[3], numel, bits8 ? 1 : 4, names[3]);
+    check_apart(at_, numel, {p0.element_size(), 0, bits8 ? 1 : 4, bits8 ? 1 : 4, 4, 4}, block);
     TORCH_CHECK_VALUE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "adamw_step: betas outside [0, 1)");
     const auto [step_host, step_dev] = scalar(step, "step", device);
     const auto [lr_host, lr_dev] = scalar(lr, "lr", device);

@@ -7,6 +7,8 @@ from ... import functional as Fn
 from ...host_utils import get_param_val
 from ..networks.help_layers import LinearNet
 
+_NO_CLASS = -2 ** 63         # no category is left out: one outside the vocabulary is an error
+
 
 def create_embed_layer(vocab, vocab_size, default_embed_layer_dims):
     """nn.Embedding from scratch or from a torchtext vocabulary's vectors (decoder.py:12-21)."""
@@ -52,7 +54,7 @@ class DecoderLinear(nn.Module):
         [..., C] log-probabilities are never written (one fused kernel per direction instead of GEMM + log-softmax + gather)."""
         last = self.layers.main_net[-1]
         hidden = self.layers.hidden_features(self._features(z_cont))
-        return -Fn.linear_cross_entropy(hidden, last.weight, z_categ, last.bias, ignore_index=-100, reduction="none")
+        return -Fn.linear_cross_entropy(hidden, last.weight, z_categ, last.bias, ignore_index=_NO_CLASS, reduction="none")
 
     def info(self):
         return "Linear model with hidden size %i and %i layers" % (self.hidden_size, self.num_layers)

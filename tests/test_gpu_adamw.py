@@ -372,6 +372,18 @@ def test_driver_trains_checkpoints_and_resumes(optimizer, graph_step, tmp_path):
     assert math.isfinite(first["val_bpd"]) and math.isfinite(second["val_bpd"])
 
 
+def test_more_elements_than_2_to_the_31():
+    n, tail = 2 ** 31 + 5000, 7000
+    p, g = torch.zeros(n, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    m, v = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    g[-tail:].normal_()
+    small = [t[-tail:].clone() for t in (p, g, m, v)]
+    ops.adamw_step([p], [g], [m], [v], step=1, lr=1e-2)
+    ops.adamw_step([small[0]], [small[1]], [small[2]], [small[3]], step=1, lr=1e-2)
+    for a, b in zip((p, m, v), (small[0], small[2], small[3])):
+        assert torch.equal(a[-tail:], b) and not a[:-tail].any()
+
+
 def test_refusals():
     t = Tensors([300, 40])
     call = lambda **kw: ops.adamw_step(kw.get("p", t.p), kw.get("g", t.g), kw.get("m", t.m), kw.get("v", t.v), step=kw.get("step", 1),
@@ -382,11 +394,20 @@ def test_refusals():
                       (dict(beta1=1.0), ValueError), (dict(ms=[1]), ValueError), (dict(g=[g.half() for g in t.g]), TypeError),
                       (dict(p=[t.p[0].cpu(), t.p[1].cpu()]), ops.HipOnlyError), (dict(g=[t.g[0], t.g[1].cpu()]), ValueError),
                       (dict(lr=torch.tensor(1e-3)), ValueError), (dict(step=torch.tensor(1, device="cuda")), ValueError),
+                      (dict(m=t.v), ValueError), (dict(p=t.m), ValueError), (dict(m=[t.p[0], t.m[1]]), ValueError),
                       (dict(v=[t.v[0].double(), t.v[1]]), ValueError), (dict(ms=[t.m[0], t.m[1]], vs=[t.v[0], t.v[1]]), ValueError)):
         with pytest.raises(kind):
             call(**bad)
     for x, y in zip(t.p, before):
         assert torch.equal(x, y)
+    # 8-bit moments whose scales are shared: between two tensors, and between the two moments
+    p, g = [torch.zeros(40, device="cuda") for _ in range(2)], [torch.ones(40, device="cuda") for _ in range(2)]
+    m, v = [torch.zeros(40, dtype=torch.int8, device="cuda") for _ in range(2)], [torch.zeros(40, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    s = [torch.zeros(1, device="cuda") for _ in range(4)]
+    for ms, vs in (([s[0], s[0]], s[2:]), (s[:2], [s[2], s[2]]), (s[:2], s[1:3])):
+        with pytest.raises(ValueError):
+            call(p=p, g=g, m=m, v=v, ms=ms, vs=vs)
+    call(p=p, g=g, m=m, v=v, ms=s[:2], vs=s[2:])
     w = torch.nn.Parameter(torch.randn(6, 4, device="cuda").t())
     opt = AdamW([w])
     w.grad = torch.randn(4, 6, device="cuda")

@@ -234,6 +234,21 @@ def test_captured_step_replays():
         del y
 
 
+def test_more_elements_than_2_to_the_31():
+    """Rows whose elements lie beyond 2^31 give what they give at the front."""
+    C, n = 512, 300
+    R = 2 ** 31 // C + n
+    x, g = torch.zeros(R, C, dtype=BF16, device="cuda"), torch.zeros(R, C, dtype=BF16, device="cuda")
+    x[-n:].normal_(), g[-n:].normal_()
+    w, b = torch.randn(C, device="cuda").to(BF16), torch.randn(C, device="cuda").to(BF16)
+    front_x, front_g = x[-n:].clone(), g[-n:].clone()
+    x.requires_grad_(), front_x.requires_grad_()
+    y, front_y = Fn.layer_norm(x, w, b), Fn.layer_norm(front_x, w, b)
+    assert torch.equal(y[-n:], front_y) and torch.equal(y[:2], b.expand(2, C))
+    (dx,), (front_dx,) = torch.autograd.grad(y, x, g), torch.autograd.grad(front_y, front_x, front_g)
+    assert torch.equal(dx[-n:], front_dx) and not dx[:-n].any()
+
+
 def test_module_is_the_kernel_on_the_gpu_and_torch_elsewhere():
     torch.manual_seed(0)
     mine, ref = LayerNorm(72).cuda(), torch.nn.LayerNorm(72)

@@ -228,6 +228,87 @@ def test_rows_that_are_not_finite_stay_alone():
     assert not torch.isfinite(loss[~rest]).any() and torch.equal(loss[rest], clean[rest])
 
 
+@pytest.mark.parametrize("shape", [(200, 300, 40), (150, 700, 200), (1100, 700, 64)], ids=str)
+def test_rows_of_very_different_sizes(shape):
+    """fp32 operands are split after a scaling: a row's loss and gradient do not suffer from larger rows beside it.  dweight adds rows
+    of all sizes: each of them, and its d, is kept to 2^-39 of the largest, so that R products are off by 2^-38 max|g| max|x| each."""
+    x, w, b, t, g = make(*shape, F32)
+    x = x * 10.0 ** torch.linspace(-3, 12, shape[0], device="cuda")[torch.randperm(shape[0], device="cuda")][:, None]
+    for v in (x, w, b):
+        v.requires_grad_()
+    loss = Fn.linear_cross_entropy(x, w, t, b, reduction="none")
+    grads = torch.autograd.grad(loss, (x, w, b), g)
+    val, tol = reference(x, w, t, b, g)
+    tol["dw"] = tol["dw"] + shape[0] * 2.0 ** -38 * float(g.max()) * float(x.detach().abs().max())
+    for name, got in zip(("loss", "dx", "dw", "db"), (loss,) + grads):
+        check(name, got, val, tol)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", [(70, 51, 64), (300, 300, 40), (300, 600, 200)], ids=str)
+def test_what_ignored_rows_hold_does_not_matter(shape, dtype):
+    """The bits of a call whose ignored rows are zeros; in fp32 (whose rows are laid out anew) also with infinities and NaN in them."""
+    x, w, b, t, g = make(*shape, dtype)
+    gone = (t == -100).nonzero()[:, 0]
+    def run(fills):
+        x2 = x.detach().clone()
+        for i, r in enumerate(gone.tolist()):
+            x2[r] = fills[i % len(fills)]
+        x2.requires_grad_()
+        leaves = (x2, w.detach().requires_grad_(), b.detach().requires_grad_())
+        loss = Fn.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], reduction="none")
+        return (loss.detach(),) + torch.autograd.grad(loss, leaves, g)
+    clean = run([0.0])
+    fills = [1e30, -3e38, 0.0] + ([math.inf, math.nan] if dtype == F32 else [])
+    for a, c in zip(run(fills), clean):
+        assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_the_loss_may_be_changed_in_place(reduction):
+    x, w, b, t, _ = make(30, 40, 16, F32)
+    grads = []
+    for inplace in (False, True):
+        leaves = [v.detach().clone().requires_grad_() for v in (x, w, b)]
+        loss = Fn.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], reduction=reduction)
+        assert loss._base is None
+        if inplace:
+            loss /= 4
+        else:
+            loss = loss / 4
+        loss.sum().backward()
+        grads.append([v.grad for v in leaves])
+    assert all(torch.equal(a, c) for a, c in zip(*grads))
+
+
+@pytest.mark.parametrize("vocab", [2 ** 24 - 1, 2 ** 24 + 3])
+def test_vocabularies_around_2_to_the_24(vocab):
+    """The most classes whose index shares a word with a row's shift, and more; targets at both ends."""
+    x, w, b, t, g = make(5, vocab, 8, BF16, ignored=0.0)
+    t[0], t[1], t[2] = vocab - 1, 0, -100
+    run_and_check(x, w, b, t, g)
+
+
+def test_more_elements_than_2_to_the_31():
+    """Rows whose elements lie beyond 2^31 give what they give at the front."""
+    H, V, n = 64, 51, 3000
+    R = 2 ** 31 // H + n
+    small, w, b, t, _ = make(n, V, H, BF16)
+    x = torch.zeros(R, H, dtype=BF16, device="cuda")
+    x[-n:] = small
+    target = torch.full((R,), -100, device="cuda")
+    target[-n:] = t
+    x.requires_grad_(), w.requires_grad_(), b.requires_grad_()
+    loss = Fn.linear_cross_entropy(x, w, target, b, reduction="sum")
+    (dx, dw, db) = torch.autograd.grad(loss, (x, w, b))
+    val, tol = reference(small, w, t, b, torch.ones(n, device="cuda"))
+    tol["dw"] = tol["dw"] * (1 + R / n)          # the reference's count of additions: n rows, here R
+    tol["db"] = tol["db"] * (1 + R / n)
+    assert abs(float(loss.detach()) - float(val["loss"].sum())) <= float(tol["loss"].sum()) + U * float(val["loss"].sum())
+    check("dx", dx[-n:], val, tol), check("dw", dw, val, tol), check("db", db, val, tol)
+    assert not dx[:-n].any()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_large_logits(dtype):
     """Logits of some thousands: the maximum is taken out before the exponential; certain rows have loss 0 and gradient 0."""
@@ -356,6 +437,18 @@ def test_refusals_on_the_gpu():
     (g,) = torch.autograd.grad(ce(x, w, t, b), x, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+def test_decoder_ignores_no_category():
+    dec = DecoderLinear(num_categories=30, embed_dim=5, hidden_size=64, num_layers=1).cuda()
+    z, c = torch.randn(8, 5, device="cuda"), torch.randint(0, 30, (8,), device="cuda")
+    for bad in (-100, -1, 30):
+        c[3] = bad
+        with torch.no_grad():
+            out = dec.class_log_prob(z, c)
+        with pytest.raises(AssertionError):
+            ops.check_flags(z.device)
+        assert torch.isnan(out[3]) and torch.isfinite(out[:3]).all()
 
 
 @pytest.mark.parametrize("num_layers", [0, 1, 2])

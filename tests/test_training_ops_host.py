@@ -85,6 +85,20 @@ def test_linear_ce_refuses_before_launching(lib):
         assert lib.cnf_linear_ce_bwd(*args) == 1
 
 
+def test_sizes_beyond_the_loop_counters_are_refused(lib):
+    """Rows, classes or features that a kernel's 32-bit counters and offsets do not reach: an error before anything is launched."""
+    for R, V, H in ((4, 2 ** 30 + 1, 8), (4, 50, 2 ** 21 + 8), (2 ** 31 - 1, 50, 16)):
+        assert lib.cnf_linear_ce_workspace_bytes(R, V, H, 1, 1) == 0
+        args = [P, H, P, H, None, P, -100, P, P, P, None, None, P, 2 ** 62, R, V, H, 1, 1, None, None]
+        assert lib.cnf_linear_ce(*args) == 1 and b"bad size" in lib.cnf_last_error()
+        args = [P, H, P, H, None, P, -100, P, P, None, P, 1, None, P, P, None, P, 2 ** 62, R, V, H, 1, 1, None]
+        assert lib.cnf_linear_ce_bwd(*args) == 1 and b"bad size" in lib.cnf_last_error()
+    C = 2 ** 30 + 1
+    assert lib.cnf_layer_norm(P, C, None, None, P, None, None, 1, C, 1e-5, 0, 0, None) == 1 and b"bad size" in lib.cnf_last_error()
+    assert lib.cnf_layer_norm_bwd(P, C, P, C, None, P, P, P, None, None, None, 0, 1, C, 0, 0, None) == 1 and b"bad size" in lib.cnf_last_error()
+    assert lib.cnf_layer_norm_bwd_workspace_floats(1, C) == 0
+
+
 def test_linear_ce_workspace_is_bounded(lib):
     """The gradient of the logits never takes more than 512 MiB beyond what one strip of 256 classes needs, however large the
     vocabulary: nothing of size rows x vocabulary is kept."""
