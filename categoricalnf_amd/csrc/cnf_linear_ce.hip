@@ -274,47 +274,62 @@ __global__ __launch_bounds__(1024) void ce_reduce_kernel(const double* sums, int
 // ---- operand layout ----------------------------------------------------------------------------------------------------------------
 
 constexpr int kMaxBlocks = 256;
-// fp32: the largest finite |element| of x's rows that count (blockIdx.y 0) and of w (1), one value per workgroup
-__global__ __launch_bounds__(kBlock) void ce_largest_kernel(const float* x, int64_t x_stride, int64_t R, const int64_t* target, int64_t ignore,
-                                                            const float* w, int64_t w_stride, int V, int H, uint32_t* largest) {
-    __shared__ uint32_t sh[kWavesPerBlock];
-    const float* src = blockIdx.y ? w : x;
-    const int64_t stride = blockIdx.y ? w_stride : x_stride, rows = blockIdx.y ? V : R;
+// the largest finite |element| (its bits) that this lane sees of fp32 rows `block`, `block` + `blocks`, ... (in units of the rows that a
+// workgroup's lanes share at a time); rows with target == ignore do not count (target: nullable).  Four rows are in flight
+__device__ __forceinline__ uint32_t largest_of(const float* src, int64_t stride, int64_t rows, int H, const int64_t* target, int64_t ignore, int block,
+                                               int blocks) {
+    int g = 1;
+    while (g < (int)blockDim.x && g * 4 < H) g <<= 1;
+    const int l = threadIdx.x & (g - 1), rpb = blockDim.x / g;
+    const bool vec = stride % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
     uint32_t top = 0;
-    // row: asked for only where an element exceeds all that the lane has seen
-    auto see = [&](float v, auto row) {
-        const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
-        if (b > top && b < 0x7f800000u && (blockIdx.y || target[row()] != ignore)) top = b;
-    };
-    const int64_t step = (int64_t)kMaxBlocks * kBlock, at = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-    if (stride == H && rows * H % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-        const f32x4* v = reinterpret_cast<const f32x4*>(src);
-        const int64_t n = rows * H / 4;
-        int64_t i = at;
-        for (; i + 3 * step < n; i += 4 * step) {           // four loads in flight
-            const f32x4 q[4] = {v[i], v[i + step], v[i + 2 * step], v[i + 3 * step]};
+    const int64_t step = (int64_t)blocks * rpb;
+    for (int64_t r = (int64_t)block * rpb + threadIdx.x / g; r < rows; r += 4 * step) {
+        bool live[4];
 #pragma unroll
-            for (int k = 0; k < 16; ++k) see(q[k / 4][k % 4], [&] { return (4 * (i + k / 4 * step) + k % 4) / H; });
-        }
-        for (; i < n; i += step) {
-            const f32x4 q = v[i];
+        for (int k = 0; k < 4; ++k) live[k] = r + k * step < rows && (!target || target[r + k * step] != ignore);
+        for (int c = l * 4; c < H; c += g * 4) {
+            f32x4 v[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) see(q[k], [&] { return (4 * i + k) / H; });
+            for (int k = 0; k < 4; ++k) {
+                const float* p = src + (r + k * step) * stride + c;
+                v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (r + k * step >= rows) continue;
+                if (vec && c + 4 <= H) {
+                    v[k] = *reinterpret_cast<const f32x4*>(p);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[k][i] = c + i < H ? p[i] : 0.f;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t b = __float_as_uint(v[k][i]) & 0x7fffffffu;
+                    if (live[k] && b < 0x7f800000u) top = max(top, b);
+                }
         }
-    } else if (stride == H) {
-        for (int64_t i = at; i < rows * H; i += step) see(src[i], [&] { return i / H; });
-    } else {
-        for (int64_t r = blockIdx.x; r < rows; r += kMaxBlocks)
-            for (int c = threadIdx.x; c < H; c += kBlock) see(src[r * stride + c], [&] { return r; });
     }
+    return top;
+}
+// of the workgroup, in every lane
+__device__ __forceinline__ uint32_t block_max(uint32_t top, uint32_t* sh) {
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, kWave));
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int k = 1; k < kWavesPerBlock; ++k) top = max(top, sh[k]);
-        largest[blockIdx.y * kMaxBlocks + blockIdx.x] = top;
-    }
+    for (int k = 0; k < (int)blockDim.x / kWave; ++k) top = max(top, sh[k]);
+    return top;
+}
+
+// fp32: the largest finite |element| of x's rows that count (blockIdx.y 0) and of w (1), one value per workgroup
+__global__ __launch_bounds__(1024) void ce_largest_kernel(const float* x, int64_t x_stride, int64_t R, const int64_t* target, int64_t ignore,
+                                                            const float* w, int64_t w_stride, int V, int H, uint32_t* largest) {
+    __shared__ uint32_t sh[16];
+    const uint32_t top = block_max(blockIdx.y ? largest_of(w, w_stride, V, H, nullptr, 0, blockIdx.x, kMaxBlocks)
+                                              : largest_of(x, x_stride, R, H, target, ignore, blockIdx.x, kMaxBlocks), sh);
+    if (threadIdx.x == 0) largest[blockIdx.y * kMaxBlocks + blockIdx.x] = top;
 }
 
 struct LayoutJob {
@@ -367,22 +382,9 @@ __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
         } else {
             __shared__ uint32_t sh[kWavesPerBlock];
             static_assert(kMaxBlocks == kBlock, "a lane reads one workgroup's value");
-            uint32_t top = 0;
-            if (a.largest) {
-                top = a.largest[which * kMaxBlocks + threadIdx.x];
-            } else {
-                for (int i = threadIdx.x; i < (int)job.rows * a.cols; i += kBlock) {
-                    const int r = i / a.cols;
-                    const uint32_t b = __float_as_uint((float)src[r * job.stride + i - r * a.cols]) & 0x7fffffffu;
-                    if (b < 0x7f800000u && counts(r)) top = max(top, b);
-                }
-            }
-#pragma unroll
-            for (int m = 32; m >= 1; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, kWave));
-            if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
-            __syncthreads();
-            for (int k = 0; k < kWavesPerBlock; ++k) top = max(top, sh[k]);
-            ex = exponent(top);
+            ex = exponent(block_max(a.largest ? a.largest[which * kMaxBlocks + threadIdx.x]
+                                              : largest_of(reinterpret_cast<const float*>(src), job.stride, job.rows, a.cols,
+                                                           which ? nullptr : a.target, a.ignore, 0, 1), sh));
         }
         if (blockIdx.x == 0 && blockIdx.y < 2 && threadIdx.x == 0) {
             a.scales->ex[which] = ex;
@@ -850,7 +852,7 @@ static void ce_operands(CeArgs& a, const CePlan& p, const void* x, int64_t x_str
         // the join, 64 tokens of 51 classes and 64 features take 11.6 us instead of 17.1
         if (!known && std::max<int64_t>(R, V) * H > 8192) {
             uint32_t* largest = reinterpret_cast<uint32_t*>(ws + p.largest_off);
-            CNF_LAUNCH(ce_largest_kernel, dim3(kMaxBlocks, 2), dim3(kBlock), 0, st, static_cast<const float*>(x), x_stride, R, target, ignore,
+            CNF_LAUNCH(ce_largest_kernel, dim3(kMaxBlocks, 2), dim3(1024), 0, st, static_cast<const float*>(x), x_stride, R, target, ignore,
                        static_cast<const float*>(w), w_stride, V, H, largest);
             l.largest = largest;
         }

@@ -10,7 +10,7 @@
 //
 // Bound by the matrix cores and the vector work beside them (exponentials, splitting): 5 products of 2 R V H operations against the
 // 3 of the definition — the logits are computed three times — but nothing of size R x V is written or read.  36864 x 10000 x 64 fp32:
-// forward 186 us (760 TF of fp16 products), dx 298 us (950 TF), dw 360 us (790 TF); matrix cores busy 40 - 50 % of the cycles, vector
+// forward 184 us (770 TF of fp16 products), dx 288 us (980 TF), dw 370 us (765 TF); matrix cores busy 40 - 50 % of the cycles, vector
 // units 50 - 60 %, and a step's products wait for its exponentials.  128 rows a workgroup: the tile of the other side is read from LDS
 // once for 32 rows of a wave; 64 rows a wave would leave registers for one wave per SIMD.
 #include <algorithm>
@@ -47,6 +47,23 @@ struct NarrowTile {
             const void* src = (e < o.ext && c * 8 < hidden) ? static_cast<const void*>(base + (int64_t)part * o.part + e * o.ld + c * 8)
                                                             : static_cast<const void*>(kZeroChunk);
             __builtin_amdgcn_global_load_lds((glb_cvoid_t*)src, (lds_void16_t*)(lds + (j * kBlock + wave * 64) * 16), 16, 0, 0);
+        }
+    }
+    // A tile whose rows and chunks all exist: a copy's rows lie kRows apart, which the swizzle does not see, so a lane has one offset for
+    // all of them and the rest is scalar (dw at 36864 x 10000 x 64 fp32: 379 -> 369 us)
+    static constexpr int kRows = kBlock / kChunks;
+    __device__ static uint32_t lane_offset(const Operand& o) {
+        const int row = threadIdx.x / kChunks, c = (threadIdx.x % kChunks) ^ narrow_swizzle<HP>(row);
+        return (uint32_t)(row * (int)o.ld + c * 8) * 2u;
+    }
+    __device__ static void copy_whole(const Operand& o, int64_t m0, uint32_t offset, char* lds) {
+        static_assert(kRows % 16 == 0 && kNarrowWalk % kRows == 0, "whole swizzles and parts");
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+        for (int j = 0; j < kCopies; ++j) {
+            const int part = j * kRows / kNarrowWalk, row = j * kRows % kNarrowWalk;
+            const char* base = static_cast<const char*>(o.base) + 2 * (part * o.part + (m0 + row) * o.ld);
+            __builtin_amdgcn_global_load_lds((glb_cvoid_t*)(base + offset), (lds_void16_t*)(lds + (j * kBlock + wave * 64) * 16), 16, 0, 0);
         }
     }
     // rows row0 ... row0 + 15, k = 32 kk ...
@@ -125,14 +142,18 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
     const int64_t tiles = (walk_n + kNarrowWalk - 1) / kNarrowWalk;
     const int64_t first = tiles * split / a.splits, last = tiles * (split + 1) / a.splits;
 
+    const uint32_t offset = Tile::lane_offset(a.walk);
     auto copy = [&](int64_t tile, int stage) {
         char* s = lds + stage * kStage;
-        Tile::copy(a.walk, tile * kNarrowWalk, a.hidden, s);
+        if (a.hidden > HP - 8 && (tile + 1) * kNarrowWalk <= a.walk.ext) Tile::copy_whole(a.walk, tile * kNarrowWalk, offset, s);
+        else Tile::copy(a.walk, tile * kNarrowWalk, a.hidden, s);
         // every wave copies the step's records (the same bytes to the same place): all waves have the same number of copies in flight
         if (JOB == kNarrowDw)
-            __builtin_amdgcn_global_load_lds((glb_cvoid_t*)(a.state + tile * kNarrowWalk + lane), (lds_void16_t*)(s + Tile::kBytes), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((glb_cvoid_t*)(reinterpret_cast<const char*>(a.state + tile * kNarrowWalk) + lane * 16u),
+                                             (lds_void16_t*)(s + Tile::kBytes), 16, 0, 0);
         else
-            __builtin_amdgcn_global_load_lds((glb_cvoid_t*)(a.bias + tile * kNarrowWalk + lane), (lds_void16_t*)(s + Tile::kBytes), 4, 0, 0);
+            __builtin_amdgcn_global_load_lds((glb_cvoid_t*)(reinterpret_cast<const char*>(a.bias + tile * kNarrowWalk) + lane * 4u),
+                                             (lds_void16_t*)(s + Tile::kBytes), 4, 0, 0);
     };
     if (first < last) copy(first, 0);
 
@@ -270,28 +291,29 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
             s16x8 early[HB];
             if constexpr (JOB == kNarrowDx) Tile::template frag_t<PARTS - 1, HB>(t_base, tile_at, early);
             s16x8 d[PARTS][NT];
-            // dw: the records of the lane's rows; their g is read only where a target is met
+            // dw: the records of the lane's rows; target and g are read again where a target is met
             const RowState* row = reinterpret_cast<const RowState*>(s + Tile::kBytes) + mp * 32 + g * 4;
-            float row_m2[8], row_scale[8];          // dw: the row's g and the lift in its scale
-            int row_target[8];
-            bool shifted = false;                   // rows that were scaled by more than the others: rare
+            float row_m2[8], row_scale[8];          // the row's g and the lift in its scale
+            bool shifted = false, met = false;      // rows scaled by more than the others; targets among the wave's entries: both rare
             if (JOB == kNarrowDw) {
                 int words = 0;
+                const int e0 = (int)(n_wave + col);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const RowState& q = row[(e / 4) * 16 + e % 4];
                     row_m2[e] = q.m2;
                     row_scale[e] = q.inv_s * q.g * a.lift;
-                    row_target[e] = target_of(q.target);
                     words |= q.target;
+                    met |= ((q.target - e0) & ~16) == 0;            // entry 0 or 1 of the lane's (NT = 2)
                 }
                 shifted = PARTS > 1 && __ballot(shift_of(words) != 0) != 0;
+                met = shifted || __ballot(met) != 0;
                 if (shifted) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const int s = shift_of(row[(e / 4) * 16 + e % 4].target);
+                        const int by = shift_of(row[(e / 4) * 16 + e % 4].target);
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) sc[e / 4][n][e % 4] = ldexpf(sc[e / 4][n][e % 4], -s);
+                        for (int n = 0; n < NT; ++n) sc[e / 4][n][e % 4] = ldexpf(sc[e / 4][n][e % 4], -by);
                     }
                 }
             }
@@ -306,7 +328,7 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
                     // the logit rounded as in the forward, then the difference: the row's maximum gives 1
                     v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e / 4][n][e % 4], back[n], b) - m) * f;
                     // an ignored row of x read as it is: its logits may have overflowed (fp32 ones are laid out as zeros)
-                    if (JOB == kNarrowDw && PARTS == 1) v[e] = row_target[e] == kNarrowVocab ? 0.f : v[e];
+                    if (JOB == kNarrowDw && PARTS == 1) v[e] = f == 0.f ? 0.f : v[e];
                 }
                 if (JOB == kNarrowDx) {
                     const int64_t at = st[n].target - m0;
@@ -316,14 +338,12 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
                             if (at == (e / 4) * 16 + e % 4) v[e] -= a.lift;
                     }
                 } else {
-                    const int e0 = (int)(n_wave + n * 16 + col);
-                    bool hit = false;
+                    if (met) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) hit |= row_target[e] == e0;
-                    if (__ballot(hit)) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (row_target[e] == e0) v[e] -= row[(e / 4) * 16 + e % 4].g * a.lift;
+                        for (int e = 0; e < 8; ++e) {
+                            const RowState& q = row[(e / 4) * 16 + e % 4];
+                            if (target_of(q.target) == (int)(n_wave + n * 16 + col)) v[e] -= q.g * a.lift;
+                        }
                     }
 #pragma unroll
                     for (int e = 0; e < 8; ++e) sum[n] += v[e];

@@ -289,6 +289,11 @@ def test_vocabularies_around_2_to_the_24(vocab):
     run_and_check(x, w, b, t, g)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_million_features(dtype):
+    run_and_check(*make(3, 5, 2 ** 20 + 8, dtype, ignored=0.0))
+
+
 def test_more_elements_than_2_to_the_31():
     """Rows whose elements lie beyond 2^31 give what they give at the front."""
     H, V, n = 64, 51, 3000
