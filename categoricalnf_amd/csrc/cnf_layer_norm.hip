@@ -62,30 +62,64 @@ struct BlockGroup {
     __device__ __forceinline__ float sum(float v) const { return sum(Sum2(v, 0.f)).a; }
 };
 
-template <typename T, int VEC, int NV>
+// 16 bytes of a row, at any address its elements may have (the hardware takes them in one access); TAIL: the row's last vector may be
+// shorter, and goes element by element
+template <bool TAIL, typename T, int VEC>
+__device__ __forceinline__ void ln_read(const T* row, int c, int cols, vec_t<T, VEC>& v) {
+    if (!TAIL || c + VEC <= cols) {
+        __builtin_memcpy(&v, row + c, sizeof(v));
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if (c + i < cols) v[i] = row[c + i];
+    }
+}
+template <bool TAIL, typename T, int VEC>
+__device__ __forceinline__ void ln_write(T* row, int c, int cols, const vec_t<T, VEC>& v) {
+    if (!TAIL || c + VEC <= cols) {
+        __builtin_memcpy(row + c, &v, sizeof(v));
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if (c + i < cols) row[c + i] = v[i];
+    }
+}
+
+template <bool TAIL, typename T, int VEC, int NV>
 __device__ __forceinline__ void ln_load(const T* row, int l, int lanes, int cols, bool on, vec_t<T, VEC>* v) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int c = (j * lanes + l) * VEC;
-        vec_t<T, VEC> z;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) z[i] = (T)0.f;
-        v[j] = (on && c < cols) ? *reinterpret_cast<const vec_t<T, VEC>*>(row + c) : z;
+        for (int i = 0; i < VEC; ++i) v[j][i] = (T)0.f;
+        if (on && c < cols) ln_read<TAIL, T, VEC>(row, c, cols, v[j]);
     }
 }
 
 template <int VEC, int NV>
 __device__ __forceinline__ void ln_load_weight(const void* w, int wdtype, int l, int lanes, int cols, float fill, float* out) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+    for (int e = 0; e < NV * VEC; ++e) out[e] = fill;
+    if (!w) return;
+    auto load = [&](auto t) {
+        typedef decltype(t) W;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const int c = (j * lanes + l) * VEC + i;
-            out[j * VEC + i] = (w && c < cols) ? load_any(w, wdtype, c) : fill;
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * lanes + l) * VEC;
+            vec_t<W, VEC> v;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[i] = (W)fill;
+            if (c < cols) ln_read<true, W, VEC>(static_cast<const W*>(w), c, cols, v);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) out[j * VEC + i] = (float)v[i];
         }
+    };
+    if (wdtype == CNF_DTYPE_F32) load(float{});
+    else if (wdtype == CNF_DTYPE_BF16) load(bf16_t{});
+    else load(f16_t{});
 }
 
-template <typename T, int VEC, int NV, typename Group>
+template <bool TAIL, typename T, int VEC, int NV, typename Group>
 __device__ __forceinline__ void ln_fwd_row(const LnArgs& a, const vec_t<T, VEC>* xv, int64_t row, bool on, int l, int lanes,
                                            const Group& grp, const float* w, const float* b) {
     float x[NV * VEC], s = 0.f;
@@ -99,11 +133,11 @@ __device__ __forceinline__ void ln_fwd_row(const LnArgs& a, const vec_t<T, VEC>*
     float q = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const bool in = (j * lanes + l) * VEC < a.cols;
+        const int c = (j * lanes + l) * VEC;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             float& v = x[j * VEC + i];
-            v = in ? v - mean : 0.f;
+            v = (TAIL ? c + i : c) < a.cols ? v - mean : 0.f;
             q += v * v;
         }
     }
@@ -117,7 +151,7 @@ __device__ __forceinline__ void ln_fwd_row(const LnArgs& a, const vec_t<T, VEC>*
         vec_t<T, VEC> o;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) o[i] = (T)(x[j * VEC + i] * rstd * w[j * VEC + i] + b[j * VEC + i]);
-        *reinterpret_cast<vec_t<T, VEC>*>(y + c) = o;
+        ln_write<TAIL, T, VEC>(y, c, a.cols, o);
     }
     if (l == 0 && a.mean) {
         a.mean[row] = mean;
@@ -125,7 +159,7 @@ __device__ __forceinline__ void ln_fwd_row(const LnArgs& a, const vec_t<T, VEC>*
     }
 }
 
-template <typename T, int VEC, int NV>
+template <bool TAIL, typename T, int VEC, int NV>
 __global__ __launch_bounds__(kBlock) void ln_fwd_wave_kernel(const LnArgs a) {
     const int g = a.group, rpw = kWave / g;
     const int lane = threadIdx.x & 63, l = lane & (g - 1);
@@ -138,17 +172,17 @@ __global__ __launch_bounds__(kBlock) void ln_fwd_wave_kernel(const LnArgs a) {
     const int64_t step = (int64_t)gridDim.x * rpb;
     vec_t<T, VEC> now[NV], next[NV];
     int64_t r = (int64_t)blockIdx.x * rpb + slot;
-    ln_load<T, VEC, NV>(static_cast<const T*>(a.x) + r * a.x_stride, l, g, a.cols, r < a.rows, next);
+    ln_load<TAIL, T, VEC, NV>(static_cast<const T*>(a.x) + r * a.x_stride, l, g, a.cols, r < a.rows, next);
     for (int64_t r0 = (int64_t)blockIdx.x * rpb; r0 < a.rows; r0 += step, r += step) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) now[j] = next[j];
         if (r0 + step < a.rows)
-            ln_load<T, VEC, NV>(static_cast<const T*>(a.x) + (r + step) * a.x_stride, l, g, a.cols, r + step < a.rows, next);
-        ln_fwd_row<T, VEC, NV>(a, now, r, r < a.rows, l, g, grp, w, b);
+            ln_load<TAIL, T, VEC, NV>(static_cast<const T*>(a.x) + (r + step) * a.x_stride, l, g, a.cols, r + step < a.rows, next);
+        ln_fwd_row<TAIL, T, VEC, NV>(a, now, r, r < a.rows, l, g, grp, w, b);
     }
 }
 
-template <typename T, int VEC, int NV>
+template <bool TAIL, typename T, int VEC, int NV>
 __global__ __launch_bounds__(1024) void ln_fwd_block_kernel(const LnArgs a) {
     __shared__ float sh[32];
     const BlockGroup grp{sh};
@@ -157,8 +191,8 @@ __global__ __launch_bounds__(1024) void ln_fwd_block_kernel(const LnArgs a) {
     ln_load_weight<VEC, NV>(a.bias, a.wdtype, threadIdx.x, blockDim.x, a.cols, 0.f, b);
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         vec_t<T, VEC> xv[NV];
-        ln_load<T, VEC, NV>(static_cast<const T*>(a.x) + r * a.x_stride, threadIdx.x, blockDim.x, a.cols, true, xv);
-        ln_fwd_row<T, VEC, NV>(a, xv, r, true, threadIdx.x, blockDim.x, grp, w, b);
+        ln_load<TAIL, T, VEC, NV>(static_cast<const T*>(a.x) + r * a.x_stride, threadIdx.x, blockDim.x, a.cols, true, xv);
+        ln_fwd_row<TAIL, T, VEC, NV>(a, xv, r, true, threadIdx.x, blockDim.x, grp, w, b);
     }
 }
 
@@ -180,31 +214,31 @@ __device__ __forceinline__ vec_t<T, VEC> opaque(vec_t<T, VEC> v) {
 }
 
 // what the backward reads of one row
-template <typename T, int VEC, int NV>
+template <bool TAIL, typename T, int VEC, int NV>
 struct LnRow {
     vec_t<T, VEC> x[NV], g[NV];
     float mean, rstd;
     __device__ __forceinline__ void load(const LnArgs& a, int64_t row, bool on, int l, int lanes) {
-        ln_load<T, VEC, NV>(static_cast<const T*>(a.x) + row * a.x_stride, l, lanes, a.cols, on, x);
-        ln_load<T, VEC, NV>(static_cast<const T*>(a.dy) + row * a.dy_stride, l, lanes, a.cols, on, g);
+        ln_load<TAIL, T, VEC, NV>(static_cast<const T*>(a.x) + row * a.x_stride, l, lanes, a.cols, on, x);
+        ln_load<TAIL, T, VEC, NV>(static_cast<const T*>(a.dy) + row * a.dy_stride, l, lanes, a.cols, on, g);
         mean = on ? a.mean[row] : 0.f;
         rstd = on ? a.rstd[row] : 0.f;
     }
 };
 
-template <typename T, int VEC, int NV, typename Group>
-__device__ __forceinline__ void ln_bwd_row(const LnArgs& a, LnRow<T, VEC, NV>& in_row, int64_t row, bool on, int l, int lanes,
+template <bool TAIL, typename T, int VEC, int NV, typename Group>
+__device__ __forceinline__ void ln_bwd_row(const LnArgs& a, LnRow<TAIL, T, VEC, NV>& in_row, int64_t row, bool on, int l, int lanes,
                                            const Group& grp, const float* w, float* dw, float* db) {
     vec_t<T, VEC>*xv = in_row.x, *gv = in_row.g;
     const float mean = in_row.mean, rstd = in_row.rstd;
     Sum2 s(0);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const bool in = (j * lanes + l) * VEC < a.cols;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             const int e = j * VEC + i;
-            const float g = (float)gv[j][i], xh = in ? ((float)xv[j][i] - mean) * rstd : 0.f, gw = g * w[e];
+            // past the last column g is 0
+            const float g = (float)gv[j][i], xh = ((float)xv[j][i] - mean) * rstd, gw = g * w[e];
             dw[e] += g * xh;
             db[e] += g;
             s += Sum2(gw, gw * xh);
@@ -230,12 +264,12 @@ __device__ __forceinline__ void ln_bwd_row(const LnArgs& a, LnRow<T, VEC, NV>& i
             const float xh = ((float)xv[j][i] - mean) * rstd, gw = (float)gv[j][i] * w[j * VEC + i];
             o[i] = (T)(rstd * (gw - c1 - xh * c2));
         }
-        *reinterpret_cast<vec_t<T, VEC>*>(dx + c) = o;
+        ln_write<TAIL, T, VEC>(dx, c, a.cols, o);
     }
 }
 
 // partials: [gridDim.x][2][cols]
-template <typename T, int VEC, int NV>
+template <bool TAIL, typename T, int VEC, int NV>
 __global__ __launch_bounds__(kBlock) void ln_bwd_wave_kernel(const LnArgs a) {
     __shared__ float sh[kWavesPerBlock][kLnWaveCols];
     const int g = a.group, rpw = kWave / g;
@@ -247,9 +281,9 @@ __global__ __launch_bounds__(kBlock) void ln_bwd_wave_kernel(const LnArgs a) {
     for (int e = 0; e < NV * VEC; ++e) acc[0][e] = acc[1][e] = 0.f;
     const WaveGroup grp{g};
     for (int64_t r0 = (int64_t)blockIdx.x * rpb; r0 < a.rows; r0 += (int64_t)gridDim.x * rpb) {
-        LnRow<T, VEC, NV> in_row;
+        LnRow<TAIL, T, VEC, NV> in_row;
         in_row.load(a, r0 + slot, r0 + slot < a.rows, l, g);
-        ln_bwd_row<T, VEC, NV>(a, in_row, r0 + slot, r0 + slot < a.rows, l, g, grp, w, acc[0], acc[1]);
+        ln_bwd_row<TAIL, T, VEC, NV>(a, in_row, r0 + slot, r0 + slot < a.rows, l, g, grp, w, acc[0], acc[1]);
     }
     if (!a.partials) return;
 #pragma unroll
@@ -273,7 +307,7 @@ __global__ __launch_bounds__(kBlock) void ln_bwd_wave_kernel(const LnArgs a) {
     }
 }
 
-template <typename T, int VEC, int NV>
+template <bool TAIL, typename T, int VEC, int NV>
 __global__ __launch_bounds__(1024) void ln_bwd_block_kernel(const LnArgs a) {
     __shared__ float sh[32];
     const BlockGroup grp{sh};
@@ -282,9 +316,9 @@ __global__ __launch_bounds__(1024) void ln_bwd_block_kernel(const LnArgs a) {
 #pragma unroll
     for (int e = 0; e < NV * VEC; ++e) acc[0][e] = acc[1][e] = 0.f;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        LnRow<T, VEC, NV> in_row;
+        LnRow<TAIL, T, VEC, NV> in_row;
         in_row.load(a, r, true, threadIdx.x, blockDim.x);
-        ln_bwd_row<T, VEC, NV>(a, in_row, r, true, threadIdx.x, blockDim.x, grp, w, acc[0], acc[1]);
+        ln_bwd_row<TAIL, T, VEC, NV>(a, in_row, r, true, threadIdx.x, blockDim.x, grp, w, acc[0], acc[1]);
     }
     if (!a.partials) return;
 #pragma unroll
@@ -389,16 +423,15 @@ __global__ __launch_bounds__(1024) void ln_reduce_kernel(const float* __restrict
 
 // How a launch deals rows to lanes.  16-byte vectors where every row allows it; otherwise single elements.
 struct LnShape {
-    int vec;        // 1: 16-byte vectors
-    int nv;         // vectors (elements) per lane: 1 or the most that keeps 16 elements
+    bool tail;      // the last 16-byte vector of a row is shorter
+    int nv;         // vectors per lane: 1, or the most that keeps 16 elements
     int group;      // lanes per row; > 64: the workgroup's size
     int kind;       // 0 wave, 1 workgroup, 2 long rows
 };
-static LnShape ln_shape(int cols, int dtype, bool aligned) {
+static LnShape ln_shape(int cols, int dtype) {
     LnShape s;
-    const int per = 16 / dtype_bytes(dtype);
-    s.vec = aligned && cols % per == 0;
-    const int width = s.vec ? per : 1, units = (cols + width - 1) / width, most = kLnElems / width;
+    const int width = 16 / dtype_bytes(dtype), units = (cols + width - 1) / width, most = kLnElems / width;
+    s.tail = cols % width != 0;
     s.nv = units <= 16 ? 1 : most;      // short rows: one load per lane keeps the lanes of a wave busy
     int g = 1;
     while ((int64_t)g * s.nv < units) g <<= 1;
@@ -415,19 +448,19 @@ static int ln_partials(int64_t rows, const LnShape& s) {
     return (int)std::min<int64_t>(steps, std::max<int64_t>(256, std::min<int64_t>(kLnMaxPartials, steps / 8)));
 }
 
+// calls wave or block with (tail, vector width, vectors per lane) as constants
 template <typename T, typename Wave, typename Block>
 static void ln_pick(const LnShape& s, Wave&& wave, Block&& block) {
     constexpr int V = 16 / (int)sizeof(T);
-    if (s.kind == 0) {
-        if (s.vec && s.nv == 1) wave(std::integral_constant<int, V>{}, std::integral_constant<int, 1>{});
-        else if (s.vec) wave(std::integral_constant<int, V>{}, std::integral_constant<int, kLnElems / V>{});
-        else if (s.nv == 1) wave(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
-        else wave(std::integral_constant<int, 1>{}, std::integral_constant<int, kLnElems>{});
-    } else if (s.vec) {
-        block(std::integral_constant<int, V>{}, std::integral_constant<int, kLnElems / V>{});
-    } else {
-        block(std::integral_constant<int, 1>{}, std::integral_constant<int, kLnElems>{});
-    }
+    auto pick = [&](auto tail) {
+        std::integral_constant<int, V> width;
+        std::integral_constant<int, kLnElems / V> most;
+        if (s.kind == 1) block(tail, width, most);
+        else if (s.nv == 1) wave(tail, width, std::integral_constant<int, 1>{});
+        else wave(tail, width, most);
+    };
+    if (s.tail) pick(std::true_type{});
+    else pick(std::false_type{});
 }
 
 }  // namespace cnf
@@ -446,7 +479,7 @@ int cnf_layer_norm(const void* x, int64_t x_stride, const void* weight, const vo
     LnArgs a{};
     a.x = x; a.weight = weight; a.bias = bias; a.y = y; a.mean = mean; a.rstd = rstd;
     a.x_stride = x_stride; a.y_stride = cols; a.rows = rows; a.cols = cols; a.wdtype = wdtype; a.eps = eps;
-    const LnShape s = ln_shape(cols, dtype, rows_aligned16(x, x_stride, dtype) && rows_aligned16(y, cols, dtype));
+    const LnShape s = ln_shape(cols, dtype);
     a.group = s.group;
     hipStream_t st = (hipStream_t)stream;
     return with_dtype(dtype, [&](auto t) {
@@ -455,13 +488,13 @@ int cnf_layer_norm(const void* x, int64_t x_stride, const void* weight, const vo
             CNF_LAUNCH((ln_fwd_long_kernel<T>), dim3((unsigned)std::min<int64_t>(rows, 2048)), dim3(1024), 0, st, a);
         } else {
             ln_pick<T>(s,
-                       [&](auto v, auto n) {
+                       [&](auto tail, auto v, auto n) {
                            const int rpb = kWavesPerBlock * (kWave / s.group);
                            const unsigned grid = (unsigned)std::min<int64_t>((rows + rpb - 1) / rpb, 4096);
-                           CNF_LAUNCH((ln_fwd_wave_kernel<T, decltype(v)::value, decltype(n)::value>), dim3(grid), dim3(kBlock), 0, st, a);
+                           CNF_LAUNCH((ln_fwd_wave_kernel<decltype(tail)::value, T, decltype(v)::value, decltype(n)::value>), dim3(grid), dim3(kBlock), 0, st, a);
                        },
-                       [&](auto v, auto n) {
-                           CNF_LAUNCH((ln_fwd_block_kernel<T, decltype(v)::value, decltype(n)::value>),
+                       [&](auto tail, auto v, auto n) {
+                           CNF_LAUNCH((ln_fwd_block_kernel<decltype(tail)::value, T, decltype(v)::value, decltype(n)::value>),
                                       dim3((unsigned)std::min<int64_t>(rows, 4096)), dim3(s.group), 0, st, a);
                        });
         }
@@ -471,11 +504,9 @@ int cnf_layer_norm(const void* x, int64_t x_stride, const void* weight, const vo
 
 int64_t cnf_layer_norm_bwd_workspace_floats(int64_t rows, int cols) {
     if (rows <= 0 || cols <= 0 || cols > kLnMaxCols) return 0;
-    // the largest partials matrix over the layouts a launch of this size may take
+    // the largest partials matrix over the types
     int64_t most = 0;
-    for (int dtype : {CNF_DTYPE_F32, CNF_DTYPE_BF16})
-        for (int aligned = 0; aligned < 2; ++aligned)
-            most = std::max<int64_t>(most, ln_partials(rows, ln_shape(cols, dtype, aligned != 0)));
+    for (int dtype : {CNF_DTYPE_F32, CNF_DTYPE_BF16}) most = std::max<int64_t>(most, ln_partials(rows, ln_shape(cols, dtype)));
     return most * 2 * cols;
 }
 
@@ -492,8 +523,7 @@ int cnf_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64_t 
     a.x = x; a.dy = dy; a.weight = weight; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd); a.dx = dx;
     a.x_stride = x_stride; a.dy_stride = dy_stride; a.y_stride = cols; a.rows = rows; a.cols = cols; a.wdtype = wdtype;
     a.partials = sums ? ws : nullptr;
-    const LnShape s = ln_shape(cols, dtype, rows_aligned16(x, x_stride, dtype) && rows_aligned16(dy, dy_stride, dtype) &&
-                                                rows_aligned16(dx, cols, dtype));
+    const LnShape s = ln_shape(cols, dtype);
     a.group = s.group;
     const int parts = rows > 0 ? ln_partials(rows, s) : 0;
     hipStream_t st = (hipStream_t)stream;
@@ -506,11 +536,11 @@ int cnf_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64_t 
                     CNF_LAUNCH((ln_columns_kernel<T>), dim3((cols + kBlock - 1) / kBlock, parts), dim3(kBlock), 0, st, a);
             } else {
                 ln_pick<T>(s,
-                           [&](auto v, auto n) {
-                               CNF_LAUNCH((ln_bwd_wave_kernel<T, decltype(v)::value, decltype(n)::value>), dim3(parts), dim3(kBlock), 0, st, a);
+                           [&](auto tail, auto v, auto n) {
+                               CNF_LAUNCH((ln_bwd_wave_kernel<decltype(tail)::value, T, decltype(v)::value, decltype(n)::value>), dim3(parts), dim3(kBlock), 0, st, a);
                            },
-                           [&](auto v, auto n) {
-                               CNF_LAUNCH((ln_bwd_block_kernel<T, decltype(v)::value, decltype(n)::value>), dim3(parts), dim3(s.group), 0, st, a);
+                           [&](auto tail, auto v, auto n) {
+                               CNF_LAUNCH((ln_bwd_block_kernel<decltype(tail)::value, T, decltype(v)::value, decltype(n)::value>), dim3(parts), dim3(s.group), 0, st, a);
                            });
             }
             return launch_status("cnf_layer_norm_bwd");
