@@ -11,9 +11,10 @@
 // launch adds the partial rows in their order (the same bits on every run, no atomics).  Longer rows take kernels that read a row
 // three times (forward) or twice (backward) and sum the columns in a launch of their own.
 //
-// Waves in flight are what keeps HBM busy: the forward holds its next row's loads while it works on one (129 -> 122 us at 131072 x
-// 1024 bf16, 4.4 TB/s); the backward has registers for that only at the price of a wave per SIMD, and computes xhat and g w twice
-// instead of holding them (202 -> 166 us, 4.85 TB/s; a plain copy: 4.97).
+// Waves in flight are what keeps HBM busy: the forward holds its next row's loads while it works on one; the backward has registers for
+// that only at the price of a wave per SIMD, and computes xhat and g w twice instead of holding them (202 -> 166 us).  131072 x 1024 bf16:
+// forward 102 us (5.2 TB/s), backward 162 us and 8 for the column sums (4.9 TB/s; a plain copy: 4.97).  Rows that begin at odd addresses
+// are read in 16-byte vectors all the same: 4933 x 7438 bf16 forward 44 us, backward 70 us (7440 columns: 27 and 54; floors 30 and 44).
 #include <algorithm>
 #include <type_traits>
 
@@ -307,8 +308,9 @@ __global__ __launch_bounds__(kBlock) void ln_bwd_wave_kernel(const LnArgs a) {
     }
 }
 
-template <bool TAIL, typename T, int VEC, int NV>
-__global__ __launch_bounds__(1024) void ln_bwd_block_kernel(const LnArgs a) {
+// THREADS at most: 1024, or 512 for fp32, whose rows want 134 registers where 1024 threads have 128 (25079 x 3034: 282 -> 250 us)
+template <int THREADS, bool TAIL, typename T, int VEC, int NV>
+__global__ __launch_bounds__(THREADS) void ln_bwd_block_kernel(const LnArgs a) {
     __shared__ float sh[32];
     const BlockGroup grp{sh};
     float w[NV * VEC], acc[2][NV * VEC];
@@ -324,9 +326,12 @@ __global__ __launch_bounds__(1024) void ln_bwd_block_kernel(const LnArgs a) {
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int e = 0; e < NV * VEC; ++e) {
-            const int c = ((e / VEC) * blockDim.x + threadIdx.x) * VEC + e % VEC;
-            if (c < a.cols) a.partials[((size_t)blockIdx.x * 2 + k) * a.cols + c] = acc[k][e];
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * blockDim.x + threadIdx.x) * VEC;
+            vec_t<float, VEC> v;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[i] = acc[k][j * VEC + i];
+            if (c < a.cols) ln_write<TAIL, float, VEC>(a.partials + ((size_t)blockIdx.x * 2 + k) * a.cols, c, a.cols, v);
         }
 }
 
@@ -428,11 +433,14 @@ struct LnShape {
     int group;      // lanes per row; > 64: the workgroup's size
     int kind;       // 0 wave, 1 workgroup, 2 long rows
 };
-static LnShape ln_shape(int cols, int dtype) {
+static LnShape ln_shape(int cols, int dtype, bool backward) {
     LnShape s;
     const int width = 16 / dtype_bytes(dtype), units = (cols + width - 1) / width, most = kLnElems / width;
     s.tail = cols % width != 0;
-    s.nv = units <= 16 ? 1 : most;      // short rows: one load per lane keeps the lanes of a wave busy
+    // Short rows: one vector per lane keeps the lanes of a wave busy; the forward, with less to do per vector, sooner takes more of them
+    // (44992 x 128 fp32, 32 vectors a row, one / four a lane: forward 11.2 / 9.6 us, backward 21.3 / 26.1; x 512 bf16, 64 vectors, one /
+    // two: 20.8 / 18.7 and 37.1 / 35.5)
+    s.nv = units <= (backward ? 32 : 16) ? 1 : most;
     int g = 1;
     while ((int64_t)g * s.nv < units) g <<= 1;
     s.kind = cols > kLnBlockCols ? 2 : (g > kWave ? 1 : 0);
@@ -444,8 +452,10 @@ static int ln_partials(int64_t rows, const LnShape& s) {
     if (s.kind == 2) return (int)std::min<int64_t>(rows, 64);
     const int rpb = s.kind == 1 ? 1 : kWavesPerBlock * (kWave / s.group);
     const int64_t steps = (rows + rpb - 1) / rpb;
-    // at least 8 steps of rows per workgroup before there are more than 256 of them: each workgroup writes 2 C sums at its end
-    return (int)std::min<int64_t>(steps, std::max<int64_t>(256, std::min<int64_t>(kLnMaxPartials, steps / 8)));
+    // at least 8 steps of rows per workgroup before there are more than 256 of them: each workgroup writes 2 C sums at its end; of large
+    // workgroups no more than run at once
+    const int64_t most = s.kind == 1 ? std::min(kLnMaxPartials, 256 * 1024 / s.group) : kLnMaxPartials;
+    return (int)std::min<int64_t>(steps, std::max<int64_t>(256, std::min<int64_t>(most, steps / 8)));
 }
 
 // calls wave or block with (tail, vector width, vectors per lane) as constants
@@ -479,7 +489,7 @@ int cnf_layer_norm(const void* x, int64_t x_stride, const void* weight, const vo
     LnArgs a{};
     a.x = x; a.weight = weight; a.bias = bias; a.y = y; a.mean = mean; a.rstd = rstd;
     a.x_stride = x_stride; a.y_stride = cols; a.rows = rows; a.cols = cols; a.wdtype = wdtype; a.eps = eps;
-    const LnShape s = ln_shape(cols, dtype);
+    const LnShape s = ln_shape(cols, dtype, false);
     a.group = s.group;
     hipStream_t st = (hipStream_t)stream;
     return with_dtype(dtype, [&](auto t) {
@@ -506,7 +516,7 @@ int64_t cnf_layer_norm_bwd_workspace_floats(int64_t rows, int cols) {
     if (rows <= 0 || cols <= 0 || cols > kLnMaxCols) return 0;
     // the largest partials matrix over the types
     int64_t most = 0;
-    for (int dtype : {CNF_DTYPE_F32, CNF_DTYPE_BF16}) most = std::max<int64_t>(most, ln_partials(rows, ln_shape(cols, dtype)));
+    for (int dtype : {CNF_DTYPE_F32, CNF_DTYPE_BF16}) most = std::max<int64_t>(most, ln_partials(rows, ln_shape(cols, dtype, true)));
     return most * 2 * cols;
 }
 
@@ -523,7 +533,7 @@ int cnf_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64_t 
     a.x = x; a.dy = dy; a.weight = weight; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd); a.dx = dx;
     a.x_stride = x_stride; a.dy_stride = dy_stride; a.y_stride = cols; a.rows = rows; a.cols = cols; a.wdtype = wdtype;
     a.partials = sums ? ws : nullptr;
-    const LnShape s = ln_shape(cols, dtype);
+    const LnShape s = ln_shape(cols, dtype, true);
     a.group = s.group;
     const int parts = rows > 0 ? ln_partials(rows, s) : 0;
     hipStream_t st = (hipStream_t)stream;
@@ -540,7 +550,12 @@ int cnf_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64_t 
                                CNF_LAUNCH((ln_bwd_wave_kernel<decltype(tail)::value, T, decltype(v)::value, decltype(n)::value>), dim3(parts), dim3(kBlock), 0, st, a);
                            },
                            [&](auto tail, auto v, auto n) {
-                               CNF_LAUNCH((ln_bwd_block_kernel<decltype(tail)::value, T, decltype(v)::value, decltype(n)::value>), dim3(parts), dim3(s.group), 0, st, a);
+                               auto launch = [&](auto threads) {
+                                   CNF_LAUNCH((ln_bwd_block_kernel<decltype(threads)::value, decltype(tail)::value, T, decltype(v)::value, decltype(n)::value>),
+                                              dim3(parts), dim3(s.group), 0, st, a);
+                               };
+                               if (sizeof(T) == 4 && s.group <= 512) launch(std::integral_constant<int, sizeof(T) == 4 ? 512 : 1024>{});
+                               else launch(std::integral_constant<int, 1024>{});
                            });
             }
             return launch_status("cnf_layer_norm_bwd");
