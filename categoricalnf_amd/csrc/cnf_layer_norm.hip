@@ -337,8 +337,19 @@ __global__ __launch_bounds__(THREADS) void ln_bwd_block_kernel(const LnArgs a) {
 
 // ---- rows wider than a workgroup's registers: the row is read again instead of held ---------------------------------------------
 
+// calls fn(first column, its 16 bytes) for this lane's part of a row
+template <typename T, typename Fn>
+__device__ __forceinline__ void ln_walk(const T* row, int cols, Fn&& fn) {
+    constexpr int V = 16 / (int)sizeof(T);
+    for (int c = threadIdx.x * V; c < cols; c += 1024 * V) {
+        vec_t<T, V> v;
+        ln_read<true, T, V>(row, c, cols, v);
+        fn(c, v);
+    }
+}
 template <typename T>
 __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const LnArgs a) {
+    constexpr int V = 16 / (int)sizeof(T);
     __shared__ float sh[32];
     const BlockGroup grp{sh};
     const float inv = 1.f / (float)a.cols;
@@ -346,17 +357,28 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const LnArgs a) {
         const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
         T* y = static_cast<T*>(a.y) + r * a.y_stride;
         float s = 0.f, q = 0.f;
-        for (int c = threadIdx.x; c < a.cols; c += 1024) s += (float)x[c];
+        ln_walk<T>(x, a.cols, [&](int c, const vec_t<T, V>& v) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) s += c + i < a.cols ? (float)v[i] : 0.f;
+        });
         const float mean = grp.sum(s) * inv;
-        for (int c = threadIdx.x; c < a.cols; c += 1024) {
-            const float d = (float)x[c] - mean;
-            q += d * d;
-        }
+        ln_walk<T>(x, a.cols, [&](int c, const vec_t<T, V>& v) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float d = c + i < a.cols ? (float)v[i] - mean : 0.f;
+                q += d * d;
+            }
+        });
         const float rstd = 1.f / sqrtf(grp.sum(q) * inv + a.eps);
-        for (int c = threadIdx.x; c < a.cols; c += 1024) {
-            const float w = a.weight ? load_any(a.weight, a.wdtype, c) : 1.f, b = a.bias ? load_any(a.bias, a.wdtype, c) : 0.f;
-            y[c] = (T)(((float)x[c] - mean) * rstd * w + b);
-        }
+        ln_walk<T>(x, a.cols, [&](int c, const vec_t<T, V>& v) {
+            float w[V], b[V];
+            ln_load_weight<V, 1>(a.weight, a.wdtype, c / V, 1, a.cols, 1.f, w);
+            ln_load_weight<V, 1>(a.bias, a.wdtype, c / V, 1, a.cols, 0.f, b);
+            vec_t<T, V> o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] = (T)(((float)v[i] - mean) * rstd * w[i] + b[i]);
+            ln_write<true, T, V>(y, c, a.cols, o);
+        });
         if (threadIdx.x == 0 && a.mean) {
             a.mean[r] = mean;
             a.rstd[r] = rstd;
@@ -366,6 +388,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const LnArgs a) {
 
 template <typename T>
 __global__ __launch_bounds__(1024) void ln_bwd_long_kernel(const LnArgs a) {
+    constexpr int V = 16 / (int)sizeof(T);
     __shared__ float sh[32];
     const BlockGroup grp{sh};
     const float inv = 1.f / (float)a.cols;
@@ -375,15 +398,28 @@ __global__ __launch_bounds__(1024) void ln_bwd_long_kernel(const LnArgs a) {
         T* dx = static_cast<T*>(a.dx) + r * a.y_stride;
         const float mean = a.mean[r], rstd = a.rstd[r];
         Sum2 s(0);
-        for (int c = threadIdx.x; c < a.cols; c += 1024) {
-            const float gw = (float)g[c] * (a.weight ? load_any(a.weight, a.wdtype, c) : 1.f);
-            s += Sum2(gw, gw * (((float)x[c] - mean) * rstd));
-        }
+        ln_walk<T>(x, a.cols, [&](int c, const vec_t<T, V>& v) {
+            vec_t<T, V> gv;
+            float w[V];
+            ln_read<true, T, V>(g, c, a.cols, gv);
+            ln_load_weight<V, 1>(a.weight, a.wdtype, c / V, 1, a.cols, 1.f, w);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float gw = c + i < a.cols ? (float)gv[i] * w[i] : 0.f, xh = c + i < a.cols ? ((float)v[i] - mean) * rstd : 0.f;
+                s += Sum2(gw, gw * xh);
+            }
+        });
         s = grp.sum(s);
-        for (int c = threadIdx.x; c < a.cols; c += 1024) {
-            const float gw = (float)g[c] * (a.weight ? load_any(a.weight, a.wdtype, c) : 1.f);
-            dx[c] = (T)(rstd * (gw - s.a * inv - ((float)x[c] - mean) * rstd * (s.b * inv)));
-        }
+        const float c1 = s.a * inv, c2 = s.b * inv;
+        ln_walk<T>(x, a.cols, [&](int c, const vec_t<T, V>& v) {
+            vec_t<T, V> gv, o;
+            float w[V];
+            ln_read<true, T, V>(g, c, a.cols, gv);
+            ln_load_weight<V, 1>(a.weight, a.wdtype, c / V, 1, a.cols, 1.f, w);
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] = (T)(rstd * ((float)gv[i] * w[i] - c1 - ((float)v[i] - mean) * rstd * c2));
+            ln_write<true, T, V>(dx, c, a.cols, o);
+        });
     }
 }
 
