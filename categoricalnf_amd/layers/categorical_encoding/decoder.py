@@ -53,7 +53,7 @@ class DecoderLinear(nn.Module):
         """log p(z_categ | z_cont) for z_categ of z_cont's shape without its last axis: forward() gathered at one class, whose
         [..., C] log-probabilities are never written (one fused kernel per direction instead of GEMM + log-softmax + gather)."""
         last = self.layers.main_net[-1]
-        hidden = self.layers.hidden_features(self._features(z_cont))
+        hidden = self.layers.hidden_features(self._features(z_cont)).to(last.weight.dtype)          # autocast: back from 16 bits
         return -Fn.linear_cross_entropy(hidden, last.weight, z_categ, last.bias, ignore_index=_NO_CLASS, reduction="none")
 
     def info(self):

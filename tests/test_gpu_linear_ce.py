@@ -444,6 +444,25 @@ def test_refusals_on_the_gpu():
         g.sum().backward()
 
 
+def test_decoder_under_autocast():
+    torch.manual_seed(0)
+    dec = DecoderLinear(num_categories=30, embed_dim=5, hidden_size=64, num_layers=1).cuda()
+    z, c = torch.randn(200, 5, device="cuda"), torch.randint(0, 30, (200,), device="cuda")
+    ref = dec.class_log_prob(z, c)
+    with torch.autocast("cuda", dtype=BF16):
+        out = dec.class_log_prob(z, c)
+    grads = torch.autograd.grad(out.sum(), dec.parameters())
+    # the products before the last are of bf16 operands with bf16 results: the features, two weights and two results round by 2^-8 of
+    # what is summed, each; a feature of the hidden layer is at most a sum of such, and a log-probability moves by at most twice a logit
+    with torch.no_grad():
+        h = dec._features(z).abs()
+        for m in list(dec.layers.inp_layer.modules()) + list(dec.layers.main_net.modules()):
+            if isinstance(m, torch.nn.Linear):
+                h = h @ m.weight.abs().t() + m.bias.abs()
+    assert out.dtype == F32 and bool(((out - ref).abs() <= 2 * 6 * 2.0 ** -8 * h.max(-1)[0]).all())
+    assert all(bool(torch.isfinite(g).all()) for g in grads)
+
+
 def test_decoder_ignores_no_category():
     dec = DecoderLinear(num_categories=30, embed_dim=5, hidden_size=64, num_layers=1).cuda()
     z, c = torch.randn(8, 5, device="cuda"), torch.randint(0, 30, (8,), device="cuda")
