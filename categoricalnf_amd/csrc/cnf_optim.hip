@@ -13,7 +13,7 @@
 // with a non-finite moment gets the scale NaN and codes 0: it reads back as NaN, as the fp32 moments of such an element would.
 //
 // Bound by HBM: 28 bytes per fp32 element (16 with 8-bit moments, plus 8 / 256).  The tensors' addresses travel in the kernel
-// arguments (up to 4 KB: 80 tensors a launch, 56 with scales): nothing is uploaded, so a launch may be captured and replayed, and
+// arguments (up to 4 KB: 98 tensors a launch, 70 with scales): nothing is uploaded, so a launch may be captured and replayed, and
 // nothing on the device has to outlive it.  A workgroup owns 1024 (2048 with 8-bit moments) consecutive elements of one tensor, found by counting
 // the tensors that begin at or before it; each lane has one or two 4-element units of every array in flight.
 #include <algorithm>
@@ -36,14 +36,14 @@ struct AdamConst {
 
 template <int BITS>
 struct AdamArgs {
-    static constexpr int kTensors = BITS == 8 ? 56 : 80;
+    static constexpr int kTensors = BITS == 8 ? 70 : 98;
     void* p[kTensors];
     const void* g[kTensors];
     void* m[kTensors];
     void* v[kTensors];
     float* ms[BITS == 8 ? kTensors : 1];
     float* vs[BITS == 8 ? kTensors : 1];
-    int64_t n[kTensors];
+    uint32_t n[kTensors];           // larger tensors are passed in parts
     uint32_t first[kTensors];       // index of the tensor's first chunk
     const float* lr;                // device scalars of a captured step (nullable): the learning rate ...
     const float* step;              // ... and the number of this step
@@ -266,34 +266,42 @@ __global__ __launch_bounds__(kBlock) void adamw_moments_kernel(const int8_t* m, 
 template <int BITS, typename PT, typename GT>
 static int adamw_launch(int count, void* const* p, const void* const* g, void* const* m, void* const* v, float* const* ms,
                         float* const* vs, const int64_t* n, AdamArgs<BITS>& a, hipStream_t st) {
-    int i = 0;
-    while (i < count) {
-        int k = 0;
-        uint64_t chunks = 0;
-        for (; i < count && k < AdamArgs<BITS>::kTensors; ++i) {
-            if (n[i] == 0) continue;
-            const uint64_t c = ((uint64_t)n[i] + kAdamChunk<BITS> - 1) / kAdamChunk<BITS>;
-            if (k > 0 && chunks + c > 0x7fffffffull) break;
-            a.p[k] = p[i];
-            a.g[k] = g[i];
-            a.m[k] = m[i];
-            a.v[k] = v[i];
-            if (BITS == 8) {
-                a.ms[k] = ms[i];
-                a.vs[k] = vs[i];
+    constexpr int64_t kMost = 1ll << 31;            // elements of an entry: whole chunks, blocks of codes and aligned vectors
+    static_assert(kMost % kAdamChunk<BITS> == 0 && kMost % 256 == 0, "a part ends where a chunk ends");
+    constexpr uint64_t kMostChunks = (1ull << 32) / kBlock - 1;             // a grid has less than 2^32 threads
+    int k = 0;
+    uint64_t chunks = 0;
+    auto flush = [&]() {
+        if (k == 0) return (int)CNF_OK;
+        a.count = k;
+        CNF_LAUNCH((adamw_kernel<BITS, PT, GT>), dim3((unsigned)chunks), dim3(kBlock), 0, st, a);
+        k = 0;
+        chunks = 0;
+        return launch_status("cnf_adamw_step");
+    };
+    for (int i = 0; i < count; ++i) {
+        for (int64_t at = 0; at < n[i]; at += kMost) {
+            const int64_t part = std::min<int64_t>(n[i] - at, kMost);
+            const uint64_t c = ((uint64_t)part + kAdamChunk<BITS> - 1) / kAdamChunk<BITS>;
+            if (k == AdamArgs<BITS>::kTensors || chunks + c > kMostChunks) {
+                const int rc = flush();
+                if (rc != CNF_OK) return rc;
             }
-            a.n[k] = n[i];
+            a.p[k] = static_cast<PT*>(p[i]) + at;
+            a.g[k] = static_cast<const GT*>(g[i]) + at;
+            a.m[k] = static_cast<char*>(m[i]) + at * (BITS / 8);
+            a.v[k] = static_cast<char*>(v[i]) + at * (BITS / 8);
+            if (BITS == 8) {
+                a.ms[k] = ms[i] + at / 256;
+                a.vs[k] = vs[i] + at / 256;
+            }
+            a.n[k] = (uint32_t)part;
             a.first[k] = (uint32_t)chunks;
             chunks += c;
             ++k;
         }
-        if (k == 0) break;
-        a.count = k;
-        CNF_LAUNCH((adamw_kernel<BITS, PT, GT>), dim3((unsigned)chunks), dim3(kBlock), 0, st, a);
-        const int rc = launch_status("cnf_adamw_step");
-        if (rc != CNF_OK) return rc;
     }
-    return CNF_OK;
+    return flush();
 }
 
 template <int BITS>

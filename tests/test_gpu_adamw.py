@@ -137,6 +137,15 @@ def test_step_is_the_chain_of_operations(bits, pdtype, gdtype, offset):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("count", [69, 70, 71, 97, 98, 99, 140, 141, 196, 197])
+def test_tensor_counts_around_a_launch(bits, count):
+    t = Tensors([(37 * i) % 700 + 1 for i in range(count)], bits=bits, seed=count)
+    before = t.host()
+    t.step()
+    t.check(before)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("count", [1, 55, 56, 57, 64, 65, 79, 80, 81, 500])
 def test_tensor_counts(bits, count):
     t = Tensors([(37 * i) % 700 + 1 for i in range(count)], bits=bits, seed=count)
@@ -372,16 +381,21 @@ def test_driver_trains_checkpoints_and_resumes(optimizer, graph_step, tmp_path):
     assert math.isfinite(first["val_bpd"]) and math.isfinite(second["val_bpd"])
 
 
-def test_more_elements_than_2_to_the_31():
-    n, tail = 2 ** 31 + 5000, 7000
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_elements_than_2_to_the_31(bits):
+    n, tail = 2 ** 31 + 5120, 7168           # whole blocks of 256, so that the tail alone has the same blocks
     p, g = torch.zeros(n, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, dtype=torch.bfloat16, device="cuda")
-    m, v = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    types = (torch.float32, torch.float32) if bits == 32 else (torch.int8, torch.uint8)
+    m, v = (torch.zeros(n, dtype=t, device="cuda") for t in types)
     g[-tail:].normal_()
-    small = [t[-tail:].clone() for t in (p, g, m, v)]
-    ops.adamw_step([p], [g], [m], [v], step=1, lr=1e-2)
-    ops.adamw_step([small[0]], [small[1]], [small[2]], [small[3]], step=1, lr=1e-2)
-    for a, b in zip((p, m, v), (small[0], small[2], small[3])):
-        assert torch.equal(a[-tail:], b) and not a[:-tail].any()
+    scales = [torch.zeros(n // 256, device="cuda") for _ in range(2)] if bits == 8 else []
+    small = [t[-tail:].clone() for t in (p, g, m, v)] + [s[-(tail // 256):].clone() for s in scales]
+    def step(p, g, m, v, *s):
+        ops.adamw_step([p], [g], [m], [v], step=1, lr=1e-2, exp_avg_scales=[s[0]] if s else None, exp_avg_sq_scales=[s[1]] if s else None)
+    step(p, g, m, v, *scales)
+    step(*small)
+    for a, b in zip([p, m, v] + scales, [small[0]] + small[2:]):
+        assert torch.equal(a[-b.numel():], b) and not a[:-b.numel()].any()
 
 
 def test_refusals():
