@@ -25,6 +25,23 @@ __device__ __forceinline__ void store_any(void* p, int dtype, long i, float v) {
     else static_cast<f16_t*>(p)[i] = (f16_t)v;
 }
 
+// four consecutive elements i ... i + 3, those below `end`; four go in one access, whatever their address
+template <typename V4>
+__device__ __forceinline__ void store4_any(void* p, int dtype, long i, long end, V4 v) {
+    if (i + 4 > end) {
+        for (int k = 0; k < 4; ++k)
+            if (i + k < end) store_any(p, dtype, i + k, v[k]);
+    } else if (dtype == CNF_DTYPE_F32) {
+        __builtin_memcpy(static_cast<float*>(p) + i, &v, 16);
+    } else if (dtype == CNF_DTYPE_BF16) {
+        const vec_t<bf16_t, 4> o = {(bf16_t)v[0], (bf16_t)v[1], (bf16_t)v[2], (bf16_t)v[3]};
+        __builtin_memcpy(static_cast<bf16_t*>(p) + i, &o, 8);
+    } else {
+        const vec_t<f16_t, 4> o = {(f16_t)v[0], (f16_t)v[1], (f16_t)v[2], (f16_t)v[3]};
+        __builtin_memcpy(static_cast<f16_t*>(p) + i, &o, 8);
+    }
+}
+
 // calls fn(T{}) with the element type of `dtype`
 template <typename Fn>
 inline int with_dtype(int dtype, Fn&& fn) {

@@ -189,22 +189,28 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_lse_kernel(const CeArgs a)
 }
 
 // the parts of the vocabulary -> row maximum, sum, loss; a category outside the vocabulary raises its flag and gives NaN.
+// `group` lanes (a power of two) share a row: few rows have many parts (one row of 32000 classes in 250 parts: a lane alone takes 40 us).
 // sums (with `reduced`): [workgroups][2] sum and number of the rows that are not ignored, in a fixed order; a single workgroup
 // writes `reduced` itself
 __global__ __launch_bounds__(kBlock) void ce_join_kernel(const float2* partial, const float* target_logit, const int64_t* target,
-                                                         int64_t ignore, int vocab, int splits, int64_t rows, float* row_max,
+                                                         int64_t ignore, int vocab, int splits, int group, int64_t rows, float* row_max,
                                                          float* row_sum, float* loss, double* sums, float* reduced, int* flags) {
-    const int64_t r = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    const int l = threadIdx.x & (group - 1);
+    const int64_t r = ((int64_t)blockIdx.x * kBlock + threadIdx.x) / group;
     float v = 0.f;
     bool counts = false;
-    if (r < rows) {
-        float m = -INFINITY, s = 0.f;
-        for (int k = 0; k < splits; ++k) m = fmaxf(m, partial[(int64_t)k * rows + r].x);
-        const float ref = m == -INFINITY ? 0.f : m;
-        for (int k = 0; k < splits; ++k) {
+    float m = -INFINITY, s = 0.f;
+    if (r < rows)
+        for (int k = l; k < splits; k += group) m = fmaxf(m, partial[(int64_t)k * rows + r].x);
+    for (int x = 1; x < group; x <<= 1) m = fmaxf(m, __shfl_xor(m, x, kWave));
+    const float ref = m == -INFINITY ? 0.f : m;
+    if (r < rows)
+        for (int k = l; k < splits; k += group) {
             const float2 o = partial[(int64_t)k * rows + r];
             s += o.y * __builtin_amdgcn_exp2f(o.x - ref);
         }
+    for (int x = 1; x < group; x <<= 1) s += __shfl_xor(s, x, kWave);
+    if (r < rows && l == 0) {
         row_max[r] = m;
         row_sum[r] = s;
         const int64_t t = target[r];
@@ -663,9 +669,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_grad_kernel(const GradArgs
                 f32x4* p = reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + ((int64_t)ks * a.n_end + row) * a.ld + h);
                 *p = a.accumulate ? *p + acc[m][n] : acc[m][n];
             } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (h + i < a.m_end) store_any(a.out, a.final_dtype, row * a.ld + h + i, acc[m][n][i]);
+                store4_any(a.out, a.final_dtype, row * a.ld + h, row * a.ld + a.m_end, acc[m][n]);
             }
         }
         if (sums && g == 0) {
@@ -751,7 +755,7 @@ struct CePlan {
     int64_t x_off, w_off, even_off, shift_off, bias_off, scales_off, largest_off;
     // forward
     bool big_lse;
-    int splits;
+    int splits, join_group;
     int64_t partial_off, logit_off, sums_off;
     // backward
     int64_t rows_pad, piece, d_off, state_off, dx_off, dw_off;
@@ -796,7 +800,9 @@ static CePlan ce_plan(int64_t R, int V, int H, int dtype, bool x_ok, bool w_ok, 
         p.splits = p.narrow ? narrow_split(R, V) : (int)std::min<int64_t>(vt, std::max<int64_t>(1, (p.big_lse ? 256 : 512) / rt));
         p.partial_off = take((int64_t)p.splits * R * 8);
         p.logit_off = take(R * 4);
-        p.sums_off = take(ceil_div(R, kNarrowOwn) * 16);
+        p.join_group = 1;
+        while (p.join_group < kWave && p.join_group * 4 < p.splits) p.join_group *= 2;
+        p.sums_off = take(std::max(ceil_div(R, kNarrowOwn), ceil_div(R * p.join_group, kBlock)) * 16);
         p.bytes = at;
         return p;
     }
@@ -976,7 +982,7 @@ int cnf_linear_ce(const void* x, int64_t x_stride, const void* weight, int64_t w
             a.target_logit = reinterpret_cast<float*>(ws + p.logit_off);
             a.splits = p.splits;
             double* sums = reinterpret_cast<double*>(ws + p.sums_off);
-            int64_t blocks = ceil_div(R, kBlock);
+            int64_t blocks = ceil_div(R * p.join_group, kBlock);
             if (p.narrow) {
                 NarrowArgs n = narrow_args(a, p, true, ws);
                 n.row_max = row_max;
@@ -994,7 +1000,7 @@ int cnf_linear_ce(const void* x, int64_t x_stride, const void* weight, int64_t w
             if (p.narrow && p.splits == 1)
                 blocks = ceil_div(R, kNarrowOwn);           // the rows are finished
             else
-                CNF_LAUNCH(ce_join_kernel, dim3((unsigned)blocks), dim3(kBlock), 0, st, a.partial, a.target_logit, target, ignore_index, V, p.splits, R,
+                CNF_LAUNCH(ce_join_kernel, dim3((unsigned)blocks), dim3(kBlock), 0, st, a.partial, a.target_logit, target, ignore_index, V, p.splits, p.join_group, R,
                            row_max, row_sum, loss, sums, reduced, flags);
             if (reduced && blocks > 1) CNF_LAUNCH(ce_reduce_kernel, dim3(1), dim3(1024), 0, st, sums, blocks, reduced);
             return launch_status("cnf_linear_ce");

@@ -472,9 +472,7 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
             if (a.final_dtype < 0) {
                 *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + ((int64_t)split * own_n + e) * a.ld + k) = acc[h][n];
             } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (k + i < a.hidden) store_any(a.out, a.final_dtype, e * a.ld + k + i, acc[h][n][i]);
+                store4_any(a.out, a.final_dtype, e * a.ld + k, e * a.ld + a.hidden, acc[h][n]);
             }
         }
     }

@@ -15,7 +15,9 @@
 // Bound by HBM: 28 bytes per fp32 element (16 with 8-bit moments, plus 8 / 256).  The tensors' addresses travel in the kernel
 // arguments (up to 4 KB: 98 tensors a launch, 70 with scales): nothing is uploaded, so a launch may be captured and replayed, and
 // nothing on the device has to outlive it.  A workgroup owns 1024 (2048 with 8-bit moments) consecutive elements of one tensor, found by counting
-// the tensors that begin at or before it; each lane has one or two 4-element units of every array in flight.
+// the tensors that begin at or before it; each lane has one or two 4-element units of every array in flight.  Measured: 420 M bf16
+// elements with fp32 moments 1595 us (5.8 TB/s), 84 M fp32 elements with 8-bit moments 280 us (4.8 TB/s), 27 M elements in 820
+// tensors 189 us in 9 launches (4.0 TB/s: a launch of 20 us fills and drains the chip for some of them).
 #include <algorithm>
 #include <cmath>
 #include <cstring>
