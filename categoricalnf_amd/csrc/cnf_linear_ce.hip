@@ -12,7 +12,7 @@
 // the piece.  db comes out of the second product: a fragment of ones in place of x.
 //
 // Bound by the matrix cores and, running one after the other without a pause, by the card's power: 8192 x 32000 x 1024 bf16, 537 GF each:
-// forward 575 us (930 TF), d 640 us (840 TF; 525 MB written beside it), dw 564 us (950 TF), dx 498 us (1080 TF); the library's 8192^3
+// forward 580 us (925 TF), d 640 us (840 TF; 525 MB written beside it), dw 517 us (1040 TF), dx 495 us (1085 TF); the library's 8192^3
 // product reaches 1236 TF.  256 x 256 tiles read an operand from LDS half as often as 128 x 128 ones (d: 340 us a half against 421);
 // those are kept for sizes whose large tiles would leave CUs empty.
 //
