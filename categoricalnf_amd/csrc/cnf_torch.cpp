@@ -11,9 +11,11 @@
 #include <utility>
 #include <vector>
 
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include "../../include/cnf_hip.h"
@@ -50,6 +52,12 @@ void bind(const std::unordered_map<std::string, uintptr_t>& at, py::object hip_o
 }
 
 // ---- checks ----------------------------------------------------------------------------------------------------------------------
+
+// Outputs are allocated by operators and filled through their pointers: a recording of the call would hold the empty tensors alone
+void refuse_recording(const char* name) {
+    TORCH_CHECK(!torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+                name, " is a HIP kernel, which torch.jit.trace and make_fx cannot record");
+}
 
 void need_gpu(const Tensor& t, const char* name) {
     if (t.is_cuda()) return;
@@ -110,6 +118,7 @@ Tensor opt(const std::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(
 // ---- layer norm --------------------------------------------------------------------------------------------------------------------
 
 std::tuple<Tensor, Tensor, Tensor> layer_norm_raw(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, bool want_stats) {
+    refuse_recording("layer_norm");
     const int code = dtype_code(x, "x");
     TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0, "layer_norm needs a last axis of at least one element, got shape ", x.sizes());
     TORCH_CHECK_VALUE(x.size(-1) <= 1 << 30, "layer_norm: ", x.size(-1), " columns");
@@ -135,6 +144,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_raw(const Tensor& x, const Tensor&
 
 std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd_raw(const Tensor& x, const Tensor& dy, const Tensor& weight, const Tensor& mean, const Tensor& rstd,
                                                       at::ScalarType pdtype, bool want_weight, bool want_bias) {
+    refuse_recording("layer_norm_bwd");
     const int code = dtype_code(x, "x");
     const int64_t C = x.size(-1);
     TORCH_CHECK_VALUE(dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type() && dy.device() == x.device(),
@@ -228,6 +238,7 @@ CeOperands ce_operands(const Tensor& x, const Tensor& weight, const Tensor& targ
 // loss, row statistics [2][R] (maximum, sum), reduced [3] or none, exponents [2]
 std::tuple<Tensor, Tensor, Tensor, Tensor> linear_ce_raw(const Tensor& x, const Tensor& weight, const Tensor& target, const Tensor& bias,
                                                          int64_t ignore_index, bool want_reduced, const Tensor& flags) {
+    refuse_recording("linear_cross_entropy");
     const c10::OptionalDeviceGuard guard(x.is_cuda() ? std::optional<at::Device>(x.device()) : std::nullopt);
     const CeOperands o = ce_operands(x, weight, target, bias);
     const auto f32 = x.options().dtype(at::kFloat);
@@ -246,6 +257,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> linear_ce_raw(const Tensor& x, const 
 std::tuple<Tensor, Tensor, Tensor> linear_ce_bwd_raw(const Tensor& x, const Tensor& weight, const Tensor& target, const Tensor& bias,
                                                      const Tensor& stats, const Tensor& exps, const Tensor& g, const Tensor& count,
                                                      int64_t ignore_index, bool want_x, bool want_w, bool want_b) {
+    refuse_recording("linear_cross_entropy_bwd");
     const c10::DeviceGuard guard(x.device());
     const CeOperands o = ce_operands(x, weight, target, bias);
     want_b = want_b && o.b.defined();
@@ -359,6 +371,7 @@ std::pair<double, Tensor> scalar(const py::object& v, const char* name, const at
 void adamw_step(const py::object& params, const py::object& grads, const py::object& exp_avgs, const py::object& exp_avg_sqs, const py::object& step,
                 const py::object& lr, double beta1, double beta2, double eps, double weight_decay, const py::object& exp_avg_scales,
                 const py::object& exp_avg_sq_scales, int64_t block) {
+    refuse_recording("adamw_step");
     TORCH_CHECK_VALUE(exp_avg_scales.is_none() == exp_avg_sq_scales.is_none(), "8-bit moments need both lists of scales");
     const bool bits8 = !exp_avg_scales.is_none();
     const char* names[6] = {"params", "grads", "exp_avgs", "exp_avg_sqs", "exp_avg_scales", "exp_avg_sq_scales"};

@@ -1,0 +1,34 @@
+"""The sub-networks' norm where something other than autograd watches the calls: what torch's norm gives there."""
+import pytest
+import torch
+
+from categoricalnf_amd import functional as Fn
+from categoricalnf_amd.layers.networks.help_layers import LayerNorm
+
+pytestmark = pytest.mark.gpu
+
+
+def pair(cols=24, dtype=torch.float32, seed=0):
+    """This package's norm and torch's with the same parameters, and an input."""
+    torch.manual_seed(seed)
+    mine, ref = LayerNorm(cols).cuda().to(dtype), torch.nn.LayerNorm(cols).cuda().to(dtype)
+    with torch.no_grad():
+        ref.weight.normal_(), ref.bias.normal_()
+    mine.load_state_dict(ref.state_dict())
+    return mine, ref, torch.randn(5, cols, device="cuda", dtype=dtype)
+
+
+def test_traced_norm_gives_what_the_eager_one_gives():
+    mine, ref, x = pair()
+    for check in (True, False):
+        traced = torch.jit.trace(mine, x, check_trace=check)
+        for seed in range(3):
+            y = torch.randn(5, 24, device="cuda", generator=torch.Generator("cuda").manual_seed(seed))
+            assert torch.equal(traced(y), ref(y))
+    graph = torch.fx.experimental.proxy_tensor.make_fx(mine)(x)
+    assert torch.equal(graph(x * 2), ref(x * 2))
+    with pytest.raises(RuntimeError, match="cannot record"):
+        torch.jit.trace(lambda v: Fn.layer_norm(v), x)
+    with pytest.raises(RuntimeError, match="cannot record"):
+        torch.jit.trace(lambda v: Fn.linear_cross_entropy(v, x, torch.arange(5, device="cuda")), x)
+    assert torch.equal(mine(x), Fn.layer_norm(x, mine.weight, mine.bias))
