@@ -66,6 +66,12 @@ void need_gpu(const Tensor& t, const char* name) {
     throw py::error_already_set();
 }
 
+// a tangent (forward-mode derivative) would be dropped: the kernels have none
+void refuse_tangents(std::initializer_list<const Tensor*> ts, const char* name) {
+    for (const Tensor* t : ts)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), name, " is a HIP kernel without a forward-mode derivative");
+}
+
 int dtype_code(const Tensor& t, const char* name) {
     need_gpu(t, name);
     switch (t.scalar_type()) {
@@ -119,6 +125,7 @@ Tensor opt(const std::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(
 
 std::tuple<Tensor, Tensor, Tensor> layer_norm_raw(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, bool want_stats) {
     refuse_recording("layer_norm");
+    refuse_tangents({&x, &weight, &bias}, "layer_norm");
     const int code = dtype_code(x, "x");
     TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0, "layer_norm needs a last axis of at least one element, got shape ", x.sizes());
     TORCH_CHECK_VALUE(x.size(-1) <= 1 << 30, "layer_norm: ", x.size(-1), " columns");
@@ -145,6 +152,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_raw(const Tensor& x, const Tensor&
 std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd_raw(const Tensor& x, const Tensor& dy, const Tensor& weight, const Tensor& mean, const Tensor& rstd,
                                                       at::ScalarType pdtype, bool want_weight, bool want_bias) {
     refuse_recording("layer_norm_bwd");
+    refuse_tangents({&x, &dy, &weight}, "layer_norm_bwd");
     const int code = dtype_code(x, "x");
     const int64_t C = x.size(-1);
     TORCH_CHECK_VALUE(dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type() && dy.device() == x.device(),
@@ -196,6 +204,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
 
 Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {
     const Tensor w = opt(weight), b = opt(bias);
+    refuse_tangents({&x, &w, &b}, "layer_norm");
     if (wants_grad({&x, &w, &b})) return LayerNormNode::apply(x, weight, bias, eps);
     return std::get<0>(layer_norm_raw(x, w, b, eps, false));
 }
@@ -239,6 +248,7 @@ CeOperands ce_operands(const Tensor& x, const Tensor& weight, const Tensor& targ
 std::tuple<Tensor, Tensor, Tensor, Tensor> linear_ce_raw(const Tensor& x, const Tensor& weight, const Tensor& target, const Tensor& bias,
                                                          int64_t ignore_index, bool want_reduced, const Tensor& flags) {
     refuse_recording("linear_cross_entropy");
+    refuse_tangents({&x, &weight, &bias}, "linear_cross_entropy");
     const c10::OptionalDeviceGuard guard(x.is_cuda() ? std::optional<at::Device>(x.device()) : std::nullopt);
     const CeOperands o = ce_operands(x, weight, target, bias);
     const auto f32 = x.options().dtype(at::kFloat);
@@ -258,6 +268,7 @@ std::tuple<Tensor, Tensor, Tensor> linear_ce_bwd_raw(const Tensor& x, const Tens
                                                      const Tensor& stats, const Tensor& exps, const Tensor& g, const Tensor& count,
                                                      int64_t ignore_index, bool want_x, bool want_w, bool want_b) {
     refuse_recording("linear_cross_entropy_bwd");
+    refuse_tangents({&x, &weight, &bias, &g}, "linear_cross_entropy_bwd");
     const c10::DeviceGuard guard(x.device());
     const CeOperands o = ce_operands(x, weight, target, bias);
     want_b = want_b && o.b.defined();
@@ -320,6 +331,7 @@ struct LinearCeNode : torch::autograd::Function<LinearCeNode> {
 Tensor linear_ce(const Tensor& x, const Tensor& weight, const Tensor& target, const std::optional<Tensor>& bias, int64_t ignore_index,
                  int64_t reduction, const Tensor& flags) {
     const Tensor b = opt(bias);
+    refuse_tangents({&x, &weight, &b}, "linear_cross_entropy");
     if (wants_grad({&x, &weight, &b})) return LinearCeNode::apply(x, weight, bias, target, ignore_index, reduction, flags);
     auto [loss, stats, reduced, exps] = linear_ce_raw(x, weight, target, b, ignore_index, reduction != kNone, flags);
     return reduction == kNone ? loss : value_of(reduced, reduction - 1);

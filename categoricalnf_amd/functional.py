@@ -777,10 +777,12 @@ def needs_grad(*tensors):
     return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
 
 
-def recorded():
-    """Whether the calls of this thread are being recorded or rewritten (torch.jit.trace, torch.compile, make_fx and every other dispatch
-    mode).  Kernels that fill their outputs through pointers are invisible there: modules take torch's operators instead."""
-    return torch._C._get_tracing_state() is not None or torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+def transformed():
+    """Whether the calls of this thread are recorded, rewritten or carry more than values: torch.jit.trace, torch.compile, make_fx and every
+    other dispatch mode, forward-mode derivatives.  Kernels that fill their outputs through pointers know nothing of it: modules take
+    torch's operators instead."""
+    return (torch._C._get_tracing_state() is not None or torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+            or torch.autograd.forward_ad._current_level >= 0)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):

@@ -15,11 +15,11 @@ _KERNEL_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 class LayerNorm(nn.LayerNorm):
     """nn.LayerNorm (same arguments, parameters and state_dict) whose last-axis norm of GPU tensors is this package's kernel,
     forward and backward.  Host tensors, float64 and norms over several axes keep torch's: the sub-networks also run there; so do
-    calls that are traced or compiled, which record operators and not kernels."""
+    calls that are traced or compiled or carry tangents (`functional.transformed`)."""
 
     def forward(self, x):
         if not x.is_cuda or x.dtype not in _KERNEL_DTYPES or len(self.normalized_shape) != 1 \
-                or x.shape[-1:] != self.normalized_shape or Fn.recorded():
+                or x.shape[-1:] != self.normalized_shape or Fn.transformed():
             return super().forward(x)
         if torch.is_autocast_enabled():
             x = x.float()                                # layer norm is an fp32 operation under autocast

@@ -2,6 +2,7 @@
 a recording does not see: they refuse, and the sub-networks' norms take torch's operators.  CPU: the checks come before the device's."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 from torch.utils.flop_counter import FlopCounterMode
 
 from categoricalnf_amd import functional as Fn
@@ -32,7 +33,7 @@ def test_modules_see_a_recording():
     seen = []
 
     def f(x):
-        seen.append(Fn.recorded())
+        seen.append(Fn.transformed())
         return x + 1
     f(X)
     torch.jit.trace(f, X, check_trace=False)
@@ -41,3 +42,27 @@ def test_modules_see_a_recording():
         f(X)
     f(X)
     assert seen == [False, True, True, True, False]
+
+
+CE = lambda x, w, b: ops.native().linear_ce(x, w, T, b, -100, 1, torch.zeros(1, dtype=torch.int32))
+TANGENTS = {**{k: (f, X) for k, f in CALLS.items() if k != "ops.adamw_step"}, "layer_norm, bias": (lambda b: Fn.layer_norm(X, None, b), X[0]),
+            "linear_cross_entropy": (lambda x: CE(x, W, None), X), "linear_cross_entropy, weight": (lambda w: CE(X, w, None), W),
+            "linear_cross_entropy, bias": (lambda b: CE(X, W, b), W[:, 0].contiguous())}
+
+
+@pytest.mark.parametrize("name", TANGENTS)
+def test_tangents_are_refused(name):
+    """With frozen operands, and under no_grad, where no autograd node would notice."""
+    call, x = TANGENTS[name]
+    with fwad.dual_level():
+        for grad in (True, False):
+            for leaf in (x.clone(), x.clone().requires_grad_()):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(fwad.make_dual(leaf, torch.ones_like(x)))
+
+
+def test_modules_see_tangents():
+    assert not Fn.transformed()
+    with fwad.dual_level():
+        assert Fn.transformed()
+    assert not Fn.transformed()
