@@ -437,6 +437,11 @@ void adamw_step(const py::object& params, const py::object& grads, const py::obj
                          beta2, eps, weight_decay, step_host, static_cast<const float*>(ptr(lr_dev)), static_cast<const float*>(ptr(step_dev)),
                          stream_of(device)),
           "cnf_adamw_step");
+    // as after any operation in place: a graph that has saved one of these raises in its backward instead of using the new values
+    for (int k = 0; k < lists; ++k)
+        if (k != 1)
+            for (const Tensor* t : l[k].t)
+                if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
 }
 
 }  // namespace
