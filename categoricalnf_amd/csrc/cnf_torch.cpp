@@ -54,9 +54,10 @@ void bind(const std::unordered_map<std::string, uintptr_t>& at, py::object hip_o
 // ---- checks ----------------------------------------------------------------------------------------------------------------------
 
 // Outputs are allocated by operators and filled through their pointers: a recording of the call would hold the empty tensors alone
-void refuse_recording(const char* name) {
+void refuse_transforms(const char* name) {
     TORCH_CHECK(!torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
                 name, " is a HIP kernel, which torch.jit.trace and make_fx cannot record");
+    TORCH_CHECK_NOT_IMPLEMENTED(!c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode), name, " is a HIP kernel, which torch.func cannot transform");
 }
 
 void need_gpu(const Tensor& t, const char* name) {
@@ -124,7 +125,7 @@ Tensor opt(const std::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(
 // ---- layer norm --------------------------------------------------------------------------------------------------------------------
 
 std::tuple<Tensor, Tensor, Tensor> layer_norm_raw(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, bool want_stats) {
-    refuse_recording("layer_norm");
+    refuse_transforms("layer_norm");
     refuse_tangents({&x, &weight, &bias}, "layer_norm");
     const int code = dtype_code(x, "x");
     TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0, "layer_norm needs a last axis of at least one element, got shape ", x.sizes());
@@ -151,7 +152,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_raw(const Tensor& x, const Tensor&
 
 std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd_raw(const Tensor& x, const Tensor& dy, const Tensor& weight, const Tensor& mean, const Tensor& rstd,
                                                       at::ScalarType pdtype, bool want_weight, bool want_bias) {
-    refuse_recording("layer_norm_bwd");
+    refuse_transforms("layer_norm_bwd");
     refuse_tangents({&x, &dy, &weight}, "layer_norm_bwd");
     const int code = dtype_code(x, "x");
     const int64_t C = x.size(-1);
@@ -204,6 +205,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
 
 Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {
     const Tensor w = opt(weight), b = opt(bias);
+    refuse_transforms("layer_norm");
     refuse_tangents({&x, &w, &b}, "layer_norm");
     if (wants_grad({&x, &w, &b})) return LayerNormNode::apply(x, weight, bias, eps);
     return std::get<0>(layer_norm_raw(x, w, b, eps, false));
@@ -247,7 +249,7 @@ CeOperands ce_operands(const Tensor& x, const Tensor& weight, const Tensor& targ
 // loss, row statistics [2][R] (maximum, sum), reduced [3] or none, exponents [2]
 std::tuple<Tensor, Tensor, Tensor, Tensor> linear_ce_raw(const Tensor& x, const Tensor& weight, const Tensor& target, const Tensor& bias,
                                                          int64_t ignore_index, bool want_reduced, const Tensor& flags) {
-    refuse_recording("linear_cross_entropy");
+    refuse_transforms("linear_cross_entropy");
     refuse_tangents({&x, &weight, &bias}, "linear_cross_entropy");
     const c10::OptionalDeviceGuard guard(x.is_cuda() ? std::optional<at::Device>(x.device()) : std::nullopt);
     const CeOperands o = ce_operands(x, weight, target, bias);
@@ -267,7 +269,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> linear_ce_raw(const Tensor& x, const 
 std::tuple<Tensor, Tensor, Tensor> linear_ce_bwd_raw(const Tensor& x, const Tensor& weight, const Tensor& target, const Tensor& bias,
                                                      const Tensor& stats, const Tensor& exps, const Tensor& g, const Tensor& count,
                                                      int64_t ignore_index, bool want_x, bool want_w, bool want_b) {
-    refuse_recording("linear_cross_entropy_bwd");
+    refuse_transforms("linear_cross_entropy_bwd");
     refuse_tangents({&x, &weight, &bias, &g}, "linear_cross_entropy_bwd");
     const c10::DeviceGuard guard(x.device());
     const CeOperands o = ce_operands(x, weight, target, bias);
@@ -331,6 +333,7 @@ struct LinearCeNode : torch::autograd::Function<LinearCeNode> {
 Tensor linear_ce(const Tensor& x, const Tensor& weight, const Tensor& target, const std::optional<Tensor>& bias, int64_t ignore_index,
                  int64_t reduction, const Tensor& flags) {
     const Tensor b = opt(bias);
+    refuse_transforms("linear_cross_entropy");
     refuse_tangents({&x, &weight, &b}, "linear_cross_entropy");
     if (wants_grad({&x, &weight, &b})) return LinearCeNode::apply(x, weight, bias, target, ignore_index, reduction, flags);
     auto [loss, stats, reduced, exps] = linear_ce_raw(x, weight, target, b, ignore_index, reduction != kNone, flags);
@@ -383,7 +386,7 @@ std::pair<double, Tensor> scalar(const py::object& v, const char* name, const at
 void adamw_step(const py::object& params, const py::object& grads, const py::object& exp_avgs, const py::object& exp_avg_sqs, const py::object& step,
                 const py::object& lr, double beta1, double beta2, double eps, double weight_decay, const py::object& exp_avg_scales,
                 const py::object& exp_avg_sq_scales, int64_t block) {
-    refuse_recording("adamw_step");
+    refuse_transforms("adamw_step");
     TORCH_CHECK_VALUE(exp_avg_scales.is_none() == exp_avg_sq_scales.is_none(), "8-bit moments need both lists of scales");
     const bool bits8 = !exp_avg_scales.is_none();
     const char* names[6] = {"params", "grads", "exp_avgs", "exp_avg_sqs", "exp_avg_scales", "exp_avg_sq_scales"};

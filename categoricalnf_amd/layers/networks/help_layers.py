@@ -15,7 +15,7 @@ _KERNEL_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 class LayerNorm(nn.LayerNorm):
     """nn.LayerNorm (same arguments, parameters and state_dict) whose last-axis norm of GPU tensors is this package's kernel,
     forward and backward.  Host tensors, float64 and norms over several axes keep torch's: the sub-networks also run there; so do
-    calls that are traced or compiled or carry tangents (`functional.transformed`)."""
+    calls that are traced, compiled, vectorised or carry tangents (`functional.transformed`)."""
 
     def forward(self, x):
         if not x.is_cuda or x.dtype not in _KERNEL_DTYPES or len(self.normalized_shape) != 1 \

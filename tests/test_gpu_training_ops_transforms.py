@@ -48,3 +48,19 @@ def test_tangents_pass_the_norm():
                 Fn.layer_norm(fwad.make_dual(x, t))
             with pytest.raises(NotImplementedError):
                 Fn.linear_cross_entropy(fwad.make_dual(x, t), x, torch.arange(5, device="cuda"))
+
+
+def test_function_transforms_pass_the_norm():
+    mine, ref, x = pair()
+    params = {k: v.detach() for k, v in mine.named_parameters()}
+    for make in (lambda m: torch.func.vmap(m)(x[None].expand(3, -1, -1) * torch.arange(1, 4, device="cuda")[:, None, None]),
+                 lambda m: torch.func.grad(lambda v: m(v).square().sum())(x),
+                 lambda m: torch.func.jvp(m, (x,), (x.flip(0),))[1],
+                 lambda m: torch.func.grad(lambda q: torch.func.functional_call(m, q, (x,)).square().sum())(params)["weight"],
+                 lambda m: torch.func.vmap(torch.func.grad(lambda q, v: torch.func.functional_call(m, q, (v,)).square().sum()), in_dims=(None, 0))(params, x)["bias"]):
+        got, want = make(mine), make(ref)
+        assert torch.equal(got, want)
+    # the function itself takes no transform
+    for call in (lambda: torch.func.vmap(Fn.layer_norm)(x), lambda: torch.func.grad(lambda v: Fn.layer_norm(v).sum())(x)):
+        with pytest.raises(NotImplementedError, match="torch.func"):
+            call()

@@ -66,3 +66,23 @@ def test_modules_see_tangents():
     with fwad.dual_level():
         assert Fn.transformed()
     assert not Fn.transformed()
+
+
+def test_modules_see_function_transforms():
+    seen = []
+
+    def f(x):
+        seen.append(Fn.transformed())
+        return (x * x).sum()
+    torch.func.vmap(f)(X), torch.func.grad(f)(X), torch.func.jvp(f, (X,), (X,)), torch.func.vjp(f, X), torch.func.hessian(f)(X)
+    assert len(seen) >= 5 and all(seen) and not Fn.transformed()
+
+
+@pytest.mark.parametrize("name", [k for k in TANGENTS])
+def test_function_transforms_are_refused(name):
+    call, x = TANGENTS[name]
+    for transform in (lambda f: lambda v: torch.func.vmap(f)(v[None]), torch.func.grad, lambda f: lambda v: torch.func.jvp(f, (v,), (v,))):
+        with pytest.raises(NotImplementedError, match="torch.func|forward-mode"):
+            transform(call)(x.clone())
+    with pytest.raises(NotImplementedError, match="torch.func"):
+        torch.func.vmap(lambda v: ops.adamw_step([v], [v], [v], [v], step=1, lr=0.1) or v)(X)
