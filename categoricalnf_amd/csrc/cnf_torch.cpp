@@ -184,30 +184,45 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd_raw(const Tensor& x, const Ten
     return {dx, dw, db};
 }
 
+// the gradients as operators that autograd knows, for a backward that is differentiated itself
+variable_list layer_norm_bwd_composed(const Tensor& x, const Tensor& dy, const Tensor& weight, at::ScalarType pdtype, double eps, bool want_weight,
+                                      bool want_bias) {
+    const Tensor xf = x.to(at::kFloat), g = dy.to(at::kFloat), gw = weight.defined() ? g * weight.to(at::kFloat) : g;
+    const Tensor centred = xf - xf.mean(-1, true), rstd = (centred.square().mean(-1, true) + eps).rsqrt(), xhat = centred * rstd;
+    const Tensor dx = rstd * (gw - gw.mean(-1, true) - xhat * (gw * xhat).mean(-1, true));
+    auto columns = [&](const Tensor& t) { return t.reshape({-1, x.size(-1)}).sum(0).to(pdtype); };
+    return {dx.to(x.scalar_type()), want_weight ? columns(g * xhat) : Tensor(), want_bias ? columns(g) : Tensor(), Tensor(), Tensor()};
+}
+
 struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
     // an absent parameter is no input of the node: the others' places in needs_input_grad move up
-    static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& w, const std::optional<Tensor>& b, double eps) {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& w, const std::optional<Tensor>& b, double eps, bool twice) {
         const Tensor weight = opt(w), bias = opt(b);
         auto [y, mean, rstd] = layer_norm_raw(x, weight, bias, eps, true);
         ctx->saved_data["bias"] = bias.defined();
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["twice"] = twice;
         ctx->save_for_backward({x, weight, mean, rstd});
         ctx->saved_data["dtype"] = (int64_t)(weight.defined() ? weight.scalar_type() : (bias.defined() ? bias.scalar_type() : x.scalar_type()));
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         const auto s = ctx->get_saved_variables();
-        auto [dx, dw, db] = layer_norm_bwd_raw(s[0], g[0], s[1], s[2], s[3], (at::ScalarType)ctx->saved_data["dtype"].toInt(),
-                                               s[1].defined() && ctx->needs_input_grad(1),
-                                               ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(s[1].defined() ? 2 : 1));
-        return once({dx, dw, db, Tensor()});
+        const auto pdtype = (at::ScalarType)ctx->saved_data["dtype"].toInt();
+        const bool want_weight = s[1].defined() && ctx->needs_input_grad(1);
+        const bool want_bias = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(s[1].defined() ? 2 : 1);
+        if (at::GradMode::is_enabled() && ctx->saved_data["twice"].toBool())
+            return layer_norm_bwd_composed(s[0], g[0], s[1], pdtype, ctx->saved_data["eps"].toDouble(), want_weight, want_bias);
+        auto [dx, dw, db] = layer_norm_bwd_raw(s[0], g[0], s[1], s[2], s[3], pdtype, want_weight, want_bias);
+        return once({dx, dw, db, Tensor(), Tensor()});
     }
 };
 
-Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {
+Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps, bool twice) {
     const Tensor w = opt(weight), b = opt(bias);
     refuse_transforms("layer_norm");
     refuse_tangents({&x, &w, &b}, "layer_norm");
-    if (wants_grad({&x, &w, &b})) return LayerNormNode::apply(x, weight, bias, eps);
+    if (wants_grad({&x, &w, &b})) return LayerNormNode::apply(x, weight, bias, eps, twice);
     return std::get<0>(layer_norm_raw(x, w, b, eps, false));
 }
 

@@ -785,9 +785,10 @@ def transformed():
             or torch._C._functorch.peek_interpreter_stack() is not None or torch.autograd.forward_ad._current_level >= 0)
 
 
-def layer_norm(x, weight=None, bias=None, eps=1e-5):
-    """Layer norm over the last axis (`ops.layer_norm`), differentiable (once) in x, weight and bias."""
-    return ops.native().layer_norm(x, weight, bias, eps)
+def layer_norm(x, weight=None, bias=None, eps=1e-5, twice=False):
+    """Layer norm over the last axis (`ops.layer_norm`), differentiable in x, weight and bias: once, or with `twice` any number of times
+    (a backward under create_graph is then made of torch's operators instead of the kernel)."""
+    return ops.native().layer_norm(x, weight, bias, eps, twice)
 
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}

@@ -23,7 +23,7 @@ class LayerNorm(nn.LayerNorm):
             return super().forward(x)
         if torch.is_autocast_enabled():
             x = x.float()                                # layer norm is an fp32 operation under autocast
-        return Fn.layer_norm(x, self.weight, self.bias, self.eps)
+        return Fn.layer_norm(x, self.weight, self.bias, self.eps, twice=True)
 
 
 class SimpleLinearLayer(nn.Module):

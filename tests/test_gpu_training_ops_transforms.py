@@ -64,3 +64,41 @@ def test_function_transforms_pass_the_norm():
     for call in (lambda: torch.func.vmap(Fn.layer_norm)(x), lambda: torch.func.grad(lambda v: Fn.layer_norm(v).sum())(x)):
         with pytest.raises(NotImplementedError, match="torch.func"):
             call()
+
+
+@pytest.mark.parametrize("affine", ["both", "weight", "none"])
+def test_second_derivatives_of_the_norm(affine):
+    """A penalty on the gradient's square, its own gradients in the input, the parameters and the upstream gradient against 64 bits.  The
+    longest chain: four sums over 24 columns, one over 5 rows, some 40 products: 150 roundings of 2^-24, of sums of absolute values
+    that exceed a tensor's largest element by less than a factor of 16; those of the first gradient enter the second squared: twice."""
+    torch.manual_seed(1)
+    mine = LayerNorm(24, elementwise_affine=affine != "none", bias=affine == "both").cuda()
+    with torch.no_grad():
+        for p in mine.parameters():
+            p.normal_()
+    ref = torch.nn.LayerNorm(24, elementwise_affine=affine != "none", bias=affine == "both").double()
+    ref.load_state_dict({k: v.double().cpu() for k, v in mine.state_dict().items()})
+    x, u = torch.randn(5, 24), torch.randn(5, 24)
+
+    def second(m, x, u):
+        x, u = x.clone().requires_grad_(), u.clone().requires_grad_()
+        wrt = [x] + list(m.parameters())
+        first = torch.autograd.grad(m(x), wrt, u, create_graph=True)
+        return first, torch.autograd.grad(sum(g.square().sum() for g in first), wrt[:2] + [u])
+    first, got = second(mine, x.cuda(), u.cuda())
+    want_first, want = second(ref, x.double(), u.double())
+    for a, b in zip(first + got, want_first + want):
+        assert float((a.detach().cpu().double() - b).abs().max()) <= 2 * 150 * 2.0 ** -24 * 16 * float(b.detach().abs().max())
+    # the gradient alone still comes from the kernel
+    xg = x.cuda().requires_grad_()
+    (a,), (b,) = (torch.autograd.grad(f(xg), xg, u.cuda()) for f in (mine, lambda v: Fn.layer_norm(v, mine.weight, mine.bias)))
+    assert torch.equal(a, b)
+
+
+def test_second_derivatives_in_16_bits_keep_the_types():
+    m = LayerNorm(16).cuda().bfloat16()
+    x = torch.randn(3, 2, 16, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    g = torch.autograd.grad(m(x).square().sum(), [x, m.weight, m.bias], create_graph=True)
+    assert all(a.dtype == torch.bfloat16 for a in g)
+    h = torch.autograd.grad(sum(a.float().square().sum() for a in g), [x, m.weight])
+    assert all(a.dtype == torch.bfloat16 and bool(torch.isfinite(a).all()) for a in h)
