@@ -10,6 +10,13 @@ from ..networks.help_layers import LinearNet
 _NO_CLASS = -2 ** 63         # no category is left out: one outside the vocabulary is an error
 
 
+def _hooked(module):
+    """Whether a call of the module runs anything besides its forward()."""
+    m = nn.modules.module
+    return bool("forward" in module.__dict__ or module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks
+                or m._global_forward_hooks or m._global_forward_pre_hooks or m._global_backward_hooks or m._global_backward_pre_hooks)
+
+
 def create_embed_layer(vocab, vocab_size, default_embed_layer_dims):
     """nn.Embedding from scratch or from a torchtext vocabulary's vectors (decoder.py:12-21)."""
     use_vectors = (vocab is not None and vocab.vectors is not None)
@@ -51,8 +58,17 @@ class DecoderLinear(nn.Module):
 
     def class_log_prob(self, z_cont, z_categ):
         """log p(z_categ | z_cont) for z_categ of z_cont's shape without its last axis: forward() gathered at one class, whose
-        [..., C] log-probabilities are never written (one fused kernel per direction instead of GEMM + log-softmax + gather)."""
-        last = self.layers.main_net[-1]
+        [..., C] log-probabilities are never written (one fused kernel per direction instead of GEMM + log-softmax + gather).  The kernel
+        reads the last Linear's parameters and does not call the modules that it stands for: where one of them is hooked, replaced or
+        watched, this is the gather."""
+        net = self.layers.main_net
+        last = net[-1] if type(net) is nn.Sequential else None
+        if type(last) is not nn.Linear or type(self.log_softmax) is not nn.LogSoftmax or Fn.transformed() \
+                or any(_hooked(m) for m in (self, self.layers, net, last, self.log_softmax)):
+            scores = self(z_cont)
+            inside = (z_categ >= 0) & (z_categ < scores.size(-1))        # outside: NaN, as the kernel's (an index error would end the process)
+            chosen = scores.gather(-1, torch.where(inside, z_categ, 0).long().unsqueeze(-1)).squeeze(-1)
+            return torch.where(inside, chosen, float("nan"))
         hidden = self.layers.hidden_features(self._features(z_cont)).to(last.weight.dtype)          # autocast: back from 16 bits
         return -Fn.linear_cross_entropy(hidden, last.weight, z_categ, last.bias, ignore_index=_NO_CLASS, reduction="none")
 

@@ -65,14 +65,20 @@ class LinearNet(nn.Module):
                 self.main_net[-1].bias.zero_()
 
     def forward(self, x, ext_input=None, **kwargs):
-        return self.main_net[-1](self.hidden_features(x, ext_input))
+        return self.main_net(self._input_features(x, ext_input))
 
-    def hidden_features(self, x, ext_input=None):
-        """What the last Linear is applied to."""
+    def _input_features(self, x, ext_input=None):
         feat = self.inp_layer(x)
         if ext_input is not None:
             feat = torch.cat([feat, ext_input], dim=-1)
-        return self.main_net[:-1](feat)
+        return feat
+
+    def hidden_features(self, x, ext_input=None):
+        """What the last Linear is applied to."""
+        feat = self._input_features(x, ext_input)
+        for layer in list(self.main_net)[:-1]:
+            feat = layer(feat)
+        return feat
 
     def set_bias(self, bias):
         # the reference assigns the tensor as it comes (help_layers.py:106); a float64 numpy prior then makes the bias

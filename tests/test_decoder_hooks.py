@@ -1,0 +1,86 @@
+"""LinearNet and DecoderLinear call the modules that a user has hooked or replaced."""
+import pytest
+import torch
+import torch.nn as nn
+
+from categoricalnf_amd import ops
+from categoricalnf_amd.layers.categorical_encoding.decoder import DecoderLinear
+from categoricalnf_amd.layers.networks.help_layers import LinearNet
+
+on_gpu = pytest.mark.gpu
+
+
+def test_hooks_of_the_main_net_run():
+    net = LinearNet(3, 5, num_layers=2, hidden_size=8)
+    x = torch.randn(4, 3)
+    plain = net(x)
+    assert torch.equal(net.main_net[-1](net.hidden_features(x)), plain)
+    calls = []
+    net.main_net.register_forward_pre_hook(lambda m, a: calls.append("pre"))
+    net.main_net.register_forward_hook(lambda m, a, out: out + 1)
+    assert torch.equal(net(x), plain + 1) and calls == ["pre"]
+
+
+def double(m, args, out):
+    return 2 * out
+
+
+def weight_norm(dec):
+    nn.utils.weight_norm(dec.layers.main_net[-1])
+    with torch.no_grad():
+        dec.layers.main_net[-1].weight_g.mul_(3)          # the weight itself is stale until the next call
+
+
+def parametrised(dec):
+    class Half(nn.Module):
+        def forward(self, w):
+            return w / 2
+    nn.utils.parametrize.register_parametrization(dec.layers.main_net[-1], "weight", Half())
+
+
+def replaced(dec):
+    dec.layers.main_net[-1].forward = lambda x: -nn.functional.linear(x, dec.layers.main_net[-1].weight)
+
+
+CHANGES = {"last": lambda d: d.layers.main_net[-1].register_forward_hook(double), "main_net": lambda d: d.layers.main_net.register_forward_hook(double),
+           "layers": lambda d: d.layers.register_forward_hook(double), "log_softmax": lambda d: d.log_softmax.register_forward_hook(double),
+           "itself": lambda d: d.register_forward_hook(double), "weight_norm": weight_norm, "parametrised": parametrised, "replaced": replaced}
+
+
+def check(device, name):
+    torch.manual_seed(0)
+    dec = DecoderLinear(num_categories=7, embed_dim=2, hidden_size=16, num_layers=1).to(device)
+    z, c = torch.randn(9, 1, 2, device=device), torch.randint(0, 7, (9, 1), device=device)
+    before = dec(z).gather(-1, c[..., None])[..., 0].detach().clone()
+    CHANGES[name](dec)
+    got, want = dec.class_log_prob(z, c), dec(z).gather(-1, c[..., None])[..., 0]
+    assert torch.equal(got, want) and not torch.allclose(got, before)
+    grads = [torch.autograd.grad(v.sum(), list(dec.parameters()), allow_unused=True) for v in (got, want)]
+    assert all((a is None and b is None) or torch.equal(a, b) for a, b in zip(*grads))
+    c[3] = 7
+    assert torch.isnan(dec.class_log_prob(z, c)[3]) and torch.equal(dec.class_log_prob(z, c)[4:], want[4:])
+
+
+@pytest.mark.parametrize("name", CHANGES)
+def test_class_log_prob_calls_hooked_modules(name):
+    check("cpu", name)
+
+
+@on_gpu
+@pytest.mark.parametrize("name", CHANGES)
+def test_class_log_prob_calls_hooked_modules_on_the_gpu(name):
+    check("cuda", name)
+
+
+def test_class_log_prob_without_hooks_is_the_kernel():
+    dec = DecoderLinear(num_categories=7, embed_dim=2, hidden_size=16, num_layers=1)
+    with pytest.raises(ops.HipOnlyError):
+        dec.class_log_prob(torch.randn(3, 1, 2), torch.zeros(3, 1, dtype=torch.long))
+
+
+def test_class_log_prob_can_be_traced():
+    dec = DecoderLinear(num_categories=7, embed_dim=2, hidden_size=16, num_layers=1)
+    z, c = torch.randn(3, 1, 2), torch.tensor([[1], [0], [6]])
+    dec.requires_grad_(False)
+    traced = torch.jit.trace(lambda a, b: dec.class_log_prob(a, b), (z, c))
+    assert torch.equal(traced(2 * z, c), dec(2 * z).gather(-1, c[..., None])[..., 0])
