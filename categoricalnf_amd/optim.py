@@ -7,6 +7,8 @@ import torch
 from . import ops
 
 _CPU = torch.device("cpu")
+# what a capture records runs again in every replay: only the step itself may be in it
+_IN_CAPTURE = "AdamW.step() inside a stream capture: %s, in every replay again; run one step with the same gradients present before the capture"
 
 
 class AdamW(torch.optim.Optimizer):
@@ -18,7 +20,7 @@ class AdamW(torch.optim.Optimizer):
     at every step, so steps below half its spacing are lost — train 16-bit models with fp32 parameters where that matters.
 
     capturable=True: the step counter is a device tensor and `lr` may be one (float32), so that a captured `step()` can be
-    replayed.  Parameters, gradients and moments must be dense (contiguous); sparse gradients are refused."""
+    replayed.  A step with the same gradients present has to run before the capture.  Parameters, gradients and moments must be dense (contiguous); sparse gradients are refused."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, min_8bit_size=4096,
                  capturable=False):
@@ -115,14 +117,18 @@ class AdamW(torch.optim.Optimizer):
                     raise RuntimeError("AdamW does not take sparse gradients")
                 home = p.device if capturable else _CPU
                 if not state:
+                    if capturing:
+                        raise RuntimeError(_IN_CAPTURE % "a parameter's state would be created")
                     if home not in fresh:
                         fresh[home] = torch.zeros((), dtype=torch.float32, device=home)
                     state = self._init_state(p, group, fresh[home])
                 step = state["step"]
-                if step.is_cuda != capturable:            # the group's flag was switched (a checkpoint of a captured run, and back)
-                    if id(step) not in moved:
-                        moved[id(step)] = (step, step.to(home))
-                    step = state["step"] = moved[id(step)][1]
+                if step.device != home:                   # the group's flag was switched (a checkpoint of a captured run, and back)
+                    if capturing:
+                        raise RuntimeError(_IN_CAPTURE % "a step counter would be moved to the device")
+                    if (id(step), home) not in moved:
+                        moved[id(step), home] = (step, step.to(home))
+                    step = state["step"] = moved[id(step), home][1]
                 bits8 = "exp_avg_scale" in state
                 key = (id(group), p.device, p.dtype, g.dtype, bits8, id(step))
                 call = calls.get(key)
@@ -140,6 +146,8 @@ class AdamW(torch.optim.Optimizer):
         for state in idle:                                # no gradient this time: the parameter's own count does not advance
             step = state["step"]
             if id(step) in steps:
+                if capturing:
+                    raise RuntimeError(_IN_CAPTURE % "the step counter of a parameter without a gradient would be split from the others'")
                 if id(step) not in stay:
                     stay[id(step)] = step.clone()
                 state["step"] = stay[id(step)]

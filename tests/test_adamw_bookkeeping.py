@@ -1,0 +1,67 @@
+"""optim.AdamW: state, counters and checkpoints around the step.  CPU: the kernel call is replaced, or never reached."""
+import pytest
+import torch
+
+from categoricalnf_amd import ops
+from categoricalnf_amd.optim import AdamW
+
+
+@pytest.fixture
+def steps(monkeypatch):
+    """Calls of the kernel, as lists of parameters; the stream is being captured while `steps.capturing`."""
+    class Calls(list):
+        capturing = False
+    calls = Calls()
+    monkeypatch.setattr(ops, "adamw_step", lambda ps, *a, **kw: calls.append([id(p) for p in ps]))
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: calls.capturing)
+    return calls
+
+
+def params(n=3):
+    ps = [torch.nn.Parameter(torch.zeros(4)) for _ in range(n)]
+    for p in ps:
+        p.grad = torch.ones(4)
+    return ps
+
+
+def test_a_capture_creates_no_state(steps):
+    ps = params()
+    opt = AdamW(ps, capturable=True)
+    steps.capturing = True
+    with pytest.raises(RuntimeError, match="before the capture"):
+        opt.step()
+    assert not steps and not opt.state
+    steps.capturing = False
+    opt.step()
+    steps.capturing = True
+    opt.step()
+    assert len(steps) == 2
+
+
+def test_a_capture_splits_no_counter(steps):
+    """A clone in the captured graph would take the shared counter's value anew in every replay."""
+    ps = params()
+    opt = AdamW(ps, capturable=True)
+    opt.step()
+    ps[1].grad = None
+    steps.capturing = True
+    with pytest.raises(RuntimeError, match="before the capture"):
+        opt.step()
+    assert len(steps) == 1 and all(float(opt.state[p]["step"]) == 1 for p in ps)
+    steps.capturing = False
+    opt.step()                                     # eagerly: the idle parameter keeps its count from here on
+    steps.capturing = True
+    opt.step()
+    assert [float(opt.state[p]["step"]) for p in ps] == [3, 1, 3]
+
+
+def test_a_capture_moves_no_counter(steps):
+    ps = params(1)
+    opt = AdamW(ps, capturable=True)
+    opt.step()
+    opt.state[ps[0]]["step"] = torch.ones((), device="meta")
+    steps.capturing = True
+    with pytest.raises(RuntimeError, match="before the capture"):
+        opt.step()
+    assert len(steps) == 1
