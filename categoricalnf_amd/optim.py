@@ -63,7 +63,14 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch's, but the moments keep the types they were saved with (torch casts a state to its parameter's type, which
-        would destroy codes, and fp32 moments of 16-bit parameters)."""
+        would destroy codes, and fp32 moments of 16-bit parameters).  A checkpoint whose steps this class does not compute (amsgrad,
+        maximize, another rule than decoupled weight decay) is refused."""
+        for group in state_dict["param_groups"]:
+            for option in ("amsgrad", "maximize"):
+                if group.get(option):
+                    raise ValueError("the checkpoint's optimiser has %s, which this AdamW does not compute" % option)
+            if "decoupled_weight_decay" in group and not group["decoupled_weight_decay"] and group.get("weight_decay"):
+                raise ValueError("the checkpoint's optimiser adds its weight decay to the gradients, which this AdamW does not")
         super().load_state_dict(state_dict)
         for group in self.param_groups:                   # a checkpoint of torch.optim.AdamW lacks this class's options
             for k, v in self.defaults.items():
@@ -123,7 +130,7 @@ class AdamW(torch.optim.Optimizer):
                         fresh[home] = torch.zeros((), dtype=torch.float32, device=home)
                     state = self._init_state(p, group, fresh[home])
                 step = state["step"]
-                if step.device != home:                   # the group's flag was switched (a checkpoint of a captured run, and back)
+                if step.is_cuda != capturable and step.device != home:        # the group's flag was switched (a checkpoint of a captured run, and back)
                     if capturing:
                         raise RuntimeError(_IN_CAPTURE % "a step counter would be moved to the device")
                     if (id(step), home) not in moved:

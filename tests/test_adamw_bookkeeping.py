@@ -65,3 +65,26 @@ def test_a_capture_moves_no_counter(steps):
     with pytest.raises(RuntimeError, match="before the capture"):
         opt.step()
     assert len(steps) == 1
+
+
+def state_of(cls, steps=1, **kw):
+    p = torch.nn.Parameter(torch.zeros(4))
+    opt = cls([p], **kw)
+    for _ in range(steps):
+        p.grad = torch.ones(4)
+        opt.step()
+    return opt.state_dict()
+
+
+@pytest.mark.parametrize("kw", [dict(amsgrad=True), dict(maximize=True)])
+def test_checkpoints_of_other_rules_are_refused(kw):
+    opt = AdamW(params(1))
+    with pytest.raises(ValueError, match=list(kw)[0]):
+        opt.load_state_dict(state_of(torch.optim.AdamW, **kw))
+    assert not opt.state and "amsgrad" not in opt.param_groups[0]
+    with pytest.raises(ValueError, match="weight decay"):
+        opt.load_state_dict(state_of(torch.optim.Adam, weight_decay=0.1))
+    opt.load_state_dict(state_of(torch.optim.AdamW, lr=0.25))
+    opt.load_state_dict(state_of(torch.optim.Adam))
+    assert opt.param_groups[0]["lr"] == 1e-3
+
