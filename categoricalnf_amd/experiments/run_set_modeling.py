@@ -149,6 +149,16 @@ def load_args(path):
         return pickle.load(f)
 
 
+def _check_same_rule(optimizer, state_dict, path):
+    """torch would load any optimiser's state into any other: 8-bit codes of moments as their values, another rule's moments and options."""
+    mine = isinstance(optimizer, AdamW)
+    for group in state_dict["param_groups"]:
+        known = "state_bits" in group or "amsgrad" in group if mine else "state_bits" not in group        # Adam's moments are AdamW's
+        if not known:
+            raise ValueError("%s was written by a run with another --optimizer than this one's %s: resume with that one, or start in another "
+                             "checkpoint path" % (path, type(optimizer).__name__))
+
+
 def load_checkpoint(path, model=None, optimizer=None, scheduler=None, device="cpu", load_best_model=False):
     """`path` = a checkpoint file or a directory (its newest `*.tar`, or with `load_best_model` the file its
     `best_save_dict` names); returns the non-state entries (general/mutils.py:66-112)."""
@@ -174,6 +184,7 @@ def load_checkpoint(path, model=None, optimizer=None, scheduler=None, device="cp
         state.update(blob["model_state_dict"])
         inner.load_state_dict(state)
     if optimizer is not None and "optimizer_state_dict" in blob:
+        _check_same_rule(optimizer, blob["optimizer_state_dict"], path)
         optimizer.load_state_dict(blob["optimizer_state_dict"])
     if scheduler is not None and "scheduler_state_dict" in blob:
         scheduler.load_state_dict(blob["scheduler_state_dict"])

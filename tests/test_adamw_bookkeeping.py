@@ -88,3 +88,21 @@ def test_checkpoints_of_other_rules_are_refused(kw):
     opt.load_state_dict(state_of(torch.optim.Adam))
     assert opt.param_groups[0]["lr"] == 1e-3
 
+
+def test_drivers_resume_with_the_optimiser_that_wrote_the_checkpoint(tmp_path, steps):
+    from categoricalnf_amd.experiments.run_set_modeling import load_checkpoint
+    made = {"radam": torch.optim.RAdam, "adamw": AdamW, "adamw8": lambda ps: AdamW(ps, state_bits=8, min_8bit_size=1)}
+    for a, write in made.items():
+        file = str(tmp_path / (a + ".tar"))
+        opt = write(params(1))
+        opt.step()
+        torch.save({"optimizer_state_dict": opt.state_dict(), "iteration": 1}, file)
+        for b, read in made.items():
+            other = read(params(1))
+            if (a == "radam") == (b == "radam"):
+                load_checkpoint(file, optimizer=other)
+                assert other.state
+            else:
+                with pytest.raises(ValueError, match="--optimizer"):
+                    load_checkpoint(file, optimizer=other)
+                assert not other.state
