@@ -444,21 +444,24 @@ __global__ __launch_bounds__(1024) void ln_reduce_kernel(const float* __restrict
                                                          void* dweight, void* dbias) {
     __shared__ float sh[64][17];
     const int cl = threadIdx.x & 15, slot = threadIdx.x >> 4;
-    const int64_t k = (int64_t)blockIdx.x * 16 + cl, width = 2 * (int64_t)cols;
-    float t = 0.f;
-    if (k < width)
-        for (int p = slot; p < nparts; p += 64) t += partials[(size_t)p * width + k];
-    sh[slot][cl] = t;
-    __syncthreads();
-    if (slot == 0 && k < width) {
-        float v = 0.f;
+    const int64_t width = 2 * (int64_t)cols;
+    for (int64_t k = (int64_t)blockIdx.x * 16 + cl; k - cl < width; k += (int64_t)gridDim.x * 16) {
+        float t = 0.f;
+        if (k < width)
+            for (int p = slot; p < nparts; p += 64) t += partials[(size_t)p * width + k];
+        sh[slot][cl] = t;
+        __syncthreads();
+        if (slot == 0 && k < width) {
+            float v = 0.f;
 #pragma unroll
-        for (int q = 0; q < 64; ++q) v += sh[q][cl];
-        if (k < cols) {
-            if (dweight) store_any(dweight, wdtype, k, v);
-        } else if (dbias) {
-            store_any(dbias, wdtype, k - cols, v);
+            for (int q = 0; q < 64; ++q) v += sh[q][cl];
+            if (k < cols) {
+                if (dweight) store_any(dweight, wdtype, k, v);
+            } else if (dbias) {
+                store_any(dbias, wdtype, k - cols, v);
+            }
         }
+        __syncthreads();                            // the sums have been read
     }
 }
 
@@ -599,7 +602,8 @@ int cnf_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64_t 
         if (rc != CNF_OK) return rc;
     }
     if (sums) {
-        const unsigned grid = (unsigned)((2 * (int64_t)cols + 15) / 16);
+        // a grid has less than 2^32 threads: 2^25 columns would reach that
+        const unsigned grid = (unsigned)std::min<int64_t>((2 * (int64_t)cols + 15) / 16, 1 << 21);
         CNF_LAUNCH(ln_reduce_kernel, dim3(grid), dim3(1024), 0, st, ws, parts, cols, wdtype, dweight, dbias);
         return launch_status("cnf_layer_norm_bwd (column sums)");
     }
