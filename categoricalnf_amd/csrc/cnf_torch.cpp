@@ -155,6 +155,8 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd_raw(const Tensor& x, const Ten
     refuse_transforms("layer_norm_bwd");
     refuse_tangents({&x, &dy, &weight}, "layer_norm_bwd");
     const int code = dtype_code(x, "x");
+    TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0 && x.size(-1) <= 1 << 30, "layer_norm_bwd needs a last axis of 1 to 2^30 elements, got shape ",
+                      x.sizes());
     const int64_t C = x.size(-1);
     TORCH_CHECK_VALUE(dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type() && dy.device() == x.device(),
                       "the gradient must have the input's shape and type, got ", dy.sizes(), " ", dy.scalar_type(), " for ", x.sizes(), " ",
@@ -304,7 +306,8 @@ std::tuple<Tensor, Tensor, Tensor> linear_ce_bwd_raw(const Tensor& x, const Tens
                       "the upstream gradient has ", gc.numel(), " values of ", gc.scalar_type(), " for ", o.R, " rows");
     for (const Tensor* s : {&stats, &count, &exps})
         TORCH_CHECK_VALUE(!s->defined() || (s->device() == x.device() && s->is_contiguous()), "row statistics are the forward's");
-    TORCH_CHECK_VALUE(stats.numel() == 2 * o.R && stats.scalar_type() == at::kFloat && (!count.defined() || count.scalar_type() == at::kFloat) &&
+    TORCH_CHECK_VALUE(stats.numel() == 2 * o.R && stats.scalar_type() == at::kFloat &&
+                          (!count.defined() || (count.scalar_type() == at::kFloat && count.numel() == 1)) &&
                           (!exps.defined() || (exps.numel() == 2 && exps.scalar_type() == at::kInt)),
                       "row statistics are the forward's: [2, ", o.R, "] float32");
     const int64_t n = api.linear_ce_workspace_bytes(o.R, (int)o.V, (int)o.H, o.code, 1);
