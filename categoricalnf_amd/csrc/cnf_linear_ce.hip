@@ -18,10 +18,10 @@
 //
 // Few features (H <= 128) take the kernels of cnf_linear_ce_narrow.hip instead, which write nothing of size R x V.
 //
-// fp32 inputs are scaled by a power of two per tensor (small rows of x: of their own) and split once into two fp16 parts (cnf_mfma.h:
-// pair_a): three fp16 products keep every product to 2^-22, and the matrix cores do them at 16 times the fp32 rate.  What is below
-// 2^-16 of the largest |w| keeps 2^-39 of that largest, not 2^-23 of itself; so does a small row's part in dw beside large rows.  16-bit inputs whose rows are not 16-byte aligned
-// are copied once into padded rows.
+// fp32 inputs are scaled by a power of two per tensor and split once into two fp16 parts (cnf_mfma.h: pair_a): three fp16 products keep
+// every product to 2^-22 of its rows' largest elements, and the matrix cores do them at 16 times the fp32 rate.  Tensors with rows below
+// 2^-14 of the largest element ("wide", kRowSpan) take fp32 matrix instructions instead, found on the device, in the same kernels and
+// order.  16-bit inputs whose rows are not 16-byte aligned are copied once into padded rows.
 // d is computed for g_r / max |g| (for fp16 operands times 2^14, so that small probabilities keep their bits) and the results are scaled
 // back: under a mean every row's -1 is then exact, where a rounded -g_r would put the same relative error on every row's largest entry.
 #include <algorithm>
@@ -47,9 +47,8 @@ struct CeArgs {
     // backward
     const RowState* state;          // [rows]
     const CeScales* scales;
-    int scaled;                     // fp32 operands: scales->ex holds, and
-    const uint8_t* shift;           // [rows] what the rows of x were scaled by beyond it
-    Operand x_even;                 // x for the product over the rows: fp32: without the rows' shifts, else x
+    int scaled;                     // fp32 operands: scales->ex and ->wide hold
+    Operand32 w32, x32;             // fp32 operands as they were given
     float lift;                     // of d
     void* d;                        // [parts][rows_pad][piece_ld]
     int64_t d_part, d_ld;
@@ -70,20 +69,27 @@ __device__ __forceinline__ void grouped_tile(unsigned t, unsigned ni, unsigned n
 
 __device__ __forceinline__ float bias_at(const CeArgs& a, int v) { return a.bias && v < a.vocab ? load_any(a.bias, a.bias_dtype, v) : 0.f; }
 
-// what takes a product of row r to its logit, times log2 e
-__device__ __forceinline__ float logit_scale(const CeArgs& a, int64_t r) {
-    const int shift = a.scaled && r < a.rows ? a.shift[r] : 0;
-    return a.scaled ? ldexpf(kLog2e, max(min(-(a.scales->ex[0] + a.scales->ex[1] + shift), 126), -300)) : kLog2e;
+// what takes a product to its logit, times log2 e
+__device__ __forceinline__ float logit_scale(const CeArgs& a) {
+    return a.scaled ? ldexpf(kLog2e, max(min(-(a.scales->ex[0] + a.scales->ex[1]), 126), -300)) : kLog2e;
 }
+// arguments of product32
+__device__ __forceinline__ bool all_live(int64_t) { return true; }
+struct NoExtra {
+    template <typename F>
+    __device__ __forceinline__ void operator()(const F&) const {}
+};
+__device__ __forceinline__ bool wide_rows(const CeScales* s) { return (s->wide[0] | s->wide[1]) != 0; }
 
 // ---- forward ---------------------------------------------------------------------------------------------------------------------
 
 // D[m = vocabulary][n = row]
-template <typename E, int BM, int BN, int WM, int WN>
+template <typename E, int PARTS, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 2) void ce_lse_kernel(const CeArgs a) {
     typedef TileProduct<E, false, false, BM, BN, WM, WN> Tile;
     __shared__ __align__(16) char lds[Tile::kLds];
     Tile tile(a.w, a.x, a.pairs, a.k_end, lds);
+    float back = logit_scale(a);
     const unsigned t = xcd_contiguous(blockIdx.x, gridDim.x);
     const int split = t % a.splits;
     const int r0 = (t / a.splits) * BN;
@@ -100,29 +106,22 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_lse_kernel(const CeArgs a)
         const int64_t tg = r < a.rows ? a.target[r] : -1;
         want[n] = tg >= 0 && tg < a.vocab && tg != a.ignore ? (int)tg : -1;
     }
-    for (int vt = first; vt < last; ++vt) {
-        const int v0 = vt * BM;
-        f32x4 acc[Tile::MT][Tile::NT];
+    auto clear = [](f32x4 (&acc)[Tile::MT][Tile::NT]) {
 #pragma unroll
         for (int m = 0; m < Tile::MT; ++m)
 #pragma unroll
             for (int n = 0; n < Tile::NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-        tile.begin(v0, r0, 0, a.k_end);         // (ahead of the last epilogue, as in ce_d_kernel, it spills more and gains nothing: 578 -> 588 us)
-        tile.multiply(acc, [](int, int) {});
+    };
+    auto enter = [&](f32x4 (&acc)[Tile::MT][Tile::NT], int v0) {
         const int vw = v0 + tile.m_wave + g * 4;        // the lane's first entry
-        {
-            float back[Tile::NT];
 #pragma unroll
-            for (int n = 0; n < Tile::NT; ++n) back[n] = logit_scale(a, (int64_t)r0 + tile.n_wave + n * 16 + col);
+        for (int m = 0; m < Tile::MT; ++m)
 #pragma unroll
-            for (int m = 0; m < Tile::MT; ++m)
+            for (int i = 0; i < 4; ++i) {
+                const float b = a.bias ? bias_at(a, vw + m * 16 + i) * kLog2e : 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float b = a.bias ? bias_at(a, vw + m * 16 + i) * kLog2e : 0.f;
-#pragma unroll
-                    for (int n = 0; n < Tile::NT; ++n) acc[m][n][i] = __builtin_fmaf(acc[m][n][i], back[n], b);
-                }
-        }
+                for (int n = 0; n < Tile::NT; ++n) acc[m][n][i] = __builtin_fmaf(acc[m][n][i], back, b);
+            }
         if (v0 + BM > a.vocab) {                        // entries past the vocabulary
 #pragma unroll
             for (int m = 0; m < Tile::MT; ++m)
@@ -157,6 +156,24 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_lse_kernel(const CeArgs a)
             sum[n] = s;
             mx[n] = top;
         }
+    };
+    bool wide = false;
+    if constexpr (PARTS > 1) {
+        wide = wide_rows(a.scales);
+        if (wide) back = kLog2e;
+        for (int vt = first; wide && vt < last; ++vt) {
+            f32x4 acc[Tile::MT][Tile::NT];
+            clear(acc);
+            product32<false, false>(a.w32, a.x32, vt * BM + tile.m_wave, (int64_t)r0 + tile.n_wave, 0, a.hidden, acc, all_live, NoExtra{});
+            enter(acc, vt * BM);
+        }
+    }
+    for (int vt = wide ? last : first; vt < last; ++vt) {
+        f32x4 acc[Tile::MT][Tile::NT];
+        clear(acc);
+        tile.begin(vt * BM, r0, 0, a.k_end);    // (ahead of the last epilogue, as in ce_d_kernel, it spills more and gains nothing: 578 -> 588 us)
+        tile.multiply(acc, [](int, int) {});
+        enter(acc, vt * BM);
     }
     // join the four lane groups, then the waves that share rows
     float2* sh = reinterpret_cast<float2*>(lds);        // [WM][BN]; every wave is past its last read of the stages
@@ -280,18 +297,27 @@ __global__ __launch_bounds__(1024) void ce_reduce_kernel(const double* sums, int
 // ---- operand layout ----------------------------------------------------------------------------------------------------------------
 
 constexpr int kMaxBlocks = 256;
-// the largest finite |element| (its bits) that this lane sees of fp32 rows `block`, `block` + `blocks`, ... (in units of the rows that a
-// workgroup's lanes share at a time); rows with target == ignore do not count (target: nullable).  Four rows are in flight
-__device__ __forceinline__ uint32_t largest_of(const float* src, int64_t stride, int64_t rows, int H, const int64_t* target, int64_t ignore, int block,
-                                               int blocks) {
+// What the layout has to know of an fp32 tensor: the bits of its largest finite |element|, and of the smallest that is largest in its row
+// (rows of zeros left out; none: all ones)
+struct Extent {
+    uint32_t top, least;
+};
+__device__ __forceinline__ int exponent_of(uint32_t bits) { return max((int)(bits >> 23), 1) - 127; }       // subnormal numbers: as if of -126
+__device__ __forceinline__ bool is_wide(Extent e) { return e.least != 0xffffffffu && exponent_of(e.top) - exponent_of(e.least) > kRowSpan; }
+
+// what this lane's rows say, of fp32 rows `block`, `block` + `blocks`, ... (in units of the rows that a workgroup's lanes share at a time);
+// rows with target == ignore do not count (target: nullable).  At most a wave shares a row; four rows are in flight
+__device__ __forceinline__ Extent extent_of(const float* src, int64_t stride, int64_t rows, int H, const int64_t* target, int64_t ignore, int block,
+                                            int blocks) {
     int g = 1;
-    while (g < (int)blockDim.x && g * 4 < H) g <<= 1;
+    while (g < kWave && g * 4 < H) g <<= 1;
     const int l = threadIdx.x & (g - 1), rpb = blockDim.x / g;
     const bool vec = stride % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
-    uint32_t top = 0;
+    Extent all = {0, 0xffffffffu};
     const int64_t step = (int64_t)blocks * rpb;
     for (int64_t r = (int64_t)block * rpb + threadIdx.x / g; r < rows; r += 4 * step) {
         bool live[4];
+        uint32_t top[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < 4; ++k) live[k] = r + k * step < rows && (!target || target[r + k * step] != ignore);
         for (int c = l * 4; c < H; c += g * 4) {
@@ -313,29 +339,43 @@ __device__ __forceinline__ uint32_t largest_of(const float* src, int64_t stride,
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t b = __float_as_uint(v[k][i]) & 0x7fffffffu;
-                    if (live[k] && b < 0x7f800000u) top = max(top, b);
+                    if (live[k] && b < 0x7f800000u) top[k] = max(top[k], b);
                 }
         }
+        for (int m = 1; m < g; m <<= 1)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) top[k] = max(top[k], (uint32_t)__shfl_xor((int)top[k], m, kWave));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            all.top = max(all.top, top[k]);
+            if (top[k]) all.least = min(all.least, top[k]);
+        }
     }
-    return top;
+    return all;
 }
 // of the workgroup, in every lane
-__device__ __forceinline__ uint32_t block_max(uint32_t top, uint32_t* sh) {
+__device__ __forceinline__ Extent block_extent(Extent e, Extent* sh) {
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, kWave));
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
+    for (int m = 32; m >= 1; m >>= 1) {
+        e.top = max(e.top, (uint32_t)__shfl_xor((int)e.top, m, kWave));
+        e.least = min(e.least, (uint32_t)__shfl_xor((int)e.least, m, kWave));
+    }
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = e;
     __syncthreads();
-    for (int k = 0; k < (int)blockDim.x / kWave; ++k) top = max(top, sh[k]);
-    return top;
+    for (int k = 0; k < (int)blockDim.x / kWave; ++k) {
+        e.top = max(e.top, sh[k].top);
+        e.least = min(e.least, sh[k].least);
+    }
+    return e;
 }
 
-// fp32: the largest finite |element| of x's rows that count (blockIdx.y 0) and of w (1), one value per workgroup
-__global__ __launch_bounds__(1024) void ce_largest_kernel(const float* x, int64_t x_stride, int64_t R, const int64_t* target, int64_t ignore,
-                                                            const float* w, int64_t w_stride, int V, int H, uint32_t* largest) {
-    __shared__ uint32_t sh[16];
-    const uint32_t top = block_max(blockIdx.y ? largest_of(w, w_stride, V, H, nullptr, 0, blockIdx.x, kMaxBlocks)
-                                              : largest_of(x, x_stride, R, H, target, ignore, blockIdx.x, kMaxBlocks), sh);
-    if (threadIdx.x == 0) largest[blockIdx.y * kMaxBlocks + blockIdx.x] = top;
+// fp32: the extents of x's rows that count (blockIdx.y 0) and of w (1), one for each workgroup
+__global__ __launch_bounds__(1024) void ce_extent_kernel(const float* x, int64_t x_stride, int64_t R, const int64_t* target, int64_t ignore,
+                                                           const float* w, int64_t w_stride, int V, int H, Extent* extents) {
+    __shared__ Extent sh[16];
+    const Extent e = block_extent(blockIdx.y ? extent_of(w, w_stride, V, H, nullptr, 0, blockIdx.x, kMaxBlocks)
+                                             : extent_of(x, x_stride, R, H, target, ignore, blockIdx.x, kMaxBlocks), sh);
+    if (threadIdx.x == 0) extents[blockIdx.y * kMaxBlocks + blockIdx.x] = e;
 }
 
 struct LayoutJob {
@@ -344,25 +384,22 @@ struct LayoutJob {
     void* dst;
 };
 struct LayoutArgs {
-    LayoutJob job[4];               // 0: x, 1: w, 3: x without its rows' shifts; [rows][cols] -> `parts` arrays of [rows][ld] 16-bit elements, zeros behind cols
+    LayoutJob job[2];               // x, w: [rows][cols] -> `parts` arrays of [rows][ld] 16-bit elements, zeros behind cols
     int cols, vec;                  // vec: bit j: 8 elements of job j's rows may be read as vectors of 16 bytes
-    int group;                      // lanes that share a row of x (a power of two)
     const int64_t* target;          // fp32: ignored rows of x are laid out as zeros, whatever they hold
     int64_t ignore;
-    uint8_t* shift;
     int64_t ld;
     const void* bias;               // -> fp32, times log2 e, -inf behind the vocabulary (nullable: zeros)
     int bias_dtype, vocab, bias_pad;
     float* bias_out;                // nullable
-    const uint32_t* largest;        // fp32: what ce_largest_kernel found (null: every workgroup looks for itself),
-    const int* known;               // or the exponents themselves;
-    CeScales* scales;               // where they go ...
+    const Extent* extents;          // fp32: what ce_extent_kernel found (null: every workgroup looks for itself),
+    const int* known;               // or the forward's exponents;
+    CeScales* scales;               // where what they say goes ...
     int* exponents;                 // ... and here (nullable)
 };
 
-// one launch for whatever a call has to lay out: blockIdx.y 0: x, 1: w, 2: the bias, 3: x for the product over the rows.  fp32: scaled,
-// then x0 + x1, each the fp16 nearest to what is left.  A row of x whose largest element is below 2^-11 of the tensor's is scaled by
-// itself (its shift): a row's results do not depend on the size of the others
+// one launch for whatever a call has to lay out: blockIdx.y 0: x, 1: w, 2: the bias.  fp32: scaled, then x0 + x1, each the fp16 nearest to
+// what is left
 template <typename T, typename E, int PARTS>
 __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
     if (blockIdx.y == 2) {
@@ -371,35 +408,38 @@ __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
                 a.bias_out[v] = v >= a.vocab ? -INFINITY : (a.bias ? load_any(a.bias, a.bias_dtype, v) * kLog2e : 0.f);
         return;
     }
-    const LayoutJob job = a.job[blockIdx.y];
+    const int which = blockIdx.y;
+    const LayoutJob job = a.job[which];
     if (!job.src) return;
     const T* src = static_cast<const T*>(job.src);
     E* dst = static_cast<E*>(job.dst);
-    const int which = blockIdx.y == 1 ? 1 : 0;
-    auto counts = [&](int64_t r) { return which == 1 || a.target[r] != a.ignore; };
-    auto exponent = [](uint32_t top) {
-        // the largest into 2^14 ... 2^15 (subnormal numbers: as if of exponent -126); zeros alone stay as they are
-        return top ? 14 - (max((int)(top >> 23), 1) - 127) : 0;
-    };
     int ex = 0;
     if (PARTS > 1) {
+        bool wide;
         if (a.known) {
-            ex = a.known[which];
+            wide = a.known[which] >= kWideMark / 2;
+            ex = a.known[which] - (wide ? kWideMark : 0);
         } else {
-            __shared__ uint32_t sh[kWavesPerBlock];
-            static_assert(kMaxBlocks == kBlock, "a lane reads one workgroup's value");
-            ex = exponent(block_max(a.largest ? a.largest[which * kMaxBlocks + threadIdx.x]
-                                              : largest_of(reinterpret_cast<const float*>(src), job.stride, job.rows, a.cols,
-                                                           which ? nullptr : a.target, a.ignore, 0, 1), sh));
+            __shared__ Extent sh[kWavesPerBlock];
+            static_assert(kMaxBlocks == kBlock, "a lane reads one workgroup's extent");
+            const Extent e = block_extent(a.extents ? a.extents[which * kMaxBlocks + threadIdx.x]
+                                                    : extent_of(reinterpret_cast<const float*>(src), job.stride, job.rows, a.cols,
+                                                                which ? nullptr : a.target, a.ignore, 0, 1), sh);
+            wide = is_wide(e);
+            ex = e.top ? 14 - exponent_of(e.top) : 0;           // the largest into 2^14 ... 2^15; zeros alone stay as they are
         }
-        if (blockIdx.x == 0 && blockIdx.y < 2 && threadIdx.x == 0) {
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
             a.scales->ex[which] = ex;
-            if (a.exponents) a.exponents[which] = ex;
+            a.scales->wide[which] = wide;
+            if (a.exponents) a.exponents[which] = ex + (wide ? kWideMark : 0);
         }
     }
     const int per = (int)(a.ld / 8);
-    const int64_t part = job.rows * a.ld;
-    auto read = [&](int64_t r, int c0) {
+    const int64_t part = job.rows * a.ld, n = job.rows * per;
+    for (int64_t q = (int64_t)blockIdx.x * kBlock + threadIdx.x; q < n; q += (int64_t)gridDim.x * kBlock) {
+        const int64_t r = q / per;
+        const int c0 = (int)(q - r * per) * 8;
+        const bool live = PARTS == 1 || which == 1 || a.target[r] != a.ignore;
         vec_t<T, 8> in;
         if (((a.vec >> which) & 1) && c0 + 8 <= a.cols) {
             in = *reinterpret_cast<const vec_t<T, 8>*>(src + r * job.stride + c0);
@@ -407,13 +447,10 @@ __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) in[i] = c0 + i < a.cols ? src[r * job.stride + c0 + i] : (T)0.f;
         }
-        return in;
-    };
-    auto write = [&](int64_t r, int c0, const vec_t<T, 8>& in, int by, bool live) {
         vec_t<E, 8> o[PARTS];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            float v = PARTS > 1 ? (live ? ldexpf((float)in[i], by) : 0.f) : (float)in[i];
+            float v = PARTS > 1 ? (live ? ldexpf((float)in[i], ex) : 0.f) : (float)in[i];
 #pragma unroll
             for (int p = 0; p < PARTS; ++p) {
                 o[p][i] = (E)v;
@@ -423,36 +460,6 @@ __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
         }
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) *reinterpret_cast<vec_t<E, 8>*>(dst + p * part + r * a.ld + c0) = o[p];
-    };
-    if (PARTS > 1 && blockIdx.y == 0) {
-        const int l = threadIdx.x & (a.group - 1), rpb = kBlock / a.group;
-        for (int64_t r = (int64_t)blockIdx.x * rpb + threadIdx.x / a.group; r < job.rows; r += (int64_t)gridDim.x * rpb) {
-            const bool live = counts(r);
-            uint32_t top = 0;
-            vec_t<T, 8> in;
-            for (int c = l; c < per; c += a.group) {
-                in = read(r, c * 8);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t b = __float_as_uint((float)in[i]) & 0x7fffffffu;
-                    if (b < 0x7f800000u) top = max(top, b);
-                }
-            }
-            for (int m = 1; m < a.group; m <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, kWave));
-            const int more = live && top ? exponent(top) - ex : 0, shift = more >= 12 ? min(more, 255) : 0;
-            if (l == 0) a.shift[r] = (uint8_t)shift;
-            for (int c = l; c < per; c += a.group) {
-                if (per > a.group) in = read(r, c * 8);
-                write(r, c * 8, in, ex + shift, live);
-            }
-        }
-        return;
-    }
-    const int64_t n = job.rows * per;
-    for (int64_t q = (int64_t)blockIdx.x * kBlock + threadIdx.x; q < n; q += (int64_t)gridDim.x * kBlock) {
-        const int64_t r = q / per;
-        const int c0 = (int)(q - r * per) * 8;
-        write(r, c0, read(r, c0), ex, PARTS == 1 || counts(r));
     }
 }
 
@@ -462,7 +469,7 @@ __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
 // divided by the largest |g|, which goes to scales
 __global__ __launch_bounds__(1024) void ce_rows_kernel(const float* g, int g_is_row, const float* count, const float* row_max, const float* row_sum,
                                                        const int64_t* target, int64_t ignore, int vocab, int64_t rows, int64_t rows_pad,
-                                                       const uint8_t* shift, int narrow, RowState* state, CeScales* scales) {
+                                                       RowState* state, CeScales* scales) {
     __shared__ uint32_t sh[16];
     const float shared = g_is_row ? 0.f : *g / *count;
     uint32_t bits = __float_as_uint(shared) & 0x7fffffffu;
@@ -486,7 +493,6 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(const float* g, int g_is_
         s.inv_s = in ? 1.f / row_sum[r] : 0.f;
         s.g = in ? (g_is_row ? g[r] : shared) / top : 0.f;
         s.target = in ? (int)t : -1;
-        if (narrow) s.target = in ? (int)((uint32_t)t | (shift ? (uint32_t)shift[r] << 24 : 0)) : kNarrowVocab;
         state[r] = s;
     }
 }
@@ -513,6 +519,41 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
         r0 = tj * BN;
         tile.begin(v0, r0, 0, a.k_end);
     };
+    if constexpr (PARTS > 1) {
+        if (wide_rows(a.scales)) {
+            // fp32 products, and d in fp32 where its two parts would be: [rows_pad][piece_ld]
+            for (; t < end; t += step) {
+                unsigned ti, tj;
+                grouped_tile(t, nv, nr, ti, tj);
+                const int64_t vw = a.v0 + (int64_t)ti * BM + tile.m_wave + g * 4, rw = (int64_t)tj * BN + tile.n_wave + col;
+                f32x4 acc[Tile::MT][Tile::NT];
+#pragma unroll
+                for (int m = 0; m < Tile::MT; ++m)
+#pragma unroll
+                    for (int n = 0; n < Tile::NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+                product32<false, false>(a.w32, a.x32, vw - g * 4, rw - col, 0, a.hidden, acc, all_live, NoExtra{});
+#pragma unroll
+                for (int n = 0; n < Tile::NT; ++n) {
+                    const RowState q = rw + n * 16 < a.rows ? a.state[rw + n * 16] : RowState{INFINITY, 0.f, 0.f, -1};
+#pragma unroll
+                    for (int m = 0; m < Tile::MT; ++m) {
+                        f32x4 p;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int64_t v = vw + m * 16 + i;
+                            const float b = a.bias ? bias_at(a, (int)v) * kLog2e : 0.f;
+                            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[m][n][i], kLog2e, b) - q.m2) * q.inv_s;
+                            if (v == q.target) p[i] -= 1.f;
+                            p[i] = q.target < 0 || v >= a.v1 ? 0.f : p[i] * q.g;
+                        }
+                        *reinterpret_cast<f32x4*>(static_cast<float*>(a.d) + (rw + n * 16) * a.d_ld + (vw - a.v0) + m * 16) = p;
+                    }
+                }
+            }
+            return;
+        }
+    }
+    const float back = logit_scale(a);
     if (t < end) begin();
     while (t < end) {
         f32x4 acc[Tile::MT][Tile::NT];
@@ -525,7 +566,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
         const int64_t rw = (int64_t)r0 + tile.n_wave + col;
         const bool edge = v0 + BM > a.v1;
         RowState st[Tile::NT];
-        float scale[Tile::NT], own_g[Tile::NT], back[Tile::NT];
+        float scale[Tile::NT], own_g[Tile::NT];
         // targets among the wave's entries are rare: their -g is applied behind a branch that most waves do not take
         int at[Tile::NT];
         bool hit = false;
@@ -534,7 +575,6 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
             st[n] = rw + n * 16 < a.rows ? a.state[rw + n * 16] : RowState{INFINITY, 0.f, 0.f, -1};
             own_g[n] = st[n].g * a.lift;
             scale[n] = st[n].inv_s * own_g[n];
-            back[n] = logit_scale(a, rw + n * 16);
             at[n] = st[n].target - vw;
             hit |= st[n].target >= 0 && at[n] >= 0 && at[n] < Tile::MT * 16;
         }
@@ -557,7 +597,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
                     f32x4 p;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)         // the logit rounded as in the forward, then the difference: the row's maximum gives 1
-                        p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[m + q][n][i], back[n], b[q][i]) - st[n].m2) * scale[n];
+                        p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[m + q][n][i], back, b[q][i]) - st[n].m2) * scale[n];
                     if (any_hit) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
@@ -604,6 +644,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
 
 struct GradArgs {
     Operand a, b;           // D[m = hidden][n = row or vocabulary entry]
+    Operand32 a32, b32;     // wide operands: the tensor itself, and d in fp32
+    const RowState* state;  // over the rows: which of them count (null: over the vocabulary)
     int pairs, k_end, ksplit;
     int m_end, n_end;       // extent of the output
     void* out;              // final: [n][ld] of the output type; partial: fp32 [ksplit][n][ld]
@@ -617,7 +659,7 @@ struct GradArgs {
     int db_dtype;
 };
 
-template <typename E, bool KMB, int BM, int BN, int WM, int WN>
+template <typename E, int PARTS, bool KMB, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 2) void ce_grad_kernel(const GradArgs a) {
     typedef TileProduct<E, true, KMB, BM, BN, WM, WN> Tile;
     __shared__ __align__(16) char lds[Tile::kLds];
@@ -641,19 +683,31 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_grad_kernel(const GradArgs
     s16x8 ones;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ones[i] = __builtin_bit_cast(short, (E)1.f);
-    // fp32: each part of d is once the partner of part 0 of x: pairs (0, 1) and (0, 0)
-    tile.begin(m0, n0, k0, k1);
-    tile.multiply(acc, [&](int stage, int pair) {
-        if (!sums || pair_a(a.pairs, pair) != 0) return;
-        const char* sb = lds + stage * Tile::kStage + Tile::kBytesA;
-        s16x8 fb[4];
-        tile_frags4<KMB, BN>(sb, tile.n_wave, 0, fb);
+    const bool wide = PARTS > 1 && wide_rows(a.scales);
+    if (wide) {
+        product32<true, KMB>(a.a32, a.b32, m0 + tile.m_wave, (int64_t)n0 + tile.n_wave, k0, k1, acc, [&](int64_t k) { return !KMB || a.state[k].target >= 0; },
+                             [&](const float (&fb)[Tile::NT][4]) {
+                                 if (!sums) return;
 #pragma unroll
-        for (int n = 0; n < Tile::NT; ++n) acc1[n] = mfma16<E>(ones, fb[n], acc1[n]);
-    });
+                                 for (int j = 0; j < 4; ++j)
+#pragma unroll
+                                     for (int n = 0; n < Tile::NT; ++n) acc1[n] = mfma32(1.f, fb[n][j], acc1[n]);
+                             });
+    } else {
+        // fp32: each part of d is once the partner of part 0 of x: pairs (0, 1) and (0, 0)
+        tile.begin(m0, n0, k0, k1);
+        tile.multiply(acc, [&](int stage, int pair) {
+            if (!sums || pair_a(a.pairs, pair) != 0) return;
+            const char* sb = lds + stage * Tile::kStage + Tile::kBytesA;
+            s16x8 fb[4];
+            tile_frags4<KMB, BN>(sb, tile.n_wave, 0, fb);
+#pragma unroll
+            for (int n = 0; n < Tile::NT; ++n) acc1[n] = mfma16<E>(ones, fb[n], acc1[n]);
+        });
+    }
     const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
-    const float down = a.scales->top / a.lift;
-    const int ex = a.scaled ? -a.scales->ex[a.scaled - 1] : 0;
+    const float down = wide ? a.scales->top : a.scales->top / a.lift;
+    const int ex = a.scaled && !wide ? -a.scales->ex[a.scaled - 1] : 0;
 #pragma unroll
     for (int n = 0; n < Tile::NT; ++n) {
         const int64_t row = (int64_t)n0 + tile.n_wave + n * 16 + col;
@@ -752,7 +806,7 @@ struct CePlan {
     int parts, pairs;
     bool copy_x, copy_w, narrow;
     int64_t ldh;                    // padded row of a copied operand
-    int64_t x_off, w_off, even_off, shift_off, bias_off, scales_off, largest_off;
+    int64_t x_off, w_off, bias_off, scales_off, extents_off;
     // forward
     bool big_lse;
     int splits, join_group;
@@ -770,7 +824,7 @@ static CePlan ce_plan(int64_t R, int V, int H, int dtype, bool x_ok, bool w_ok, 
     p.pairs = dtype == CNF_DTYPE_F32 ? 3 : 1;
     p.copy_x = p.parts > 1 || !x_ok;
     p.copy_w = p.parts > 1 || !w_ok;
-    p.narrow = narrow_supported(H, V);
+    p.narrow = narrow_supported(H);
     p.ldh = round_up(H, p.narrow ? 8 : kStepK);     // whole steps of the products
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -781,11 +835,7 @@ static CePlan ce_plan(int64_t R, int V, int H, int dtype, bool x_ok, bool w_ok, 
     if (p.copy_x) p.x_off = take((int64_t)p.parts * R * p.ldh * 2);
     if (p.copy_w) p.w_off = take((int64_t)p.parts * V * p.ldh * 2);
     p.scales_off = take(sizeof(CeScales));
-    if (p.parts > 1) {
-        p.largest_off = take(2 * kMaxBlocks * 4);
-        p.shift_off = take(R);
-        if (backward && !p.narrow) p.even_off = take((int64_t)p.parts * R * p.ldh * 2);
-    }
+    if (p.parts > 1) p.extents_off = take(2 * kMaxBlocks * sizeof(Extent));
     if (p.narrow) p.bias_off = take(round_up(V, kNarrowWalk) * 4);
     // about four workgroups for every CU, at least two steps of the walk each
     auto narrow_split = [](int64_t own, int64_t walk) {
@@ -849,7 +899,7 @@ static bool rows_aligned32(const void* p, int64_t stride) { return (reinterpret_
 
 template <typename T, typename E, int PARTS>
 static void ce_operands(CeArgs& a, const CePlan& p, const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias,
-                        int bias_dtype, const int64_t* target, int64_t ignore, const int* known, int* exponents, bool even, int64_t R, int V, int H,
+                        int bias_dtype, const int64_t* target, int64_t ignore, const int* known, int* exponents, int64_t R, int V, int H,
                         char* ws, hipStream_t st) {
     LayoutArgs l{};
     CeScales* scales = reinterpret_cast<CeScales*>(ws + p.scales_off);
@@ -857,21 +907,18 @@ static void ce_operands(CeArgs& a, const CePlan& p, const void* x, int64_t x_str
         // operands of few elements (at most 32 loads a lane): one launch less; with the rows finished by the walk itself, which saves
         // the join, 64 tokens of 51 classes and 64 features take 11.6 us instead of 17.1
         if (!known && std::max<int64_t>(R, V) * H > 8192) {
-            uint32_t* largest = reinterpret_cast<uint32_t*>(ws + p.largest_off);
-            CNF_LAUNCH(ce_largest_kernel, dim3(kMaxBlocks, 2), dim3(1024), 0, st, static_cast<const float*>(x), x_stride, R, target, ignore,
-                       static_cast<const float*>(w), w_stride, V, H, largest);
-            l.largest = largest;
+            Extent* extents = reinterpret_cast<Extent*>(ws + p.extents_off);
+            CNF_LAUNCH(ce_extent_kernel, dim3(kMaxBlocks, 2), dim3(1024), 0, st, static_cast<const float*>(x), x_stride, R, target, ignore,
+                       static_cast<const float*>(w), w_stride, V, H, extents);
+            l.extents = extents;
         }
         l.known = known;
         l.scales = scales;
         l.exponents = exponents;
-        l.shift = reinterpret_cast<uint8_t*>(ws + p.shift_off);
         l.target = target;
         l.ignore = ignore;
-        l.group = 8;
-        while (l.group < kWave && l.group < p.ldh / 8) l.group *= 2;
-        if (even) l.job[3] = LayoutJob{x, x_stride, R, ws + p.even_off};
-        a.shift = l.shift;
+        a.x32 = Operand32{static_cast<const float*>(x), x_stride, R};
+        a.w32 = Operand32{static_cast<const float*>(w), w_stride, V};
     }
     if (p.copy_x) l.job[0] = LayoutJob{x, x_stride, R, ws + p.x_off};
     if (p.copy_w) l.job[1] = LayoutJob{w, w_stride, V, ws + p.w_off};
@@ -889,11 +936,10 @@ static void ce_operands(CeArgs& a, const CePlan& p, const void* x, int64_t x_str
     if (p.copy_x || p.copy_w || p.narrow) {
         const int64_t chunks = std::max(p.copy_x ? R * (p.ldh / 8) : 0, p.copy_w ? V * (p.ldh / 8) : 0);
         const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(std::max<int64_t>(chunks, l.bias_pad), kBlock), 4096));
-        CNF_LAUNCH((ce_layout_kernel<T, E, PARTS>), dim3(grid, even ? 4 : 3), dim3(kBlock), 0, st, l);
+        CNF_LAUNCH((ce_layout_kernel<T, E, PARTS>), dim3(grid, 3), dim3(kBlock), 0, st, l);
     }
     a.x = p.copy_x ? Operand{ws + p.x_off, p.ldh, R * p.ldh, (int)R} : Operand{x, x_stride, 0, (int)R};
     a.w = p.copy_w ? Operand{ws + p.w_off, p.ldh, V * p.ldh, V} : Operand{w, w_stride, 0, V};
-    a.x_even = even ? Operand{ws + p.even_off, p.ldh, R * p.ldh, (int)R} : a.x;
     a.pairs = p.pairs;
     a.parts = p.parts;
     a.rows = R;
@@ -911,6 +957,8 @@ static NarrowArgs narrow_args(const CeArgs& a, const CePlan& p, bool rows_own, c
     NarrowArgs n{};
     n.own = rows_own ? a.x : a.w;
     n.walk = rows_own ? a.w : a.x;
+    n.own32 = rows_own ? a.x32 : a.w32;
+    n.walk32 = rows_own ? a.w32 : a.x32;
     n.hidden = a.hidden;
     n.vocab = a.vocab;
     n.rows = a.rows;
@@ -923,7 +971,6 @@ static NarrowArgs narrow_args(const CeArgs& a, const CePlan& p, bool rows_own, c
     n.state = a.state;
     n.scales = a.scales;
     n.scaled = a.scaled;
-    n.shift = a.shift;
     n.lift = a.lift;
     return n;
 }
@@ -974,7 +1021,7 @@ int cnf_linear_ce(const void* x, int64_t x_stride, const void* weight, int64_t w
             typedef decltype(t) T;
             typedef decltype(e) E;
             CeArgs a{};
-            ce_operands<T, E, decltype(parts)::value>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, target, ignore_index, nullptr, exponents, false, R, V, H,
+            ce_operands<T, E, decltype(parts)::value>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, target, ignore_index, nullptr, exponents, R, V, H,
                                                      ws, st);
             a.target = target;
             a.ignore = ignore_index;
@@ -994,9 +1041,9 @@ int cnf_linear_ce(const void* x, int64_t x_stride, const void* weight, int64_t w
                 const int rc = narrow_launch(kNarrowLse, dtype, n, st);
                 if (rc != CNF_OK) return rc;
             } else if (p.big_lse)
-                CNF_LAUNCH((ce_lse_kernel<E, kBig, kBig, 2, 4>), dim3((unsigned)(ceil_div(R, kBig) * p.splits)), dim3(512), 0, st, a);
+                CNF_LAUNCH((ce_lse_kernel<E, decltype(parts)::value, kBig, kBig, 2, 4>), dim3((unsigned)(ceil_div(R, kBig) * p.splits)), dim3(512), 0, st, a);
             else
-                CNF_LAUNCH((ce_lse_kernel<E, kSmall, kSmall, 2, 2>), dim3((unsigned)(ceil_div(R, kSmall) * p.splits)), dim3(256), 0, st, a);
+                CNF_LAUNCH((ce_lse_kernel<E, decltype(parts)::value, kSmall, kSmall, 2, 2>), dim3((unsigned)(ceil_div(R, kSmall) * p.splits)), dim3(256), 0, st, a);
             if (p.narrow && p.splits == 1)
                 blocks = ceil_div(R, kNarrowOwn);           // the rows are finished
             else
@@ -1031,13 +1078,13 @@ int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64
         typedef decltype(e) E;
         constexpr int PARTS = decltype(parts)::value;
         CeArgs a{};
-        ce_operands<T, E, PARTS>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, target, ignore_index, exponents, nullptr,
-                                 PARTS > 1 && !p.narrow && dweight, R, V, H, ws, st);
+        ce_operands<T, E, PARTS>(a, p, x, x_stride, weight, w_stride, bias, bias_dtype, target, ignore_index, exponents, nullptr, R, V, H,
+                                 ws, st);
         RowState* state = reinterpret_cast<RowState*>(ws + p.state_off);
         a.state = state;
         // per-row gradients: every workgroup finds the largest |g| itself; few of them
         CNF_LAUNCH(ce_rows_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(p.rows_pad, 1024), g_per_row ? 16 : 1024)), dim3(1024), 0, st, g,
-                   g_per_row, count, row_max, row_sum, target, ignore_index, V, R, p.rows_pad, a.shift, p.narrow, state,
+                   g_per_row, count, row_max, row_sum, target, ignore_index, V, R, p.rows_pad, state,
                    reinterpret_cast<CeScales*>(ws + p.scales_off));
         const int64_t ld4 = round_up(H, 4);
         if (p.narrow) {
@@ -1085,6 +1132,8 @@ int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64
             q.a = Operand{static_cast<const uint16_t*>(a.w.base) + v0 * a.w.ld, a.w.ld, a.w.part, H};
             q.b = d;
             q.b.ext = (int)R;
+            q.a32 = Operand32{a.w32.base + v0 * a.w32.ld, a.w32.ld, H};
+            q.b32 = Operand32{static_cast<const float*>(a.d), a.d_ld, R};
             q.k_end = (int)width;
             q.n_end = (int)R;
             q.ksplit = p.dx_split;
@@ -1098,20 +1147,23 @@ int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64
             auto grad = [&](bool kmb, bool big, int64_t n) {
                 const int64_t edge = big ? kBig : kSmall;
                 const dim3 grid((unsigned)(ceil_div(n, edge) * ceil_div(H, edge) * q.ksplit));
-                if (kmb && big) CNF_LAUNCH((ce_grad_kernel<E, true, kBig, kBig, 2, 4>), grid, dim3(512), 0, st, q);
-                else if (kmb) CNF_LAUNCH((ce_grad_kernel<E, true, kSmall, kSmall, 2, 2>), grid, dim3(256), 0, st, q);
-                else if (big) CNF_LAUNCH((ce_grad_kernel<E, false, kBig, kBig, 2, 4>), grid, dim3(512), 0, st, q);
-                else CNF_LAUNCH((ce_grad_kernel<E, false, kSmall, kSmall, 2, 2>), grid, dim3(256), 0, st, q);
+                if (kmb && big) CNF_LAUNCH((ce_grad_kernel<E, PARTS, true, kBig, kBig, 2, 4>), grid, dim3(512), 0, st, q);
+                else if (kmb) CNF_LAUNCH((ce_grad_kernel<E, PARTS, true, kSmall, kSmall, 2, 2>), grid, dim3(256), 0, st, q);
+                else if (big) CNF_LAUNCH((ce_grad_kernel<E, PARTS, false, kBig, kBig, 2, 4>), grid, dim3(512), 0, st, q);
+                else CNF_LAUNCH((ce_grad_kernel<E, PARTS, false, kSmall, kSmall, 2, 2>), grid, dim3(256), 0, st, q);
             };
             if (dx) grad(false, p.big_dx, R);
             if (!dweight) continue;
             // dw[v][h] = sum_r x[r][h] d[r][v]; db[v] = sum_r d[r][v]
             char* dw = static_cast<char*>(dweight) + v0 * H * dtype_bytes(dtype);
             char* db = dbias ? static_cast<char*>(dbias) + v0 * dtype_bytes(bias_dtype) : nullptr;
-            q.a = a.x_even;
+            q.a = a.x;
             q.a.ext = H;
             q.b = d;
             q.b.ext = (int)width;
+            q.a32 = Operand32{a.x32.base, a.x32.ld, H};
+            q.b32.ext = width;
+            q.state = state;
             q.k_end = (int)R;
             q.n_end = (int)width;
             q.ksplit = p.dw_split;

@@ -10,15 +10,19 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 struct RowState {       // backward: what an element d = (exp2(l2 - m2) inv_s - [target]) g, l2 = l log2 e, needs of its row
     float m2, inv_s;    // maximum times log2 e (+inf: the row is ignored); 1 / s
     float g;            // over the largest |g|
-    int target;         // -1: ignored.  Few features: target_of(), and in the upper 8 bits the row's shift
+    int target;         // -1: ignored
 };
-constexpr int kNarrowVocab = (1 << 24) - 1;             // so many classes at most; its value as a target: ignored
-__device__ __forceinline__ int target_of(int word) { return word & kNarrowVocab; }
-__device__ __forceinline__ int shift_of(int word) { return (int)((uint32_t)word >> 24); }
+
+// Two fp16 parts of an operand scaled by one power of two hold 22 bits of what is above 2^-16 of its largest element, and 2^-39 of that
+// largest of the rest.  An operand with a row whose largest element is below 2^-kRowSpan of the tensor's is "wide": its call takes the fp32
+// matrix instructions (product32), so that no row's results depend on the size of the others.
+constexpr int kRowSpan = 14;
+constexpr int kWideMark = 4096;         // in an exponent that the forward hands to the backward: the operand is wide
 
 // what the operands of a call were scaled by; in device memory
 struct CeScales {
-    int ex[2];          // fp32: x was multiplied by 2^ex[0] (its row r by 2^(ex[0] + shift[r])), w by 2^ex[1]
+    int ex[2];          // fp32: x was multiplied by 2^ex[0], w by 2^ex[1]
+    int wide[2];        // fp32: whether x, w are wide
     float top;          // largest |g|
 };
 
@@ -46,8 +50,8 @@ struct NarrowArgs {
     int64_t ld;
     int final_dtype;
     const CeScales* scales;
-    int scaled;                         // fp32 operands: scales->ex holds, and
-    const uint8_t* shift;               // [rows] what the rows of x were scaled by beyond it (forward)
+    int scaled;                         // fp32 operands: scales->ex and ->wide hold
+    Operand32 own32, walk32;            // the operands as they were given, for wide ones
     float lift;                         // d is computed times lift (a power of two): small probabilities stay normal numbers in fp16
     void* db;                           // nullable; partial sums: in column ld - 4 of out
     int db_dtype;
@@ -55,7 +59,7 @@ struct NarrowArgs {
 
 enum NarrowJob { kNarrowLse, kNarrowDx, kNarrowDw };
 
-bool narrow_supported(int hidden, int vocab);
+bool narrow_supported(int hidden);
 int narrow_launch(NarrowJob job, int dtype, const NarrowArgs& a, hipStream_t st);
 
 }  // namespace cnf

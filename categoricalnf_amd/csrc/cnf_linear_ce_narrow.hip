@@ -126,6 +126,95 @@ __device__ __forceinline__ void static_for(Fn&& fn) {
     static_for_impl(static_cast<Fn&&>(fn), std::make_integer_sequence<int, N>{});
 }
 
+// forward: two blocks of 16 walk entries (the lane's: m0 + 16 t + i) enter the running maximum and sum of the lane's own rows own0 + 16 n
+template <int NT>
+__device__ __forceinline__ void lse_step(const NarrowArgs& a, f32x4 (&sc)[2][NT], const float (&back)[NT], const f32x4 (&bias)[2], int64_t m0,
+                                         int64_t own0, const int (&want)[NT], float (&mx)[NT], float (&sum)[NT], float (&own_logit)[NT]) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[t][n][i] = __builtin_fmaf(sc[t][n][i], back[n], bias[t][i]);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int64_t at = want[n] - m0;
+        if (want[n] >= 0 && at >= 0 && at < 32 && (at & 15) < 4) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (at == t * 16 + i) own_logit[n] = sc[t][n][i];
+            if (a.splits > 1) a.target_logit[own0 + n * 16] = own_logit[n];
+        }
+        float top = mx[n];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[t][n][i]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float q = sum[n] * __builtin_amdgcn_exp2f(mx[n] - ref);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q += __builtin_amdgcn_exp2f(sc[t][n][i] - ref);
+        sum[n] = q;
+        mx[n] = top;
+    }
+}
+
+// The walk with fp32 products of the operands as they were given (kRowSpan), read where they lie; no lift, and nothing is split
+template <int HT, int NT, NarrowJob JOB>
+__device__ __forceinline__ void narrow_walk32(const NarrowArgs& a, int64_t first, int64_t last, int64_t n_wave, const RowState (&st)[NT],
+                                              const float (&bias_n)[NT], const int (&want)[NT], float (&mx)[NT], float (&sum)[NT],
+                                              float (&own_logit)[NT], f32x4 (&acc)[HT][NT]) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+    float back[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) back[n] = kLog2e;
+    for (int64_t m_half = first * kNarrowWalk; m_half < last * kNarrowWalk; m_half += 32) {
+        f32x4 sc[2][NT];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) sc[t][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        product32<false, false, 2, NT>(a.walk32, a.own32, m_half, n_wave, 0, a.hidden, sc, [](int64_t) { return true; }, [](const float (&)[NT][4]) {});
+        const int64_t m0 = m_half + g * 4;
+        f32x4 bias[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) bias[t] = JOB == kNarrowDw ? f32x4{0.f, 0.f, 0.f, 0.f} : *reinterpret_cast<const f32x4*>(a.bias + m0 + t * 16);
+        if (JOB == kNarrowLse) {
+            lse_step(a, sc, back, bias, m0, n_wave + col, want, mx, sum, own_logit);
+            continue;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int64_t at = m0 + (e / 4) * 16 + e % 4;                // the walk entry, one of this lane's eight
+            // the rows' records are padded to whole tiles
+            const RowState q = JOB == kNarrowDw ? a.state[at] : RowState{0.f, 0.f, 0.f, 0};
+            float v[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const RowState& row = JOB == kNarrowDw ? q : st[n];
+                const float b = JOB == kNarrowDw ? bias_n[n] : bias[e / 4][e % 4];
+                v[n] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e / 4][n][e % 4], kLog2e, b) - row.m2) * row.inv_s;
+                if (row.target == (JOB == kNarrowDw ? n_wave + n * 16 + col : at)) v[n] -= 1.f;
+                if (JOB == kNarrowDw) v[n] *= row.g;                     // dx: at the end
+                if (row.target < 0) v[n] = 0.f;                          // an ignored row's logits may be anything
+                if (JOB == kNarrowDw) sum[n] += v[n];
+            }
+            const bool live = at < a.walk32.ext && (JOB == kNarrowDx || q.target >= 0);
+#pragma unroll
+            for (int h = 0; h < HT; ++h) {
+                const int k = h * 16 + col;
+                const float f = live && k < a.hidden ? a.walk32.base[at * a.walk32.ld + k] : 0.f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) acc[h][n] = mfma32(f, v[n], acc[h][n]);
+            }
+        }
+    }
+}
+
 template <typename E, int PARTS, int HP, NarrowJob JOB>
 __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(const NarrowArgs a) {
     typedef NarrowTile<HP, PARTS> Tile;
@@ -155,7 +244,9 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
             __builtin_amdgcn_global_load_lds((glb_cvoid_t*)(reinterpret_cast<const char*>(a.bias + tile * kNarrowWalk) + lane * 4u),
                                              (lds_void16_t*)(s + Tile::kBytes), 4, 0, 0);
     };
-    if (first < last) copy(first, 0);
+    const bool wide = PARTS > 1 && (a.scales->wide[0] | a.scales->wide[1]) != 0;
+    const float lift = wide ? 1.f : a.lift;
+    if (!wide && first < last) copy(first, 0);
 
     // this lane's own entries
     RowState st[NT];
@@ -168,24 +259,20 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
     for (int n = 0; n < NT; ++n) {
         const int64_t e = n_wave + n * 16 + col;
         bool in = e < own_n;
-        st[n] = RowState{INFINITY, 0.f, 0.f, kNarrowVocab};
+        st[n] = RowState{INFINITY, 0.f, 0.f, -1};
         bias_n[n] = 0.f;
         want[n] = -1;
-        int shift = 0;
         if (JOB == kNarrowLse) {
             const int64_t t = in ? a.target[e] : -1;
-            shift = in && a.scaled ? a.shift[e] : 0;
             want[n] = t >= 0 && t < a.vocab && t != a.ignore ? (int)t : -1;
         } else if (JOB == kNarrowDx) {
             if (in) st[n] = a.state[e];
-            st[n].inv_s *= a.lift;
-            shift = shift_of(st[n].target);
-            st[n].target = target_of(st[n].target);
-            in = in && st[n].target != kNarrowVocab;               // an ignored row: operand 0, maximum +inf, so that d = 0 whatever the row holds
+            st[n].inv_s *= lift;
+            in = in && st[n].target >= 0;               // an ignored row: operand 0, maximum +inf, so that d = 0 whatever the row holds
         } else {
             bias_n[n] = in ? a.bias[e] : -INFINITY;     // d = 0
         }
-        back[n] = a.scaled ? ldexpf(kLog2e, max(min(-(a.scales->ex[0] + a.scales->ex[1] + shift), 126), -300)) : kLog2e;
+        back[n] = a.scaled ? ldexpf(kLog2e, max(min(-(a.scales->ex[0] + a.scales->ex[1]), 126), -300)) : kLog2e;
 #pragma unroll
         for (int p = 0; p < PARTS; ++p)
 #pragma unroll
@@ -210,8 +297,11 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
         for (int h = 0; h < HT; ++h) acc[h][n] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
+    if constexpr (PARTS > 1) {
+        if (wide) narrow_walk32<HT, NT, JOB>(a, first, last, n_wave, st, bias_n, want, mx, sum, own_logit, acc);
+    }
     int stage = 0;
-    for (int64_t tile = first; tile < last; ++tile, stage ^= 1) {
+    for (int64_t tile = wide ? last : first; tile < last; ++tile, stage ^= 1) {
         if (tile + 1 < last) {
             copy(tile + 1, stage ^ 1);
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Tile::kCopies + 1) : "memory");
@@ -251,37 +341,7 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
                 for (int t = 0; t < 2; ++t) bias[t] = *reinterpret_cast<const f32x4*>(s + Tile::kBytes + (mp * 32 + t * 16 + g * 4) * 4);
             }
             if (JOB == kNarrowLse) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) sc[t][n][i] = __builtin_fmaf(sc[t][n][i], back[n], bias[t][i]);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const int64_t at = want[n] - m0;
-                    if (want[n] >= 0 && at >= 0 && at < 32 && (at & 15) < 4) {
-#pragma unroll
-                        for (int t = 0; t < 2; ++t)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (at == t * 16 + i) own_logit[n] = sc[t][n][i];
-                        if (a.splits > 1) a.target_logit[n_wave + n * 16 + col] = own_logit[n];
-                    }
-                    float top = mx[n];
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[t][n][i]);
-                    const float ref = top == -INFINITY ? 0.f : top;
-                    float q = sum[n] * __builtin_amdgcn_exp2f(mx[n] - ref);
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) q += __builtin_amdgcn_exp2f(sc[t][n][i] - ref);
-                    sum[n] = q;
-                    mx[n] = top;
-                }
+                lse_step(a, sc, back, bias, m0, n_wave + col, want, mx, sum, own_logit);
                 continue;
             }
             // d, split into its parts: the second product's operand
@@ -294,28 +354,17 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
             // dw: the records of the lane's rows; target and g are read again where a target is met
             const RowState* row = reinterpret_cast<const RowState*>(s + Tile::kBytes) + mp * 32 + g * 4;
             float row_m2[8], row_scale[8];          // the row's g and the lift in its scale
-            bool shifted = false, met = false;      // rows scaled by more than the others; targets among the wave's entries: both rare
+            bool met = false;                       // targets among the wave's entries: rare
             if (JOB == kNarrowDw) {
-                int words = 0;
                 const int e0 = (int)(n_wave + col);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const RowState& q = row[(e / 4) * 16 + e % 4];
                     row_m2[e] = q.m2;
-                    row_scale[e] = q.inv_s * q.g * a.lift;
-                    words |= q.target;
+                    row_scale[e] = q.inv_s * q.g * lift;
                     met |= ((q.target - e0) & ~16) == 0;            // entry 0 or 1 of the lane's (NT = 2)
                 }
-                shifted = PARTS > 1 && __ballot(shift_of(words) != 0) != 0;
-                met = shifted || __ballot(met) != 0;
-                if (shifted) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int by = shift_of(row[(e / 4) * 16 + e % 4].target);
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) sc[e / 4][n][e % 4] = ldexpf(sc[e / 4][n][e % 4], -by);
-                    }
-                }
+                met = __ballot(met) != 0;
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -332,25 +381,21 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
                 }
                 if (JOB == kNarrowDx) {
                     const int64_t at = st[n].target - m0;
-                    if (__ballot(st[n].target != kNarrowVocab && at >= 0 && at < 32)) {
+                    if (__ballot(at >= 0 && at < 32)) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            if (at == (e / 4) * 16 + e % 4) v[e] -= a.lift;
+                            if (at == (e / 4) * 16 + e % 4) v[e] -= lift;
                     }
                 } else {
                     if (met) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const RowState& q = row[(e / 4) * 16 + e % 4];
-                            if (target_of(q.target) == (int)(n_wave + n * 16 + col)) v[e] -= q.g * a.lift;
+                            if (q.target == (int)(n_wave + n * 16 + col)) v[e] -= q.g * lift;
                         }
                     }
 #pragma unroll
                     for (int e = 0; e < 8; ++e) sum[n] += v[e];
-                    if (shifted) {                  // x's row is that much larger in the second product
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], -shift_of(row[(e / 4) * 16 + e % 4].target));
-                    }
                 }
                 vec_t<E, 8> o[PARTS];
 #pragma unroll
@@ -447,8 +492,8 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
         }
         return;
     }
-    const float down = a.scales->top / a.lift;
-    const int ex_out = a.scaled ? -a.scales->ex[JOB == kNarrowDw ? 0 : 1] : 0;
+    const float down = a.scales->top / lift;
+    const int ex_out = a.scaled && !wide ? -a.scales->ex[JOB == kNarrowDw ? 0 : 1] : 0;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int64_t e = n_wave + n * 16 + col;
@@ -494,7 +539,7 @@ static void narrow_width(NarrowJob job, const NarrowArgs& a, hipStream_t st) {
     else narrow_job<E, PARTS, 128>(job, a, st);
 }
 
-bool narrow_supported(int hidden, int vocab) { return hidden <= 128 && vocab <= kNarrowVocab; }
+bool narrow_supported(int hidden) { return hidden <= 128; }
 
 int narrow_launch(NarrowJob job, int dtype, const NarrowArgs& a, hipStream_t st) {
     if (dtype == CNF_DTYPE_F32) narrow_width<f16_t, 2>(job, a, st);

@@ -320,4 +320,51 @@ struct TileProduct {
     }
 };
 
+// ---- fp32 products on the fp32 matrix instructions -------------------------------------------------------------------------------------
+//
+// For operands that two fp16 parts do not hold: v_mfma_f32_16x16x4, an eighth of the rate, over the full range of fp32.  Fragments come
+// straight from memory in steps of 16 k (16 rows of 64 bytes each where k is contiguous), and stay in the caches between the workgroups.
+// D lies as with the 16-bit instructions; A and B hold one k of row l % 16 a lane: in instruction j of a step, k = 4 (l / 16) + j.
+
+struct Operand32 {
+    const float* base;
+    int64_t ld, ext;        // ext: rows of D (columns) that exist
+};
+__device__ __forceinline__ f32x4 mfma32(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+// elements k ... k + 3 of row (column) e: 0 where e or k is outside, or k is not live
+template <bool KMAJOR, typename Live>
+__device__ __forceinline__ void load32(const Operand32& o, int64_t e, int64_t k, int64_t k_end, Live&& live, float (&out)[4]) {
+    const bool in = e < o.ext;
+    if (!KMAJOR && in && k + 4 <= k_end) {
+        __builtin_memcpy(out, o.base + e * o.ld + k, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) out[j] = in && k + j < k_end && (!KMAJOR || live(k + j)) ? o.base[KMAJOR ? (k + j) * o.ld + e : e * o.ld + k + j] : 0.f;
+    }
+}
+
+// acc += A B over k0 <= k < k1 for this wave's rows m_wave ... and columns n_wave ...; live(k): whether k counts where A is k-major (a dead
+// one may hold anything); extra(B's elements) sees every step.  The order of the sums depends on k0 alone, and on nothing of A and B: a
+// logit has the same bits wherever it is computed
+template <bool KMA, bool KMB, int MT, int NT, typename Live, typename Extra>
+__device__ __forceinline__ void product32(const Operand32& a, const Operand32& b, int64_t m_wave, int64_t n_wave, int64_t k0, int64_t k1,
+                                          f32x4 (&acc)[MT][NT], Live&& live, Extra&& extra) {
+    const int l = threadIdx.x & 63, g = l >> 4, i = l & 15;
+    for (int64_t k = k0; k < k1; k += 16) {
+        float fa[MT][4], fb[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) load32<KMB>(b, n_wave + n * 16 + i, k + 4 * g, k1, [](int64_t) { return true; }, fb[n]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) load32<KMA>(a, m_wave + m * 16 + i, k + 4 * g, k1, live, fa[m]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) acc[m][n] = mfma32(fa[m][j], fb[n][j], acc[m][n]);
+        extra(fb);
+    }
+}
+
 }  // namespace cnf

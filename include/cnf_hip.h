@@ -647,11 +647,12 @@ int cnf_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64_t 
  * stride, `x_stride` / `w_stride` elements between rows; bias [V] of `bias_dtype` (nullable); target int64 [R].  Rows with target ==
  * ignore_index have loss 0; any other target outside [0, V) raises CNF_FLAG_CATEGORY and its loss is NaN.  row_max, row_sum [R]: the
  * maximum logit times log2(e) and sum_v exp(logit - maximum), which the backward takes; reduced [3] (nullable): mean (NaN over no rows), sum and
- * number of the rows that are not ignored; exponents [2] (nullable): the powers of two that fp32 operands were scaled by, which the
- * backward takes back instead of looking for the largest elements again.  fp32 products are exact to 2^-22 of the operands' sizes (three fp16
- * products of operands scaled by a power of two per tensor and split in two; a row of x below 2^-11 of x's largest element is scaled by
- * itself; elements of weight below 2^-16 of its largest keep 2^-39 of that), 16-bit products are exact; sums, maxima and exponentials
- * are fp32.  What ignored rows hold does not matter for the other rows; dweight wants it finite in 16 bits.  R <= 2^31 - 256,
+ * number of the rows that are not ignored; exponents [2] (nullable): the powers of two that fp32 operands were scaled by (4096 more: see
+ * below), which the backward takes back instead of looking for the largest elements again.  fp32 products are exact to 2^-22 of the largest
+ * elements of their two rows: three fp16 products of operands scaled by a power of two per tensor and split in two, or — where a row of
+ * either (zeros and ignored ones aside) is below 2^-14 of its tensor's largest element — products on the fp32 matrix instructions, two to
+ * seven times slower.  16-bit products are exact; sums, maxima and exponentials are fp32.  What ignored rows hold does not matter for the
+ * other rows; dweight wants it finite in 16 bits.  R <= 2^31 - 256,
  * V <= 2^30, H <= 2^21.  workspace_bytes >= cnf_linear_ce_workspace_bytes(R, V, H, dtype, 0). */
 int64_t cnf_linear_ce_workspace_bytes(int64_t R, int V, int H, int dtype, int backward);
 int cnf_linear_ce(const void* x, int64_t x_stride, const void* weight, int64_t w_stride, const void* bias, const int64_t* target,

@@ -1,0 +1,179 @@
+"""Linear cross entropy in fp32 where rows of x or of weight differ so much in size that two fp16 parts of a tensor scaled as a whole do not
+hold them: losses and gradients to the same tolerances as everywhere (test_gpu_linear_ce.py: fp32 products and sums stay below its count)."""
+import math
+
+import pytest
+import torch
+
+from categoricalnf_amd import functional as Fn
+from categoricalnf_amd import ops
+from tests.test_gpu_linear_ce import F32, check, make, reference, run_and_check
+
+pytestmark = pytest.mark.gpu
+
+SHAPES = [(1, 2, 3), (70, 51, 64), (200, 300, 40), (1100, 700, 64), (130, 90, 128), (150, 700, 200), (5, 3000, 264), (700, 17, 1000)]
+
+
+def spread(n, lo, hi, seed=0):
+    """n sizes from 10^lo to 10^hi in random order"""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return (10.0 ** torch.linspace(lo, hi, n, device="cuda"))[torch.randperm(n, generator=gen, device="cuda")][:, None]
+
+
+@pytest.mark.parametrize("factor", [1e3, 1e6, 1e9, 1e20])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_beside_one_large_class(shape, factor):
+    """One class with far larger weights: its probability is 0 where its logit is far below, and 1 in some rows where it is not."""
+    x, w, b, t, g = make(*shape, F32)
+    last = shape[1] - 1
+    t[t == last] = 0
+    w[last] = -w[last].abs() * factor
+    run_and_check(x.abs(), w, b, t, g)                  # never chosen
+    run_and_check(x.detach(), w.detach(), b.detach(), t, g)
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_rows_of_both_operands_of_all_sizes(shape):
+    x, w, b, t, g = make(*shape, F32)
+    run_and_check(x * spread(shape[0], -6, 3), w * spread(shape[1], -8, 1, 1), b, t, g)
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_gradients_of_small_rows_beside_large_ones(shape):
+    """dweight, too: rows that are certain of their class (d = 0) may be of any size beside the rows whose sum a class's gradient is."""
+    x, w, b, t, g = make(*shape, F32)
+    x = x * spread(shape[0], -3, 12)
+    run_and_check(x, w, b, t, g)
+
+
+@pytest.mark.parametrize("by", [12, 13, 14, 15, 16, 17, 40])
+@pytest.mark.parametrize("which", ["x", "w"])
+@pytest.mark.parametrize("shape", [(200, 300, 40), (150, 700, 200)], ids=str)
+def test_around_the_change_of_products(shape, which, by):
+    x, w, b, t, g = make(*shape, F32)
+    (x if which == "x" else w)[3] *= 2.0 ** -by
+    run_and_check(x, w, b, t, g)
+
+
+@pytest.mark.parametrize("shape", [(4100, 9000, 136), (8300, 17000, 136), (600, 9000, 1024), (3000, 9000, 100)], ids=str)
+def test_large_tiles_splits_and_pieces(shape):
+    x, w, b, t, g = make(*shape, F32)
+    run_and_check(x, w * spread(shape[1], -7, 0), b, t, g)
+
+
+@pytest.mark.parametrize("shape", [(70, 51, 64), (300, 600, 200)], ids=str)
+def test_rows_of_zeros_change_nothing(shape):
+    """A padding class without weights and rows without features are no reason for other products: the bits of the rest are the same."""
+    x, w, b, t, g = make(*shape, F32, ignored=0.0)
+    loss, grads = run_and_check(x, w, b, t, g)
+    x2, w2, b2 = torch.cat([x.detach(), x.detach()[:1] * 0]), torch.cat([w.detach(), w.detach()[:1] * 0]), torch.cat([b.detach(), b.detach()[:1] * 0 - math.inf])
+    loss2, grads2 = Fn.linear_cross_entropy(x2, w2, torch.cat([t, t[:1]]), b2, reduction="none"), None
+    assert torch.equal(loss2[:-1], loss) and torch.isfinite(loss2).all()
+
+
+@pytest.mark.parametrize("shape", [(70, 51, 64), (300, 300, 40), (300, 600, 200)], ids=str)
+def test_ignored_rows_hold_anything(shape):
+    """Beside rows of all sizes: the bits of a call whose ignored rows are zeros."""
+    x, w, b, t, g = make(*shape, F32)
+    x = x * spread(shape[0], -6, 3)
+    gone = (t == -100).nonzero()[:, 0]
+
+    def run(fills):
+        x2 = x.detach().clone()
+        for i, r in enumerate(gone.tolist()):
+            x2[r] = fills[i % len(fills)]
+        leaves = [v.detach().clone().requires_grad_() for v in (x2, w, b)]
+        loss = Fn.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], reduction="none")
+        return (loss.detach(),) + torch.autograd.grad(loss, leaves, g)
+    clean = run([0.0])
+    for a, c in zip(run([1e30, -3e38, 0.0, math.inf, math.nan]), clean):
+        assert torch.equal(a, c)
+    # ... and they are no reason for other products
+    leaves = [v.detach().clone() for v in make(*shape, F32)[:3]]
+    plain = Fn.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], reduction="none")
+    leaves[0][gone] = 1e30
+    assert torch.equal(Fn.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], reduction="none"), plain)
+
+
+@pytest.mark.parametrize("shape", [(40, 600, 24), (40, 600, 160)], ids=str)
+def test_masked_classes_and_categories_outside(shape):
+    x, w, b, t, g = make(*shape, F32, ignored=0.0)
+    x, w = x * spread(shape[0], -5, 1), w * spread(shape[1], -6, 0)
+    t[:] = torch.randint(0, 100, (shape[0],), device="cuda")
+    for low in (-math.inf, torch.finfo(F32).min):
+        b2 = b.clone()
+        b2[100:420] = low
+        leaves = [v.detach().clone().requires_grad_() for v in (x, w, b2)]
+        loss = Fn.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], reduction="none")
+        dx, dw, db = torch.autograd.grad(loss, leaves, g)
+        keep = torch.ones(shape[1], dtype=torch.bool, device="cuda")
+        keep[100:420] = False
+        val, tol = reference(x, w[keep], t, b[keep], g)
+        tol["loss"] = tol["loss"] + (shape[1] / 8) * 2.0 ** -24
+        check("loss", loss, val, tol), check("dx", dx, val, tol), check("dw", dw[keep], val, tol), check("db", db[keep], val, tol)
+        assert not dw[~keep].any() and not db[~keep].any()
+    # a masked class as the target: loss inf, gradient p - 1
+    t2, b2 = t.clone(), b.clone()
+    t2[3], b2[200], t2[5] = 200, -math.inf, shape[1]
+    t2[3] = 200
+    leaves = [v.detach().clone().requires_grad_() for v in (x, w, b2)]
+    loss = Fn.linear_cross_entropy(leaves[0], leaves[1], t2, leaves[2], reduction="none")
+    dx, dw, db = torch.autograd.grad(loss, leaves, g)
+    with pytest.raises(AssertionError):
+        ops.check_flags(x.device)
+    rest = torch.ones(shape[0], dtype=torch.bool, device="cuda")
+    rest[[3, 5]] = False
+    assert torch.isinf(loss[3]) and torch.isnan(loss[5]) and torch.isfinite(loss[rest]).all() and not dx[5].any() and torch.isfinite(dx).all()
+    assert torch.equal(db[200], -g[3]) and torch.isfinite(dw).all()
+
+
+def test_strides_and_targets_of_32_bits():
+    wide = torch.randn(6, 10, 200, device="cuda") * spread(6, -6, 2)[:, None]
+    ww = torch.randn(40, 210, device="cuda") * spread(40, -6, 0)
+    b, t, g = torch.randn(40, device="cuda"), torch.randint(0, 40, (6, 10), device="cuda"), torch.rand(60, device="cuda")
+    for H in (32, 150):
+        for x, w in ((wide[:, :, :H], ww[:, :H]), (wide[:, :, 1:H + 1], ww[:, 3:H + 3]), (wide[:, :, :H].transpose(0, 1).contiguous().transpose(0, 1), ww[:, 5:H + 5])):
+            run_and_check(x.detach(), w.detach(), b.detach(), t, g)
+        run_and_check(wide[:, :, :H].detach(), ww[:, :H].detach(), b.detach(), t.int(), g)
+
+
+@pytest.mark.parametrize("shape", [(300, 51, 64), (200, 600, 200)], ids=str)
+def test_a_captured_step_follows_its_inputs(shape):
+    """Replays with operands of all sizes and of one, in turn: each the bits of the eager call."""
+    x, w, b, t, _ = make(*shape, F32)
+    xs, ws, bs = (s.clone().requires_grad_() for s in (x, w, b))
+
+    def step(x, w, b):
+        loss = Fn.linear_cross_entropy(x, w, t, b)
+        return (loss.detach(),) + torch.autograd.grad(loss, (x, w, b))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(xs, ws, bs)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(xs, ws, bs)
+    for seed in range(1, 7):
+        x1, w1, b1, _, _ = make(*shape, F32, seed=seed)
+        if seed % 3 == 1:
+            x1 = x1 * spread(shape[0], -6, 0)
+        if seed % 3 == 2:
+            w1 = w1 * spread(shape[1], -6, 0)
+        with torch.no_grad():
+            xs.copy_(x1), ws.copy_(w1), bs.copy_(b1)
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, q in zip(out, step(x1.requires_grad_(), w1.requires_grad_(), b1.requires_grad_())):
+            assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("shape", [(70, 51, 64), (300, 300, 40), (300, 600, 200)], ids=str)
+def test_the_backward_finds_by_itself_what_the_forward_hands_over(shape):
+    for sizes in (False, True):
+        x, w, b, t, g = make(*shape, F32)
+        if sizes:
+            w = w * spread(shape[1], -9, 0)
+        loss, stats, _, exps = ops.linear_cross_entropy(x, w, t, b)
+        with_them, without = (ops.linear_cross_entropy_bwd(x, w, t, b, stats, g, exponents=e) for e in (exps, None))
+        assert all(torch.equal(p, q) for p, q in zip(with_them, without))
