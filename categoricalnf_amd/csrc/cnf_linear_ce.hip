@@ -53,6 +53,7 @@ struct CeArgs {
     void* d;                        // [parts][rows_pad][piece_ld]
     int64_t d_part, d_ld;
     int v0, v1;                     // the piece
+    int g_pass;                     // 1: d for dx, 2: for dw behind it (if g is apart), 0: for both
 };
 
 // tiles in the order that lets the workgroups of one XCD (dispatched round-robin over the 8) work on neighbouring tiles
@@ -80,6 +81,15 @@ struct NoExtra {
     __device__ __forceinline__ void operator()(const F&) const {}
 };
 __device__ __forceinline__ bool wide_rows(const CeScales* s) { return (s->wide[0] | s->wide[1]) != 0; }
+// of the backward
+__device__ __forceinline__ bool wide_call(const CeScales* s) { return (s->wide[0] | s->wide[1] | (s->wide_g == 2)) != 0; }
+// fp16 operands (bf16 has fp32's exponents): whether d comes without g for dx, and then again with it for dw, since x, which the product over
+// the rows takes as it lies, cannot carry a row's g
+template <typename E, int PARTS>
+__device__ __forceinline__ bool g_apart(const CeScales* s) {
+    if (!std::is_same<E, f16_t>::value) return false;
+    return s->wide_g != 0 && !(PARTS > 1 && wide_call(s));
+}
 
 // ---- forward ---------------------------------------------------------------------------------------------------------------------
 
@@ -303,7 +313,7 @@ struct Extent {
     uint32_t top, least;
 };
 __device__ __forceinline__ int exponent_of(uint32_t bits) { return max((int)(bits >> 23), 1) - 127; }       // subnormal numbers: as if of -126
-__device__ __forceinline__ bool is_wide(Extent e) { return e.least != 0xffffffffu && exponent_of(e.top) - exponent_of(e.least) > kRowSpan; }
+__device__ __forceinline__ bool is_wide(Extent e, int span) { return e.least != 0xffffffffu && exponent_of(e.top) - exponent_of(e.least) > span; }
 
 // what this lane's rows say, of fp32 rows `block`, `block` + `blocks`, ... (in units of the rows that a workgroup's lanes share at a time);
 // rows with target == ignore do not count (target: nullable).  At most a wave shares a row; four rows are in flight
@@ -425,7 +435,7 @@ __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
             const Extent e = block_extent(a.extents ? a.extents[which * kMaxBlocks + threadIdx.x]
                                                     : extent_of(reinterpret_cast<const float*>(src), job.stride, job.rows, a.cols,
                                                                 which ? nullptr : a.target, a.ignore, 0, 1), sh);
-            wide = is_wide(e);
+            wide = is_wide(e, kRowSpan);
             ex = e.top ? 14 - exponent_of(e.top) : 0;           // the largest into 2^14 ... 2^15; zeros alone stay as they are
         }
         if (blockIdx.x == 0 && threadIdx.x == 0) {
@@ -468,26 +478,33 @@ __global__ __launch_bounds__(kBlock) void ce_layout_kernel(const LayoutArgs a) {
 // upstream gradients (per row, or one over the count) -> row records, ignored ones behind the last row up to rows_pad.  Every g is
 // divided by the largest |g|, which goes to scales
 __global__ __launch_bounds__(1024) void ce_rows_kernel(const float* g, int g_is_row, const float* count, const float* row_max, const float* row_sum,
-                                                       const int64_t* target, int64_t ignore, int vocab, int64_t rows, int64_t rows_pad,
+                                                       const int64_t* target, int64_t ignore, int vocab, int64_t rows, int64_t rows_pad, GradSpan span,
                                                        RowState* state, CeScales* scales) {
-    __shared__ uint32_t sh[16];
+    __shared__ Extent sh[16];
     const float shared = g_is_row ? 0.f : *g / *count;
-    uint32_t bits = __float_as_uint(shared) & 0x7fffffffu;
+    auto counts = [&](int64_t t) { return t != ignore && t >= 0 && t < vocab; };
+    Extent e = {__float_as_uint(shared) & 0x7fffffffu, 0xffffffffu};
     if (g_is_row) {
         for (int64_t r = threadIdx.x; r < rows; r += 1024)
-            if (target[r] != ignore) bits = max(bits, __float_as_uint(g[r]) & 0x7fffffffu);
-#pragma unroll
-        for (int m = 32; m >= 1; m >>= 1) bits = max(bits, (uint32_t)__shfl_xor((int)bits, m, kWave));
-        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = bits;
-        __syncthreads();
-        for (int w = 0; w < 16; ++w) bits = max(bits, sh[w]);
+            if (counts(target[r])) {
+                const uint32_t bits = __float_as_uint(g[r]) & 0x7fffffffu;
+                e.top = max(e.top, bits);
+                if (bits) e.least = min(e.least, bits);
+            }
+        e = block_extent(e, sh);
     }
+    // an infinite or NaN one among them: the others are any distance from it
+    const bool finite = e.top < 0x7f800000u;
+    const int wide = !g_is_row ? 0 : (!finite || is_wide(e, span.plain) ? 2 : (is_wide(e, span.apart) ? 1 : 0));
     // all gradients zero, or an infinite or NaN one among them: as they are
-    const float top = bits != 0 && bits < 0x7f800000u ? __uint_as_float(bits) : 1.f;
-    if (threadIdx.x == 0 && blockIdx.x == 0) scales->top = top;
+    const float top = e.top != 0 && finite ? __uint_as_float(e.top) : 1.f;
+    if (threadIdx.x == 0 && blockIdx.x == 0) {
+        scales->top = top;
+        scales->wide_g = wide;
+    }
     for (int64_t r = (int64_t)blockIdx.x * 1024 + threadIdx.x; r < rows_pad; r += (int64_t)gridDim.x * 1024) {
         const int64_t t = r < rows ? target[r] : -1;
-        const bool in = r < rows && t != ignore && t >= 0 && t < vocab;
+        const bool in = r < rows && counts(t);
         RowState s;
         s.m2 = in ? row_max[r] : INFINITY;
         s.inv_s = in ? 1.f / row_sum[r] : 0.f;
@@ -520,7 +537,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
         tile.begin(v0, r0, 0, a.k_end);
     };
     if constexpr (PARTS > 1) {
-        if (wide_rows(a.scales)) {
+        if (wide_call(a.scales)) {
+            if (a.g_pass == 2) return;
             // fp32 products, and d in fp32 where its two parts would be: [rows_pad][piece_ld]
             for (; t < end; t += step) {
                 unsigned ti, tj;
@@ -553,6 +571,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
             return;
         }
     }
+    const bool apart = a.g_pass != 0 && g_apart<E, PARTS>(a.scales), without_g = apart && a.g_pass == 1;
+    if (a.g_pass == 2 && !apart) return;
     const float back = logit_scale(a);
     if (t < end) begin();
     while (t < end) {
@@ -573,7 +593,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
 #pragma unroll
         for (int n = 0; n < Tile::NT; ++n) {
             st[n] = rw + n * 16 < a.rows ? a.state[rw + n * 16] : RowState{INFINITY, 0.f, 0.f, -1};
-            own_g[n] = st[n].g * a.lift;
+            own_g[n] = without_g ? a.lift : st[n].g * a.lift;
             scale[n] = st[n].inv_s * own_g[n];
             at[n] = st[n].target - vw;
             hit |= st[n].target >= 0 && at[n] >= 0 && at[n] < Tile::MT * 16;
@@ -645,7 +665,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
 struct GradArgs {
     Operand a, b;           // D[m = hidden][n = row or vocabulary entry]
     Operand32 a32, b32;     // wide operands: the tensor itself, and d in fp32
-    const RowState* state;  // over the rows: which of them count (null: over the vocabulary)
+    const RowState* state;  // over the rows: which of them count; over the vocabulary: their g, where it may be apart, or null
     int pairs, k_end, ksplit;
     int m_end, n_end;       // extent of the output
     void* out;              // final: [n][ld] of the output type; partial: fp32 [ksplit][n][ld]
@@ -683,7 +703,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_grad_kernel(const GradArgs
     s16x8 ones;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ones[i] = __builtin_bit_cast(short, (E)1.f);
-    const bool wide = PARTS > 1 && wide_rows(a.scales);
+    const bool wide = PARTS > 1 && wide_call(a.scales);
     if (wide) {
         product32<true, KMB>(a.a32, a.b32, m0 + tile.m_wave, (int64_t)n0 + tile.n_wave, k0, k1, acc, [&](int64_t k) { return !KMB || a.state[k].target >= 0; },
                              [&](const float (&fb)[Tile::NT][4]) {
@@ -706,12 +726,15 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void ce_grad_kernel(const GradArgs
         });
     }
     const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
-    const float down = wide ? a.scales->top : a.scales->top / a.lift;
+    const bool apart = !KMB && a.state && g_apart<E, PARTS>(a.scales);
+    const float all_down = wide ? a.scales->top : a.scales->top / a.lift;
     const int ex = a.scaled && !wide ? -a.scales->ex[a.scaled - 1] : 0;
 #pragma unroll
     for (int n = 0; n < Tile::NT; ++n) {
         const int64_t row = (int64_t)n0 + tile.n_wave + n * 16 + col;
         if (row >= a.n_end) continue;
+        float down = all_down;
+        if (!KMB && apart) down *= a.state[row].g;
 #pragma unroll
         for (int m = 0; m < Tile::MT; ++m) {
             const int h = m0 + tile.m_wave + m * 16 + g * 4;
@@ -1084,7 +1107,7 @@ int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64
         a.state = state;
         // per-row gradients: every workgroup finds the largest |g| itself; few of them
         CNF_LAUNCH(ce_rows_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(p.rows_pad, 1024), g_per_row ? 16 : 1024)), dim3(1024), 0, st, g,
-                   g_per_row, count, row_max, row_sum, target, ignore_index, V, R, p.rows_pad, state,
+                   g_per_row, count, row_max, row_sum, target, ignore_index, V, R, p.rows_pad, PARTS > 1 ? kGradSpan32 : kGradSpan16, state,
                    reinterpret_cast<CeScales*>(ws + p.scales_off));
         const int64_t ld4 = round_up(H, 4);
         if (p.narrow) {
@@ -1122,8 +1145,13 @@ int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64
             a.v1 = (int)v1;
             const int edge = p.big_d ? kBig : kSmall;
             const unsigned d_grid = (unsigned)std::min<int64_t>(ceil_div(width, edge) * ceil_div(R, edge), p.big_d ? 256 : 512);
-            if (p.big_d) CNF_LAUNCH((ce_d_kernel<E, PARTS, kBig, kBig, 2, 4>), dim3(d_grid), dim3(512), 0, st, a);
-            else CNF_LAUNCH((ce_d_kernel<E, PARTS, kSmall, kSmall, 2, 2>), dim3(d_grid), dim3(256), 0, st, a);
+            auto logit_gradient = [&](int pass) {
+                a.g_pass = pass;
+                if (p.big_d) CNF_LAUNCH((ce_d_kernel<E, PARTS, kBig, kBig, 2, 4>), dim3(d_grid), dim3(512), 0, st, a);
+                else CNF_LAUNCH((ce_d_kernel<E, PARTS, kSmall, kSmall, 2, 2>), dim3(d_grid), dim3(256), 0, st, a);
+            };
+            const bool may_part = std::is_same<E, f16_t>::value && g_per_row && dx;
+            logit_gradient(may_part ? 1 : 0);
             const Operand d{a.d, a.d_ld, a.d_part, 0};
             GradArgs q{};
             q.pairs = p.pairs;
@@ -1152,8 +1180,10 @@ int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64
                 else if (big) CNF_LAUNCH((ce_grad_kernel<E, PARTS, false, kBig, kBig, 2, 4>), grid, dim3(512), 0, st, q);
                 else CNF_LAUNCH((ce_grad_kernel<E, PARTS, false, kSmall, kSmall, 2, 2>), grid, dim3(256), 0, st, q);
             };
+            q.state = may_part ? state : nullptr;
             if (dx) grad(false, p.big_dx, R);
             if (!dweight) continue;
+            if (may_part) logit_gradient(2);
             // dw[v][h] = sum_r x[r][h] d[r][v]; db[v] = sum_r d[r][v]
             char* dw = static_cast<char*>(dweight) + v0 * H * dtype_bytes(dtype);
             char* db = dbias ? static_cast<char*>(dbias) + v0 * dtype_bytes(bias_dtype) : nullptr;

@@ -17,13 +17,21 @@ struct RowState {       // backward: what an element d = (exp2(l2 - m2) inv_s - 
 // largest of the rest.  An operand with a row whose largest element is below 2^-kRowSpan of the tensor's is "wide": its call takes the fp32
 // matrix instructions (product32), so that no row's results depend on the size of the others.
 constexpr int kRowSpan = 14;
+// The gradient of the logits in fp16 (one part or two) is kept to 2^-39 of the largest |g|.  Where a row's |g| is that many powers of two
+// below the largest, more than `apart`, its dx would be short of bits: dx applies g behind its product then; further than `plain` below
+// (or beside an infinite or NaN g), fp32 operands take fp32 products, so that also a class that only such rows have gets its dw.
+struct GradSpan {
+    int apart, plain;
+};
+constexpr GradSpan kGradSpan32 = {12, 24}, kGradSpan16 = {18, 18};
 constexpr int kWideMark = 4096;         // in an exponent that the forward hands to the backward: the operand is wide
 
 // what the operands of a call were scaled by; in device memory
 struct CeScales {
     int ex[2];          // fp32: x was multiplied by 2^ex[0], w by 2^ex[1]
     int wide[2];        // fp32: whether x, w are wide
-    float top;          // largest |g|
+    float top;          // largest |g|, or 1
+    int wide_g;         // the rows' g: 0, 1: apart, 2: plain
 };
 
 constexpr int kNarrowOwn = 128;         // rows (or vocabulary entries) of a workgroup

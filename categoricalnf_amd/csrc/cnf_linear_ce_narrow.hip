@@ -244,7 +244,8 @@ __global__ __launch_bounds__(kBlock, HP <= 64 ? 3 : 2) void ce_narrow_kernel(con
             __builtin_amdgcn_global_load_lds((glb_cvoid_t*)(reinterpret_cast<const char*>(a.bias + tile * kNarrowWalk) + lane * 4u),
                                              (lds_void16_t*)(s + Tile::kBytes), 4, 0, 0);
     };
-    const bool wide = PARTS > 1 && (a.scales->wide[0] | a.scales->wide[1]) != 0;
+    // (dx applies g at its end)
+    const bool wide = PARTS > 1 && (a.scales->wide[0] | a.scales->wide[1] | (JOB == kNarrowDw && a.scales->wide_g == 2)) != 0;
     const float lift = wide ? 1.f : a.lift;
     if (!wide && first < last) copy(first, 0);
 

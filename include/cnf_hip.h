@@ -661,7 +661,10 @@ int cnf_linear_ce(const void* x, int64_t x_stride, const void* weight, int64_t w
 /* Its gradients (exponents: the forward's, or NULL): dx [R, H], dweight [V, H] dense of `dtype`, dbias [V] of `bias_dtype` (each nullable; dbias needs dweight) for the
  * upstream gradient g: fp32 [R] (g_per_row != 0), or one value that is divided by *count (the mean's).  Ignored rows and rows with a
  * target outside the vocabulary have gradient 0.  The gradient of the logits is computed in pieces of the vocabulary and rounded to
- * `dtype` (fp32: to 2^-22), relative to the largest |g|; sums are fp32, in a fixed order.  workspace_bytes >= cnf_linear_ce_workspace_bytes(..., 1). */
+ * `dtype` (fp32: to 2^-22); what dx takes of it is also kept to 2^-27 of the row's own |g| in fp32 and 2^-21 in
+ * fp16, what dweight and dbias take to 2^-39 of the largest |g|, and to 2^-15 of the row's own in fp32.  (A |g| below 2^-12 of the largest in fp32, 2^-18 in fp16, zeros aside, costs a
+ * second pass over the logits where H > 128; below 2^-24 in fp32 the fp32 matrix instructions.)  Sums are fp32, in a fixed order.
+ * workspace_bytes >= cnf_linear_ce_workspace_bytes(..., 1). */
 int cnf_linear_ce_bwd(const void* x, int64_t x_stride, const void* weight, int64_t w_stride, const void* bias, const int64_t* target,
                       int64_t ignore_index, const float* row_max, const float* row_sum, const int* exponents, const float* g,
                       int g_per_row, const float* count, void* dx, void* dweight, void* dbias, void* workspace, int64_t workspace_bytes, int64_t R, int V, int H, int dtype,

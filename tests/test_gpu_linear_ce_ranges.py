@@ -7,7 +7,7 @@ import torch
 
 from categoricalnf_amd import functional as Fn
 from categoricalnf_amd import ops
-from tests.test_gpu_linear_ce import F32, check, make, reference, run_and_check
+from tests.test_gpu_linear_ce import BF16, F16, F32, check, half_step, make, reference, run_and_check
 
 pytestmark = pytest.mark.gpu
 
@@ -177,3 +177,81 @@ def test_the_backward_finds_by_itself_what_the_forward_hands_over(shape):
         loss, stats, _, exps = ops.linear_cross_entropy(x, w, t, b)
         with_them, without = (ops.linear_cross_entropy_bwd(x, w, t, b, stats, g, exponents=e) for e in (exps, None))
         assert all(torch.equal(p, q) for p, q in zip(with_them, without))
+
+
+def check_dx_by_rows(x, w, b, t, g):
+    """dx of each row against its own g alone: the tolerance of g = 1, times g, and the quotient's and the product's rounding.  dw and db take
+    d g as two fp16 parts after a scaling that brings the largest |g| to 2^14: the second part's smallest step there is 2^-24, so that an
+    element is off by at most 2^-25 2^-14 max |g| more, times |x| (a sum of which counts where a class's own gradients are that small)."""
+    leaves = [v.detach().clone().requires_grad_() for v in (x, w, b)]
+    loss = Fn.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], reduction="none")
+    dx, dw, db = torch.autograd.grad(loss, leaves, g)
+    (alone,) = torch.autograd.grad(Fn.linear_cross_entropy(leaves[0], w, t, b, reduction="none"), leaves[0], g)
+    assert torch.equal(dx, alone)                       # whether the other gradients are asked for or not
+    val, tol = reference(x, w, t, b, torch.ones_like(g))
+    check("dx", dx, {"dx": val["dx"] * g.double()[:, None]}, {"dx": g.double()[:, None] * (tol["dx"] + 4 * 2.0 ** -24 * val["dx"].abs())})
+    val, tol = reference(x, w, t, b, g)
+    if x.dtype == F32:
+        live = (t != -100).double() * 2.0 ** -39 * float(g.max())
+        tol["dw"], tol["db"] = tol["dw"] + (live[:, None] * x.detach().double().abs()).sum(0), tol["db"] + live.sum()
+    check("dw", dw, val, tol), check("db", db, val, tol)
+    return dx, dw, db
+
+
+GRADS = [(300, 700, 200), (150, 90, 40), (1100, 51, 64), (3, 5000, 264), (600, 9000, 1024)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("shape", GRADS, ids=str)
+def test_upstream_gradients_of_all_sizes(shape, dtype):
+    """A row's dx does not depend on the other rows' gradients.  fp16: sizes at which dx is not yet below that type's normal numbers."""
+    x, w, b, t, _ = make(*shape, dtype)
+    g = spread(shape[0], -12, 0)[:, 0] if dtype != F16 else 1e4 * spread(shape[0], -9, 0)[:, 0]
+    check_dx_by_rows(x, w, b, t, g)
+    g = g * torch.where(torch.arange(shape[0], device="cuda") % 5 == 1, 0.0, 1.0)         # zeros are no reason for anything
+    check_dx_by_rows(x, w, b, t, g)
+
+
+@pytest.mark.parametrize("by", [11, 12, 13, 14, 17, 18, 19, 20, 23, 24, 25, 26, 40])
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("shape", [(300, 700, 200), (150, 90, 40)], ids=str)
+def test_around_the_change_of_gradients(shape, dtype, by):
+    x, w, b, t, g = make(*shape, dtype)
+    g[2] = 2.0 ** -by
+    g[3] = 1.0
+    t[2:4] = torch.tensor([5, 7], device="cuda")
+    check_dx_by_rows(x, w, b, t, 512 * g)
+
+
+def test_two_pieces_with_gradients_of_all_sizes():
+    for dtype, rows in ((F16, 16500), (F32, 8300)):
+        x, w, b, t, _ = make(rows, 17000, 136, dtype)
+        check_dx_by_rows(x, w, b, t, 100 * spread(rows, -6, 0)[:, 0])
+
+
+@pytest.mark.parametrize("shape", [(300, 700, 200), (150, 90, 40)], ids=str)
+def test_gradients_of_classes_that_only_rows_of_small_g_have(shape):
+    """A class's dweight where the other rows are certain of another one (their p is 0): the sum of the small rows', not of nothing."""
+    x, w, b, t, g = make(*shape, F32, ignored=0.0)
+    x = x.abs()
+    w[0] = 300.0                                        # rows of the first half are certain of class 0, the others of not
+    half = shape[0] // 2
+    x[half:] *= -1
+    t[:half], g[half:] = 0, g[half:] * 1e-11
+    t[half:] = 1 + t[half:] % (shape[1] - 1)
+    run_and_check(x, w, b, t, g)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_one_gradient_that_is_not_finite(dtype):
+    x, w, b, t, g = make(40, 300, 200, dtype, ignored=0.0)
+    # (two runs' difference is no bound: each rounds its d, and a sum's terms cancel; the reference's tolerance counts both)
+    val, tol = reference(x, w, t, b, g * 1e-3)
+    x.requires_grad_()
+    for bad in (math.inf, math.nan):
+        g2 = g * 1e-3
+        g2[7] = bad
+        (dx,) = torch.autograd.grad(Fn.linear_cross_entropy(x, w, t, b, reduction="none"), x, g2)
+        assert not torch.isfinite(dx[7]).any()
+        rest = torch.arange(40, device="cuda") != 7
+        check("dx", dx[rest], {"dx": val["dx"][rest]}, {"dx": tol["dx"][rest]})
