@@ -255,3 +255,18 @@ def test_one_gradient_that_is_not_finite(dtype):
         assert not torch.isfinite(dx[7]).any()
         rest = torch.arange(40, device="cuda") != 7
         check("dx", dx[rest], {"dx": val["dx"][rest]}, {"dx": tol["dx"][rest]})
+
+
+def test_the_largest_and_the_smallest_numbers():
+    """Operands at both ends of fp32: x the largest numbers, weights around 2^-126 (partly subnormal), logits up to 163.  Scaled by a power of
+    two they are ordinary numbers, split in two fp16 parts: the tolerances of everywhere, 128 2^-24 of the sum of |x w| here (1.2e-3 at a
+    logit of 163; a kernel that dropped the second part would be off by 163 2^-12 = 0.04)."""
+    big = torch.full((4, 8), torch.finfo(F32).max, device="cuda")
+    small = torch.full((6, 8), 1e-38, device="cuda") * torch.arange(1, 7, device="cuda")[:, None]
+    for signs in (torch.ones(8, device="cuda"), torch.tensor([1, -1, 1, 1, -1, 1, -1, 1], device="cuda")):
+        for x, w, t in ((big * signs, small.clone(), [0, 5, 2, -100]), (small.clone(), (big * signs)[:2].clone(), [0, 1, 0, 1, -100, 0])):
+            t, b = torch.tensor(t, device="cuda"), torch.zeros(len(w), device="cuda")
+            g = torch.full((len(x),), 2.0 ** -4, device="cuda")
+            val, tol = reference(x, w, t, b, g)
+            check("loss", Fn.linear_cross_entropy(x, w, t, b, reduction="none"), val, tol)
+            check_dx_by_rows(x, w, b, t, g)             # classes of p = exp(-100) beside others: dw is held to 2^-39 of the largest |g| |x|
