@@ -781,7 +781,7 @@ def transformed():
     """Whether the calls of this thread are recorded, rewritten or carry more than values: torch.jit.trace, torch.compile, make_fx and every
     other dispatch mode, torch.func transforms, forward-mode derivatives.  Kernels that fill their outputs through pointers know nothing of it: modules take
     torch's operators instead."""
-    return (torch._C._get_tracing_state() is not None or torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+    return (torch.compiler.is_compiling() or torch._C._get_tracing_state() is not None or torch._C._len_torch_dispatch_stack() > 0
             or torch._C._functorch.peek_interpreter_stack() is not None or torch.autograd.forward_ad._current_level >= 0)
 
 

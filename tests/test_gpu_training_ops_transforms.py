@@ -102,3 +102,15 @@ def test_second_derivatives_in_16_bits_keep_the_types():
     assert all(a.dtype == torch.bfloat16 for a in g)
     h = torch.autograd.grad(sum(a.float().square().sum() for a in g), [x, m.weight])
     assert all(a.dtype == torch.bfloat16 and bool(torch.isfinite(a).all()) for a in h)
+
+
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_compiled_norm_is_one_graph(backend):
+    mine, ref, x = pair()
+    torch._dynamo.reset()
+    compiled = torch.compile(mine, backend=backend, fullgraph=True)
+    xs = [x.clone().requires_grad_() for _ in range(2)]
+    got, want = compiled(xs[0]), ref(xs[1])
+    assert torch.equal(got, want)
+    got.square().sum().backward(), want.square().sum().backward()
+    assert torch.equal(xs[0].grad, xs[1].grad) and torch.equal(mine.weight.grad, ref.weight.grad)

@@ -86,3 +86,10 @@ def test_function_transforms_are_refused(name):
             transform(call)(x.clone())
     with pytest.raises(NotImplementedError, match="torch.func"):
         torch.func.vmap(lambda v: ops.adamw_step([v], [v], [v], [v], step=1, lr=0.1) or v)(X)
+
+
+def test_modules_see_a_compilation():
+    def f(x):
+        return x + 1 if Fn.transformed() else x - 1
+    torch._dynamo.reset()
+    assert torch.equal(torch.compile(f, backend="eager", fullgraph=True)(X), X + 1) and torch.equal(f(X), X - 1)
