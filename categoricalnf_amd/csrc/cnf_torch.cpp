@@ -469,6 +469,7 @@ void adamw_step(const py::object& params, const py::object& grads, const py::obj
 
 PYBIND11_MODULE(_cnf_torch, m) {
     m.def("bind", &bind);
+    m.def("refuse_transforms", [](const std::string& name) { refuse_transforms(name.c_str()); });
     m.def("layer_norm", &layer_norm);
     m.def("layer_norm_raw", [](const Tensor& x, const std::optional<Tensor>& w, const std::optional<Tensor>& b, double eps, bool stats) {
         return layer_norm_raw(x, opt(w), opt(b), eps, stats);

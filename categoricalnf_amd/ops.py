@@ -1086,6 +1086,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, beta1=0.9, bet
 
 def adamw_moments(exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale):
     """(m, v) in fp32: the values that a tensor's 8-bit moments stand for."""
+    native().refuse_transforms("adamw_moments")
     dev = _dev(exp_avg)
     n = exp_avg.numel()
     for t, dt, k, name in ((exp_avg, torch.int8, n, "exp_avg"), (exp_avg_sq, torch.uint8, n, "exp_avg_sq"),

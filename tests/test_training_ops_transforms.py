@@ -15,6 +15,7 @@ CALLS = {
     "ops.layer_norm": lambda x: ops.layer_norm(x),
     "ops.layer_norm_bwd": lambda x: ops.layer_norm_bwd(x, x, None, x[:, 0], x[:, 0])[0],
     "ops.linear_cross_entropy_bwd": lambda x: ops.linear_cross_entropy_bwd(x, W, T, None, x[:2, :3], x[0, :3])[0],
+    "ops.adamw_moments": lambda x: ops.adamw_moments(x, x, x, x)[0],
     "ops.adamw_step": lambda x: ops.adamw_step([x], [x], [x], [x], step=1, lr=0.1) or x,
 }
 
@@ -45,7 +46,7 @@ def test_modules_see_a_recording():
 
 
 CE = lambda x, w, b: ops.native().linear_ce(x, w, T, b, -100, 1, torch.zeros(1, dtype=torch.int32))
-TANGENTS = {**{k: (f, X) for k, f in CALLS.items() if k != "ops.adamw_step"}, "layer_norm, bias": (lambda b: Fn.layer_norm(X, None, b), X[0]),
+TANGENTS = {**{k: (f, X) for k, f in CALLS.items() if not k.startswith("ops.adamw")}, "layer_norm, bias": (lambda b: Fn.layer_norm(X, None, b), X[0]),
             "linear_cross_entropy": (lambda x: CE(x, W, None), X), "linear_cross_entropy, weight": (lambda w: CE(X, w, None), W),
             "linear_cross_entropy, bias": (lambda b: CE(X, W, b), W[:, 0].contiguous())}
 
