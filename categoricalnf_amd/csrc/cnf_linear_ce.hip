@@ -12,7 +12,7 @@
 // the piece.  db comes out of the second product: a fragment of ones in place of x.
 //
 // Bound by the matrix cores and, running one after the other without a pause, by the card's power: 8192 x 32000 x 1024 bf16, 537 GF each:
-// forward 580 us (925 TF), d 640 us (840 TF; 525 MB written beside it), dw 517 us (1040 TF), dx 495 us (1085 TF); the library's 8192^3
+// forward 587 us (915 TF), d 632 us (850 TF; 525 MB written beside it), dw 515 us (1043 TF), dx 494 us (1087 TF); the library's 8192^3
 // product reaches 1236 TF.  256 x 256 tiles read an operand from LDS half as often as 128 x 128 ones (d: 340 us a half against 421);
 // those are kept for sizes whose large tiles would leave CUs empty.
 //
@@ -21,7 +21,7 @@
 // fp32 inputs are scaled by a power of two per tensor and split once into two fp16 parts (cnf_mfma.h: pair_a): three fp16 products keep
 // every product to 2^-22 of its rows' largest elements, and the matrix cores do them at 16 times the fp32 rate.  Tensors with rows below
 // 2^-14 of the largest element ("wide", kRowSpan) take fp32 matrix instructions instead, found on the device, in the same kernels and
-// order.  16-bit inputs whose rows are not 16-byte aligned are copied once into padded rows.
+// order: 8192 x 32000 x 1024 fp32 forward 1.50 ms (1070 TF of fp16 products), wide 7.45 ms (72 TF of fp32 ones, whose peak is 157).  16-bit inputs whose rows are not 16-byte aligned are copied once into padded rows.
 // d is computed for g_r / max |g| (for fp16 operands times 2^14, so that small probabilities keep their bits) and the results are scaled
 // back: under a mean every row's -1 is then exact, where a rounded -g_r would put the same relative error on every row's largest entry.
 #include <algorithm>
@@ -515,8 +515,8 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(const float* g, int g_is_
 }
 
 // d, a few tiles per workgroup (as many workgroups as run at once), so that a tile's first copies land during the epilogue of the one
-// before; D[m = vocabulary][n = row].  An XCD's workgroups share one run of tiles.  8192 x 32000 x 1024 bf16: 726 -> 682 us (790 TF) with
-// the copies ahead and 16-byte stores
+// before; D[m = vocabulary][n = row].  An XCD's workgroups share one run of tiles.  8192 x 32000 x 1024 bf16: 632 us (850 TF); the copies
+// ahead and the 16-byte stores together took 6 % off (726 -> 682 us, measured alone)
 template <typename E, int PARTS, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 2) void ce_d_kernel(const CeArgs a) {
     typedef TileProduct<E, false, false, BM, BN, WM, WN> Tile;

@@ -15,11 +15,14 @@ struct RowState {       // backward: what an element d = (exp2(l2 - m2) inv_s - 
 
 // Two fp16 parts of an operand scaled by one power of two hold 22 bits of what is above 2^-16 of its largest element, and 2^-39 of that
 // largest of the rest.  An operand with a row whose largest element is below 2^-kRowSpan of the tensor's is "wide": its call takes the fp32
-// matrix instructions (product32), so that no row's results depend on the size of the others.
+// matrix instructions (product32), so that no row's results depend on the size of the others.  14: a row at the border still has its
+// 22 bits, and two are left for the sums over a vocabulary in which it alone has any probability.
 constexpr int kRowSpan = 14;
 // The gradient of the logits in fp16 (one part or two) is kept to 2^-39 of the largest |g|.  Where a row's |g| is that many powers of two
 // below the largest, more than `apart`, its dx would be short of bits: dx applies g behind its product then; further than `plain` below
-// (or beside an infinite or NaN g), fp32 operands take fp32 products, so that also a class that only such rows have gets its dw.
+// (or beside an infinite or NaN g), fp32 operands take fp32 products, so that also a class that only such rows have gets its dw.  fp32:
+// 2^-39 of the largest is 2^-27 of a row at `apart`, 2^-15 at `plain`; fp16: 2^-21 at 18, a few bits below d's own rounding.  The second pass
+// over the logits takes 260 us of 1034 at 8192 x 8000 x 512 in fp32.
 struct GradSpan {
     int apart, plain;
 };

@@ -787,7 +787,8 @@ def transformed():
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, twice=False):
     """Layer norm over the last axis (`ops.layer_norm`), differentiable in x, weight and bias: once, or with `twice` any number of times
-    (a backward under create_graph is then made of torch's operators instead of the kernel)."""
+    (a backward under create_graph is then made of torch's operators instead of the kernel).  A recorded, transformed or forward-mode call
+    raises (`transformed`)."""
     return ops.native().layer_norm(x, weight, bias, eps, twice)
 
 
@@ -797,7 +798,8 @@ _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduction="mean"):
     """Softmax cross entropy of x @ weight.T + bias against integer targets without keeping the logits (`ops.linear_cross_entropy`),
     differentiable (once) in x, weight and bias.  reduction: "mean" over the rows that are not ignored (NaN if there are none), "sum",
-    or "none" (fp32 losses of target's shape; ignored rows 0)."""
+    or "none" (fp32 losses of target's shape; ignored rows 0).  As of `layer_norm`, a recorded, transformed or forward-mode call raises
+    (`transformed`)."""
     if reduction not in _REDUCTIONS:
         raise ValueError("reduction is mean, sum or none, got %r" % (reduction,))
     loss = ops.native().linear_ce(x, weight, target, bias, ignore_index, _REDUCTIONS[reduction], ops.flag_word(ops._dev(x)))
