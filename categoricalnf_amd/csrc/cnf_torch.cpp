@@ -186,7 +186,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd_raw(const Tensor& x, const Ten
     return {dx, dw, db};
 }
 
-// the gradients as operators that autograd knows, for a backward that is differentiated itself
+// the gradients as operators that autograd knows, for a backward that is differentiated itself, batched or given a tangent
 variable_list layer_norm_bwd_composed(const Tensor& x, const Tensor& dy, const Tensor& weight, at::ScalarType pdtype, double eps, bool want_weight,
                                       bool want_bias) {
     const Tensor xf = x.to(at::kFloat), g = dy.to(at::kFloat), gw = weight.defined() ? g * weight.to(at::kFloat) : g;
@@ -213,7 +213,8 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
         const auto pdtype = (at::ScalarType)ctx->saved_data["dtype"].toInt();
         const bool want_weight = s[1].defined() && ctx->needs_input_grad(1);
         const bool want_bias = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(s[1].defined() ? 2 : 1);
-        if (at::GradMode::is_enabled() && ctx->saved_data["twice"].toBool())
+        // (batched gradients are wrappers without memory of their own)
+        if (ctx->saved_data["twice"].toBool() && (at::GradMode::is_enabled() || !g[0].has_storage() || g[0]._fw_grad(0).defined()))
             return layer_norm_bwd_composed(s[0], g[0], s[1], pdtype, ctx->saved_data["eps"].toDouble(), want_weight, want_bias);
         auto [dx, dw, db] = layer_norm_bwd_raw(s[0], g[0], s[1], s[2], s[3], pdtype, want_weight, want_bias);
         return once({dx, dw, db, Tensor(), Tensor()});

@@ -787,7 +787,7 @@ def transformed():
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, twice=False):
     """Layer norm over the last axis (`ops.layer_norm`), differentiable in x, weight and bias: once, or with `twice` any number of times
-    (a backward under create_graph is then made of torch's operators instead of the kernel).  A recorded, transformed or forward-mode call
+    (a backward under create_graph, or of batched gradients, is then made of torch's operators instead of the kernel).  A recorded, transformed or forward-mode call
     raises (`transformed`)."""
     return ops.native().layer_norm(x, weight, bias, eps, twice)
 

@@ -114,3 +114,37 @@ def test_compiled_norm_is_one_graph(backend):
     assert torch.equal(got, want)
     got.square().sum().backward(), want.square().sum().backward()
     assert torch.equal(xs[0].grad, xs[1].grad) and torch.equal(mine.weight.grad, ref.weight.grad)
+
+
+def test_batched_gradients_of_the_norm():
+    """Several upstream gradients at once: each one's gradients as they come alone from torch's norm (the operators of the composed
+    backward: the bound of test_second_derivatives_of_the_norm for one derivative)."""
+    mine, ref, x = pair()
+    u = torch.randn(3, 5, 24, device="cuda")
+    ref.double()
+    wrt = lambda m, v: [v] + list(m.parameters())
+    xg, xr = x.clone().requires_grad_(), x.double().requires_grad_()
+    got = torch.autograd.grad(mine(xg), wrt(mine, xg), u, is_grads_batched=True)
+    for k in range(3):
+        want = torch.autograd.grad(ref(xr), wrt(ref, xr), u[k].double())
+        for a, b in zip(got, want):
+            assert float((a[k].double() - b).abs().max()) <= 150 * 2.0 ** -24 * 16 * float(b.abs().max())
+    j = torch.autograd.functional.jacobian(lambda v: mine(v).sum(0), x, vectorize=True)
+    r = torch.autograd.functional.jacobian(lambda v: ref(v).sum(0), x.double())
+    assert float((j.double() - r).abs().max()) <= 150 * 2.0 ** -24 * 16 * float(r.abs().max())
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(Fn.layer_norm(xg), xg, u, is_grads_batched=True)
+
+
+def test_tangents_of_the_upstream_gradient():
+    mine, ref, x = pair()
+    u, t = torch.randn(2, 5, 24, device="cuda")
+    out = []
+    for m in (mine, ref):
+        xg = x.clone().requires_grad_()
+        y = m(xg)
+        with fwad.dual_level():
+            (d,) = torch.autograd.grad(y, xg, fwad.make_dual(u, t))
+            out.append(fwad.unpack_dual(d))
+    for a, b in ((out[0].primal, out[1].primal), (out[0].tangent, out[1].tangent)):
+        assert float((a - b).abs().max()) <= 2 * 150 * 2.0 ** -24 * 16 * float(b.abs().max())
